@@ -40,6 +40,21 @@ FMXQ_SYMBOLS = {
     "fmxq_route_softmax_topk": (_int, [_p, _int, _i64, _i64, _int, _bool, _p, _p, _int, _p]),
     "fmxq_route_group_topk": (_int, [_p, _int, _p, _i64, _i64, _int, _int, _int, ctypes.c_float,
                                      _bool, _p, _p, _int, _p]),
+    "fmxq_head_cross_entropy": (_int, [_p] * 9 + [_i64] * 3 + [ctypes.c_int32, _int, _int, _p,
+                                                               ctypes.c_size_t, _p]),
+    "fmxq_head_distill": (_int, [_p] * 6 + [_int] + [_p] * 4 + [_i64] * 3 +
+                          [_int, ctypes.c_float, _int, _int, _p, ctypes.c_size_t, _p]),
+    "fmxq_head_workspace": (_int, [_i64] * 3 + [_int, _bool, _p]),
+    "fmxq_quantized_matmul_grad": (_int, [_p] * 5 + [_i64] * 3 + [_int, _int, _p, ctypes.c_size_t,
+                                                                  _p]),
+    "fmxq_quantized_matmul_grad_workspace": (_int, [_i64] * 3 + [_p]),
+    "fmxq_gather_qmm_grad": (_int, [_p] * 6 + [_i64] * 4 + [_int, _int, _p, ctypes.c_size_t, _p]),
+    "fmxq_gather_qmm_grad_workspace": (_int, [_i64] * 4 + [_p]),
+    "fmxq_moe_sort": (_int, [_p] * 6 + [_i64] * 4 + [_p, ctypes.c_size_t, _p]),
+    "fmxq_moe_sort_workspace": (_int, [_i64] * 3 + [_p]),
+    "fmxq_moe_sort_grad": (_int, [_p] * 3 + [_i64] * 3 + [_p]),
+    "fmxq_moe_unsort": (_int, [_p] * 3 + [_int, _p] + [_i64] * 3 + [_p]),
+    "fmxq_moe_unsort_grad": (_int, [_p] * 4 + [_int, _p, _p] + [_i64] * 3 + [_p]),
 }
 
 

@@ -1,0 +1,120 @@
+// fmxq_grad.hpp -- launchers of the losses over a quantized head, the input gradients of
+// the quantized products and the sorted expert rows (fmxq_grad_gemm.hip, fmxq_head.hip,
+// fmxq_rows.hip), shared with their C ABI (fmxq_grad_capi.cpp).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace fmxq {
+
+// One product D [M, N] = A [M, C] . B with B the dequantized weights (the bits of
+// fmxq_dequantize):
+//   nn = false: B = deq(W)^T, W [N, C] packed along the contraction (logits);
+//   nn = true:  B = deq(W),   W [C, N] packed along the outputs (input gradients).
+// A's rows are 16-byte aligned and lda a multiple of 8; columns of A from a_cols (a multiple
+// of 8) on are read as zero.
+struct GradGemm {
+  const uint16_t* a = nullptr;
+  int64_t lda = 0, a_cols = 0;
+  int64_t M = 0, N = 0, C = 0;
+  const uint32_t* w = nullptr;
+  const uint16_t* scales = nullptr;
+  const uint16_t* biases = nullptr;
+  int group_size = 64, bits = 4;
+  // The contraction in `splits` parts of c_split (a multiple of 64) values; part p goes to
+  // slice p of out.
+  int splits = 1;
+  int64_t c_split = 0;
+  // nn: fp32 slices out [splits][M][N], added to what is there times factor[row] when
+  // factor is given; or, with y, bf16 rows y [M][ldy] (one part only).
+  float* out = nullptr;
+  const float* factor = nullptr;
+  uint16_t* y = nullptr;
+  int64_t ldy = 0;
+  // nt: what a softmax needs of the logits l = D * logit_scale (in units of log 2) by
+  // tiles of stat_width columns: stats[row][tile] = (m, sum 2^(l - m)) with m the tile's
+  // largest l rounded up to an integer, and, with e, e[row][col] = bf16(2^(l - m)) with
+  // zeros in columns N .. lde.
+  float2* stats = nullptr;
+  int64_t stat_tiles = 0;
+  uint16_t* e = nullptr;
+  int64_t lde = 0;
+  float logit_scale = 1.f;
+  // Expert runs (nn only): tile t of the list covers rows [tiles[3t], + tiles[3t+1]) with
+  // expert tiles[3t+2], whose weights are C rows into w.
+  const uint32_t* tiles = nullptr;
+  const uint32_t* ntile = nullptr;
+  int64_t max_tiles = 0;
+};
+
+// Rows of a block's tile, for M rows (or expert runs of about that many).
+int grad_gemm_rows(int64_t M);
+// Columns of a tile of the statistics for M rows.
+int grad_gemm_stat_width(int64_t M);
+constexpr int kGradTileCols = 256;
+hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
+
+// bf16 y [M, N] = the sum of the slices of out [splits][M][N].
+hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64_t M, int64_t N,
+                             hipStream_t stream);
+// dst [M, ld] = src [M, N] with zeros in columns N .. ld.
+hipError_t launch_pad_rows(const uint16_t* src, uint16_t* dst, int64_t M, int64_t N, int64_t ld,
+                           hipStream_t stream);
+// Tiles of `bm` rows of the expert runs [offsets[e], offsets[e + 1]) of S rows as (row, rows,
+// expert) triples, their number, and zeros in the rows of dx [S, N] that no run covers.
+// Offsets that decrease or leave 0 .. S give no tiles, zero rows and raise *flag.
+hipError_t launch_run_tiles(const int32_t* offsets, int64_t E, int64_t S, int bm, uint32_t* tiles,
+                            uint32_t* ntile, uint16_t* dx, int64_t N, uint32_t* flag,
+                            hipStream_t stream);
+
+// A loss over a quantized head (fmxq_head.hip).  ids [M, k]: the targets (k = 1, teacher
+// null) or the teacher's entries.  An id that names no token: `ignore` for targets, below
+// zero for a teacher.
+struct HeadLoss {
+  const uint16_t* h;
+  const uint32_t* w;
+  const uint16_t *scales, *biases;
+  const int32_t* ids;
+  const void* teacher;  // null: cross entropy
+  bool teacher_bf16;
+  const float* grad_loss;
+  float *loss, *lse;
+  uint16_t* dh;  // null: no gradient
+  int64_t M, V, K;
+  int k;
+  int32_t ignore;
+  float temperature;
+  int group_size, bits;
+  uint32_t* flag;
+};
+struct HeadPlan {
+  int bm, stat_width, pieces, splits;
+  int64_t piece, c_split, stat_tiles;
+  size_t stats, e, slices, state, factor, sel, coef, row, bytes;  // offsets in the workspace
+};
+HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);
+hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipStream_t stream);
+
+// Rows sorted by expert and back (fmxq_rows.hip); S = T k slots, slot s of token s / k.
+struct MoeSort {
+  const uint16_t* x;     // [T, D]
+  const uint32_t* inds;  // [S]
+  uint16_t* xs;          // [S, D]
+  uint32_t *order, *pos; // [S]
+  uint32_t* offsets;     // [E + 1]
+  int64_t T, k, E, D;
+  uint32_t* hist;        // moe_sort_hist_bytes
+  uint32_t* flag;
+};
+size_t moe_sort_hist_bytes(int64_t S, int64_t E);
+hipError_t launch_moe_sort(const MoeSort& a, hipStream_t stream);
+// out[t] = sum_j weights[t, j] y[pos[t, j]], weights bf16, fp32 or null (ones).
+hipError_t launch_moe_unsort(const uint16_t* y, const uint32_t* pos, const void* weights,
+                             bool weights_bf16, uint16_t* out, int64_t T, int64_t k, int64_t D,
+                             uint32_t* flag, hipStream_t stream);
+hipError_t launch_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t* pos,
+                                  const void* weights, bool weights_bf16, uint16_t* dy,
+                                  void* dweights, int64_t T, int64_t k, int64_t D, uint32_t* flag,
+                                  hipStream_t stream);
+
+}  // namespace fmxq

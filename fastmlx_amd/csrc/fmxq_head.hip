@@ -1,0 +1,340 @@
+// fmxq_head.hip -- losses over a quantized vocabulary head: cross entropy and the divergence
+// from a teacher's top logits, with the gradient of the hidden states.
+//
+// With l = h . deq(W)^T / T (T = 1 for cross entropy), p = softmax(l) and q the wanted
+// distribution, which has at most k entries a row (one for cross entropy):
+//   lse  = log sum_v exp(l_v)
+//   loss = T^2 sum_j q_j (log q_j - l_j + lse)
+//   dh   = g T (sum_v p_v W_v - sum_j q_j W_j)
+// The vocabulary is walked in pieces.  A piece's product leaves e = 2^(l - m) in bf16 with m
+// the largest l of the row in a tile, rounded up to an integer, and the tile's sum; the join
+// brings the tiles of a row to one m (a power of two: no second rounding), and e . deq(W) is
+// added to fp32 sums that are scaled by the change of m.  The wanted entries' e are zeroed
+// and their share p_j - q_j enters at the end in fp32: where p_j nears q_j the two cancel,
+// and bf16 values of them would leave their rounding.
+#include <algorithm>
+
+#include "fmxq_common.hpp"
+#include "fmxq_grad.hpp"
+
+namespace fmxq {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// 8 dequantized values (fmxq_dequantize's bits) of packed row `row` from column c on.
+__device__ __forceinline__ void deq8(const HeadLoss& a, int64_t row, int64_t c, float* v) {
+  const int64_t grp = (row * a.K + c) / a.group_size;
+  const float s = bf16_bits_to_f32(a.scales[grp]), b = bf16_bits_to_f32(a.biases[grp]);
+  uint32_t w0, w1 = 0;
+  const int64_t at = (row * a.K + c) * a.bits / 32;
+  w0 = a.w[at];
+  if (a.bits == 8) w1 = a.w[at + 1];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float q0, q1;
+    if (a.bits == 4) {
+      q0 = (float)((w0 >> (4 * j)) & 15u);
+      q1 = (float)((w0 >> (4 * j + 4)) & 15u);
+    } else {
+      const uint32_t w = j < 4 ? w0 : w1;
+      q0 = (float)((w >> (8 * (j & 3))) & 255u);
+      q1 = (float)((w >> (8 * (j & 3) + 8)) & 255u);
+    }
+    const uint32_t m = pack_bf16x2(q0 * s, q1 * s);
+    const uint32_t r = pack_bf16x2(bf16_lo(m) + b, bf16_hi(m) + b);
+    v[j] = bf16_lo(r);
+    v[j + 1] = bf16_hi(r);
+  }
+}
+
+// The token of entry j of row m, or -1: absent, or out of range (which raises the flag).
+__device__ __forceinline__ int64_t token_of(const HeadLoss& a, int64_t m, int j, bool report) {
+  const int32_t id = a.ids[m * a.k + j];
+  if (a.teacher ? id < 0 : id == a.ignore) return -1;
+  if (id < 0 || id >= a.V) {
+    if (report) atomicOr(a.flag, 1u);
+    return -1;
+  }
+  return id;
+}
+
+// One wave per wanted entry: its logit in units of log 2, fp32 sums.
+__global__ __launch_bounds__(256) void head_dots_kernel(HeadLoss a, float scale,
+                                                        float* __restrict__ sel) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= a.M * a.k) return;
+  const int64_t m = i / a.k;
+  const int64_t v = token_of(a, m, (int)(i - m * a.k), lane == 0);
+  float t = 0.f;
+  if (v >= 0)
+    for (int64_t c = 8 * lane; c < a.K; c += 512) {
+      float wv[8];
+      deq8(a, v, c, wv);
+      const u32x4 x = *reinterpret_cast<const u32x4*>(a.h + m * a.K + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t = __builtin_fmaf(wv[2 * j], bf16_lo(x[j]), t);
+        t = __builtin_fmaf(wv[2 * j + 1], bf16_hi(x[j]), t);
+      }
+    }
+  t = wave_sum(t);
+  if (lane == 0) sel[i] = t * scale;
+}
+
+// Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought
+// to it with the wanted entries zeroed.  in / out are the states before and after; chunk 0
+// writes out and the factor of the earlier pieces' sums.
+constexpr int kJoinCols = 8192;
+__global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2* __restrict__ stats,
+                                                        int64_t stat_tiles, int tw,
+                                                        const float2* in, float2* out,
+                                                        float* factor, uint16_t* e, int64_t lde,
+                                                        int64_t v0, int64_t tiles) {
+  __shared__ float red[4], red2[4];
+  const int64_t m = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float2* st = stats + m * stat_tiles;
+  const float2 old = in ? in[m] : make_float2(-INFINITY, 0.f);
+  float top = old.x;
+  for (int64_t t = tid; t < tiles; t += 256) top = fmaxf(top, st[t].x);
+  top = wave_max(top);
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (blockIdx.y == 0) {
+    float sum = 0.f;
+    for (int64_t t = tid; t < tiles; t += 256)
+      sum = __builtin_fmaf(st[t].y, __builtin_amdgcn_exp2f(st[t].x - top), sum);
+    sum = wave_sum(sum);
+    if (lane == 0) red2[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      // The first piece starts from nothing: its factor is never used on anything but zeros.
+      const float f = in ? __builtin_amdgcn_exp2f(old.x - top) : 0.f;
+      out[m] = make_float2(top, (in ? old.y * f : 0.f) + (red2[0] + red2[1]) + (red2[2] + red2[3]));
+      if (factor) factor[m] = f;
+    }
+  }
+  if (!e) return;
+  uint16_t* row = e + m * lde;
+  const int64_t c0 = (int64_t)blockIdx.y * kJoinCols;
+  const int64_t c1 = c0 + kJoinCols < lde ? c0 + kJoinCols : lde;
+  for (int64_t c = c0 + 8 * tid; c < c1; c += 2048) {
+    const int64_t t = c / tw;
+    if (t >= tiles) break;  // columns past the vocabulary hold zeros
+    const float f = __builtin_amdgcn_exp2f(st[t].x - top);
+    if (f == 1.f) continue;
+    u32x4 v = *reinterpret_cast<u32x4*>(row + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2(bf16_lo(v[j]) * f, bf16_hi(v[j]) * f);
+    *reinterpret_cast<u32x4*>(row + c) = v;
+  }
+  __syncthreads();
+  for (int j = tid; j < a.k; j += 256) {
+    const int64_t v = token_of(a, m, j, false) - v0;
+    if (v >= c0 && v < c1) row[v] = 0;
+  }
+}
+
+// One wave per row: lse, the loss, each wanted entry's coefficient of W_id and the factor of
+// the sums over e.  A row without a wanted entry has loss 0 and gradient 0 (row factor NaN
+// marks it; the gradient kernel writes zeros without reading the sums).
+__global__ __launch_bounds__(256) void head_loss_kernel(HeadLoss a, const float2* __restrict__ state,
+                                                        const float* __restrict__ sel,
+                                                        float* __restrict__ coef,
+                                                        float2* __restrict__ row) {
+  const int lane = threadIdx.x & 63;
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= a.M) return;
+  const float2 st = state[m];
+  const float lse2 = st.x + __builtin_amdgcn_logf(st.y);  // in units of log 2
+  const float T = a.temperature;
+  const bool on = lane < a.k;
+  const int64_t v = on ? token_of(a, m, lane, false) : -1;
+  float q = v >= 0 ? 1.f : 0.f, logq = 0.f;
+  bool empty;
+  if (a.teacher) {
+    float t = -INFINITY;
+    if (v >= 0)
+      t = (a.teacher_bf16
+               ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.teacher)[m * a.k + lane])
+               : reinterpret_cast<const float*>(a.teacher)[m * a.k + lane]) * (kLog2e / T);
+    const float top = wave_max(t);
+    const bool nan = __any(t != t);
+    empty = top == -INFINITY && !nan;
+    q = empty ? 0.f : __builtin_amdgcn_exp2f(t - top);
+    const float s = wave_sum(q);
+    logq = (t - top) - __builtin_amdgcn_logf(s);
+    q = empty ? 0.f : q / s;
+  } else {
+    empty = !__any(v >= 0);
+  }
+  const float l2 = on ? sel[m * a.k + lane] : 0.f;
+  // Entries of no weight add nothing (0 log 0 = 0); NaN stays.
+  const float term = v >= 0 && q != 0.f ? q * (logq - l2 + lse2) : 0.f;
+  const float loss = wave_sum(term) * (T * T * kLn2);
+  if (lane == 0) {
+    a.lse[m] = lse2 * kLn2;
+    a.loss[m] = empty ? 0.f : loss;
+  }
+  if (!a.dh) return;
+  // p of an id that a row names twice counts once.
+  bool first = v >= 0;
+  for (int j = 0; j < a.k; ++j) {
+    const int32_t vj = __shfl((int)v, j, 64);
+    if (j < lane && vj == (int32_t)v) first = false;
+  }
+  const float g = (a.grad_loss ? a.grad_loss[m] : 1.f) * T;
+  const float p = first ? __builtin_amdgcn_exp2f(l2 - lse2) : 0.f;
+  if (on) coef[m * a.k + lane] = v >= 0 ? g * (p - q) : 0.f;
+  if (lane == 0) row[m] = make_float2(g / st.y, empty ? 1.f : 0.f);
+}
+
+// Thread: 8 columns of a row: the slices' sum times the row's factor, plus the wanted
+// entries' share.
+__global__ __launch_bounds__(256) void head_dh_kernel(HeadLoss a, const float* __restrict__ slices,
+                                                      int splits, const float* __restrict__ coef,
+                                                      const float2* __restrict__ row) {
+  const int64_t m = blockIdx.x;
+  const int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
+  if (c >= a.K) return;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (row[m].y == 0.f) {
+    for (int s = 0; s < splits; ++s) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(slices + ((int64_t)s * a.M + m) * a.K + c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += p[j >> 2][j & 3];
+    }
+    const float f = row[m].x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+    for (int i = 0; i < a.k; ++i) {
+      const int64_t id = token_of(a, m, i, false);
+      if (id < 0) continue;
+      const float co = coef[m * a.k + i];
+      float wv[8];
+      deq8(a, id, c, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(co, wv[j], v[j]);
+    }
+  }
+  *reinterpret_cast<u32x4*>(a.dh + m * a.K + c) =
+      u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+            pack_bf16x2(v[6], v[7])};
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+}  // namespace
+
+// Most bytes of a piece's e.
+constexpr int64_t kHeadPieceBytes = 256 << 20;
+
+HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
+  HeadPlan p{};
+  p.bm = grad_gemm_rows(M);
+  p.stat_width = grad_gemm_stat_width(M);
+  int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
+  p.pieces = (int)((V + piece - 1) / piece);
+  piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
+  p.pieces = (int)((V + piece - 1) / piece);
+  p.piece = piece;
+  p.stat_tiles = up(piece, p.stat_width) / p.stat_width;
+  // Parts of the gradient product's contraction: enough blocks for the chip, each walking
+  // 256 tokens at least.
+  const int64_t tiles = (M + p.bm - 1) / p.bm * ((K + kGradTileCols - 1) / kGradTileCols);
+  const int64_t want = (p.bm >= 128 ? cus : 2 * cus) / tiles;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, piece / 256));
+  p.c_split = up((piece + p.splits - 1) / p.splits, 64);
+  size_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const size_t o = at;
+    at += (size_t)up(bytes, 256);
+    return o;
+  };
+  p.stats = take(M * p.stat_tiles * 8);
+  p.state = take(2 * M * 8);
+  p.sel = take(M * k * 4);
+  p.coef = take(M * k * 4);
+  p.row = take(M * 8);
+  p.factor = take(M * 4);
+  if (grad) {
+    p.e = take(M * piece * 2);
+    p.slices = take((int64_t)p.splits * M * K * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipStream_t stream) {
+  char* base = static_cast<char*>(ws);
+  float2* stats = reinterpret_cast<float2*>(base + p.stats);
+  float2* state = reinterpret_cast<float2*>(base + p.state);
+  float* sel = reinterpret_cast<float*>(base + p.sel);
+  float* coef = reinterpret_cast<float*>(base + p.coef);
+  float2* row = reinterpret_cast<float2*>(base + p.row);
+  float* factor = reinterpret_cast<float*>(base + p.factor);
+  uint16_t* e = a.dh ? reinterpret_cast<uint16_t*>(base + p.e) : nullptr;
+  float* slices = a.dh ? reinterpret_cast<float*>(base + p.slices) : nullptr;
+  const float scale = kLog2e / a.temperature;
+  head_dots_kernel<<<(unsigned)((a.M * a.k + 3) / 4), 256, 0, stream>>>(a, scale, sel);
+  if (hipError_t r = hipGetLastError()) return r;
+  for (int i = 0; i < p.pieces; ++i) {
+    const int64_t v0 = i * p.piece, n = std::min(a.V - v0, p.piece);
+    GradGemm g;
+    g.a = a.h;
+    g.lda = g.a_cols = a.K;
+    g.M = a.M;
+    g.N = n;
+    g.C = a.K;
+    g.c_split = up(a.K, 64);
+    g.w = a.w + v0 * (a.K * a.bits / 32);
+    g.scales = a.scales + v0 * (a.K / a.group_size);
+    g.biases = a.biases + v0 * (a.K / a.group_size);
+    g.group_size = a.group_size;
+    g.bits = a.bits;
+    g.stats = stats;
+    g.stat_tiles = p.stat_tiles;
+    g.e = e;
+    g.lde = up(n, kGradTileCols);
+    g.logit_scale = scale;
+    if (hipError_t r = launch_grad_gemm(g, false, p.bm, stream)) return r;
+    const int64_t tiles = (n + p.stat_width - 1) / p.stat_width;
+    const dim3 grid((unsigned)a.M, e ? (unsigned)((g.lde + kJoinCols - 1) / kJoinCols) : 1u);
+    head_join_kernel<<<grid, 256, 0, stream>>>(a, stats, p.stat_tiles, p.stat_width,
+                                               i ? state + (i & 1) * a.M : nullptr,
+                                               state + ((i + 1) & 1) * a.M, factor, e, g.lde, v0,
+                                               tiles);
+    if (hipError_t r = hipGetLastError()) return r;
+    if (!e) continue;
+    GradGemm d = g;
+    d.a = e;
+    d.lda = d.a_cols = g.lde;
+    d.N = a.K;
+    d.C = n;
+    d.splits = p.splits;
+    d.c_split = p.c_split;
+    d.out = slices;
+    d.factor = i ? factor : nullptr;
+    if (hipError_t r = launch_grad_gemm(d, true, p.bm, stream)) return r;
+  }
+  head_loss_kernel<<<(unsigned)((a.M + 3) / 4), 256, 0, stream>>>(a, state + (p.pieces & 1) * a.M, sel,
+                                                                  coef, row);
+  if (hipError_t r = hipGetLastError()) return r;
+  if (!a.dh) return hipSuccess;
+  const dim3 grid((unsigned)a.M, (unsigned)((a.K + 2047) / 2048));
+  head_dh_kernel<<<grid, 256, 0, stream>>>(a, slices, p.splits, coef, row);
+  return hipGetLastError();
+}
+
+}  // namespace fmxq

@@ -1,0 +1,307 @@
+// fmxq_rows.hip -- token rows sorted by expert and back, for MoE layers whose expert
+// products run over sorted rows, with the gradients of both directions.
+//
+// The sort is a stable counting sort of the S = T k routing slots: order is the one a stable
+// argsort of the ids gives, pos its inverse, offsets[e] the first sorted position of expert
+// e.  Ids >= E sort behind offsets[E]; their rows are zero and they raise the error flag.
+// The row kernels work by token: x (or dout) is read once for its k slots, and the sums of a
+// token are fp32, rounded once.
+#include <algorithm>
+
+#include "fmxq_common.hpp"
+#include "fmxq_grad.hpp"
+
+namespace fmxq {
+namespace {
+
+// Slots of a block of the sort, in 4 waves of consecutive slots each.
+constexpr int kSortSlots = 1024;
+constexpr int kWaveSlots = kSortSlots / 4;
+
+__device__ __forceinline__ uint32_t bucket_of(uint32_t e, int64_t E) {
+  return e < (uint64_t)E ? e : (uint32_t)E;
+}
+
+// hist[block][e]: slots of each expert (bucket E: ids out of range) in the block's range.
+__global__ __launch_bounds__(256) void sort_hist_kernel(MoeSort a, int64_t S) {
+  extern __shared__ uint32_t cnt[];
+  const int64_t nb = a.E + 1, s0 = (int64_t)blockIdx.x * kSortSlots;
+  for (int64_t i = threadIdx.x; i < nb; i += 256) cnt[i] = 0;
+  __syncthreads();
+  for (int64_t s = s0 + threadIdx.x; s < s0 + kSortSlots && s < S; s += 256)
+    atomicAdd(&cnt[bucket_of(a.inds[s], a.E)], 1u);
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < nb; i += 256) a.hist[blockIdx.x * nb + i] = cnt[i];
+}
+
+// Exclusive prefix sum over 256 threads.
+__device__ __forceinline__ uint32_t scan256(uint32_t v, uint32_t* wsum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = (uint32_t)__shfl_up((int)inc, o, 64);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();
+  if (lane == 63) wsum[wave] = inc;
+  __syncthreads();
+  uint32_t r = inc - v;
+  for (int i = 0; i < wave; ++i) r += wsum[i];
+  return r;
+}
+
+// Lanes of the wave with the same bucket: one ballot per bit of the bucket.
+__device__ __forceinline__ uint64_t same_bucket(uint32_t b, bool on, int bits) {
+  uint64_t m = __ballot(on);
+  for (int i = 0; i < bits; ++i) {
+    const uint64_t set = __ballot((b >> i) & 1u);
+    m &= (b >> i) & 1u ? set : ~set;
+  }
+  return m;
+}
+
+// Orders the wave's own LDS accesses (no instruction; the LDS serves a wave in order).
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Each block adds up the histograms before its own (every block reads the few tables again,
+// which costs less than a launch for the scan), then its waves place their slots in order.
+__global__ __launch_bounds__(256) void sort_place_kernel(MoeSort a, int64_t S, int bits) {
+  extern __shared__ uint32_t lds[];  // cursors of each wave: 4 x (E + 1)
+  __shared__ uint32_t wsum[4];
+  const int64_t nb = a.E + 1, s0 = (int64_t)blockIdx.x * kSortSlots;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t* cur = lds;
+  // Per-wave counts of the block's slots.
+  for (int64_t i = tid; i < 4 * nb; i += 256) cur[i] = 0;
+  __syncthreads();
+  const int64_t w0 = s0 + wave * kWaveSlots, w1 = w0 + kWaveSlots < S ? w0 + kWaveSlots : S;
+  for (int64_t s = w0 + lane; s < w1; s += 64)
+    atomicAdd(&cur[wave * nb + bucket_of(a.inds[s], a.E)], 1u);
+  __syncthreads();
+  // Each thread takes a run of buckets: total over all blocks and over the earlier ones.
+  const int64_t per = (nb + 255) / 256;
+  const int64_t b0 = tid * per < nb ? tid * per : nb, b1 = b0 + per < nb ? b0 + per : nb;
+  uint32_t total = 0;
+  for (int64_t e = b0; e < b1; ++e)
+    for (unsigned k = 0; k < gridDim.x; ++k) total += a.hist[k * nb + e];
+  uint32_t base = scan256(total, wsum);
+  for (int64_t e = b0; e < b1; ++e) {
+    if (blockIdx.x == 0) {
+      a.offsets[e] = base;
+      if (e == a.E && base < S) atomicOr(a.flag, 1u);
+    }
+    uint32_t before = 0, all = 0;
+    for (unsigned k = 0; k < gridDim.x; ++k) {
+      const uint32_t v = a.hist[k * nb + e];
+      if (k < blockIdx.x) before += v;
+      all += v;
+    }
+    uint32_t at = base + before;
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t n = cur[w * nb + e];
+      cur[w * nb + e] = at;
+      at += n;
+    }
+    base += all;
+  }
+  __syncthreads();
+  for (int64_t s = w0 + lane; s - lane < w1; s += 64) {
+    const bool on = s < w1;
+    const uint32_t b = on ? bucket_of(a.inds[s], a.E) : 0u;
+    const uint64_t same = same_bucket(b, on, bits);
+    if (on) {
+      const uint32_t p = cur[wave * nb + b] + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+      a.order[p] = (uint32_t)s;
+      a.pos[s] = p;
+    }
+    wave_fence();
+    if (on && (same & ((1ull << lane) - 1)) == 0)
+      cur[wave * nb + b] += (uint32_t)__popcll(same);
+    wave_fence();
+  }
+}
+
+// 8 (or 1) bf16 values.
+template <int VEC>
+struct Row;
+template <>
+struct Row<8> {
+  u32x4 v;
+  __device__ __forceinline__ static Row load(const uint16_t* p) {
+    return {*reinterpret_cast<const u32x4*>(p)};
+  }
+  __device__ __forceinline__ void store(uint16_t* p) const { *reinterpret_cast<u32x4*>(p) = v; }
+  __device__ __forceinline__ float at(int i) const {
+    return i & 1 ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]);
+  }
+  __device__ __forceinline__ static Row of(const float* f) {
+    return {u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                  pack_bf16x2(f[6], f[7])}};
+  }
+};
+template <>
+struct Row<1> {
+  uint16_t v;
+  __device__ __forceinline__ static Row load(const uint16_t* p) { return {*p}; }
+  __device__ __forceinline__ void store(uint16_t* p) const { *p = v; }
+  __device__ __forceinline__ float at(int) const { return bf16_bits_to_f32(v); }
+  __device__ __forceinline__ static Row of(const float* f) {
+    return {(uint16_t)f32_to_bf16_rne(f[0])};
+  }
+};
+
+__device__ __forceinline__ float weight_of(const void* w, bool bf16, int64_t i) {
+  return bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(w)[i])
+              : reinterpret_cast<const float*>(w)[i];
+}
+
+// xs[pos[t, j]] = x[t], or zeros for ids out of range.
+template <int VEC>
+__global__ __launch_bounds__(256) void rows_out_kernel(MoeSort a) {
+  const int64_t t = blockIdx.x;
+  const uint32_t valid = a.offsets[a.E];
+  for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * VEC; c < a.D;
+       c += (int64_t)gridDim.y * 256 * VEC) {
+    const Row<VEC> x = Row<VEC>::load(a.x + t * a.D + c);
+    for (int64_t j = 0; j < a.k; ++j) {
+      const uint32_t p = a.pos[t * a.k + j];
+      (p < valid ? x : Row<VEC>{}).store(a.xs + (int64_t)p * a.D + c);
+    }
+  }
+}
+
+// out[t] = sum_j w[t, j] y[pos[t, j]]; a position outside the rows adds nothing.
+template <int VEC>
+__global__ __launch_bounds__(256) void rows_sum_kernel(const uint16_t* __restrict__ y,
+                                                       const uint32_t* __restrict__ pos,
+                                                       const void* __restrict__ weights,
+                                                       bool wbf16, uint16_t* __restrict__ out,
+                                                       int64_t S, int64_t k, int64_t D,
+                                                       uint32_t* flag) {
+  const int64_t t = blockIdx.x;
+  for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * VEC; c < D;
+       c += (int64_t)gridDim.y * 256 * VEC) {
+    float s[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+    for (int64_t j = 0; j < k; ++j) {
+      const int64_t p = pos[t * k + j];
+      if (p >= S) {
+        if (c == 0) atomicOr(flag, 1u);
+        continue;
+      }
+      const float w = weights ? weight_of(weights, wbf16, t * k + j) : 1.f;
+      const Row<VEC> v = Row<VEC>::load(y + p * D + c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] = __builtin_fmaf(w, v.at(i), s[i]);
+    }
+    Row<VEC>::of(s).store(out + t * D + c);
+  }
+}
+
+// One block per token: dy[pos] = w dout, dweights = <dout, y[pos]>.
+template <int VEC>
+__global__ __launch_bounds__(256) void rows_grad_kernel(const uint16_t* __restrict__ dout,
+                                                        const uint16_t* __restrict__ y,
+                                                        const uint32_t* __restrict__ pos,
+                                                        const void* __restrict__ weights,
+                                                        bool wbf16, uint16_t* __restrict__ dy,
+                                                        void* __restrict__ dweights, int64_t S,
+                                                        int64_t k, int64_t D, uint32_t* flag) {
+  __shared__ float red[4];
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t j = 0; j < k; ++j) {
+    const int64_t p = pos[t * k + j];
+    const float w = weight_of(weights, wbf16, t * k + j);
+    float dot = 0.f;
+    if (p < S) {
+      for (int64_t c = threadIdx.x * VEC; c < D; c += 256 * VEC) {
+        const Row<VEC> d = Row<VEC>::load(dout + t * D + c), v = Row<VEC>::load(y + p * D + c);
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          dot = __builtin_fmaf(d.at(i), v.at(i), dot);
+          o[i] = w * d.at(i);
+        }
+        Row<VEC>::of(o).store(dy + p * D + c);
+      }
+    } else if (threadIdx.x == 0) {
+      atomicOr(flag, 1u);
+    }
+    dot = wave_sum(dot);
+    if (lane == 0) red[wave] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const float v = (red[0] + red[1]) + (red[2] + red[3]);
+      if (wbf16) reinterpret_cast<uint16_t*>(dweights)[t * k + j] = (uint16_t)f32_to_bf16_rne(v);
+      else reinterpret_cast<float*>(dweights)[t * k + j] = v;
+    }
+    __syncthreads();
+  }
+}
+
+bool vec8(int64_t D, const void* a, const void* b, const void* c) {
+  return D % 8 == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
+                         reinterpret_cast<uintptr_t>(c)) & 15) == 0;
+}
+
+dim3 row_grid(int64_t T, int64_t D, int vec) {
+  const int64_t y = (D + 256 * vec - 1) / (256 * vec);
+  return dim3((unsigned)T, (unsigned)std::min<int64_t>(std::max<int64_t>(y, 1), 1024));
+}
+
+}  // namespace
+
+size_t moe_sort_hist_bytes(int64_t S, int64_t E) {
+  return (size_t)((S + kSortSlots - 1) / kSortSlots) * (E + 1) * sizeof(uint32_t);
+}
+
+hipError_t launch_moe_sort(const MoeSort& a, hipStream_t stream) {
+  const int64_t S = a.T * a.k, nb = a.E + 1;
+  const unsigned blocks = (unsigned)((S + kSortSlots - 1) / kSortSlots);
+  int bits = 1;
+  while (nb > ((int64_t)1 << bits)) ++bits;
+  sort_hist_kernel<<<blocks, 256, nb * sizeof(uint32_t), stream>>>(a, S);
+  if (hipError_t e = hipGetLastError()) return e;
+  sort_place_kernel<<<blocks, 256, 4 * nb * sizeof(uint32_t), stream>>>(a, S, bits);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (a.D == 0) return hipSuccess;
+  if (vec8(a.D, a.x, a.xs, nullptr))
+    rows_out_kernel<8><<<row_grid(a.T, a.D, 8), 256, 0, stream>>>(a);
+  else
+    rows_out_kernel<1><<<row_grid(a.T, a.D, 1), 256, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_moe_unsort(const uint16_t* y, const uint32_t* pos, const void* weights,
+                             bool weights_bf16, uint16_t* out, int64_t T, int64_t k, int64_t D,
+                             uint32_t* flag, hipStream_t stream) {
+  if (vec8(D, y, out, nullptr))
+    rows_sum_kernel<8><<<row_grid(T, D, 8), 256, 0, stream>>>(y, pos, weights, weights_bf16, out,
+                                                              T * k, k, D, flag);
+  else
+    rows_sum_kernel<1><<<row_grid(T, D, 1), 256, 0, stream>>>(y, pos, weights, weights_bf16, out,
+                                                              T * k, k, D, flag);
+  return hipGetLastError();
+}
+
+hipError_t launch_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t* pos,
+                                  const void* weights, bool weights_bf16, uint16_t* dy,
+                                  void* dweights, int64_t T, int64_t k, int64_t D, uint32_t* flag,
+                                  hipStream_t stream) {
+  if (vec8(D, dout, y, dy))
+    rows_grad_kernel<8><<<(unsigned)T, 256, 0, stream>>>(dout, y, pos, weights, weights_bf16, dy,
+                                                         dweights, T * k, k, D, flag);
+  else
+    rows_grad_kernel<1><<<(unsigned)T, 256, 0, stream>>>(dout, y, pos, weights, weights_bf16, dy,
+                                                         dweights, T * k, k, D, flag);
+  return hipGetLastError();
+}
+
+}  // namespace fmxq

@@ -298,6 +298,260 @@ def route_group_topk(gates, bias, top_k, n_group, topk_group, routed_scaling_fac
     return inds, weights
 
 
+# ---- training and scoring over quantized weights --------------------------------
+# Plain functions, forward and backward, without autograd: a gradient is a call of its own.
+
+
+def _same_device(**tensors):
+    """The tensors' device; ValueError where they are on several."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None and name == "grad_loss":
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, other operands on {dev}")
+        dev = t.device
+    if dev is None or dev.type != "cuda":
+        raise ValueError(f"operands must live on the GPU (got {dev})")
+    return dev
+
+
+def _shape(name, t, *shape):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _quant_shapes(w, scales, biases, lead, K, group_size, bits):
+    if bits not in (4, 8) or group_size not in (32, 64, 128):
+        return  # refused by the library, which names the supported ones
+    if K % group_size:
+        raise ValueError(f"K={K} is not a multiple of group_size={group_size}")
+    _shape("w", w, *lead, K * bits // 32)
+    _shape("scales", scales, *lead, K // group_size)
+    _shape("biases", biases, *lead, K // group_size)
+
+
+def _workspace(fn, dev, *sizes):
+    """A workspace for a call with these sizes, from torch's allocator: its own in every
+    call, stream and captured graph.  (pointer, bytes, the tensor that keeps it)"""
+    import ctypes
+
+    n = ctypes.c_size_t()
+    check(fn(*sizes, ctypes.byref(n)))
+    t = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    return (t.data_ptr() if n.value else None), n.value, t
+
+
+def _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits):
+    if h.dim() != 2 or w.dim() != 2:
+        raise ValueError("h must be [M, K] and w [V, K*bits/32]")
+    M, K = h.shape
+    V = w.shape[0]
+    _quant_shapes(w, scales, biases, (V,), K, group_size, bits)
+    if grad_loss is not None:
+        if not grad:
+            raise ValueError("grad_loss without grad=True")
+        _shape("grad_loss", grad_loss, M)
+        _dev(grad_loss, "grad_loss", (torch.float32,))
+    ptrs = (_dev(h, "h", _BF16_LIKE), _dev(w, "w", _U32_LIKE), _dev(scales, "scales", _BF16_LIKE),
+            _dev(biases, "biases", _BF16_LIKE))
+    return M, V, K, ptrs
+
+
+def _head_results(M, K, dev, grad):
+    loss = torch.empty(M, dtype=torch.float32, device=dev)
+    lse = torch.empty(M, dtype=torch.float32, device=dev)
+    dh = torch.empty(M, K, dtype=torch.bfloat16, device=dev) if grad else None
+    return loss, lse, dh
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def head_cross_entropy(h, w, scales, biases, targets, ignore_index: int = -100, grad: bool = False,
+                       grad_loss=None, group_size: int = 64, bits: int = 4):
+    """Cross entropy of a quantized vocabulary head, its logits never stored.
+
+    h [M, K] bf16; w [V, K*bits/32] with scales and biases [V, K/group]; targets [M] int32.
+    Returns (loss [M], lse [M]) float32 with lse the log of the row's sum of exponentials, and
+    with ``grad`` also dh [M, K] bf16, the gradient of sum_t grad_loss[t] loss[t] (grad_loss
+    [M] float32, ones without).  A target equal to ignore_index has loss and gradient 0; one
+    outside the vocabulary too, which device_error reports."""
+    dev = _same_device(h=h, w=w, scales=scales, biases=biases, targets=targets,
+                       grad_loss=grad_loss)
+    M, V, K, ptrs = _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits)
+    _shape("targets", targets, M)
+    tp = _dev(targets, "targets", (torch.int32,))
+    lib = load()
+    with torch.cuda.device(dev):
+        loss, lse, dh = _head_results(M, K, dev, grad)
+        ws, n, keep = _workspace(lib.fmxq_head_workspace, dev, M, V, K, 1, bool(grad))
+        check(lib.fmxq_head_cross_entropy(*ptrs, tp, _ptr(grad_loss), loss.data_ptr(),
+                                          lse.data_ptr(), _ptr(dh), M, V, K, ignore_index,
+                                          group_size, bits, ws, n, _stream(h)))
+    return (loss, lse, dh) if grad else (loss, lse)
+
+
+def head_distill(h, w, scales, biases, ids, teacher, temperature: float = 1.0, grad: bool = False,
+                 grad_loss=None, group_size: int = 64, bits: int = 4):
+    """Divergence of a quantized head's softmax from a teacher's top logits.
+
+    ids [M, k] int32 and teacher [M, k] (bfloat16 or float32): the tokens and logits the
+    teacher kept, k <= 64, an id below zero for an absent entry.  With q = softmax(teacher / T)
+    over the entries and p = softmax(logits / T) over the vocabulary, returns (loss [M] =
+    T^2 KL(q || p), lse [M] = log sum exp(logits / T)) float32, and with ``grad`` dh [M, K] as
+    head_cross_entropy does."""
+    dev = _same_device(h=h, w=w, scales=scales, biases=biases, ids=ids, teacher=teacher,
+                       grad_loss=grad_loss)
+    M, V, K, ptrs = _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits)
+    if ids.dim() != 2:
+        raise ValueError("ids must be [M, k]")
+    k = ids.shape[1]
+    _shape("ids", ids, M, k)
+    _shape("teacher", teacher, M, k)
+    ip = _dev(ids, "ids", (torch.int32,))
+    tp = _dev(teacher, "teacher", (torch.bfloat16, torch.float32))
+    lib = load()
+    with torch.cuda.device(dev):
+        loss, lse, dh = _head_results(M, K, dev, grad)
+        ws, n, keep = _workspace(lib.fmxq_head_workspace, dev, M, V, K, k, bool(grad))
+        check(lib.fmxq_head_distill(*ptrs, ip, tp, int(teacher.dtype == torch.bfloat16),
+                                    _ptr(grad_loss), loss.data_ptr(), lse.data_ptr(), _ptr(dh), M,
+                                    V, K, k, temperature, group_size, bits, ws, n, _stream(h)))
+    return (loss, lse, dh) if grad else (loss, lse)
+
+
+def quantized_matmul_grad(dy, w, scales, biases, group_size: int = 64, bits: int = 4):
+    """Gradient of x in quantized_matmul: dx = dy @ deq(W), dy [..., N] bf16, w [N, K*bits/32];
+    dx [..., K] bf16."""
+    dev = _same_device(dy=dy, w=w, scales=scales, biases=biases)
+    if w.dim() != 2 or dy.dim() < 1:
+        raise ValueError("dy must be [..., N] and w [N, K*bits/32]")
+    N, K = w.shape[0], w.shape[1] * 32 // bits if bits in (4, 8) else 0
+    if dy.shape[-1] != N:
+        raise ValueError(f"dy has {dy.shape[-1]} columns but w {N} rows")
+    _quant_shapes(w, scales, biases, (N,), K, group_size, bits)
+    M = 1
+    for d in dy.shape[:-1]:
+        M *= d
+    args = (_dev(dy, "dy", _BF16_LIKE), _dev(w, "w", _U32_LIKE),
+            _dev(scales, "scales", _BF16_LIKE), _dev(biases, "biases", _BF16_LIKE))
+    lib = load()
+    with torch.cuda.device(dev):
+        dx = torch.empty(*dy.shape[:-1], K, dtype=torch.bfloat16, device=dev)
+        ws, n, keep = _workspace(lib.fmxq_quantized_matmul_grad_workspace, dev, M, N, K)
+        check(lib.fmxq_quantized_matmul_grad(*args, dx.data_ptr(), M, N, K, group_size, bits, ws,
+                                             n, _stream(dy)))
+    return dx
+
+
+def gather_qmm_grad(dy, w, scales, biases, offsets, group_size: int = 64, bits: int = 4):
+    """Gradient of x in gather_qmm over rows sorted by expert (moe_sort): rows offsets[e] ..
+    offsets[e + 1] of dx are dy @ deq(W[e]).  dy [S, N] bf16; w [E, N, K*bits/32]; offsets
+    [E + 1] int32; dx [S, K] bf16, zero in rows of no expert."""
+    dev = _same_device(dy=dy, w=w, scales=scales, biases=biases, offsets=offsets)
+    if w.dim() != 3 or dy.dim() != 2:
+        raise ValueError("dy must be [S, N] and w [E, N, K*bits/32]")
+    E, N = w.shape[:2]
+    K = w.shape[2] * 32 // bits if bits in (4, 8) else 0
+    S = dy.shape[0]
+    _shape("dy", dy, S, N)
+    _shape("offsets", offsets, E + 1)
+    _quant_shapes(w, scales, biases, (E, N), K, group_size, bits)
+    args = (_dev(dy, "dy", _BF16_LIKE), _dev(w, "w", _U32_LIKE),
+            _dev(scales, "scales", _BF16_LIKE), _dev(biases, "biases", _BF16_LIKE),
+            _dev(offsets, "offsets", (torch.int32,)))
+    lib = load()
+    with torch.cuda.device(dev):
+        dx = torch.empty(S, K, dtype=torch.bfloat16, device=dev)
+        ws, n, keep = _workspace(lib.fmxq_gather_qmm_grad_workspace, dev, S, E, N, K)
+        check(lib.fmxq_gather_qmm_grad(*args, dx.data_ptr(), S, E, N, K, group_size, bits, ws, n,
+                                       _stream(dy)))
+    return dx
+
+
+def moe_sort(x, inds, n_experts: int):
+    """Token rows sorted by expert: x [T, D] bf16, inds [T, k] int32/uint32 ->
+    (xs [T k, D], order [T k], pos [T, k], offsets [n_experts + 1]), the last three int32.
+
+    Slot t k + j goes to row pos[t, j]; order is the stable argsort of the ids; expert e has
+    rows offsets[e] .. offsets[e + 1].  Ids out of range sort last with zero rows, and
+    device_error reports them."""
+    dev = _same_device(x=x, inds=inds)
+    if x.dim() != 2 or inds.dim() != 2:
+        raise ValueError("x must be [T, D] and inds [T, k]")
+    T, D = x.shape
+    k = inds.shape[1]
+    _shape("inds", inds, T, k)
+    xp, ip = _dev(x, "x", _BF16_LIKE), _dev(inds, "inds", _U32_LIKE)
+    lib = load()
+    with torch.cuda.device(dev):
+        ws, n, keep = _workspace(lib.fmxq_moe_sort_workspace, dev, T, k, n_experts)
+        xs = torch.empty(T * k, D, dtype=torch.bfloat16, device=dev)
+        order = torch.empty(T * k, dtype=torch.int32, device=dev)
+        pos = torch.empty(T, k, dtype=torch.int32, device=dev)
+        offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+        check(lib.fmxq_moe_sort(xp, ip, xs.data_ptr(), order.data_ptr(), pos.data_ptr(),
+                                offsets.data_ptr(), T, k, n_experts, D, ws, n, _stream(x)))
+    return xs, order, pos, offsets
+
+
+def _sorted_rows(name, y, pos):
+    if y.dim() != 2 or pos.dim() != 2:
+        raise ValueError(f"{name} must be [T k, D] and pos [T, k]")
+    T, k = pos.shape
+    _shape(name, y, T * k, y.shape[1])
+    return T, k, y.shape[1], _dev(y, name, _BF16_LIKE), _dev(pos, "pos", _U32_LIKE)
+
+
+def _row_weights(weights, T, k):
+    _shape("weights", weights, T, k)
+    return (_dev(weights, "weights", (torch.bfloat16, torch.float32)),
+            int(weights.dtype == torch.bfloat16))
+
+
+def moe_sort_grad(dxs, pos):
+    """Gradient of moe_sort's x: dxs [T k, D] bf16 -> dx [T, D] bf16, each token's slots summed
+    in float32."""
+    dev = _same_device(dxs=dxs, pos=pos)
+    T, k, D, yp, pp = _sorted_rows("dxs", dxs, pos)
+    with torch.cuda.device(dev):
+        dx = torch.empty(T, D, dtype=torch.bfloat16, device=dev)
+        check(load().fmxq_moe_sort_grad(yp, pp, dx.data_ptr(), T, k, D, _stream(dxs)))
+    return dx
+
+
+def moe_unsort(y, pos, weights):
+    """Sorted rows back to tokens: out[t] = sum_j weights[t, j] y[pos[t, j]] in float32, rounded
+    once.  y [T k, D] bf16; weights [T, k] bfloat16 or float32; out [T, D] bf16."""
+    dev = _same_device(y=y, pos=pos, weights=weights)
+    T, k, D, yp, pp = _sorted_rows("y", y, pos)
+    wp, wb = _row_weights(weights, T, k)
+    with torch.cuda.device(dev):
+        out = torch.empty(T, D, dtype=torch.bfloat16, device=dev)
+        check(load().fmxq_moe_unsort(yp, pp, wp, wb, out.data_ptr(), T, k, D, _stream(y)))
+    return out
+
+
+def moe_unsort_grad(dout, y, pos, weights):
+    """Gradients of moe_unsort: dout [T, D] bf16 -> (dy [T k, D] bf16, dweights [T, k] in the
+    weights' type)."""
+    dev = _same_device(dout=dout, y=y, pos=pos, weights=weights)
+    T, k, D, yp, pp = _sorted_rows("y", y, pos)
+    _shape("dout", dout, T, D)
+    dp = _dev(dout, "dout", _BF16_LIKE)
+    wp, wb = _row_weights(weights, T, k)
+    with torch.cuda.device(dev):
+        dy = torch.empty(T * k, D, dtype=torch.bfloat16, device=dev)
+        dw = torch.empty(T, k, dtype=weights.dtype, device=dev)
+        check(load().fmxq_moe_unsort_grad(dp, yp, pp, wp, wb, dy.data_ptr(), dw.data_ptr(), T, k, D,
+                                          _stream(dout)))
+    return dy, dw
+
+
 def device_error(device=None) -> None:
     """Raise FmxqError(FMXQ_ERR_INDEX) if a gather met an out-of-range index."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device

@@ -32,6 +32,7 @@
 #define FMXQ_H
 
 #include <stdbool.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -270,6 +271,93 @@ int fmxq_route_group_topk(const void* gates, int gates_bf16, const float* bias, 
                           int64_t E, int top_k, int n_group, int topk_group,
                           float routed_scaling_factor, bool norm_topk_prob, uint32_t* inds,
                           void* weights, int weights_bf16, void* stream);
+
+/* ---- training and scoring over quantized weights ----
+ * No counterpart in the reference, whose models only answer: the losses of a quantized
+ * vocabulary head, the input gradients of the quantized products and the row order that a
+ * trained mixture-of-experts layer needs, so that adapters, norms and routers around frozen
+ * quantized weights can be trained or distilled, and text can be scored.
+ * deq(W) is fmxq_dequantize's, bit for bit.  Sums, softmax statistics and losses are fp32;
+ * dh, dx and rows are rounded to bf16 once.
+ * These calls own no memory: `workspace` holds the bytes that the call's _workspace function
+ * reports for the same sizes, is 16-byte aligned, needs no contents and may be reused once
+ * the call's work is done.  Calls that may overlap (two streams, two graphs replayed at once)
+ * need a workspace each.  They can be captured into a graph at any time. */
+
+/* Cross entropy of a quantized head: logits l = h . deq(W)^T over V tokens, which are never
+ * stored;
+ *     lse[t] = log sum_v exp(l[t, v]),  loss[t] = lse[t] - l[t, targets[t]],
+ * and, with dh non-NULL, the gradient of the hidden states
+ *     dh[t] = grad_loss[t] (sum_v softmax(l[t])_v deq(W)_v - deq(W)_targets[t])
+ * (grad_loss NULL: ones).  h [M, K] bf16; w, scales, biases as for quantized_matmul with N = V;
+ * targets [M]; loss, lse, grad_loss [M]; dh [M, K] bf16.  A target equal to ignore_index gives
+ * loss 0 and a zero row of dh; so does one outside 0 .. V - 1, which raises the error flag. */
+int fmxq_head_cross_entropy(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
+                            const uint16_t* biases, const int32_t* targets,
+                            const float* grad_loss, float* loss, float* lse, uint16_t* dh,
+                            int64_t M, int64_t V, int64_t K, int32_t ignore_index, int group_size,
+                            int bits, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation through the same head from a teacher's top_k (1 .. 64) logits.  With
+ * T = temperature > 0, l as above, p = softmax(l / T) over all tokens and q = softmax(teacher / T)
+ * over the row's entries:
+ *     lse[t] = log sum_v exp(l[t, v] / T),  loss[t] = T^2 sum_j q_j (log q_j - log p_ids[j]),
+ *     dh[t] = grad_loss[t] T (sum_v p_v deq(W)_v - sum_j q_j deq(W)_ids[j]).
+ * ids [M, top_k], an id below zero for an absent entry; teacher [M, top_k] (bf16 when
+ * teacher_bf16, else fp32).  An id may occur twice (its q add up).  A row whose entries are all
+ * absent or -infinity gives loss 0 and a zero row of dh.  An id of V or more counts as absent
+ * and raises the error flag. */
+int fmxq_head_distill(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
+                      const uint16_t* biases, const int32_t* ids, const void* teacher,
+                      int teacher_bf16, const float* grad_loss, float* loss, float* lse,
+                      uint16_t* dh, int64_t M, int64_t V, int64_t K, int top_k, float temperature,
+                      int group_size, int bits, void* workspace, size_t workspace_bytes,
+                      void* stream);
+/* Workspace of the two losses (top_k = 1 for cross entropy). */
+int fmxq_head_workspace(int64_t M, int64_t V, int64_t K, int top_k, bool with_grad, size_t* bytes);
+
+/* Gradient of x in quantized_matmul's y = x . deq(W)^T:
+ *     dx [M, K] = dy [M, N] . deq(W),  dy and dx bf16, N any size. */
+int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
+                               const uint16_t* biases, uint16_t* dx, int64_t M, int64_t N,
+                               int64_t K, int group_size, int bits, void* workspace,
+                               size_t workspace_bytes, void* stream);
+int fmxq_quantized_matmul_grad_workspace(int64_t M, int64_t N, int64_t K, size_t* bytes);
+
+/* The same for gather_qmm over rows sorted by expert: row r of dx [S, K] is dy[r] . deq(W[e])
+ * for offsets[e] <= r < offsets[e + 1] (offsets [E + 1], as fmxq_moe_sort writes them), and
+ * zero where no expert has the row.  Offsets that decrease or leave 0 .. S give zero rows and
+ * raise the error flag. */
+int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
+                         const uint16_t* biases, const int32_t* offsets, uint16_t* dx, int64_t S,
+                         int64_t E, int64_t N, int64_t K, int group_size, int bits,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int fmxq_gather_qmm_grad_workspace(int64_t S, int64_t E, int64_t N, int64_t K, size_t* bytes);
+
+/* Token rows sorted by expert.  The S = T top_k routing slots (slot t top_k + j is inds[t, j])
+ * are ordered by expert, slots of one expert in their own order:
+ *     order [S]: the slot at each sorted position;  pos [T, top_k]: each slot's position;
+ *     offsets [E + 1]: the first position of each expert;  xs [S, D] = x[order / top_k].
+ * x [T, D] bf16; E <= 2048.  Ids outside 0 .. E - 1 sort behind offsets[E]; their rows are zero
+ * and they raise the error flag. */
+int fmxq_moe_sort(const uint16_t* x, const uint32_t* inds, uint16_t* xs, uint32_t* order,
+                  uint32_t* pos, uint32_t* offsets, int64_t T, int64_t top_k, int64_t E, int64_t D,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int fmxq_moe_sort_workspace(int64_t T, int64_t top_k, int64_t E, size_t* bytes);
+/* Gradient of moe_sort's x: dx[t] = sum_j dxs[pos[t, j]]. */
+int fmxq_moe_sort_grad(const uint16_t* dxs, const uint32_t* pos, uint16_t* dx, int64_t T,
+                       int64_t top_k, int64_t D, void* stream);
+/* The way back: out[t] = sum_j weights[t, j] y[pos[t, j]], y [S, D] sorted, weights [T, top_k]
+ * (bf16 when weights_bf16, else fp32), one rounding (moe_combine, which this resembles, keeps
+ * the reference's rounding of each product).  A position outside 0 .. S - 1 adds nothing and
+ * raises the error flag. */
+int fmxq_moe_unsort(const uint16_t* y, const uint32_t* pos, const void* weights, int weights_bf16,
+                    uint16_t* out, int64_t T, int64_t top_k, int64_t D, void* stream);
+/* Its gradients: dy[pos[t, j]] = weights[t, j] dout[t] (rows of dy that no position names are
+ * left as they were), dweights[t, j] = <dout[t], y[pos[t, j]]> in the weights' type. */
+int fmxq_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t* pos,
+                         const void* weights, int weights_bf16, uint16_t* dy, void* dweights,
+                         int64_t T, int64_t top_k, int64_t D, void* stream);
 
 /* Synchronizes `stream`, then reports (and clears) the device-side error flags
  * that gather kernels raise on an out-of-range index: returns FMXQ_OK or
