@@ -21,6 +21,10 @@ struct GradGemm {
   const uint16_t* scales = nullptr;
   const uint16_t* biases = nullptr;
   int group_size = 64, bits = 4;
+  // launch_panel_gemm: the weights as bf16, row n of panel [N][ldp] the C contraction values
+  // of output column n (ldp a multiple of 8; values from C on are not read).
+  const uint16_t* panel = nullptr;
+  int64_t ldp = 0;
   // The contraction in `splits` parts of c_split (a multiple of 64) values; part p goes to
   // slice p of out.
   int splits = 1;
@@ -53,6 +57,17 @@ int grad_gemm_rows(int64_t M);
 int grad_gemm_stat_width(int64_t M);
 constexpr int kGradTileCols = 256;
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
+
+// The same products over a panel of weights dequantized beforehand (fmxq_grad_panel.hip), in
+// tiles of kPanelRows rows.
+constexpr int kPanelRows = 256;
+constexpr int kPanelStatWidth = 128;
+hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream);
+// panel [K][ld] = deq(W)^T for packed rows W [n, K], ld >= n a multiple of 8; columns n .. of
+// the last 8 hold zeros.
+hipError_t launch_dequant_transposed(const uint32_t* w, const uint16_t* scales,
+                                     const uint16_t* biases, uint16_t* panel, int64_t n, int64_t K,
+                                     int64_t ld, int group_size, int bits, hipStream_t stream);
 
 // bf16 y [M, N] = the sum of the slices of out [splits][M][N].
 hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64_t M, int64_t N,
@@ -90,7 +105,8 @@ struct HeadLoss {
 struct HeadPlan {
   int bm, stat_width, pieces, splits;
   int64_t piece, c_split, stat_tiles;
-  size_t stats, e, slices, state, factor, sel, coef, row, bytes;  // offsets in the workspace
+  bool panel;  // the products run over panels of dequantized weights
+  size_t stats, e, slices, state, factor, sel, coef, row, panel_at, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);
 hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipStream_t stream);

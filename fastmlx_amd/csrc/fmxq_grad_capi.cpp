@@ -80,15 +80,19 @@ int head_loss(fmxq::HeadLoss a, void* ws, size_t ws_bytes, void* stream, const c
 struct GradPlan {
   int bm, splits;
   int64_t c_split;
-  size_t pad, slices, bytes;
+  bool panel;
+  size_t pad, slices, panel_at, bytes;
 };
+// Rows from which the weights are dequantized to a panel beforehand.
+constexpr int64_t kGradPanelRows = 256;
 
 // The rows of dy are copied to a stride of 8 values where N (or the address) is not one.
 int64_t pad_cols(int64_t N) { return up(N, 8); }
 
 GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
-  p.bm = fmxq::grad_gemm_rows(M);
+  p.panel = M >= kGradPanelRows;
+  p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M);
   const int64_t tiles = (M + p.bm - 1) / p.bm * ((K + fmxq::kGradTileCols - 1) / fmxq::kGradTileCols);
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at
   // least.
@@ -98,7 +102,8 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   p.splits = (int)std::max<int64_t>(1, (N + p.c_split - 1) / std::max<int64_t>(p.c_split, 1));
   p.pad = 0;
   p.slices = up(M * pad_cols(N) * 2, 256);
-  p.bytes = p.slices + (p.splits > 1 ? (size_t)p.splits * M * K * 4 : 0);
+  p.panel_at = p.slices + (p.splits > 1 ? up(p.splits * M * K * 4, 256) : 0);
+  p.bytes = p.panel_at + (p.panel ? pad_cols(N) * K * 2 : 0);
   return p;
 }
 
@@ -239,7 +244,18 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
     g.y = dx;
     g.ldy = K;
   }
-  if (int rc = hip_status(fmxq::launch_grad_gemm(g, true, p.bm, s), op)) return rc;
+  if (p.panel) {
+    uint16_t* panel = reinterpret_cast<uint16_t*>(ws + p.panel_at);
+    g.panel = panel;
+    g.C = g.ldp = pad_cols(N);
+    if (int rc = hip_status(fmxq::launch_dequant_transposed(w, scales, biases, panel, N, K, g.ldp,
+                                                            group_size, bits, s),
+                            op))
+      return rc;
+    if (int rc = hip_status(fmxq::launch_panel_gemm(g, true, s), op)) return rc;
+  } else if (int rc = hip_status(fmxq::launch_grad_gemm(g, true, p.bm, s), op)) {
+    return rc;
+  }
   if (p.splits == 1) return FMXQ_OK;
   return hip_status(fmxq::launch_sum_slices(slices, p.splits, dx, M, K, s), op);
 }

@@ -10,28 +10,13 @@
 // the transposition costs nothing: the roundings pack any two values.
 #include <type_traits>
 
-#include "fmxq_common.hpp"
-#include "fmxq_grad.hpp"
+#include "fmxq_grad_tile.hpp"
 
 namespace fmxq {
 namespace {
 
-typedef __attribute__((address_space(3))) void lds_t;
-
 constexpr int kS = 64;   // contraction values per step
 constexpr int kN = kGradTileCols;
-
-// 16-byte chunk c of row r sits at chunk position c ^ swz(r) of the row's 128 LDS bytes.
-__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
-
-__device__ __forceinline__ constexpr int wait_enc(int vm, int lgkm) {
-  return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8);
-}
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t bytes) {
-  const int64_t b = bytes < 0 ? 0 : bytes < 0x7fffffff ? bytes : 0x7fffffff;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)b, 0x00020000);
-}
 
 template <int BM>
 struct GradCfg {
@@ -285,7 +270,7 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], bf[j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
       dequant(pk[st ^ 1], st ^ 1, s);
     }
     // The next step's A has landed (only the packed loads of the step after it are
@@ -311,61 +296,9 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
   }
 
-  // ---- epilogue: register r of acc[i][j] is row 8 (r / 4) + 4 h + r % 4 of the 32-row
-  // group, column r32 of the 32-column group.
   const int64_t mw = m0 + wm * MI * 32, nw = n0 + wn * NJ * 32;
-  const int64_t mend = m0 + rows;
-  if constexpr (NN) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t m = mw + 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
-        if (m >= mend) continue;
-        if (g.y) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const int64_t n = nw + 32 * j + r32;
-            if (n < g.N) g.y[m * g.ldy + n] = (uint16_t)f32_to_bf16_rne(acc[i][j][r]);
-          }
-        } else {
-          float* o = g.out + (split * g.M + m) * g.N;
-          const float f = g.factor ? g.factor[m] : 0.f;
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const int64_t n = nw + 32 * j + r32;
-            if (n < g.N) o[n] = g.factor ? __builtin_fmaf(o[n], f, acc[i][j][r]) : acc[i][j][r];
-          }
-        }
-      }
-  } else {
-    constexpr int TW = NJ * 32;
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t m = mw + 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          if (nw + 32 * j + r32 < g.N) top = fmaxf(top, acc[i][j][r] * g.logit_scale);
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        const float mx = ceilf(top);
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int64_t n = nw + 32 * j + r32;
-          float v = 0.f;
-          if (n < g.N) v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], g.logit_scale, -mx));
-          sum += v;
-          if (g.e && m < mend && n < g.lde) g.e[m * g.lde + n] = (uint16_t)f32_to_bf16_rne(v);
-        }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        if (r32 == 0 && m < mend && nw < g.N) g.stats[m * g.stat_tiles + nw / TW] = make_float2(mx, sum);
-      }
-  }
+  if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
+  else store_stats<MI, NJ>(g, acc, mw, m0 + rows, nw);
 }
 
 template <int BM, bool NN>

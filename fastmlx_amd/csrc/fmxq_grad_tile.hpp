@@ -1,0 +1,130 @@
+// fmxq_grad_tile.hpp -- what the products of fmxq_grad_gemm.hip and fmxq_grad_panel.hip
+// share: the LDS layout of a 64-deep stage, buffer resources, and the epilogues.
+//
+// The weights are the first operand of v_mfma_f32_32x32x16_bf16, so a lane holds 16 columns
+// of one output row (8 g + 4 h + 0..3 for g = 0..3, h its half of the wave): what a softmax
+// wants of a row is reduced in registers, and stores take 4 neighbouring columns.
+#pragma once
+#include "fmxq_common.hpp"
+#include "fmxq_grad.hpp"
+
+namespace fmxq {
+
+typedef __attribute__((address_space(3))) void lds_t;
+
+// 16-byte chunk c of row r sits at chunk position c ^ swz(r) of the row's 128 LDS bytes: 8
+// consecutive rows at one chunk hit 8 distinct positions.
+__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+// s_waitcnt with vmcnt = vm and lgkmcnt = lgkm (expcnt left alone).
+__device__ __forceinline__ constexpr int wait_enc(int vm, int lgkm) {
+  return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t bytes) {
+  const int64_t b = bytes < 0 ? 0 : bytes < 0x7fffffff ? bytes : 0x7fffffff;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)b, 0x00020000);
+}
+
+// The other half of the wave's value.
+__device__ __forceinline__ float other_half(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
+}
+
+// Rows mw .. of 32 MI (below mend), columns nw .. of 32 NJ: input gradients.
+template <int MI, int NJ>
+__device__ __forceinline__ void store_grad(const GradGemm& g, const f32x16 (&acc)[MI][NJ],
+                                           int64_t mw, int64_t mend, int64_t nw, int64_t split) {
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = mw + 32 * i + r32;
+    if (m >= mend) continue;
+    if (g.y) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t n = nw + 32 * j + 8 * q + 4 * h;
+          if (n < g.N)
+            *reinterpret_cast<u32x2*>(g.y + m * g.ldy + n) =
+                u32x2{pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
+                      pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+        }
+    } else {
+      float* o = g.out + (split * g.M + m) * g.N;
+      const float f = g.factor ? g.factor[m] : 0.f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t n = nw + 32 * j + 8 * q + 4 * h;
+          if (n >= g.N) continue;
+          f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                     acc[i][j][4 * q + 3]};
+          if (g.factor) {
+            const f32x4 old = *reinterpret_cast<const f32x4*>(o + n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(old[e], f, v[e]);
+          }
+          *reinterpret_cast<f32x4*>(o + n) = v;
+        }
+    }
+  }
+}
+
+// The softmax statistics of a tile of 32 NJ columns, and e.
+template <int MI, int NJ>
+__device__ __forceinline__ void store_stats(const GradGemm& g, const f32x16 (&acc)[MI][NJ],
+                                            int64_t mw, int64_t mend, int64_t nw) {
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  if (nw >= g.N) {  // no token here: zeros where a product reads whole tiles
+    if (g.e)
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int64_t m = mw + 32 * i + r32, n = nw + 32 * j + 8 * q + 4 * h;
+            if (m < mend && n < g.lde) *reinterpret_cast<u32x2*>(g.e + m * g.lde + n) = u32x2{0u, 0u};
+          }
+    return;
+  }
+  const bool full = nw + 32 * NJ <= g.N;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = mw + 32 * i + r32;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (full || nw + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) < g.N)
+          top = fmaxf(top, acc[i][j][r] * g.logit_scale);
+    const float mx = ceilf(fmaxf(top, other_half(top)));
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t n = nw + 32 * j + 8 * q + 4 * h;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * q + e], g.logit_scale, -mx));
+          if (!full && n + e >= g.N) v[e] = 0.f;
+          sum += v[e];
+        }
+        if (g.e && m < mend)
+          *reinterpret_cast<u32x2*>(g.e + m * g.lde + n) =
+              u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      }
+    sum += other_half(sum);
+    if (h == 0 && m < mend) g.stats[m * g.stat_tiles + nw / (32 * NJ)] = make_float2(mx, sum);
+  }
+}
+
+}  // namespace fmxq

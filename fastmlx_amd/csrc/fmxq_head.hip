@@ -16,6 +16,7 @@
 
 #include "fmxq_common.hpp"
 #include "fmxq_grad.hpp"
+#include "fmxq_internal.hpp"
 
 namespace fmxq {
 namespace {
@@ -237,19 +238,25 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 }  // namespace
 
-// Most bytes of a piece's e.
+// Most bytes of a piece's e, and of its panel of dequantized weights.
 constexpr int64_t kHeadPieceBytes = 256 << 20;
+constexpr int64_t kHeadPanelBytes = 256 << 20;
+// Rows from which the weights are dequantized to panels beforehand.
+constexpr int64_t kHeadPanelRows = 256;
 
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
-  p.bm = grad_gemm_rows(M);
-  p.stat_width = grad_gemm_stat_width(M);
+  p.panel = M >= kHeadPanelRows;
+  p.bm = p.panel ? kPanelRows : grad_gemm_rows(M);
+  p.stat_width = p.panel ? kPanelStatWidth : grad_gemm_stat_width(M);
   int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
+  if (p.panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
   p.pieces = (int)((V + piece - 1) / piece);
   piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
   p.pieces = (int)((V + piece - 1) / piece);
   p.piece = piece;
-  p.stat_tiles = up(piece, p.stat_width) / p.stat_width;
+  // Without a gradient the tiles of all pieces are joined at once.
+  p.stat_tiles = (grad ? piece : up(V, kGradTileCols)) / p.stat_width;
   // Parts of the gradient product's contraction: enough blocks for the chip, each walking
   // 256 tokens at least.
   const int64_t tiles = (M + p.bm - 1) / p.bm * ((K + kGradTileCols - 1) / kGradTileCols);
@@ -272,6 +279,7 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
     p.e = take(M * piece * 2);
     p.slices = take((int64_t)p.splits * M * K * 4);
   }
+  if (p.panel) p.panel_at = take(piece * K * 2);
   p.bytes = at;
   return p;
 }
@@ -289,6 +297,16 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   const float scale = kLog2e / a.temperature;
   head_dots_kernel<<<(unsigned)((a.M * a.k + 3) / 4), 256, 0, stream>>>(a, scale, sel);
   if (hipError_t r = hipGetLastError()) return r;
+  uint16_t* panel = p.panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
+  // (in, out): the running state before and after the pieces joined so far.
+  auto join = [&](int i, int64_t v0, int64_t n, int64_t lde) {
+    const dim3 grid((unsigned)a.M, e ? (unsigned)((lde + kJoinCols - 1) / kJoinCols) : 1u);
+    head_join_kernel<<<grid, 256, 0, stream>>>(a, stats, p.stat_tiles, p.stat_width,
+                                               i ? state + (i & 1) * a.M : nullptr,
+                                               state + ((i + 1) & 1) * a.M, factor, e, lde, v0,
+                                               (n + p.stat_width - 1) / p.stat_width);
+    return hipGetLastError();
+  };
   for (int i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, n = std::min(a.V - v0, p.piece);
     GradGemm g;
@@ -303,20 +321,23 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     g.biases = a.biases + v0 * (a.K / a.group_size);
     g.group_size = a.group_size;
     g.bits = a.bits;
-    g.stats = stats;
+    g.stats = stats + (e ? 0 : v0 / p.stat_width);
     g.stat_tiles = p.stat_tiles;
     g.e = e;
     g.lde = up(n, kGradTileCols);
     g.logit_scale = scale;
-    if (hipError_t r = launch_grad_gemm(g, false, p.bm, stream)) return r;
-    const int64_t tiles = (n + p.stat_width - 1) / p.stat_width;
-    const dim3 grid((unsigned)a.M, e ? (unsigned)((g.lde + kJoinCols - 1) / kJoinCols) : 1u);
-    head_join_kernel<<<grid, 256, 0, stream>>>(a, stats, p.stat_tiles, p.stat_width,
-                                               i ? state + (i & 1) * a.M : nullptr,
-                                               state + ((i + 1) & 1) * a.M, factor, e, g.lde, v0,
-                                               tiles);
-    if (hipError_t r = hipGetLastError()) return r;
+    if (p.panel) {
+      if (hipError_t r = launch_dequantize(g.w, g.scales, g.biases, panel, n, a.K, a.group_size, a.bits,
+                                           stream))
+        return r;
+      g.panel = panel;
+      g.ldp = a.K;
+      if (hipError_t r = launch_panel_gemm(g, false, stream)) return r;
+    } else if (hipError_t r = launch_grad_gemm(g, false, p.bm, stream)) {
+      return r;
+    }
     if (!e) continue;
+    if (hipError_t r = join(i, v0, n, g.lde)) return r;
     GradGemm d = g;
     d.a = e;
     d.lda = d.a_cols = g.lde;
@@ -326,9 +347,19 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     d.c_split = p.c_split;
     d.out = slices;
     d.factor = i ? factor : nullptr;
-    if (hipError_t r = launch_grad_gemm(d, true, p.bm, stream)) return r;
+    if (p.panel) {
+      d.C = d.ldp = up(n, 8);
+      if (hipError_t r = launch_dequant_transposed(g.w, g.scales, g.biases, panel, n, a.K, d.ldp,
+                                                   a.group_size, a.bits, stream))
+        return r;
+      if (hipError_t r = launch_panel_gemm(d, true, stream)) return r;
+    } else if (hipError_t r = launch_grad_gemm(d, true, p.bm, stream)) {
+      return r;
+    }
   }
-  head_loss_kernel<<<(unsigned)((a.M + 3) / 4), 256, 0, stream>>>(a, state + (p.pieces & 1) * a.M, sel,
+  if (!e)
+    if (hipError_t r = join(0, 0, a.V, 0)) return r;
+  head_loss_kernel<<<(unsigned)((a.M + 3) / 4), 256, 0, stream>>>(a, state + ((e ? p.pieces : 1) & 1) * a.M, sel,
                                                                   coef, row);
   if (hipError_t r = hipGetLastError()) return r;
   if (!a.dh) return hipSuccess;
