@@ -58,6 +58,13 @@ int grad_gemm_stat_width(int64_t M);
 constexpr int kGradTileCols = 256;
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
 
+// The same products for up to kSkinnyRows rows, where reading the weights is the work
+// (fmxq_grad_skinny.hip).  weight_rows: rows of a part of the contraction (nn).
+constexpr int64_t kSkinnyRows = 64;
+constexpr int kSkinnyStatWidth = 32;
+bool skinny_gemm_supported(int64_t M, int64_t lda, int64_t weight_rows, int64_t weight_cols);
+hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
+
 // The same products over a panel of weights dequantized beforehand (fmxq_grad_panel.hip), in
 // tiles of kPanelRows rows.
 constexpr int kPanelRows = 256;
@@ -105,8 +112,9 @@ struct HeadLoss {
 struct HeadPlan {
   int bm, stat_width, pieces, splits;
   int64_t piece, c_split, stat_tiles;
-  bool panel;  // the products run over panels of dequantized weights
-  size_t stats, e, slices, state, factor, sel, coef, row, panel_at, bytes;  // in the workspace
+  bool panel;   // the products run over panels of dequantized weights
+  bool skinny;  // ... or on the kernels for few rows
+  size_t stats, e, slices, state, factor, coef, row, panel_at, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);
 hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipStream_t stream);

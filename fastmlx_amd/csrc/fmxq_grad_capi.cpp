@@ -80,7 +80,7 @@ int head_loss(fmxq::HeadLoss a, void* ws, size_t ws_bytes, void* stream, const c
 struct GradPlan {
   int bm, splits;
   int64_t c_split;
-  bool panel;
+  bool panel, skinny;
   size_t pad, slices, panel_at, bytes;
 };
 // Rows from which the weights are dequantized to a panel beforehand.
@@ -93,7 +93,9 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
   p.panel = M >= kGradPanelRows;
   p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M);
-  const int64_t tiles = (M + p.bm - 1) / p.bm * ((K + fmxq::kGradTileCols - 1) / fmxq::kGradTileCols);
+  p.skinny = fmxq::skinny_gemm_supported(M, pad_cols(N), N + 64, K);
+  const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) *
+                        ((K + fmxq::kGradTileCols - 1) / fmxq::kGradTileCols);
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at
   // least.
   const int64_t want = tiles ? (p.bm >= 128 ? kCus : 2 * kCus) / tiles : 1;
@@ -253,7 +255,9 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
                             op))
       return rc;
     if (int rc = hip_status(fmxq::launch_panel_gemm(g, true, s), op)) return rc;
-  } else if (int rc = hip_status(fmxq::launch_grad_gemm(g, true, p.bm, s), op)) {
+  } else if (int rc = hip_status(p.skinny ? fmxq::launch_skinny_gemm(g, true, s)
+                                          : fmxq::launch_grad_gemm(g, true, p.bm, s),
+                                 op)) {
     return rc;
   }
   if (p.splits == 1) return FMXQ_OK;

@@ -26,13 +26,6 @@ struct GradCfg {
   static constexpr int NJ = kN / WN / 32;        // 32-column groups
 };
 
-// dequantize's value: bf16(bf16(q s) + b), two at a time (low half first).
-__device__ __forceinline__ uint32_t deq_pair(float q0, float q1, float s0, float s1, float b0,
-                                             float b1) {
-  const uint32_t m = pack_bf16x2(q0 * s0, q1 * s1);
-  return pack_bf16x2(bf16_lo(m) + b0, bf16_hi(m) + b1);
-}
-
 // Value j (0..7) of 8 packed values as a float; the masks let each be one byte conversion.
 template <int BITS>
 struct Q8;

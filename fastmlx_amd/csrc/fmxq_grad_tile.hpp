@@ -26,6 +26,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t by
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)b, 0x00020000);
 }
 
+// dequantize's value: bf16(bf16(q s) + b), two at a time (low half first).  The empty asm hides
+// where the pair comes from: the compiler takes a pack whose halves are used apart for two
+// conversions.
+__device__ __forceinline__ uint32_t deq_pair(float q0, float q1, float s0, float s1, float b0,
+                                             float b1) {
+  uint32_t m = pack_bf16x2(q0 * s0, q1 * s1);
+  asm("" : "+v"(m));
+  return pack_bf16x2(bf16_lo(m) + b0, bf16_hi(m) + b1);
+}
+
 // The other half of the wave's value.
 __device__ __forceinline__ float other_half(float v) {
   const uint32_t u = __float_as_uint(v);

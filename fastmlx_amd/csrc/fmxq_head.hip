@@ -31,10 +31,10 @@ __device__ __forceinline__ float wave_max(float v) {
 
 // 8 dequantized values (fmxq_dequantize's bits) of packed row `row` from column c on.
 __device__ __forceinline__ void deq8(const HeadLoss& a, int64_t row, int64_t c, float* v) {
-  const int64_t grp = (row * a.K + c) / a.group_size;
+  const int64_t grp = (row * a.K + c) >> __builtin_ctz(a.group_size);
   const float s = bf16_bits_to_f32(a.scales[grp]), b = bf16_bits_to_f32(a.biases[grp]);
   uint32_t w0, w1 = 0;
-  const int64_t at = (row * a.K + c) * a.bits / 32;
+  const int64_t at = (row * a.K + c) >> (a.bits == 4 ? 3 : 2);
   w0 = a.w[at];
   if (a.bits == 8) w1 = a.w[at + 1];
 #pragma unroll
@@ -66,100 +66,34 @@ __device__ __forceinline__ int64_t token_of(const HeadLoss& a, int64_t m, int j,
   return id;
 }
 
-// One wave per wanted entry: its logit in units of log 2, fp32 sums.
-__global__ __launch_bounds__(256) void head_dots_kernel(HeadLoss a, float scale,
-                                                        float* __restrict__ sel) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= a.M * a.k) return;
-  const int64_t m = i / a.k;
-  const int64_t v = token_of(a, m, (int)(i - m * a.k), lane == 0);
+// The logit of token v for row m in units of log 2, fp32 sums over the wave.
+__device__ __forceinline__ float logit_of(const HeadLoss& a, int64_t m, int64_t v, float scale) {
   float t = 0.f;
-  if (v >= 0)
-    for (int64_t c = 8 * lane; c < a.K; c += 512) {
-      float wv[8];
-      deq8(a, v, c, wv);
-      const u32x4 x = *reinterpret_cast<const u32x4*>(a.h + m * a.K + c);
+  for (int64_t c = 8 * (threadIdx.x & 63); c < a.K; c += 512) {
+    float wv[8];
+    deq8(a, v, c, wv);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(a.h + m * a.K + c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        t = __builtin_fmaf(wv[2 * j], bf16_lo(x[j]), t);
-        t = __builtin_fmaf(wv[2 * j + 1], bf16_hi(x[j]), t);
-      }
-    }
-  t = wave_sum(t);
-  if (lane == 0) sel[i] = t * scale;
-}
-
-// Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought
-// to it with the wanted entries zeroed.  in / out are the states before and after; chunk 0
-// writes out and the factor of the earlier pieces' sums.
-constexpr int kJoinCols = 8192;
-__global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2* __restrict__ stats,
-                                                        int64_t stat_tiles, int tw,
-                                                        const float2* in, float2* out,
-                                                        float* factor, uint16_t* e, int64_t lde,
-                                                        int64_t v0, int64_t tiles) {
-  __shared__ float red[4], red2[4];
-  const int64_t m = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float2* st = stats + m * stat_tiles;
-  const float2 old = in ? in[m] : make_float2(-INFINITY, 0.f);
-  float top = old.x;
-  for (int64_t t = tid; t < tiles; t += 256) top = fmaxf(top, st[t].x);
-  top = wave_max(top);
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  if (blockIdx.y == 0) {
-    float sum = 0.f;
-    for (int64_t t = tid; t < tiles; t += 256)
-      sum = __builtin_fmaf(st[t].y, __builtin_amdgcn_exp2f(st[t].x - top), sum);
-    sum = wave_sum(sum);
-    if (lane == 0) red2[wave] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      // The first piece starts from nothing: its factor is never used on anything but zeros.
-      const float f = in ? __builtin_amdgcn_exp2f(old.x - top) : 0.f;
-      out[m] = make_float2(top, (in ? old.y * f : 0.f) + (red2[0] + red2[1]) + (red2[2] + red2[3]));
-      if (factor) factor[m] = f;
+    for (int j = 0; j < 4; ++j) {
+      t = __builtin_fmaf(wv[2 * j], bf16_lo(x[j]), t);
+      t = __builtin_fmaf(wv[2 * j + 1], bf16_hi(x[j]), t);
     }
   }
-  if (!e) return;
-  uint16_t* row = e + m * lde;
-  const int64_t c0 = (int64_t)blockIdx.y * kJoinCols;
-  const int64_t c1 = c0 + kJoinCols < lde ? c0 + kJoinCols : lde;
-  for (int64_t c = c0 + 8 * tid; c < c1; c += 2048) {
-    const int64_t t = c / tw;
-    if (t >= tiles) break;  // columns past the vocabulary hold zeros
-    const float f = __builtin_amdgcn_exp2f(st[t].x - top);
-    if (f == 1.f) continue;
-    u32x4 v = *reinterpret_cast<u32x4*>(row + c);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2(bf16_lo(v[j]) * f, bf16_hi(v[j]) * f);
-    *reinterpret_cast<u32x4*>(row + c) = v;
-  }
-  __syncthreads();
-  for (int j = tid; j < a.k; j += 256) {
-    const int64_t v = token_of(a, m, j, false) - v0;
-    if (v >= c0 && v < c1) row[v] = 0;
-  }
+  return wave_sum(t) * scale;
 }
 
-// One wave per row: lse, the loss, each wanted entry's coefficient of W_id and the factor of
-// the sums over e.  A row without a wanted entry has loss 0 and gradient 0 (row factor NaN
-// marks it; the gradient kernel writes zeros without reading the sums).
-__global__ __launch_bounds__(256) void head_loss_kernel(HeadLoss a, const float2* __restrict__ state,
-                                                        const float* __restrict__ sel,
-                                                        float* __restrict__ coef,
-                                                        float2* __restrict__ row) {
+// One wave: lse, the loss, each wanted entry's coefficient of W_id and the factor of the sums
+// over e, from the row's final (m, sum) and its entries' logits.  A row without a wanted
+// entry has loss 0 and gradient 0 (row[m].y marks it; the gradient kernel writes zeros
+// without reading the sums).
+__device__ __forceinline__ void finish_row(const HeadLoss& a, int64_t m, float2 st,
+                                           const float* sel, float* __restrict__ coef,
+                                           float2* __restrict__ row) {
   const int lane = threadIdx.x & 63;
-  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (m >= a.M) return;
-  const float2 st = state[m];
   const float lse2 = st.x + __builtin_amdgcn_logf(st.y);  // in units of log 2
   const float T = a.temperature;
   const bool on = lane < a.k;
-  const int64_t v = on ? token_of(a, m, lane, false) : -1;
+  const int64_t v = on ? token_of(a, m, lane, true) : -1;
   float q = v >= 0 ? 1.f : 0.f, logq = 0.f;
   bool empty;
   if (a.teacher) {
@@ -178,7 +112,7 @@ __global__ __launch_bounds__(256) void head_loss_kernel(HeadLoss a, const float2
   } else {
     empty = !__any(v >= 0);
   }
-  const float l2 = on ? sel[m * a.k + lane] : 0.f;
+  const float l2 = v >= 0 ? sel[lane] : 0.f;
   // Entries of no weight add nothing (0 log 0 = 0); NaN stays.
   const float term = v >= 0 && q != 0.f ? q * (logq - l2 + lse2) : 0.f;
   const float loss = wave_sum(term) * (T * T * kLn2);
@@ -197,6 +131,74 @@ __global__ __launch_bounds__(256) void head_loss_kernel(HeadLoss a, const float2
   const float p = first ? __builtin_amdgcn_exp2f(l2 - lse2) : 0.f;
   if (on) coef[m * a.k + lane] = v >= 0 ? g * (p - q) : 0.f;
   if (lane == 0) row[m] = make_float2(g / st.y, empty ? 1.f : 0.f);
+}
+
+// Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought
+// to it with the wanted entries zeroed.  in / out are the states before and after; chunk 0
+// writes out and the factor of the earlier pieces' sums and, after the last piece, finishes
+// the row: its waves take the wanted entries' logits in turn.
+constexpr int kJoinCols = 8192;
+__global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2* __restrict__ stats,
+                                                        int64_t stat_tiles, int tw,
+                                                        const float2* in, float2* out,
+                                                        float* factor, uint16_t* e, int64_t lde,
+                                                        int64_t v0, int64_t tiles, bool last,
+                                                        float scale, float* coef, float2* rowf) {
+  __shared__ float red[4], red2[4], sel[64];
+  const int64_t m = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float2* st = stats + m * stat_tiles;
+  const float2 old = in ? in[m] : make_float2(-INFINITY, 0.f);
+  float top = old.x;
+  for (int64_t t = tid; t < tiles; t += 256) top = fmaxf(top, st[t].x);
+  top = wave_max(top);
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (blockIdx.y == 0) {
+    float sum = 0.f;
+    for (int64_t t = tid; t < tiles; t += 256)
+      sum = __builtin_fmaf(st[t].y, __builtin_amdgcn_exp2f(st[t].x - top), sum);
+    sum = wave_sum(sum);
+    if (lane == 0) red2[wave] = sum;
+    if (last)
+      for (int j = wave; j < a.k; j += 4) {
+        const int64_t v = token_of(a, m, j, false);
+        const float l2 = v >= 0 ? logit_of(a, m, v, scale) : 0.f;
+        if (lane == 0) sel[j] = l2;
+      }
+    __syncthreads();
+    if (wave == 0) {
+      // The first piece starts from nothing: its factor is never used on anything but zeros.
+      const float f = in ? __builtin_amdgcn_exp2f(old.x - top) : 0.f;
+      const float2 now =
+          make_float2(top, (in ? old.y * f : 0.f) + (red2[0] + red2[1]) + (red2[2] + red2[3]));
+      if (lane == 0) {
+        out[m] = now;
+        if (factor) factor[m] = f;
+      }
+      if (last) finish_row(a, m, now, sel, coef, rowf);
+    }
+  }
+  if (!e) return;
+  uint16_t* row = e + m * lde;
+  const int64_t c0 = (int64_t)blockIdx.y * kJoinCols;
+  const int64_t c1 = c0 + kJoinCols < lde ? c0 + kJoinCols : lde;
+  for (int64_t c = c0 + 8 * tid; c < c1; c += 2048) {
+    const int64_t t = c >> __builtin_ctz(tw);
+    if (t >= tiles) break;  // columns past the vocabulary hold zeros
+    const float f = __builtin_amdgcn_exp2f(st[t].x - top);
+    if (f == 1.f) continue;
+    u32x4 v = *reinterpret_cast<u32x4*>(row + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2(bf16_lo(v[j]) * f, bf16_hi(v[j]) * f);
+    *reinterpret_cast<u32x4*>(row + c) = v;
+  }
+  __syncthreads();
+  for (int j = tid; j < a.k; j += 256) {
+    const int64_t v = token_of(a, m, j, false) - v0;
+    if (v >= c0 && v < c1) row[v] = 0;
+  }
 }
 
 // Thread: 8 columns of a row: the slices' sum times the row's factor, plus the wanted
@@ -248,18 +250,20 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
   p.panel = M >= kHeadPanelRows;
   p.bm = p.panel ? kPanelRows : grad_gemm_rows(M);
-  p.stat_width = p.panel ? kPanelStatWidth : grad_gemm_stat_width(M);
   int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
   if (p.panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
   p.pieces = (int)((V + piece - 1) / piece);
   piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
   p.pieces = (int)((V + piece - 1) / piece);
   p.piece = piece;
+  p.skinny = skinny_gemm_supported(M, std::max(K, piece), piece, K);
+  p.stat_width = p.skinny ? kSkinnyStatWidth : p.panel ? kPanelStatWidth : grad_gemm_stat_width(M);
   // Without a gradient the tiles of all pieces are joined at once.
   p.stat_tiles = (grad ? piece : up(V, kGradTileCols)) / p.stat_width;
   // Parts of the gradient product's contraction: enough blocks for the chip, each walking
   // 256 tokens at least.
-  const int64_t tiles = (M + p.bm - 1) / p.bm * ((K + kGradTileCols - 1) / kGradTileCols);
+  const int64_t tiles =
+      (p.skinny ? 1 : (M + p.bm - 1) / p.bm) * ((K + kGradTileCols - 1) / kGradTileCols);
   const int64_t want = (p.bm >= 128 ? cus : 2 * cus) / tiles;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, piece / 256));
   p.c_split = up((piece + p.splits - 1) / p.splits, 64);
@@ -271,7 +275,6 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   };
   p.stats = take(M * p.stat_tiles * 8);
   p.state = take(2 * M * 8);
-  p.sel = take(M * k * 4);
   p.coef = take(M * k * 4);
   p.row = take(M * 8);
   p.factor = take(M * 4);
@@ -288,15 +291,12 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   char* base = static_cast<char*>(ws);
   float2* stats = reinterpret_cast<float2*>(base + p.stats);
   float2* state = reinterpret_cast<float2*>(base + p.state);
-  float* sel = reinterpret_cast<float*>(base + p.sel);
   float* coef = reinterpret_cast<float*>(base + p.coef);
   float2* row = reinterpret_cast<float2*>(base + p.row);
   float* factor = reinterpret_cast<float*>(base + p.factor);
   uint16_t* e = a.dh ? reinterpret_cast<uint16_t*>(base + p.e) : nullptr;
   float* slices = a.dh ? reinterpret_cast<float*>(base + p.slices) : nullptr;
   const float scale = kLog2e / a.temperature;
-  head_dots_kernel<<<(unsigned)((a.M * a.k + 3) / 4), 256, 0, stream>>>(a, scale, sel);
-  if (hipError_t r = hipGetLastError()) return r;
   uint16_t* panel = p.panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
   // (in, out): the running state before and after the pieces joined so far.
   auto join = [&](int i, int64_t v0, int64_t n, int64_t lde) {
@@ -304,7 +304,8 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     head_join_kernel<<<grid, 256, 0, stream>>>(a, stats, p.stat_tiles, p.stat_width,
                                                i ? state + (i & 1) * a.M : nullptr,
                                                state + ((i + 1) & 1) * a.M, factor, e, lde, v0,
-                                               (n + p.stat_width - 1) / p.stat_width);
+                                               (n + p.stat_width - 1) / p.stat_width,
+                                               v0 + n == a.V, scale, coef, row);
     return hipGetLastError();
   };
   for (int i = 0; i < p.pieces; ++i) {
@@ -333,14 +334,16 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
       g.panel = panel;
       g.ldp = a.K;
       if (hipError_t r = launch_panel_gemm(g, false, stream)) return r;
-    } else if (hipError_t r = launch_grad_gemm(g, false, p.bm, stream)) {
+    } else if (hipError_t r = p.skinny ? launch_skinny_gemm(g, false, stream)
+                                       : launch_grad_gemm(g, false, p.bm, stream)) {
       return r;
     }
     if (!e) continue;
     if (hipError_t r = join(i, v0, n, g.lde)) return r;
     GradGemm d = g;
     d.a = e;
-    d.lda = d.a_cols = g.lde;
+    d.lda = g.lde;
+    d.a_cols = up(n, p.stat_width);  // columns that the tiles have written
     d.N = a.K;
     d.C = n;
     d.splits = p.splits;
@@ -353,15 +356,13 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
                                                    a.group_size, a.bits, stream))
         return r;
       if (hipError_t r = launch_panel_gemm(d, true, stream)) return r;
-    } else if (hipError_t r = launch_grad_gemm(d, true, p.bm, stream)) {
+    } else if (hipError_t r = p.skinny ? launch_skinny_gemm(d, true, stream)
+                                       : launch_grad_gemm(d, true, p.bm, stream)) {
       return r;
     }
   }
   if (!e)
     if (hipError_t r = join(0, 0, a.V, 0)) return r;
-  head_loss_kernel<<<(unsigned)((a.M + 3) / 4), 256, 0, stream>>>(a, state + ((e ? p.pieces : 1) & 1) * a.M, sel,
-                                                                  coef, row);
-  if (hipError_t r = hipGetLastError()) return r;
   if (!a.dh) return hipSuccess;
   const dim3 grid((unsigned)a.M, (unsigned)((a.K + 2047) / 2048));
   head_dh_kernel<<<grid, 256, 0, stream>>>(a, slices, p.splits, coef, row);

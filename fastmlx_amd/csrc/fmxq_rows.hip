@@ -71,7 +71,7 @@ __device__ __forceinline__ void wave_fence() {
 // Each block adds up the histograms before its own (every block reads the few tables again,
 // which costs less than a launch for the scan), then its waves place their slots in order.
 __global__ __launch_bounds__(256) void sort_place_kernel(MoeSort a, int64_t S, int bits) {
-  extern __shared__ uint32_t lds[];  // cursors of each wave: 4 x (E + 1)
+  extern __shared__ uint32_t lds[];  // E + 1 cursors of each wave, then two tables more
   __shared__ uint32_t wsum[4];
   const int64_t nb = a.E + 1, s0 = (int64_t)blockIdx.x * kSortSlots;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -83,31 +83,38 @@ __global__ __launch_bounds__(256) void sort_place_kernel(MoeSort a, int64_t S, i
   for (int64_t s = w0 + lane; s < w1; s += 64)
     atomicAdd(&cur[wave * nb + bucket_of(a.inds[s], a.E)], 1u);
   __syncthreads();
-  // Each thread takes a run of buckets: total over all blocks and over the earlier ones.
+  // Each bucket's slots in all blocks and in the earlier ones, then the buckets' first
+  // positions, then each wave's cursors.
+  uint32_t *all = lds + 4 * nb, *before = lds + 5 * nb;
+  for (int64_t e = tid; e < nb; e += 256) {
+    uint32_t n = 0, m = 0;
+#pragma unroll 8
+    for (unsigned k = 0; k < gridDim.x; ++k) {
+      const uint32_t v = a.hist[k * nb + e];
+      n += v;
+      m += k < blockIdx.x ? v : 0u;
+    }
+    all[e] = n;
+    before[e] = m;
+  }
+  __syncthreads();
   const int64_t per = (nb + 255) / 256;
   const int64_t b0 = tid * per < nb ? tid * per : nb, b1 = b0 + per < nb ? b0 + per : nb;
   uint32_t total = 0;
-  for (int64_t e = b0; e < b1; ++e)
-    for (unsigned k = 0; k < gridDim.x; ++k) total += a.hist[k * nb + e];
+  for (int64_t e = b0; e < b1; ++e) total += all[e];
   uint32_t base = scan256(total, wsum);
   for (int64_t e = b0; e < b1; ++e) {
     if (blockIdx.x == 0) {
       a.offsets[e] = base;
       if (e == a.E && base < S) atomicOr(a.flag, 1u);
     }
-    uint32_t before = 0, all = 0;
-    for (unsigned k = 0; k < gridDim.x; ++k) {
-      const uint32_t v = a.hist[k * nb + e];
-      if (k < blockIdx.x) before += v;
-      all += v;
-    }
-    uint32_t at = base + before;
+    uint32_t at = base + before[e];
     for (int w = 0; w < 4; ++w) {
       const uint32_t n = cur[w * nb + e];
       cur[w * nb + e] = at;
       at += n;
     }
-    base += all;
+    base += all[e];
   }
   __syncthreads();
   for (int64_t s = w0 + lane; s - lane < w1; s += 64) {
@@ -175,7 +182,79 @@ __global__ __launch_bounds__(256) void rows_out_kernel(MoeSort a) {
   }
 }
 
-// out[t] = sum_j w[t, j] y[pos[t, j]]; a position outside the rows adds nothing.
+// Few slots: the whole sort in one launch.  Block t counts, for each slot of token t, the
+// slots that sort before it (a smaller bucket, or the same one earlier), then writes the
+// token's rows; block T counts the buckets for the offsets.  Every block reads all the ids.
+constexpr int kSmallK = 16;
+constexpr int64_t kSmallSlots = 2048;
+template <int VEC>
+__global__ __launch_bounds__(256) void sort_small_kernel(MoeSort a, int S) {
+  extern __shared__ uint32_t cnt[];  // E + 1
+  __shared__ uint32_t before[4][kSmallK], all[4], wsum[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t t = blockIdx.x;
+  const int nb = (int)a.E + 1, k = (int)a.k;
+  if (t == a.T) {
+    for (int i = tid; i < nb; i += 256) cnt[i] = 0;
+    __syncthreads();
+    for (int s = tid; s < S; s += 256) atomicAdd(&cnt[bucket_of(a.inds[s], a.E)], 1u);
+    __syncthreads();
+    const int per = (nb + 255) / 256;
+    const int b0 = tid * per < nb ? tid * per : nb, b1 = b0 + per < nb ? b0 + per : nb;
+    uint32_t n = 0;
+    for (int e = b0; e < b1; ++e) n += cnt[e];
+    uint32_t at = scan256(n, wsum);
+    for (int e = b0; e < b1; ++e) {
+      a.offsets[e] = at;
+      if (e == nb - 1 && at < (uint32_t)S) atomicOr(a.flag, 1u);
+      at += cnt[e];
+    }
+    return;
+  }
+  // Counted by ballots: a wave's totals need no sum over its lanes.
+  uint32_t mine[kSmallK], n[kSmallK], valid = 0;
+#pragma unroll
+  for (int j = 0; j < kSmallK; ++j) {
+    mine[j] = j < k ? bucket_of(a.inds[t * k + j], a.E) : 0u;
+    n[j] = 0;
+  }
+  for (int s0 = 64 * wave; s0 < S; s0 += 256) {
+    const int s = s0 + lane;
+    const bool on = s < S;
+    const uint32_t e = on ? bucket_of(a.inds[s], a.E) : ~0u;
+    valid += __popcll(__ballot(e < (uint32_t)a.E));
+#pragma unroll
+    for (int j = 0; j < kSmallK; ++j)
+      if (j < k) n[j] += __popcll(__ballot(e < mine[j] || (e == mine[j] && s < (int)t * k + j)));
+  }
+#pragma unroll
+  for (int j = 0; j < kSmallK; ++j)
+    if (j < k && lane == 0) before[wave][j] = n[j];
+  if (lane == 0) all[wave] = valid;
+  __syncthreads();
+  valid = all[0] + all[1] + all[2] + all[3];
+  uint32_t p[kSmallK];
+#pragma unroll
+  for (int j = 0; j < kSmallK; ++j)
+    p[j] = j < k ? before[0][j] + before[1][j] + before[2][j] + before[3][j] : 0u;
+  if (tid == 0) {
+#pragma unroll
+    for (int j = 0; j < kSmallK; ++j)
+      if (j < k) {
+        a.pos[t * k + j] = p[j];
+        a.order[p[j]] = (uint32_t)(t * k + j);
+      }
+  }
+  for (int64_t c = (int64_t)tid * VEC; c < a.D; c += 256 * VEC) {
+    const Row<VEC> x = Row<VEC>::load(a.x + t * a.D + c);
+#pragma unroll
+    for (int j = 0; j < kSmallK; ++j)
+      if (j < k) (p[j] < valid ? x : Row<VEC>{}).store(a.xs + (int64_t)p[j] * a.D + c);
+  }
+}
+
+// out[t] = sum_j w[t, j] y[pos[t, j]] in the order of j; a position outside the rows adds
+// nothing.  Eight rows are requested before any is added.
 template <int VEC>
 __global__ __launch_bounds__(256) void rows_sum_kernel(const uint16_t* __restrict__ y,
                                                        const uint32_t* __restrict__ pos,
@@ -189,22 +268,36 @@ __global__ __launch_bounds__(256) void rows_sum_kernel(const uint16_t* __restric
     float s[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) s[i] = 0.f;
-    for (int64_t j = 0; j < k; ++j) {
-      const int64_t p = pos[t * k + j];
-      if (p >= S) {
-        if (c == 0) atomicOr(flag, 1u);
-        continue;
-      }
-      const float w = weights ? weight_of(weights, wbf16, t * k + j) : 1.f;
-      const Row<VEC> v = Row<VEC>::load(y + p * D + c);
+    for (int64_t j0 = 0; j0 < k; j0 += 8) {
+      Row<VEC> v[8];
+      float w[8];
+      bool on[8];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s[i] = __builtin_fmaf(w, v.at(i), s[i]);
+      for (int j = 0; j < 8; ++j) {
+        const bool in = j0 + j < k;
+        const int64_t p = in ? pos[t * k + j0 + j] : S;
+        on[j] = p < S;
+        v[j] = Row<VEC>{};
+        w[j] = 0.f;
+        if (on[j]) {
+          v[j] = Row<VEC>::load(y + p * D + c);
+          w[j] = weights ? weight_of(weights, wbf16, t * k + j0 + j) : 1.f;
+        } else if (in && c == 0) {
+          atomicOr(flag, 1u);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (on[j])
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) s[i] = __builtin_fmaf(w[j], v[j].at(i), s[i]);
     }
     Row<VEC>::of(s).store(out + t * D + c);
   }
 }
 
-// One block per token: dy[pos] = w dout, dweights = <dout, y[pos]>.
+// One wave per slot: dy[pos] = w dout, dweights = <dout, y[pos]>.  The waves of a block take
+// neighbouring slots, which mostly share a token's dout.
 template <int VEC>
 __global__ __launch_bounds__(256) void rows_grad_kernel(const uint16_t* __restrict__ dout,
                                                         const uint16_t* __restrict__ y,
@@ -213,36 +306,33 @@ __global__ __launch_bounds__(256) void rows_grad_kernel(const uint16_t* __restri
                                                         bool wbf16, uint16_t* __restrict__ dy,
                                                         void* __restrict__ dweights, int64_t S,
                                                         int64_t k, int64_t D, uint32_t* flag) {
-  __shared__ float red[4];
-  const int64_t t = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t j = 0; j < k; ++j) {
-    const int64_t p = pos[t * k + j];
-    const float w = weight_of(weights, wbf16, t * k + j);
-    float dot = 0.f;
-    if (p < S) {
-      for (int64_t c = threadIdx.x * VEC; c < D; c += 256 * VEC) {
-        const Row<VEC> d = Row<VEC>::load(dout + t * D + c), v = Row<VEC>::load(y + p * D + c);
-        float o[VEC];
+  const int lane = threadIdx.x & 63;
+  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (s >= S) return;
+  const int64_t t = s / k, p = pos[s];
+  const float w = weight_of(weights, wbf16, s);
+  float dot = 0.f;
+  if (p < S) {
+    const uint16_t *dr = dout + t * D, *yr = y + p * D;
+    uint16_t* o = dy + p * D;
+#pragma unroll 4
+    for (int64_t c = (int64_t)lane * VEC; c < D; c += 64 * VEC) {
+      const Row<VEC> d = Row<VEC>::load(dr + c), v = Row<VEC>::load(yr + c);
+      float f[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          dot = __builtin_fmaf(d.at(i), v.at(i), dot);
-          o[i] = w * d.at(i);
-        }
-        Row<VEC>::of(o).store(dy + p * D + c);
+      for (int i = 0; i < VEC; ++i) {
+        dot = __builtin_fmaf(d.at(i), v.at(i), dot);
+        f[i] = w * d.at(i);
       }
-    } else if (threadIdx.x == 0) {
-      atomicOr(flag, 1u);
+      Row<VEC>::of(f).store(o + c);
     }
-    dot = wave_sum(dot);
-    if (lane == 0) red[wave] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const float v = (red[0] + red[1]) + (red[2] + red[3]);
-      if (wbf16) reinterpret_cast<uint16_t*>(dweights)[t * k + j] = (uint16_t)f32_to_bf16_rne(v);
-      else reinterpret_cast<float*>(dweights)[t * k + j] = v;
-    }
-    __syncthreads();
+  } else if (lane == 0) {
+    atomicOr(flag, 1u);
+  }
+  dot = wave_sum(dot);
+  if (lane == 0) {
+    if (wbf16) reinterpret_cast<uint16_t*>(dweights)[s] = (uint16_t)f32_to_bf16_rne(dot);
+    else reinterpret_cast<float*>(dweights)[s] = dot;
   }
 }
 
@@ -265,14 +355,21 @@ size_t moe_sort_hist_bytes(int64_t S, int64_t E) {
 hipError_t launch_moe_sort(const MoeSort& a, hipStream_t stream) {
   const int64_t S = a.T * a.k, nb = a.E + 1;
   const unsigned blocks = (unsigned)((S + kSortSlots - 1) / kSortSlots);
+  const bool vec = vec8(a.D, a.x, a.xs, nullptr);
+  if (S <= kSmallSlots && a.k <= kSmallK) {
+    const dim3 grid((unsigned)a.T + 1);
+    if (vec) sort_small_kernel<8><<<grid, 256, nb * sizeof(uint32_t), stream>>>(a, (int)S);
+    else sort_small_kernel<1><<<grid, 256, nb * sizeof(uint32_t), stream>>>(a, (int)S);
+    return hipGetLastError();
+  }
   int bits = 1;
   while (nb > ((int64_t)1 << bits)) ++bits;
   sort_hist_kernel<<<blocks, 256, nb * sizeof(uint32_t), stream>>>(a, S);
   if (hipError_t e = hipGetLastError()) return e;
-  sort_place_kernel<<<blocks, 256, 4 * nb * sizeof(uint32_t), stream>>>(a, S, bits);
+  sort_place_kernel<<<blocks, 256, 6 * nb * sizeof(uint32_t), stream>>>(a, S, bits);
   if (hipError_t e = hipGetLastError()) return e;
   if (a.D == 0) return hipSuccess;
-  if (vec8(a.D, a.x, a.xs, nullptr))
+  if (vec)
     rows_out_kernel<8><<<row_grid(a.T, a.D, 8), 256, 0, stream>>>(a);
   else
     rows_out_kernel<1><<<row_grid(a.T, a.D, 1), 256, 0, stream>>>(a);
@@ -296,10 +393,10 @@ hipError_t launch_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const
                                   void* dweights, int64_t T, int64_t k, int64_t D, uint32_t* flag,
                                   hipStream_t stream) {
   if (vec8(D, dout, y, dy))
-    rows_grad_kernel<8><<<(unsigned)T, 256, 0, stream>>>(dout, y, pos, weights, weights_bf16, dy,
+    rows_grad_kernel<8><<<(unsigned)((T * k + 3) / 4), 256, 0, stream>>>(dout, y, pos, weights, weights_bf16, dy,
                                                          dweights, T * k, k, D, flag);
   else
-    rows_grad_kernel<1><<<(unsigned)T, 256, 0, stream>>>(dout, y, pos, weights, weights_bf16, dy,
+    rows_grad_kernel<1><<<(unsigned)((T * k + 3) / 4), 256, 0, stream>>>(dout, y, pos, weights, weights_bf16, dy,
                                                          dweights, T * k, k, D, flag);
   return hipGetLastError();
 }

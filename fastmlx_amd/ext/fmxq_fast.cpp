@@ -326,9 +326,226 @@ PyObject* route_group_topk(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- training over quantized weights.  These take the plain case on the current device;
+// their workspace comes from torch's allocator, as in ops.py.
+
+bool on_current(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
+
+bool same(const at::Tensor& t, const at::Tensor& like, at::IntArrayRef sizes) {
+  return t.device() == like.device() && t.sizes() == sizes;
+}
+
+// f(bytes*) reports the workspace; its memory, or an undefined tensor after an error.
+template <class F>
+bool workspace(const at::Tensor& like, F&& f, at::Tensor* out, size_t* n) {
+  if (f(n) != FMXQ_OK) return false;
+  *out = make(like, {(int64_t)*n}, at::kByte);
+  return true;
+}
+
+// A weight [*lead, K * bits / 32] with scales and biases [*lead, K / group].
+bool weight_ok(const at::Tensor& like, const at::Tensor& w, const at::Tensor& s, const at::Tensor& b,
+               int64_t K, int64_t group, int64_t bits) {
+  if (w.device() != like.device() || w.size(-1) * 32 / bits != K || K % group) return false;
+  at::DimVector sizes(w.sizes());
+  sizes.back() = K / group;
+  return same(s, like, sizes) && same(b, like, sizes);
+}
+
+// (h, w, scales, biases, ids, teacher | None, temperature, ignore, grad, grad_loss | None,
+// group_size, bits): cross entropy without a teacher.
+PyObject* head_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 12 || !PyFloat_CheckExact(a[6]) || !PyBool_Check(a[8])) return nullptr;
+    Call c;
+    int64_t group, bits, ignore;
+    const at::Tensor *h = c.tensor(a[0], kBf16Like), *w = c.tensor(a[1], kU32Like),
+                     *s = c.tensor(a[2], kBf16Like), *b = c.tensor(a[3], kBf16Like),
+                     *ids = c.tensor(a[4], kU32Like);
+    const bool distill = a[5] != Py_None, grad = a[8] == Py_True;
+    const at::Tensor* t = distill ? c.tensor(a[5], kBf16 | kF32) : nullptr;
+    const at::Tensor* gl = a[9] == Py_None ? nullptr : c.tensor(a[9], kF32);
+    if (!c.integer(a[7], &ignore) || !c.format(a[10], a[11], &group, &bits)) return nullptr;
+    if (h->dim() != 2 || w->dim() != 2 || ids->scalar_type() != at::kInt || !on_current(*h) ||
+        (gl && !grad) || ignore < INT32_MIN || ignore > INT32_MAX)
+      return nullptr;
+    const int64_t M = h->size(0), K = h->size(1), V = w->size(0);
+    if (!weight_ok(*h, *w, *s, *b, K, group, bits) || (gl && !same(*gl, *h, {M}))) return nullptr;
+    const int64_t k = distill ? ids->size(-1) : 1;
+    if (distill ? ids->dim() != 2 || !same(*ids, *h, {M, k}) || !same(*t, *h, {M, k})
+                : !same(*ids, *h, {M}))
+      return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*h, [&](size_t* o) { return fmxq_head_workspace(M, V, K, (int)k, grad, o); }, &ws,
+                   &bytes))
+      return nullptr;
+    at::Tensor loss = make(*h, {M}, at::kFloat), lse = make(*h, {M}, at::kFloat), dh;
+    if (grad) dh = make(*h, {M, K}, at::kBFloat16);
+    const uint16_t* hp = static_cast<uint16_t*>(h->data_ptr());
+    const uint32_t* wp = static_cast<uint32_t*>(w->data_ptr());
+    const uint16_t *sp = static_cast<uint16_t*>(s->data_ptr()), *bp = static_cast<uint16_t*>(b->data_ptr());
+    const int32_t* ip = static_cast<int32_t*>(ids->data_ptr());
+    const float* gp = gl ? static_cast<float*>(gl->data_ptr()) : nullptr;
+    float *lp = static_cast<float*>(loss.data_ptr()), *ep = static_cast<float*>(lse.data_ptr());
+    uint16_t* dp = grad ? static_cast<uint16_t*>(dh.data_ptr()) : nullptr;
+    const float temperature = (float)PyFloat_AS_DOUBLE(a[6]);
+    void* st = stream_of(*h);
+    if (!enqueue([&] {
+          return distill
+                     ? fmxq_head_distill(hp, wp, sp, bp, ip, t->data_ptr(),
+                                         t->scalar_type() == at::kBFloat16, gp, lp, ep, dp, M, V, K,
+                                         (int)k, temperature, (int)group, (int)bits, ws.data_ptr(),
+                                         bytes, st)
+                     : fmxq_head_cross_entropy(hp, wp, sp, bp, ip, gp, lp, ep, dp, M, V, K,
+                                               (int32_t)ignore, (int)group, (int)bits, ws.data_ptr(),
+                                               bytes, st);
+        }))
+      return nullptr;
+    if (!grad)
+      return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(lse)));
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(lse)),
+                         THPVariable_Wrap(std::move(dh)));
+  });
+}
+
+// (dy, w, scales, biases, offsets | None, group_size, bits): quantized_matmul_grad, or
+// gather_qmm_grad with offsets.
+PyObject* qmm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 7) return nullptr;
+    Call c;
+    int64_t group, bits;
+    const at::Tensor *dy = c.tensor(a[0], kBf16Like), *w = c.tensor(a[1], kU32Like),
+                     *s = c.tensor(a[2], kBf16Like), *b = c.tensor(a[3], kBf16Like);
+    const bool runs = a[4] != Py_None;
+    const at::Tensor* off = runs ? c.tensor(a[4], kU32Like) : nullptr;
+    if (!c.format(a[5], a[6], &group, &bits) || dy->dim() < 1 || w->dim() != (runs ? 3 : 2) ||
+        !on_current(*dy))
+      return nullptr;
+    const int64_t N = w->size(-2), K = w->size(-1) * 32 / bits, M = dy->numel() / N;
+    const int64_t E = runs ? w->size(0) : 0;
+    if (dy->size(-1) != N || !weight_ok(*dy, *w, *s, *b, K, group, bits)) return nullptr;
+    if (runs && (dy->dim() != 2 || off->scalar_type() != at::kInt || !same(*off, *dy, {E + 1})))
+      return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*dy,
+                   [&](size_t* o) {
+                     return runs ? fmxq_gather_qmm_grad_workspace(M, E, N, K, o)
+                                 : fmxq_quantized_matmul_grad_workspace(M, N, K, o);
+                   },
+                   &ws, &bytes))
+      return nullptr;
+    at::DimVector sizes(dy->sizes());
+    sizes.back() = K;
+    at::Tensor dx = make(*dy, sizes, at::kBFloat16);
+    const uint16_t* yp = static_cast<uint16_t*>(dy->data_ptr());
+    const uint32_t* wp = static_cast<uint32_t*>(w->data_ptr());
+    const uint16_t *sp = static_cast<uint16_t*>(s->data_ptr()), *bp = static_cast<uint16_t*>(b->data_ptr());
+    uint16_t* xp = static_cast<uint16_t*>(dx.data_ptr());
+    void* st = stream_of(*dy);
+    if (!enqueue([&] {
+          return runs ? fmxq_gather_qmm_grad(yp, wp, sp, bp, static_cast<int32_t*>(off->data_ptr()), xp, M,
+                                             E, N, K, (int)group, (int)bits, ws.data_ptr(), bytes, st)
+                      : fmxq_quantized_matmul_grad(yp, wp, sp, bp, xp, M, N, K, (int)group, (int)bits,
+                                                   ws.data_ptr(), bytes, st);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(std::move(dx));
+  });
+}
+
+// (x, inds, n_experts) -> (xs, order, pos, offsets)
+PyObject* moe_sort(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 3) return nullptr;
+    Call c;
+    int64_t E;
+    const at::Tensor *x = c.tensor(a[0], kBf16Like), *inds = c.tensor(a[1], kU32Like);
+    if (!c.integer(a[2], &E) || x->dim() != 2 || inds->dim() != 2 || E < 1 || E > 2048 || !on_current(*x))
+      return nullptr;
+    const int64_t T = x->size(0), D = x->size(1), k = inds->size(1);
+    if (!same(*inds, *x, {T, k})) return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*x, [&](size_t* o) { return fmxq_moe_sort_workspace(T, k, E, o); }, &ws, &bytes))
+      return nullptr;
+    at::Tensor xs = make(*x, {T * k, D}, at::kBFloat16), order = make(*x, {T * k}, at::kInt),
+               pos = make(*x, {T, k}, at::kInt), off = make(*x, {E + 1}, at::kInt);
+    const uint16_t* xp = static_cast<uint16_t*>(x->data_ptr());
+    const uint32_t* ip = static_cast<uint32_t*>(inds->data_ptr());
+    void* st = stream_of(*x);
+    if (!enqueue([&] {
+          return fmxq_moe_sort(xp, ip, static_cast<uint16_t*>(xs.data_ptr()),
+                               static_cast<uint32_t*>(order.data_ptr()),
+                               static_cast<uint32_t*>(pos.data_ptr()),
+                               static_cast<uint32_t*>(off.data_ptr()), T, k, E, D, ws.data_ptr(), bytes,
+                               st);
+        }))
+      return nullptr;
+    return Py_BuildValue("(NNNN)", THPVariable_Wrap(std::move(xs)), THPVariable_Wrap(std::move(order)),
+                         THPVariable_Wrap(std::move(pos)), THPVariable_Wrap(std::move(off)));
+  });
+}
+
+// (y, pos, weights | None): moe_unsort, or moe_sort_grad without weights.
+PyObject* moe_unsort(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 3) return nullptr;
+    Call c;
+    const at::Tensor *y = c.tensor(a[0], kBf16Like), *pos = c.tensor(a[1], kU32Like);
+    const bool weighted = a[2] != Py_None;
+    const at::Tensor* w = weighted ? c.tensor(a[2], kBf16 | kF32) : nullptr;
+    if (!c.ok || y->dim() != 2 || pos->dim() != 2 || !on_current(*y)) return nullptr;
+    const int64_t T = pos->size(0), k = pos->size(1), D = y->size(1);
+    if (y->size(0) != T * k || pos->device() != y->device() || (w && !same(*w, *y, {T, k})))
+      return nullptr;
+    at::Tensor out = make(*y, {T, D}, at::kBFloat16);
+    const uint16_t* yp = static_cast<uint16_t*>(y->data_ptr());
+    const uint32_t* pp = static_cast<uint32_t*>(pos->data_ptr());
+    uint16_t* op = static_cast<uint16_t*>(out.data_ptr());
+    void* st = stream_of(*y);
+    if (!enqueue([&] {
+          return w ? fmxq_moe_unsort(yp, pp, w->data_ptr(), w->scalar_type() == at::kBFloat16, op, T, k, D,
+                                     st)
+                   : fmxq_moe_sort_grad(yp, pp, op, T, k, D, st);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// (dout, y, pos, weights) -> (dy, dweights)
+PyObject* moe_unsort_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 4) return nullptr;
+    Call c;
+    const at::Tensor *d = c.tensor(a[0], kBf16Like), *y = c.tensor(a[1], kBf16Like),
+                     *pos = c.tensor(a[2], kU32Like), *w = c.tensor(a[3], kBf16 | kF32);
+    if (!c.ok || y->dim() != 2 || pos->dim() != 2 || !on_current(*y)) return nullptr;
+    const int64_t T = pos->size(0), k = pos->size(1), D = y->size(1);
+    if (y->size(0) != T * k || pos->device() != y->device() || !same(*w, *y, {T, k}) ||
+        !same(*d, *y, {T, D}))
+      return nullptr;
+    at::Tensor dy = make(*y, {T * k, D}, at::kBFloat16), dw = make(*y, {T, k}, w->scalar_type());
+    const uint16_t *dp = static_cast<uint16_t*>(d->data_ptr()), *yp = static_cast<uint16_t*>(y->data_ptr());
+    const uint32_t* pp = static_cast<uint32_t*>(pos->data_ptr());
+    void* st = stream_of(*y);
+    if (!enqueue([&] {
+          return fmxq_moe_unsort_grad(dp, yp, pp, w->data_ptr(), w->scalar_type() == at::kBFloat16,
+                                      static_cast<uint16_t*>(dy.data_ptr()), dw.data_ptr(), T, k, D, st);
+        }))
+      return nullptr;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(dy)), THPVariable_Wrap(std::move(dw)));
+  });
+}
+
 #define FMXQ_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FMXQ_FAST(quantized_matmul), FMXQ_FAST(dequantize),       FMXQ_FAST(quantize),
                          FMXQ_FAST(moe_layer),        FMXQ_FAST(route_softmax_topk), FMXQ_FAST(route_group_topk),
+                         FMXQ_FAST(head_loss),        FMXQ_FAST(qmm_grad),           FMXQ_FAST(moe_sort),
+                         FMXQ_FAST(moe_unsort),       FMXQ_FAST(moe_unsort_grad),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

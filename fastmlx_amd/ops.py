@@ -380,6 +380,11 @@ def head_cross_entropy(h, w, scales, biases, targets, ignore_index: int = -100, 
     with ``grad`` also dh [M, K] bf16, the gradient of sum_t grad_loss[t] loss[t] (grad_loss
     [M] float32, ones without).  A target equal to ignore_index has loss and gradient 0; one
     outside the vocabulary too, which device_error reports."""
+    if _fast is not None:
+        r = _fast.head_loss(h, w, scales, biases, targets, None, 1.0, ignore_index, bool(grad),
+                            grad_loss, group_size, bits)
+        if r is not None:
+            return r
     dev = _same_device(h=h, w=w, scales=scales, biases=biases, targets=targets,
                        grad_loss=grad_loss)
     M, V, K, ptrs = _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits)
@@ -404,6 +409,11 @@ def head_distill(h, w, scales, biases, ids, teacher, temperature: float = 1.0, g
     over the entries and p = softmax(logits / T) over the vocabulary, returns (loss [M] =
     T^2 KL(q || p), lse [M] = log sum exp(logits / T)) float32, and with ``grad`` dh [M, K] as
     head_cross_entropy does."""
+    if _fast is not None and teacher is not None:
+        r = _fast.head_loss(h, w, scales, biases, ids, teacher, float(temperature), 0, bool(grad),
+                            grad_loss, group_size, bits)
+        if r is not None:
+            return r
     dev = _same_device(h=h, w=w, scales=scales, biases=biases, ids=ids, teacher=teacher,
                        grad_loss=grad_loss)
     M, V, K, ptrs = _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits)
@@ -427,6 +437,10 @@ def head_distill(h, w, scales, biases, ids, teacher, temperature: float = 1.0, g
 def quantized_matmul_grad(dy, w, scales, biases, group_size: int = 64, bits: int = 4):
     """Gradient of x in quantized_matmul: dx = dy @ deq(W), dy [..., N] bf16, w [N, K*bits/32];
     dx [..., K] bf16."""
+    if _fast is not None:
+        r = _fast.qmm_grad(dy, w, scales, biases, None, group_size, bits)
+        if r is not None:
+            return r
     dev = _same_device(dy=dy, w=w, scales=scales, biases=biases)
     if w.dim() != 2 or dy.dim() < 1:
         raise ValueError("dy must be [..., N] and w [N, K*bits/32]")
@@ -452,6 +466,10 @@ def gather_qmm_grad(dy, w, scales, biases, offsets, group_size: int = 64, bits: 
     """Gradient of x in gather_qmm over rows sorted by expert (moe_sort): rows offsets[e] ..
     offsets[e + 1] of dx are dy @ deq(W[e]).  dy [S, N] bf16; w [E, N, K*bits/32]; offsets
     [E + 1] int32; dx [S, K] bf16, zero in rows of no expert."""
+    if _fast is not None and offsets is not None:
+        r = _fast.qmm_grad(dy, w, scales, biases, offsets, group_size, bits)
+        if r is not None:
+            return r
     dev = _same_device(dy=dy, w=w, scales=scales, biases=biases, offsets=offsets)
     if w.dim() != 3 or dy.dim() != 2:
         raise ValueError("dy must be [S, N] and w [E, N, K*bits/32]")
@@ -480,6 +498,10 @@ def moe_sort(x, inds, n_experts: int):
     Slot t k + j goes to row pos[t, j]; order is the stable argsort of the ids; expert e has
     rows offsets[e] .. offsets[e + 1].  Ids out of range sort last with zero rows, and
     device_error reports them."""
+    if _fast is not None:
+        r = _fast.moe_sort(x, inds, n_experts)
+        if r is not None:
+            return r
     dev = _same_device(x=x, inds=inds)
     if x.dim() != 2 or inds.dim() != 2:
         raise ValueError("x must be [T, D] and inds [T, k]")
@@ -516,6 +538,10 @@ def _row_weights(weights, T, k):
 def moe_sort_grad(dxs, pos):
     """Gradient of moe_sort's x: dxs [T k, D] bf16 -> dx [T, D] bf16, each token's slots summed
     in float32."""
+    if _fast is not None:
+        r = _fast.moe_unsort(dxs, pos, None)
+        if r is not None:
+            return r
     dev = _same_device(dxs=dxs, pos=pos)
     T, k, D, yp, pp = _sorted_rows("dxs", dxs, pos)
     with torch.cuda.device(dev):
@@ -527,6 +553,10 @@ def moe_sort_grad(dxs, pos):
 def moe_unsort(y, pos, weights):
     """Sorted rows back to tokens: out[t] = sum_j weights[t, j] y[pos[t, j]] in float32, rounded
     once.  y [T k, D] bf16; weights [T, k] bfloat16 or float32; out [T, D] bf16."""
+    if _fast is not None and weights is not None:
+        r = _fast.moe_unsort(y, pos, weights)
+        if r is not None:
+            return r
     dev = _same_device(y=y, pos=pos, weights=weights)
     T, k, D, yp, pp = _sorted_rows("y", y, pos)
     wp, wb = _row_weights(weights, T, k)
@@ -539,6 +569,10 @@ def moe_unsort(y, pos, weights):
 def moe_unsort_grad(dout, y, pos, weights):
     """Gradients of moe_unsort: dout [T, D] bf16 -> (dy [T k, D] bf16, dweights [T, k] in the
     weights' type)."""
+    if _fast is not None:
+        r = _fast.moe_unsort_grad(dout, y, pos, weights)
+        if r is not None:
+            return r
     dev = _same_device(dout=dout, y=y, pos=pos, weights=weights)
     T, k, D, yp, pp = _sorted_rows("y", y, pos)
     _shape("dout", dout, T, D)
