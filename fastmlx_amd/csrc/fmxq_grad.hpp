@@ -25,6 +25,8 @@ struct GradGemm {
   // of output column n (ldp a multiple of 8; values from C on are not read).
   const uint16_t* panel = nullptr;
   int64_t ldp = 0;
+  // launch_skinny_gemm (nt): skinny_pack_bytes of memory for x, or null to read it as it is.
+  void* xp = nullptr;
   // The contraction in `splits` parts of c_split (a multiple of 64) values; part p goes to
   // slice p of out.
   int splits = 1;
@@ -62,6 +64,12 @@ hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stre
 // (fmxq_grad_skinny.hip).  weight_rows: rows of a part of the contraction (nn).
 constexpr int64_t kSkinnyRows = 64;
 constexpr int kSkinnyStatWidth = 32;
+constexpr int kSkinnyCols = 128;  // outputs of a block (nn)
+// Rows from which the logits' x is packed beforehand, and the bytes that takes.
+constexpr int64_t kSkinnyPackRows = 17;
+inline int64_t skinny_pack_bytes(int64_t M, int64_t K) {
+  return M < kSkinnyPackRows ? 0 : (K + 63) / 64 * 4096 * (M <= 32 ? 1 : 2);
+}
 bool skinny_gemm_supported(int64_t M, int64_t lda, int64_t weight_rows, int64_t weight_cols);
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 
@@ -114,7 +122,7 @@ struct HeadPlan {
   int64_t piece, c_split, stat_tiles;
   bool panel;   // the products run over panels of dequantized weights
   bool skinny;  // ... or on the kernels for few rows
-  size_t stats, e, slices, state, factor, coef, row, panel_at, bytes;  // in the workspace
+  size_t stats, e, slices, state, factor, sel, panel_at, xp, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);
 hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipStream_t stream);

@@ -82,18 +82,16 @@ __device__ __forceinline__ float logit_of(const HeadLoss& a, int64_t m, int64_t 
   return wave_sum(t) * scale;
 }
 
-// One wave: lse, the loss, each wanted entry's coefficient of W_id and the factor of the sums
-// over e, from the row's final (m, sum) and its entries' logits.  A row without a wanted
-// entry has loss 0 and gradient 0 (row[m].y marks it; the gradient kernel writes zeros
-// without reading the sums).
-__device__ __forceinline__ void finish_row(const HeadLoss& a, int64_t m, float2 st,
-                                           const float* sel, float* __restrict__ coef,
-                                           float2* __restrict__ row) {
+// One wave: lse and the loss (stored where `store`) from the row's final (m, sum) and lane j's
+// logit l2 of entry j; the lane's coefficient of W_id and the factor of the sums over e.
+// False for a row without a wanted entry, whose loss and gradient are 0.
+__device__ __forceinline__ bool finish_row(const HeadLoss& a, int64_t m, float2 st, float l2,
+                                           bool store, float* coef, float* factor) {
   const int lane = threadIdx.x & 63;
   const float lse2 = st.x + __builtin_amdgcn_logf(st.y);  // in units of log 2
   const float T = a.temperature;
   const bool on = lane < a.k;
-  const int64_t v = on ? token_of(a, m, lane, true) : -1;
+  const int64_t v = on ? token_of(a, m, lane, false) : -1;
   float q = v >= 0 ? 1.f : 0.f, logq = 0.f;
   bool empty;
   if (a.teacher) {
@@ -112,15 +110,14 @@ __device__ __forceinline__ void finish_row(const HeadLoss& a, int64_t m, float2 
   } else {
     empty = !__any(v >= 0);
   }
-  const float l2 = v >= 0 ? sel[lane] : 0.f;
   // Entries of no weight add nothing (0 log 0 = 0); NaN stays.
   const float term = v >= 0 && q != 0.f ? q * (logq - l2 + lse2) : 0.f;
   const float loss = wave_sum(term) * (T * T * kLn2);
-  if (lane == 0) {
+  if (store && lane == 0) {
     a.lse[m] = lse2 * kLn2;
     a.loss[m] = empty ? 0.f : loss;
   }
-  if (!a.dh) return;
+  if (!a.dh) return !empty;
   // p of an id that a row names twice counts once.
   bool first = v >= 0;
   for (int j = 0; j < a.k; ++j) {
@@ -129,22 +126,24 @@ __device__ __forceinline__ void finish_row(const HeadLoss& a, int64_t m, float2 
   }
   const float g = (a.grad_loss ? a.grad_loss[m] : 1.f) * T;
   const float p = first ? __builtin_amdgcn_exp2f(l2 - lse2) : 0.f;
-  if (on) coef[m * a.k + lane] = v >= 0 ? g * (p - q) : 0.f;
-  if (lane == 0) row[m] = make_float2(g / st.y, empty ? 1.f : 0.f);
+  *coef = v >= 0 ? g * (p - q) : 0.f;
+  *factor = g / st.y;
+  return !empty;
 }
 
 // Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought
 // to it with the wanted entries zeroed.  in / out are the states before and after; chunk 0
 // writes out and the factor of the earlier pieces' sums and, after the last piece, finishes
-// the row: its waves take the wanted entries' logits in turn.
+// the row where no gradient follows.  After the last piece the blocks of a row share its
+// wanted entries' logits (sel).
 constexpr int kJoinCols = 8192;
 __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2* __restrict__ stats,
                                                         int64_t stat_tiles, int tw,
                                                         const float2* in, float2* out,
                                                         float* factor, uint16_t* e, int64_t lde,
                                                         int64_t v0, int64_t tiles, bool last,
-                                                        float scale, float* coef, float2* rowf) {
-  __shared__ float red[4], red2[4], sel[64];
+                                                        float scale, float* sel) {
+  __shared__ float red[4], red2[4], l2s[64];
   const int64_t m = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float2* st = stats + m * stat_tiles;
@@ -155,30 +154,38 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
   if (lane == 0) red[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float2 now = make_float2(0.f, 0.f);
   if (blockIdx.y == 0) {
     float sum = 0.f;
     for (int64_t t = tid; t < tiles; t += 256)
       sum = __builtin_fmaf(st[t].y, __builtin_amdgcn_exp2f(st[t].x - top), sum);
     sum = wave_sum(sum);
     if (lane == 0) red2[wave] = sum;
-    if (last)
-      for (int j = wave; j < a.k; j += 4) {
-        const int64_t v = token_of(a, m, j, false);
-        const float l2 = v >= 0 ? logit_of(a, m, v, scale) : 0.f;
-        if (lane == 0) sel[j] = l2;
-      }
     __syncthreads();
     if (wave == 0) {
       // The first piece starts from nothing: its factor is never used on anything but zeros.
       const float f = in ? __builtin_amdgcn_exp2f(old.x - top) : 0.f;
-      const float2 now =
-          make_float2(top, (in ? old.y * f : 0.f) + (red2[0] + red2[1]) + (red2[2] + red2[3]));
+      now = make_float2(top, 
+                        (in ? old.y * f : 0.f) + (red2[0] + red2[1]) + (red2[2] + red2[3]));
       if (lane == 0) {
         out[m] = now;
         if (factor) factor[m] = f;
       }
-      if (last) finish_row(a, m, now, sel, coef, rowf);
     }
+  }
+  if (last)
+    for (int j = 4 * blockIdx.y + wave; j < a.k; j += 4 * gridDim.y) {
+      const int64_t v = token_of(a, m, j, lane == 0);
+      const float l2 = v >= 0 ? logit_of(a, m, v, scale) : 0.f;
+      if (lane == 0) {
+        if (e) sel[m * a.k + j] = l2;
+        else l2s[j] = l2;
+      }
+    }
+  if (last && !e) {
+    __syncthreads();
+    if (wave == 0)
+      finish_row(a, m, now, lane < a.k ? l2s[lane] : 0.f, true, nullptr, nullptr);
   }
   if (!e) return;
   uint16_t* row = e + m * lde;
@@ -201,39 +208,74 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
   }
 }
 
-// Thread: 8 columns of a row: the slices' sum times the row's factor, plus the wanted
-// entries' share.
+// A row's loss and gradient: the slices' sum times the row's factor, plus the wanted entries'
+// share, 8 columns a thread.  With WS = 4 the waves of a block share the slices and the
+// entries of 512 columns (many slices, or entries), else each takes columns of its own.
+template <int WS>
 __global__ __launch_bounds__(256) void head_dh_kernel(HeadLoss a, const float* __restrict__ slices,
-                                                      int splits, const float* __restrict__ coef,
-                                                      const float2* __restrict__ row) {
+                                                      int splits, const float2* __restrict__ state,
+                                                      const float* __restrict__ sel) {
+  __shared__ float coef[64], factor;
+  __shared__ int any;
+  __shared__ f32x4 part[WS > 1 ? 2 * 256 : 1];
   const int64_t m = blockIdx.x;
-  const int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
-  if (c >= a.K) return;
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  if (row[m].y == 0.f) {
-    for (int s = 0; s < splits; ++s) {
-      const f32x4* p = reinterpret_cast<const f32x4*>(slices + ((int64_t)s * a.M + m) * a.K + c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += p[j >> 2][j & 3];
-    }
-    const float f = row[m].x;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= f;
-    for (int i = 0; i < a.k; ++i) {
-      const int64_t id = token_of(a, m, i, false);
-      if (id < 0) continue;
-      const float co = coef[m * a.k + i];
-      float wv[8];
-      deq8(a, id, c, wv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(co, wv[j], v[j]);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c0 = (int64_t)blockIdx.y * (WS > 1 ? 512 : 2048);
+  const int64_t c = c0 + 8 * (WS > 1 ? lane : (int)threadIdx.x);
+  if (wave == 0) {
+    float co = 0.f, f = 0.f;
+    const bool on = finish_row(a, m, state[m], lane < a.k ? sel[m * a.k + lane] : 0.f,
+                               blockIdx.y == 0, &co, &f);
+    coef[lane] = co;
+    if (lane == 0) {
+      factor = f;
+      any = on;
     }
   }
-  *reinterpret_cast<u32x4*>(a.dh + m * a.K + c) =
-      u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-            pack_bf16x2(v[6], v[7])};
+  f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  if (c < a.K) {
+#pragma unroll 8
+    for (int s = WS > 1 ? wave : 0; s < splits; s += WS) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(slices + ((int64_t)s * a.M + m) * a.K + c);
+      v[0] += p[0];
+      v[1] += p[1];
+    }
+  }
+  __syncthreads();
+  v[0] *= factor;
+  v[1] *= factor;
+  if (c < a.K) {
+#pragma unroll 4
+    for (int i = WS > 1 ? wave : 0; i < a.k; i += WS) {
+      const int64_t id = token_of(a, m, i, false);
+      const float co = coef[i];
+      float wv[8];
+      deq8(a, id < 0 ? 0 : id, c, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (id >= 0) v[j >> 2][j & 3] = __builtin_fmaf(co, wv[j], v[j >> 2][j & 3]);
+    }
+  }
+  if constexpr (WS > 1) {
+    part[2 * threadIdx.x] = v[0];
+    part[2 * threadIdx.x + 1] = v[1];
+    __syncthreads();
+    const float* p = reinterpret_cast<const float*>(part) + 2 * threadIdx.x;
+    float lo = 0.f, hi = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      lo += p[512 * w];
+      hi += p[512 * w + 1];
+    }
+    const int64_t n = c0 + 2 * threadIdx.x;
+    if (n < a.K)
+      *reinterpret_cast<uint32_t*>(a.dh + m * a.K + n) = any ? pack_bf16x2(lo, hi) : 0u;
+  } else if (c < a.K) {
+    u32x4 o = {pack_bf16x2(v[0][0], v[0][1]), pack_bf16x2(v[0][2], v[0][3]),
+               pack_bf16x2(v[1][0], v[1][1]), pack_bf16x2(v[1][2], v[1][3])};
+    if (!any) o = u32x4{0u, 0u, 0u, 0u};
+    *reinterpret_cast<u32x4*>(a.dh + m * a.K + c) = o;
+  }
 }
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -262,8 +304,8 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   p.stat_tiles = (grad ? piece : up(V, kGradTileCols)) / p.stat_width;
   // Parts of the gradient product's contraction: enough blocks for the chip, each walking
   // 256 tokens at least.
-  const int64_t tiles =
-      (p.skinny ? 1 : (M + p.bm - 1) / p.bm) * ((K + kGradTileCols - 1) / kGradTileCols);
+  const int64_t cols = p.skinny ? kSkinnyCols : kGradTileCols;
+  const int64_t tiles = (p.skinny ? 1 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
   const int64_t want = (p.bm >= 128 ? cus : 2 * cus) / tiles;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, piece / 256));
   p.c_split = up((piece + p.splits - 1) / p.splits, 64);
@@ -275,14 +317,14 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   };
   p.stats = take(M * p.stat_tiles * 8);
   p.state = take(2 * M * 8);
-  p.coef = take(M * k * 4);
-  p.row = take(M * 8);
+  p.sel = take(M * k * 4);
   p.factor = take(M * 4);
   if (grad) {
     p.e = take(M * piece * 2);
     p.slices = take((int64_t)p.splits * M * K * 4);
   }
   if (p.panel) p.panel_at = take(piece * K * 2);
+  if (p.skinny) p.xp = take(skinny_pack_bytes(M, K));
   p.bytes = at;
   return p;
 }
@@ -291,8 +333,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   char* base = static_cast<char*>(ws);
   float2* stats = reinterpret_cast<float2*>(base + p.stats);
   float2* state = reinterpret_cast<float2*>(base + p.state);
-  float* coef = reinterpret_cast<float*>(base + p.coef);
-  float2* row = reinterpret_cast<float2*>(base + p.row);
+  float* sel = reinterpret_cast<float*>(base + p.sel);
   float* factor = reinterpret_cast<float*>(base + p.factor);
   uint16_t* e = a.dh ? reinterpret_cast<uint16_t*>(base + p.e) : nullptr;
   float* slices = a.dh ? reinterpret_cast<float*>(base + p.slices) : nullptr;
@@ -300,12 +341,13 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   uint16_t* panel = p.panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
   // (in, out): the running state before and after the pieces joined so far.
   auto join = [&](int i, int64_t v0, int64_t n, int64_t lde) {
-    const dim3 grid((unsigned)a.M, e ? (unsigned)((lde + kJoinCols - 1) / kJoinCols) : 1u);
+    const int64_t chunks = (lde + kJoinCols - 1) / kJoinCols, shares = (a.k + 3) / 4;
+    const dim3 grid((unsigned)a.M, e ? (unsigned)std::max(chunks, v0 + n == a.V ? shares : 1) : 1u);
     head_join_kernel<<<grid, 256, 0, stream>>>(a, stats, p.stat_tiles, p.stat_width,
                                                i ? state + (i & 1) * a.M : nullptr,
                                                state + ((i + 1) & 1) * a.M, factor, e, lde, v0,
                                                (n + p.stat_width - 1) / p.stat_width,
-                                               v0 + n == a.V, scale, coef, row);
+                                               v0 + n == a.V, scale, sel);
     return hipGetLastError();
   };
   for (int i = 0; i < p.pieces; ++i) {
@@ -327,6 +369,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     g.e = e;
     g.lde = up(n, kGradTileCols);
     g.logit_scale = scale;
+    if (p.skinny && skinny_pack_bytes(a.M, a.K)) g.xp = base + p.xp;
     if (p.panel) {
       if (hipError_t r = launch_dequantize(g.w, g.scales, g.biases, panel, n, a.K, a.group_size, a.bits,
                                            stream))
@@ -364,8 +407,14 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   if (!e)
     if (hipError_t r = join(0, 0, a.V, 0)) return r;
   if (!a.dh) return hipSuccess;
-  const dim3 grid((unsigned)a.M, (unsigned)((a.K + 2047) / 2048));
-  head_dh_kernel<<<grid, 256, 0, stream>>>(a, slices, p.splits, coef, row);
+  const float2* end = state + (p.pieces & 1) * a.M;
+  if (p.splits >= 8 || a.k >= 8) {
+    const dim3 grid((unsigned)a.M, (unsigned)((a.K + 511) / 512));
+    head_dh_kernel<4><<<grid, 256, 0, stream>>>(a, slices, p.splits, end, sel);
+  } else {
+    const dim3 grid((unsigned)a.M, (unsigned)((a.K + 2047) / 2048));
+    head_dh_kernel<1><<<grid, 256, 0, stream>>>(a, slices, p.splits, end, sel);
+  }
   return hipGetLastError();
 }
 
