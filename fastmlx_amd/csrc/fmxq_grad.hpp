@@ -46,18 +46,23 @@ struct GradGemm {
   uint16_t* e = nullptr;
   int64_t lde = 0;
   float logit_scale = 1.f;
-  // Expert runs (nn only): tile t of the list covers rows [tiles[3t], + tiles[3t+1]) with
-  // expert tiles[3t+2], whose weights are C rows into w.
-  const uint32_t* tiles = nullptr;
-  const uint32_t* ntile = nullptr;
-  int64_t max_tiles = 0;
+  // Expert runs (nn only, into y): rows offsets[e] .. offsets[e + 1] of M take expert e, whose
+  // weights are C rows into w; other rows get zeros.  max_tiles: grad_gemm_run_tiles.  *flag
+  // is raised where the offsets decrease or leave 0 .. M (all rows are zero then).
+  const int32_t* offsets = nullptr;
+  int64_t experts = 0, max_tiles = 0;
+  uint32_t* flag = nullptr;
 };
 
 // Rows of a block's tile, for M rows (or expert runs of about that many).
-int grad_gemm_rows(int64_t M);
-// Columns of a tile of the statistics for M rows.
-int grad_gemm_stat_width(int64_t M);
+int grad_gemm_rows(int64_t M, bool nn);
+constexpr int kGradStatWidth = 64;  // columns of a tile of the statistics (128 rows and more)
 constexpr int kGradTileCols = 256;
+constexpr int kLogitCols = 256, kGradCols = 128;  // of launch_grad_gemm's tiles
+// Tiles of bm rows that cover any runs of S rows, and one more that none does.
+inline int64_t grad_gemm_run_tiles(int64_t S, int64_t E, int bm) {
+  return S / bm + (E < S ? E : S) + 1;
+}
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
 
 // The same products for up to kSkinnyRows rows, where reading the weights is the work
@@ -90,13 +95,6 @@ hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64
 // dst [M, ld] = src [M, N] with zeros in columns N .. ld.
 hipError_t launch_pad_rows(const uint16_t* src, uint16_t* dst, int64_t M, int64_t N, int64_t ld,
                            hipStream_t stream);
-// Tiles of `bm` rows of the expert runs [offsets[e], offsets[e + 1]) of S rows as (row, rows,
-// expert) triples, their number, and zeros in the rows of dx [S, N] that no run covers.
-// Offsets that decrease or leave 0 .. S give no tiles, zero rows and raise *flag.
-hipError_t launch_run_tiles(const int32_t* offsets, int64_t E, int64_t S, int bm, uint32_t* tiles,
-                            uint32_t* ntile, uint16_t* dx, int64_t N, uint32_t* flag,
-                            hipStream_t stream);
-
 // A loss over a quantized head (fmxq_head.hip).  ids [M, k]: the targets (k = 1, teacher
 // null) or the teacher's entries.  An id that names no token: `ignore` for targets, below
 // zero for a teacher.
@@ -118,10 +116,11 @@ struct HeadLoss {
   uint32_t* flag;
 };
 struct HeadPlan {
-  int bm, stat_width, pieces, splits;
+  int bm, grad_bm, stat_width, pieces, splits;
   int64_t piece, c_split, stat_tiles;
-  bool panel;   // the products run over panels of dequantized weights
-  bool skinny;  // ... or on the kernels for few rows
+  // The logits and the gradient run over panels of dequantized weights, or both on the
+  // kernels for few rows.
+  bool panel, grad_panel, skinny;
   size_t stats, e, slices, state, factor, sel, panel_at, xp, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);

@@ -92,13 +92,13 @@ int64_t pad_cols(int64_t N) { return up(N, 8); }
 GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
   p.panel = M >= kGradPanelRows;
-  p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M);
+  p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M, true);
   p.skinny = fmxq::skinny_gemm_supported(M, pad_cols(N), N + 64, K);
-  const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) *
-                        ((K + fmxq::kGradTileCols - 1) / fmxq::kGradTileCols);
+  const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.panel ? fmxq::kGradTileCols : fmxq::kGradCols;
+  const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at
   // least.
-  const int64_t want = tiles ? (p.bm >= 128 ? kCus : 2 * kCus) / tiles : 1;
+  const int64_t want = tiles ? (p.panel ? kCus : 2 * kCus) / tiles : 1;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, N / 256));
   p.c_split = up((N + p.splits - 1) / p.splits, 64);
   p.splits = (int)std::max<int64_t>(1, (N + p.c_split - 1) / std::max<int64_t>(p.c_split, 1));
@@ -136,21 +136,7 @@ int bytes_out(size_t v, size_t* out, const char* op) {
   return FMXQ_OK;
 }
 
-struct RunPlan {
-  int bm;
-  int64_t max_tiles;
-  size_t ntile, tiles, bytes;  // the padded dy first
-};
-
-RunPlan run_plan(int64_t S, int64_t E, int64_t N) {
-  RunPlan p{};
-  p.bm = fmxq::grad_gemm_rows(E > 0 ? (S + E - 1) / E : S);
-  p.max_tiles = S / p.bm + std::min(E, S);
-  p.ntile = up(S * pad_cols(N) * 2, 256);
-  p.tiles = p.ntile + 256;
-  p.bytes = p.tiles + p.max_tiles * 3 * sizeof(uint32_t);
-  return p;
-}
+int run_rows(int64_t S, int64_t E) { return fmxq::grad_gemm_rows(E > 0 ? (S + E - 1) / E : S, true); }
 
 // ---- sorted rows --------------------------------------------------------------------
 
@@ -268,7 +254,7 @@ int fmxq_gather_qmm_grad_workspace(int64_t S, int64_t E, int64_t N, int64_t K, s
   const char* op = "gather_qmm_grad_workspace";
   if (int rc = grad_sizes(S, N, K, op)) return rc;
   if (E < 0) return fail(FMXQ_ERR_SHAPE, "%s: negative size E=%lld", op, (long long)E);
-  return bytes_out(run_plan(S, E, N).bytes, bytes, op);
+  return bytes_out(S * pad_cols(N) * 2, bytes, op);
 }
 
 int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
@@ -289,17 +275,12 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
   if (!dy || !w || !scales || !biases || !offsets)
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
   if (!aligned16(w)) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: w must be 16-byte aligned", op);
-  const RunPlan p = run_plan(S, E, N);
-  if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, op)) return rc;
+  if (E > kMaxCount) return fail(FMXQ_ERR_SHAPE, "%s: %lld experts are too many", op, (long long)E);
+  if (int rc = check_workspace(workspace, workspace_bytes, S * pad_cols(N) * 2, op)) return rc;
   uint32_t* flag = nullptr;
   if (int rc = device_flag(s, &flag)) return rc;
-  char* ws = static_cast<char*>(workspace);
-  uint32_t* ntile = reinterpret_cast<uint32_t*>(ws + p.ntile);
-  uint32_t* tiles = reinterpret_cast<uint32_t*>(ws + p.tiles);
   fmxq::GradGemm g;
-  if (int rc = grad_operand(dy, ws, S, N, s, &g, op)) return rc;
-  if (int rc = hip_status(fmxq::launch_run_tiles(offsets, E, S, p.bm, tiles, ntile, dx, K, flag, s), op))
-    return rc;
+  if (int rc = grad_operand(dy, workspace, S, N, s, &g, op)) return rc;
   g.M = S;
   g.N = K;
   g.C = N;
@@ -311,10 +292,12 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
   g.c_split = up(N, 64);
   g.y = dx;
   g.ldy = K;
-  g.tiles = tiles;
-  g.ntile = ntile;
-  g.max_tiles = p.max_tiles;
-  return hip_status(fmxq::launch_grad_gemm(g, true, p.bm, s), op);
+  const int bm = run_rows(S, E);
+  g.offsets = offsets;
+  g.experts = E;
+  g.max_tiles = fmxq::grad_gemm_run_tiles(S, E, bm);
+  g.flag = flag;
+  return hip_status(fmxq::launch_grad_gemm(g, true, bm, s), op);
 }
 
 int fmxq_moe_sort_workspace(int64_t T, int64_t top_k, int64_t E, size_t* bytes) {

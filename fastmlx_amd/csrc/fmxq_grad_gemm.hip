@@ -2,12 +2,20 @@
 // a quantized head with the statistics of their softmax (nt), and the input gradient
 // dx = dy . deq(W) of a quantized product (nn), of one matrix or of expert runs.
 //
-// Tile: BM rows by 256 columns, 64 deep contraction steps, 4 waves.  A goes global -> LDS
-// with buffer_load ... lds; the packed weights go global -> registers two steps ahead, are
+// Tile: BM rows by BN columns, 64 deep contraction steps in two LDS stages, a wave for every 32
+// columns; two waves on a SIMD, so that one's dequantization runs under the other's MFMAs: of
+// one block for the logits (BN = 256), of two for the gradients (BN = 128), whose
+// contraction is often short and whose first loads and last stores then run under the other
+// block's steps.  A goes global -> LDS with
+// buffer_load ... lds; the packed weights go global -> registers some steps ahead, are
 // dequantized there to fmxq_dequantize's bits and written to LDS.  Both stages hold rows of
 // 64 contraction values (128 bytes), so one fragment read serves both forms: where the
-// weights are packed along the outputs (nn), a thread takes 8 rows of one word column, and
+// weights are packed along the outputs (nn), a thread takes 8 rows of half a word column, and
 // the transposition costs nothing: the roundings pack any two values.
+//
+// The barrier of a step sits before its last quarter's MFMAs, when every wave has read the
+// stage: the next fragments, the DMA that refills this stage and the first share of its
+// weights' dequantization run under them.
 #include <type_traits>
 
 #include "fmxq_grad_tile.hpp"
@@ -16,25 +24,100 @@ namespace fmxq {
 namespace {
 
 constexpr int kS = 64;   // contraction values per step
-constexpr int kN = kGradTileCols;
 
-template <int BM>
+// Chunk c of row r at position c ^ swz8(r): distinct for 8 consecutive rows (fragment reads),
+// and for 8 rows 8 apart (the transposing writes).
+__device__ __forceinline__ int swz8(int r) { return (r ^ (r >> 3)) & 7; }
+
+template <int BM, int BN>
 struct GradCfg {
-  static constexpr int WM = BM >= 128 ? 2 : 1;   // waves along the rows
-  static constexpr int WN = 4 / WM;              // and along the columns
+  static constexpr int W = BN / 32;              // waves
+  static constexpr int WM = BM >= 64 ? 2 : 1;    // ... along the rows
+  static constexpr int WN = W / WM;              // and along the columns
   static constexpr int MI = BM / WM / 32;        // 32-row groups of a wave
-  static constexpr int NJ = kN / WN / 32;        // 32-column groups
+  static constexpr int NJ = BN / WN / 32;        // 32-column groups
+  static constexpr int CB = BN / 64;             // 64-column blocks
 };
 
-// Value j (0..7) of 8 packed values as a float; the masks let each be one byte conversion.
+// Tile mt of BM-row tiles over the expert runs [offsets[e], offsets[e + 1]): its first row,
+// rows and expert, or rows = 0 behind the last tile.  Then *spare is the number of tiles
+// behind the last one up to and with this one, of *spares in all, and rows *lo .. *hi are
+// what the runs cover (nothing where the offsets decrease or leave 0 .. S).  All threads of
+// the block take part, each in a range of experts.
+template <int T>
+__device__ __forceinline__ int64_t run_tile(const GradGemm& g, int64_t mt, int BM, int64_t* m0,
+                                            int64_t* expert, int64_t* spare, int64_t* spares,
+                                            int64_t* lo, int64_t* hi) {
+  __shared__ uint32_t wsum[T / 64];
+  __shared__ int found[3], bad;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int32_t* off = g.offsets;
+  const int E = (int)g.experts, S = (int)g.M;
+  const int per = (E + T - 1) / T, e0 = tid * per < E ? tid * per : E, e1 = e0 + per < E ? e0 + per : E;
+  if (tid == 0) {
+    bad = 0;
+    found[1] = 0;
+  }
+  __syncthreads();
+  uint32_t n = 0;
+  bool ok = true;
+  for (int e = e0; e < e1; ++e) {
+    const int a = off[e], b = off[e + 1];
+    ok = ok && a >= 0 && b >= a && b <= S;
+    n += (uint32_t)((b - a + BM - 1) / BM);
+  }
+  if (!ok) bad = 1;
+  uint32_t inc = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = (uint32_t)__shfl_up((int)inc, o, 64);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 63) wsum[wave] = inc;
+  __syncthreads();
+  uint32_t at = inc - n, all = 0;
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) {
+    if (i < wave) at += wsum[i];
+    all += wsum[i];
+  }
+  if (bad) all = 0;
+  else if (mt >= at && mt < at + n) {
+    for (int e = e0; e < e1; ++e) {
+      const int a = off[e], b = off[e + 1], k = (b - a + BM - 1) / BM;
+      if (mt < at + k) {
+        const int r = a + (int)(mt - at) * BM;
+        found[0] = r;
+        found[1] = b - r < BM ? b - r : BM;
+        found[2] = e;
+        break;
+      }
+      at += k;
+    }
+  }
+  __syncthreads();
+  // Uniform for the compiler too: buffer resources made of them stay in scalar registers.
+  *m0 = __builtin_amdgcn_readfirstlane(found[0]);
+  *expert = __builtin_amdgcn_readfirstlane(found[2]);
+  all = __builtin_amdgcn_readfirstlane(all);
+  *spare = mt - all;
+  *spares = g.max_tiles - all;
+  *lo = all ? off[0] : S;
+  *hi = all ? off[E] : S;
+  if (bad && blockIdx.x == 0 && tid == 0) atomicOr(g.flag, 1u);
+  return __builtin_amdgcn_readfirstlane(found[1]);
+}
+
+// Value j (0..3) of 4 packed values as a float: a byte conversion each.
 template <int BITS>
-struct Q8;
+struct Q4;
 template <>
-struct Q8<4> {
+struct Q4<4> {
   uint32_t e, o;
-  __device__ __forceinline__ explicit Q8(const uint32_t* w) {
-    e = w[0] & 0x0F0F0F0Fu;
-    o = (w[0] >> 4) & 0x0F0F0F0Fu;
+  __device__ __forceinline__ explicit Q4(uint32_t w, int half) {
+    const uint32_t v = w >> (16 * half);
+    e = v & 0x0F0Fu;
+    o = (v >> 4) & 0x0F0Fu;
     asm("" : "+v"(e), "+v"(o));
   }
   __device__ __forceinline__ float at(int j) const {
@@ -42,27 +125,27 @@ struct Q8<4> {
   }
 };
 template <>
-struct Q8<8> {
-  uint32_t w0, w1;
-  __device__ __forceinline__ explicit Q8(const uint32_t* w) : w0(w[0]), w1(w[1]) {}
-  __device__ __forceinline__ float at(int j) const {
-    return (float)(((j < 4 ? w0 : w1) >> (8 * (j & 3))) & 0xffu);
-  }
+struct Q4<8> {
+  uint32_t w;
+  __device__ __forceinline__ explicit Q4(uint32_t v, int) : w(v) {}
+  __device__ __forceinline__ float at(int j) const { return (float)((w >> (8 * j)) & 0xffu); }
 };
 
-template <int BM, int BITS, bool G32, bool NN>
-__global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
-  using C = GradCfg<BM>;
-  constexpr int WN = C::WN, MI = C::MI, NJ = C::NJ;
-  constexpr int WPU = BITS / 4;              // words of 8 values
-  constexpr int XI = BM / 32;                // A DMA instructions per wave and step
-  constexpr int NSB = G32 ? 4 : 2;           // scale and bias loads per thread and step
-  constexpr int NLD = (NN ? 8 : 2 * WPU) + NSB;  // loads per thread and step
+template <int BM, int BN, int BITS, bool G32, bool NN>
+__global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kernel(GradGemm g) {
+  using C = GradCfg<BM, BN>;
+  constexpr int W = C::W, WN = C::WN, MI = C::MI, NJ = C::NJ, CB = C::CB;
+  constexpr int XI = BM / (8 * W);           // A DMA instructions per wave and step
+  static_assert(XI * 8 * W == BM, "the waves' DMA instructions fill the rows");
+  constexpr int NSB = NN && G32 ? 4 : 2;     // scale and bias loads per thread and step
+  constexpr int NW = NN ? 8 : 4 * (BITS / 4);  // packed words per thread and step
+  constexpr int NLD = (NN ? 8 : BITS / 4) + NSB;  // loads per thread and step
+  // Each stage an LDS object of its own, so that the compiler can tell a DMA's target from
+  // the reads of another stage.
   __shared__ __attribute__((aligned(1024))) uint8_t as0[BM * 128];
   __shared__ __attribute__((aligned(1024))) uint8_t as1[BM * 128];
-  __shared__ __attribute__((aligned(1024))) uint8_t bs0[kN * 128];
-  __shared__ __attribute__((aligned(1024))) uint8_t bs1[kN * 128];
-  __shared__ __attribute__((aligned(16))) uint32_t sbx[NN ? 4 * 64 * (G32 ? 2 : 1) : 4];
+  __shared__ __attribute__((aligned(1024))) uint8_t bs0[BN * 128];
+  __shared__ __attribute__((aligned(1024))) uint8_t bs1[BN * 128];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -71,25 +154,36 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
 
   // Tile of this block: row tiles fastest, so that the blocks of one XCD (every eighth)
   // share weight columns.
-  const int64_t tn = (g.N + kN - 1) / kN;
-  const int64_t tm = g.tiles ? g.max_tiles : (g.M + BM - 1) / BM;
-  const int64_t total = (int64_t)gridDim.x;
-  int64_t b = blockIdx.x;
+  const int tn = (int)((g.N + BN - 1) / BN);
+  const int tm = (int)(g.offsets ? g.max_tiles : (g.M + BM - 1) / BM);
+  const uint32_t total = gridDim.x;
+  uint32_t b = blockIdx.x;
   if ((total & 7) == 0) b = (b & 7) * (total >> 3) + (b >> 3);
-  const int64_t split = b / (tm * tn);
-  b -= split * tm * tn;
-  const int64_t mt = b % tm, nt = b / tm;
+  const uint32_t split = b / ((uint32_t)tm * tn);
+  b -= split * ((uint32_t)tm * tn);
+  const int64_t mt = b % (uint32_t)tm, nt = b / (uint32_t)tm;
   int64_t m0 = mt * BM, rows = g.M - m0 < BM ? g.M - m0 : BM;
-  const int64_t n0 = nt * kN;
+  const int64_t n0 = nt * BN;
   const uint32_t* w = g.w;
   const uint16_t *scales = g.scales, *biases = g.biases;
+  const int gs = __builtin_ctz(g.group_size);
   const int64_t wk = NN ? g.N : g.C;             // values of a weight row
-  const int64_t wpr = wk * BITS / 32, gpr = wk / g.group_size;
-  if (NN && g.tiles) {
-    if (mt >= (int64_t)*g.ntile) return;
-    m0 = g.tiles[3 * mt];
-    rows = g.tiles[3 * mt + 1];
-    const int64_t e = g.tiles[3 * mt + 2];
+  const int64_t wpr = wk * BITS / 32, gpr = wk >> gs;
+  if (NN && g.offsets) {
+    int64_t e, spare, spares, lo, hi;
+    rows = run_tile<C::W * 64>(g, mt, BM, &m0, &e, &spare, &spares, &lo, &hi);
+    if (rows == 0) {
+      // The tiles behind the last one zero the rows of no expert.
+      const int64_t units = (g.N - n0 < BN ? g.N - n0 : BN) / 8;
+      for (int64_t i = tid + spare * (C::W * 64); i < (lo + g.M - hi) * units;
+           i += spares * (C::W * 64)) {
+        int64_t r = i / units;
+        const int64_t c = i - r * units;
+        if (r >= lo) r += hi - lo;
+        *reinterpret_cast<u32x4*>(g.y + r * g.ldy + n0 + 8 * c) = u32x4{0u, 0u, 0u, 0u};
+      }
+      return;
+    }
     w += e * g.C * wpr;
     scales += e * g.C * gpr;
     biases += e * g.C * gpr;
@@ -101,22 +195,22 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
   auto as = [&](int st) -> uint8_t* { return st == 0 ? as0 : as1; };
   auto bs = [&](int st) -> uint8_t* { return st == 0 ? bs0 : bs1; };
 
-  // ---- A: wave w, instruction i fills rows 8 (XI w + i) .. + 8 of the stage.
+  // ---- A: instruction i of a wave fills rows 8 (XI wave + i) .. + 8 of the stage.
   const __amdgpu_buffer_rsrc_t ares = rsrc(g.a + m0 * g.lda, rows * g.lda * 2);
   uint32_t ao[XI], ac[XI];
 #pragma unroll
   for (int i = 0; i < XI; ++i) {
     const int row = 8 * (XI * wave + i) + (lane >> 3);
-    ac[i] = ((lane & 7) ^ swz(row)) * 8;
-    ao[i] = row < rows ? (uint32_t)(row * g.lda * 2) : 0xffffffffu;
+    ac[i] = ((lane & 7) ^ swz8(row)) * 8;
+    ao[i] = row < rows ? (uint32_t)(row * g.lda * 2) : 0x7ffffff0u;
   }
+  const uint32_t acols = (uint32_t)g.a_cols;
   auto issue_a = [&](int k, int st) {
-    const int64_t kc = c0 + (int64_t)k * kS;
+    const uint32_t kc = (uint32_t)c0 + (uint32_t)k * kS;
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
-      const uint32_t off = (ao[i] != 0xffffffffu && kc + ac[i] < g.a_cols && k < nk)
-                               ? ao[i] + (uint32_t)(kc + ac[i]) * 2
-                               : 0x7ffffff0u;
+      const uint32_t col = kc + ac[i];
+      const uint32_t off = col < acols && k < nk ? ao[i] + col * 2 : 0x7ffffff0u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lds_t*)(as(st) + 8 * (XI * wave + i) * 128),
                                                16, (int)off, 0, 0, 0);
     }
@@ -124,108 +218,108 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
 
   // ---- B: packed words and scales of a step in registers.
   struct Packed {
-    uint32_t w[8 * WPU];
+    uint32_t w[NW];
     uint16_t s[NSB / 2], b[NSB / 2];
   };
   Packed pk[2];
-  const int q = lane & 7, c = lane >> 3;  // nn: rows 8 q .. + 8, word column c of the wave's 8
+  // nn: wave (column block, half word); lane: rows 8 q .. + 8, word column c.
+  const int cb = wave % CB, half = wave / CB, q = lane >> 3, c = lane & 7;
+  // nt: row (token) tid % BN, its contraction half tid / BN.
+  const int trow = tid % BN, kh = tid / BN;
+  uint32_t wo, so;
+  if constexpr (NN) {
+    // Columns past the weight's last are clamped into its rows; they are not stored.
+    const int64_t u = n0 / 8 + 8 * cb + c;
+    const int unit = (int)(u < wk / 8 ? u : wk / 8 - 1);
+    wo = (uint32_t)(8 * q * wpr * 4 + unit * BITS + (BITS == 8 ? 4 * half : 0));
+    so = (uint32_t)(((8 * q + (G32 ? c & 3 : c)) * gpr + (unit * 8 >> gs)) * 2);
+  } else {
+    wo = (uint32_t)(trow * wpr * 4);
+    so = (uint32_t)(trow * gpr * 2);
+  }
+  const int64_t nrows = g.N - n0 < BN ? g.N - n0 : BN;
   auto issue_b = [&](int k, Packed& p) {
     const int64_t kc = c0 + (int64_t)k * kS;
     if constexpr (NN) {
       const int64_t left = k < nk ? (c1 - kc < kS ? c1 - kc : kS) : 0;
-      const int64_t col = n0 + 64 * wave;
-      // Columns past the weight's last are clamped into its rows; they are not stored.
-      const int64_t wcol = col / 8 + c < wk / 8 ? col / 8 + c : wk / 8 - 1;
       const __amdgpu_buffer_rsrc_t wr = rsrc(w + kc * wpr, left * wpr * 4);
-      const uint32_t o = (uint32_t)((8 * q) * wpr * 4 + wcol * WPU * 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int oi = (int)(o + (uint32_t)(i * wpr * 4));
-        if constexpr (WPU == 1) {
-          p.w[i] = __builtin_amdgcn_raw_buffer_load_b32(wr, oi, 0, 0);
-        } else {
-          const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(wr, oi, 0, 0));
-          p.w[2 * i] = v[0];
-          p.w[2 * i + 1] = v[1];
-        }
-      }
+      for (int i = 0; i < 8; ++i)
+        p.w[i] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)(wo + (uint32_t)(i * wpr * 4)), 0, 0);
       const __amdgpu_buffer_rsrc_t sr = rsrc(scales + kc * gpr, left * gpr * 2);
       const __amdgpu_buffer_rsrc_t br = rsrc(biases + kc * gpr, left * gpr * 2);
 #pragma unroll
       for (int i = 0; i < NSB / 2; ++i) {
-        int64_t grp = (col + 32 * i) / g.group_size;
-        if (grp > gpr - 1) grp = gpr - 1;
-        const int so = (int)((lane * gpr + grp) * 2);
-        p.s[i] = __builtin_amdgcn_raw_buffer_load_b16(sr, so, 0, 0);
-        p.b[i] = __builtin_amdgcn_raw_buffer_load_b16(br, so, 0, 0);
+        const int o = (int)(so + (uint32_t)(4 * i * gpr * 2));
+        p.s[i] = __builtin_amdgcn_raw_buffer_load_b16(sr, o, 0, 0);
+        p.b[i] = __builtin_amdgcn_raw_buffer_load_b16(br, o, 0, 0);
       }
     } else {
-      const int64_t nrows = g.N - n0 < kN ? g.N - n0 : kN;
+      // A half step past the row's end takes the row's last values against zeros of A.
+      const int kq = (int)(kc + 32 * kh < wk ? kc + 32 * kh : wk - 32);
       const __amdgpu_buffer_rsrc_t wr = rsrc(w + n0 * wpr, nrows * wpr * 4);
-      const uint32_t o = (uint32_t)(tid * wpr * 4 + kc / 8 * WPU * 4);
 #pragma unroll
-      for (int i = 0; i < 2 * WPU; ++i) {
-        const u32x4 v =
-            __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, (int)o + 16 * i, 0, 0));
+      for (int i = 0; i < NW / 4; ++i) {
+        const u32x4 v = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, (int)(wo + kq * BITS / 8), 16 * i, 0));
 #pragma unroll
         for (int j = 0; j < 4; ++j) p.w[4 * i + j] = v[j];
       }
       const __amdgpu_buffer_rsrc_t sr = rsrc(scales + n0 * gpr, nrows * gpr * 2);
       const __amdgpu_buffer_rsrc_t br = rsrc(biases + n0 * gpr, nrows * gpr * 2);
-#pragma unroll
-      for (int i = 0; i < NSB / 2; ++i) {
-        // A step past the row's end takes the row's last group: finite weights against
-        // zeros of A.
-        int64_t grp = (kc + 32 * i) / g.group_size;
-        if (grp > gpr - 1) grp = gpr - 1;
-        const int so = (int)((tid * gpr + grp) * 2);
-        p.s[i] = __builtin_amdgcn_raw_buffer_load_b16(sr, so, 0, 0);
-        p.b[i] = __builtin_amdgcn_raw_buffer_load_b16(br, so, 0, 0);
-      }
+      const int o = (int)(so + 2 * (kq >> gs));
+      p.s[0] = __builtin_amdgcn_raw_buffer_load_b16(sr, o, 0, 0);
+      p.b[0] = __builtin_amdgcn_raw_buffer_load_b16(br, o, 0, 0);
     }
   };
-  // nn: the scales and biases of the wave's 64 rows, one pair a word, through LDS.
-  uint32_t sb8[8];
-  auto share_sb = [&](const Packed& p) {
+  // nn: lane c of an octet holds the scale and bias of row 8 q + c (rows c & 3 and + 4 of its
+  // half octet's group in groups of 32) and the others take them from there.
+  uint32_t rs[8];
+  auto share = [&](const Packed& p) {
+    if constexpr (NN) {
+      uint32_t sb[NSB / 2];
+#pragma unroll
+      for (int i = 0; i < NSB / 2; ++i) sb[i] = (uint32_t)p.s[i] | ((uint32_t)p.b[i] << 16);
+      auto from = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        constexpr int pattern = G32 ? (0x1c | ((i & 3) << 5)) : (0x18 | (i << 5));
+        rs[i] = (uint32_t)__builtin_amdgcn_ds_swizzle((int)sb[G32 ? i >> 2 : 0], pattern);
+      };
+      from(std::integral_constant<int, 0>{});
+      from(std::integral_constant<int, 1>{});
+      from(std::integral_constant<int, 2>{});
+      from(std::integral_constant<int, 3>{});
+      from(std::integral_constant<int, 4>{});
+      from(std::integral_constant<int, 5>{});
+      from(std::integral_constant<int, 6>{});
+      from(std::integral_constant<int, 7>{});
+    }
+  };
+  // Quarter t of the thread's weights: one 16-byte chunk of the stage.
+  auto dequant = [&](const Packed& p, int st, int t) {
+    u32x4 o;
+    int row, chunk;
     if constexpr (NN) {
 #pragma unroll
-      for (int i = 0; i < NSB / 2; ++i)
-        sbx[(wave * (NSB / 2) + i) * 64 + lane] = (uint32_t)p.s[i] | ((uint32_t)p.b[i] << 16);
-      const int half = G32 ? c >> 2 : 0;
-      const u32x4* v = reinterpret_cast<const u32x4*>(sbx + (wave * (NSB / 2) + half) * 64 + 8 * q);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sb8[4 * i + j] = v[i][j];
-    }
-  };
-  // Quarter t of the step's weights: two 16-byte chunks of the stage.
-  auto dequant = [&](const Packed& p, int st, int t) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int j = 2 * t + u;
-      u32x4 o;
-      int row, chunk;
-      if constexpr (NN) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const Q8<BITS> q0(p.w + 2 * i * WPU), q1(p.w + (2 * i + 1) * WPU);
-          o[i] = deq_pair(q0.at(j), q1.at(j), bf16_lo(sb8[2 * i]), bf16_lo(sb8[2 * i + 1]),
-                          bf16_hi(sb8[2 * i]), bf16_hi(sb8[2 * i + 1]));
-        }
-        row = 64 * wave + 8 * c + j;
-        chunk = q;
-      } else {
-        const float s = bf16_bits_to_f32(p.s[G32 ? j >> 2 : 0]);
-        const float bb = bf16_bits_to_f32(p.b[G32 ? j >> 2 : 0]);
-        const Q8<BITS> qq(p.w + j * WPU);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = deq_pair(qq.at(2 * i), qq.at(2 * i + 1), s, s, bb, bb);
-        row = tid;
-        chunk = j;
+      for (int i = 0; i < 4; ++i) {
+        const Q4<BITS> a(p.w[2 * i], half), z(p.w[2 * i + 1], half);
+        o[i] = deq_pair(a.at(t), z.at(t), bf16_lo(rs[2 * i]), bf16_lo(rs[2 * i + 1]),
+                        bf16_hi(rs[2 * i]), bf16_hi(rs[2 * i + 1]));
       }
-      *reinterpret_cast<u32x4*>(bs(st) + row * 128 + ((chunk ^ swz(row)) << 4)) = o;
+      row = 64 * cb + 8 * c + 4 * half + t;
+      chunk = q;
+    } else {
+      const float s = bf16_bits_to_f32(p.s[0]), bb = bf16_bits_to_f32(p.b[0]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Q4<BITS> v(BITS == 4 ? p.w[t] : p.w[2 * t + i], i);
+        o[2 * i] = deq_pair(v.at(0), v.at(1), s, s, bb, bb);
+        o[2 * i + 1] = deq_pair(v.at(2), v.at(3), s, s, bb, bb);
+      }
+      row = trow;
+      chunk = 4 * kh + t;
     }
+    *reinterpret_cast<u32x4*>(bs(st) + row * 128 + ((chunk ^ swz8(row)) << 4)) = o;
   };
 
   f32x16 acc[MI][NJ];
@@ -236,59 +330,83 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  // Fragment of sub-step s: row r32 of a 32-row group, chunk 2 s + h.
-  uint32_t fo[4];
+  // Fragment of sub-step s in a 32-row group: row r32, chunk 2 s + h; the group's parity
+  // flips the position's highest bit.
+  uint32_t fo[2][4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) fo[s] = r32 * 128 + (((2 * s + h) ^ swz(r32)) << 4);
-
-  // Step k, staged in st: the next step's A and the packed weights of the one after are
-  // requested, then the MFMAs run with the next step's dequantization between them.
-  auto step = [&](int k, auto stc) {
-    constexpr int st = decltype(stc)::value;
-    issue_a(k + 1, st ^ 1);
-    __builtin_amdgcn_sched_barrier(0);
-    issue_b(k + 2, pk[st]);
-    __builtin_amdgcn_sched_barrier(0);
-    share_sb(pk[st ^ 1]);
+  for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      bf16x8 af[MI], bf[NJ];
+    for (int s = 0; s < 4; ++s)
+      fo[p][s] = r32 * 128 + (((2 * s + h) ^ swz8(32 * p + r32)) << 4);
+  auto frag = [&](const uint8_t* stage, int group0, int i, int s) {
+    const int par = (group0 + i) & 1;  // group0 is even unless a wave has one group
+    return *reinterpret_cast<const bf16x8*>(stage + (group0 + i) * 4096 + fo[par][s]);
+  };
+  bf16x8 a0[MI], a1[MI], b0[NJ], b1[NJ];
+  auto read = [&](bf16x8 (&af)[MI], bf16x8 (&bf)[NJ], int st, int s) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
-        af[i] = *reinterpret_cast<const bf16x8*>(as(st) + (wm * MI + i) * 4096 + fo[s]);
+    for (int j = 0; j < NJ; ++j) bf[j] = frag(bs(st), wn * NJ, j, s);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) af[i] = frag(as(st), wm * MI, i, s);
+  };
+  auto mfmas = [&](const bf16x8 (&af)[MI], const bf16x8 (&bf)[NJ]) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
-        bf[j] = *reinterpret_cast<const bf16x8*>(bs(st) + (wn * NJ + j) * 4096 + fo[s]);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
-      dequant(pk[st ^ 1], st ^ 1, s);
-    }
-    // The next step's A has landed (only the packed loads of the step after it are
-    // younger) and its weights are written.
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
+  };
+  // Step k, staged in st; the weights of step k + 1 (set st ^ 1) go to the other stage, their
+  // first chunk during the step before.
+  auto step = [&](int k, auto stc) {
+    constexpr int st = decltype(stc)::value;
+    read(a1, b1, st, 1);
+    mfmas(a0, b0);
+    dequant(pk[st ^ 1], st ^ 1, 1);
+    read(a0, b0, st, 2);
+    mfmas(a1, b1);
+    dequant(pk[st ^ 1], st ^ 1, 2);
+    read(a1, b1, st, 3);
+    mfmas(a0, b0);
+    dequant(pk[st ^ 1], st ^ 1, 3);
+    // Step k + 1's A has landed (only the packed loads of step k + 2 are younger), its weights
+    // are written, and this stage is read.
     __builtin_amdgcn_s_waitcnt(wait_enc(NLD, 0));
     __builtin_amdgcn_s_barrier();
+    issue_a(k + 2, st);
+    __builtin_amdgcn_sched_barrier(0);
+    issue_b(k + 3, pk[st ^ 1]);
+    __builtin_amdgcn_sched_barrier(0);
+    read(a0, b0, st ^ 1, 0);
+    share(pk[st]);
+    mfmas(a1, b1);
+    dequant(pk[st], st, 0);
   };
   if (nk > 0) {
-    issue_a(0, 0);
     issue_b(0, pk[0]);
+    issue_a(0, 0);
+    __builtin_amdgcn_sched_barrier(0);  // the waits count on this order
     issue_b(1, pk[1]);
-    share_sb(pk[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    share(pk[0]);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) dequant(pk[0], 0, s);
-    __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
+    for (int t = 0; t < 4; ++t) dequant(pk[0], 0, t);
+    __builtin_amdgcn_s_waitcnt(wait_enc(NLD, 0));
     __builtin_amdgcn_s_barrier();
-    int k = 0;
-    for (; k + 1 < nk; k += 2) {
+    issue_a(1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    issue_b(2, pk[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    read(a0, b0, 0, 0);
+    share(pk[1]);
+    dequant(pk[1], 1, 0);
+    // Two steps a turn, the last one on zeros where nk is odd.
+    for (int k = 0; k < nk; k += 2) {
       step(k, std::integral_constant<int, 0>{});
       step(k + 1, std::integral_constant<int, 1>{});
     }
-    if (k < nk) step(k, std::integral_constant<int, 0>{});
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
   }
-
   const int64_t mw = m0 + wm * MI * 32, nw = n0 + wn * NJ * 32;
   if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
   else store_stats<MI, NJ>(g, acc, mw, m0 + rows, nw);
@@ -296,36 +414,38 @@ __global__ __launch_bounds__(256, 1) void grad_gemm_kernel(GradGemm g) {
 
 template <int BM, bool NN>
 hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
-  const int64_t tn = (g.N + kN - 1) / kN, tm = g.tiles ? g.max_tiles : (g.M + BM - 1) / BM;
+  constexpr int BN = NN ? kGradCols : kLogitCols;
+  const int64_t tn = (g.N + BN - 1) / BN, tm = g.offsets ? g.max_tiles : (g.M + BM - 1) / BM;
   const int64_t blocks = tm * tn * g.splits;
   if (blocks < 1) return hipSuccess;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks), block(256);
+  const dim3 grid((unsigned)blocks), block(BN * 2);
+  const bool g32 = NN && g.group_size == 32;
   if (g.bits == 4) {
-    if (g.group_size == 32) grad_gemm_kernel<BM, 4, true, NN><<<grid, block, 0, stream>>>(g);
-    else grad_gemm_kernel<BM, 4, false, NN><<<grid, block, 0, stream>>>(g);
+    if (g32) grad_gemm_kernel<BM, BN, 4, NN, NN><<<grid, block, 0, stream>>>(g);
+    else grad_gemm_kernel<BM, BN, 4, false, NN><<<grid, block, 0, stream>>>(g);
   } else {
-    if (g.group_size == 32) grad_gemm_kernel<BM, 8, true, NN><<<grid, block, 0, stream>>>(g);
-    else grad_gemm_kernel<BM, 8, false, NN><<<grid, block, 0, stream>>>(g);
+    if (g32) grad_gemm_kernel<BM, BN, 8, NN, NN><<<grid, block, 0, stream>>>(g);
+    else grad_gemm_kernel<BM, BN, 8, false, NN><<<grid, block, 0, stream>>>(g);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-int grad_gemm_rows(int64_t M) { return M <= 32 ? 32 : M <= 64 ? 64 : 128; }
-
-int grad_gemm_stat_width(int64_t M) { return grad_gemm_rows(M) >= 128 ? 128 : 64; }
+int grad_gemm_rows(int64_t M, bool nn) { return M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 || nn ? 128 : 256; }
 
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream) {
   // Offsets into one tile's rows and into 64 or 256 weight rows are 32 bits.
-  if (128 * g.lda * 2 >= 0x7ffffff0LL || 256 * (nn ? g.N : g.C) >= 0x7ffffff0LL || g.c_split % kS ||
-      g.lda % 8 || g.a_cols % 8)
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats) || 256 * g.lda * 2 >= 0x7ffffff0LL ||
+      256 * (nn ? g.N : g.C) >= 0x7ffffff0LL || g.c_split % kS || g.lda % 8 || g.a_cols % 8 ||
+      (g.offsets && (!nn || !g.y || !g.flag || g.splits != 1)))
     return hipErrorInvalidValue;
   switch (bm) {
-    case 32: return nn ? launch_bm<32, true>(g, stream) : launch_bm<32, false>(g, stream);
-    case 64: return nn ? launch_bm<64, true>(g, stream) : launch_bm<64, false>(g, stream);
+    case 32: return nn ? launch_bm<32, true>(g, stream) : hipErrorInvalidValue;
+    case 64: return nn ? launch_bm<64, true>(g, stream) : hipErrorInvalidValue;
     case 128: return nn ? launch_bm<128, true>(g, stream) : launch_bm<128, false>(g, stream);
+    case 256: return nn ? hipErrorInvalidValue : launch_bm<256, false>(g, stream);
   }
   return hipErrorInvalidValue;
 }
@@ -366,68 +486,6 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restric
   }
 }
 
-// One block: the offsets are checked, then each thread cuts a range of experts' runs.
-__global__ __launch_bounds__(1024) void run_tiles_kernel(const int32_t* __restrict__ offsets,
-                                                         int64_t E, int64_t S, int bm,
-                                                         uint32_t* __restrict__ tiles,
-                                                         uint32_t* __restrict__ ntile,
-                                                         uint32_t* flag) {
-  __shared__ uint32_t wsum[16], bad;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (tid == 0) bad = 0;
-  __syncthreads();
-  for (int64_t e = tid; e <= E; e += 1024) {
-    const int64_t o = offsets[e];
-    if (o < 0 || o > S || (e > 0 && o < offsets[e - 1])) bad = 1;
-  }
-  __syncthreads();
-  if (bad) {
-    if (tid == 0) {
-      *ntile = 0;
-      atomicOr(flag, 1u);
-    }
-    return;
-  }
-  const int64_t per = (E + 1023) / 1024;
-  const int64_t e0 = tid * per < E ? tid * per : E, e1 = e0 + per < E ? e0 + per : E;
-  uint32_t n = 0;
-  for (int64_t e = e0; e < e1; ++e) n += (uint32_t)((offsets[e + 1] - offsets[e] + bm - 1) / bm);
-  uint32_t inc = n;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t t = (uint32_t)__shfl_up((int)inc, o, 64);
-    if (lane >= o) inc += t;
-  }
-  if (lane == 63) wsum[wave] = inc;
-  __syncthreads();
-  uint32_t at = inc - n;
-  for (int i = 0; i < wave; ++i) at += wsum[i];
-  if (tid == 1023) *ntile = at + n;
-  for (int64_t e = e0; e < e1; ++e)
-    for (int64_t r = offsets[e]; r < offsets[e + 1]; r += bm, ++at) {
-      const int64_t left = offsets[e + 1] - r;
-      tiles[3 * at] = (uint32_t)r;
-      tiles[3 * at + 1] = (uint32_t)(left < bm ? left : bm);
-      tiles[3 * at + 2] = (uint32_t)e;
-    }
-}
-
-// Rows before the first run and behind the last (all of them where the offsets are bad, which
-// run_tiles_kernel shows by listing no tile).
-__global__ __launch_bounds__(256) void zero_uncovered_kernel(const int32_t* __restrict__ offsets,
-                                                             int64_t E, int64_t S,
-                                                             const uint32_t* __restrict__ ntile,
-                                                             uint16_t* __restrict__ dx, int64_t N) {
-  const bool none = *ntile == 0;
-  const int64_t lo = none ? S : offsets[0], hi = none ? S : offsets[E];
-  const int64_t units = N / 8, n = (lo + S - hi) * units;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    int64_t r = i / units;
-    const int64_t c = i - r * units;
-    if (r >= lo) r += hi - lo;
-    *reinterpret_cast<u32x4*>(dx + r * N + 8 * c) = u32x4{0u, 0u, 0u, 0u};
-  }
-}
-
 unsigned blocks_for(int64_t items, int64_t per, int64_t most) {
   const int64_t b = (items + per - 1) / per;
   return (unsigned)(b < 1 ? 1 : b < most ? b : most);
@@ -444,15 +502,6 @@ hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64
 hipError_t launch_pad_rows(const uint16_t* src, uint16_t* dst, int64_t M, int64_t N, int64_t ld,
                            hipStream_t stream) {
   pad_rows_kernel<<<blocks_for(M * ld / 8, 256, 8192), 256, 0, stream>>>(src, dst, M, N, ld);
-  return hipGetLastError();
-}
-
-hipError_t launch_run_tiles(const int32_t* offsets, int64_t E, int64_t S, int bm, uint32_t* tiles,
-                            uint32_t* ntile, uint16_t* dx, int64_t N, uint32_t* flag,
-                            hipStream_t stream) {
-  run_tiles_kernel<<<1, 1024, 0, stream>>>(offsets, E, S, bm, tiles, ntile, flag);
-  if (hipError_t e = hipGetLastError()) return e;
-  zero_uncovered_kernel<<<256, 256, 0, stream>>>(offsets, E, S, ntile, dx, N);
   return hipGetLastError();
 }
 

@@ -142,6 +142,7 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   };
   if (nk > 0) {
     issue(0, 0);
+    __builtin_amdgcn_sched_barrier(0);  // the wait counts on this order
     issue(1, 1);
     __builtin_amdgcn_s_waitcnt(wait_enc(XI + YI, 15));
     __builtin_amdgcn_s_barrier();
@@ -205,8 +206,8 @@ __global__ __launch_bounds__(256) void dequant_transposed_kernel(
 }  // namespace
 
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (kPanelRows * g.lda * 2 >= 0x7ffffff0LL || kN * g.ldp * 2 >= 0x7ffffff0LL || g.c_split % kS ||
-      g.lda % 8 || g.a_cols % 8 || g.ldp % 8 || g.tiles)
+  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats) || kPanelRows * g.lda * 2 >= 0x7ffffff0LL || kN * g.ldp * 2 >= 0x7ffffff0LL || g.c_split % kS ||
+      g.lda % 8 || g.a_cols % 8 || g.ldp % 8 || g.offsets)
     return hipErrorInvalidValue;
   const int64_t blocks = (g.M + kPanelRows - 1) / kPanelRows * ((g.N + kN - 1) / kN) * g.splits;
   if (blocks < 1) return hipSuccess;

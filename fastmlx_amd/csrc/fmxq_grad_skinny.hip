@@ -335,7 +335,8 @@ bool skinny_gemm_supported(int64_t M, int64_t lda, int64_t weight_rows, int64_t 
 }
 
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!skinny_gemm_supported(g.M, g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.tiles || g.lda % 8 ||
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats) ||
+      !skinny_gemm_supported(g.M, g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.offsets || g.lda % 8 ||
       g.a_cols % 8 || g.c_split % 16)
     return hipErrorInvalidValue;
   if (g.M < 1 || g.N < 1 || g.splits < 1) return hipSuccess;

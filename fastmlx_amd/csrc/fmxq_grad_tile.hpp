@@ -21,9 +21,16 @@ __device__ __forceinline__ constexpr int wait_enc(int vm, int lgkm) {
   return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8);
 }
 
+// A buffer of `bytes` at p, both the same in every lane.  They pass through readfirstlane
+// because the compiler may hold a uniform value in vector registers, and then loops over the
+// lanes' resources at every load.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t bytes) {
   const int64_t b = bytes < 0 ? 0 : bytes < 0x7fffffff ? bytes : 0x7fffffff;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)b, 0x00020000);
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), (short)0,
+                                           __builtin_amdgcn_readfirstlane((int)b), 0x00020000);
 }
 
 // dequantize's value: bf16(bf16(q s) + b), two at a time (low half first).  The empty asm hides

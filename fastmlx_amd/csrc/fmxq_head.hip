@@ -285,28 +285,32 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // Most bytes of a piece's e, and of its panel of dequantized weights.
 constexpr int64_t kHeadPieceBytes = 256 << 20;
 constexpr int64_t kHeadPanelBytes = 256 << 20;
-// Rows from which the weights are dequantized to panels beforehand.
-constexpr int64_t kHeadPanelRows = 256;
+// Rows from which the weights are dequantized to panels beforehand, for the logits and for the
+// gradient.
+constexpr int64_t kHeadPanelRows = 1001;
+constexpr int64_t kHeadGradPanelRows = 257;
 
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
   p.panel = M >= kHeadPanelRows;
-  p.bm = p.panel ? kPanelRows : grad_gemm_rows(M);
+  p.grad_panel = grad && M >= kHeadGradPanelRows;
+  p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M, false), 128);
+  p.grad_bm = p.grad_panel ? kPanelRows : std::max(grad_gemm_rows(M, true), 128);
   int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
-  if (p.panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
+  if (p.panel || p.grad_panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
   p.pieces = (int)((V + piece - 1) / piece);
   piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
   p.pieces = (int)((V + piece - 1) / piece);
   p.piece = piece;
   p.skinny = skinny_gemm_supported(M, std::max(K, piece), piece, K);
-  p.stat_width = p.skinny ? kSkinnyStatWidth : p.panel ? kPanelStatWidth : grad_gemm_stat_width(M);
+  p.stat_width = p.skinny ? kSkinnyStatWidth : p.panel ? kPanelStatWidth : kGradStatWidth;
   // Without a gradient the tiles of all pieces are joined at once.
   p.stat_tiles = (grad ? piece : up(V, kGradTileCols)) / p.stat_width;
   // Parts of the gradient product's contraction: enough blocks for the chip, each walking
   // 256 tokens at least.
-  const int64_t cols = p.skinny ? kSkinnyCols : kGradTileCols;
-  const int64_t tiles = (p.skinny ? 1 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
-  const int64_t want = (p.bm >= 128 ? cus : 2 * cus) / tiles;
+  const int64_t cols = p.skinny ? kSkinnyCols : p.grad_panel ? kGradTileCols : kGradCols;
+  const int64_t tiles = (p.skinny ? 1 : (M + p.grad_bm - 1) / p.grad_bm) * ((K + cols - 1) / cols);
+  const int64_t want = (p.grad_panel ? cus : 2 * cus) / tiles;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, piece / 256));
   p.c_split = up((piece + p.splits - 1) / p.splits, 64);
   size_t at = 0;
@@ -323,7 +327,7 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
     p.e = take(M * piece * 2);
     p.slices = take((int64_t)p.splits * M * K * 4);
   }
-  if (p.panel) p.panel_at = take(piece * K * 2);
+  if (p.panel || p.grad_panel) p.panel_at = take(piece * K * 2);
   if (p.skinny) p.xp = take(skinny_pack_bytes(M, K));
   p.bytes = at;
   return p;
@@ -338,7 +342,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   uint16_t* e = a.dh ? reinterpret_cast<uint16_t*>(base + p.e) : nullptr;
   float* slices = a.dh ? reinterpret_cast<float*>(base + p.slices) : nullptr;
   const float scale = kLog2e / a.temperature;
-  uint16_t* panel = p.panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
+  uint16_t* panel = p.panel || p.grad_panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
   // (in, out): the running state before and after the pieces joined so far.
   auto join = [&](int i, int64_t v0, int64_t n, int64_t lde) {
     const int64_t chunks = (lde + kJoinCols - 1) / kJoinCols, shares = (a.k + 3) / 4;
@@ -393,14 +397,15 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     d.c_split = p.c_split;
     d.out = slices;
     d.factor = i ? factor : nullptr;
-    if (p.panel) {
+    if (p.grad_panel) {
+      d.panel = panel;
       d.C = d.ldp = up(n, 8);
       if (hipError_t r = launch_dequant_transposed(g.w, g.scales, g.biases, panel, n, a.K, d.ldp,
                                                    a.group_size, a.bits, stream))
         return r;
       if (hipError_t r = launch_panel_gemm(d, true, stream)) return r;
     } else if (hipError_t r = p.skinny ? launch_skinny_gemm(d, true, stream)
-                                       : launch_grad_gemm(d, true, p.bm, stream)) {
+                                       : launch_grad_gemm(d, true, p.grad_bm, stream)) {
       return r;
     }
   }
