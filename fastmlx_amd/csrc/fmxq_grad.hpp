@@ -59,9 +59,9 @@ int grad_gemm_rows(int64_t M, bool nn);
 constexpr int kGradStatWidth = 64;  // columns of a tile of the statistics (128 rows and more)
 constexpr int kGradTileCols = 256;
 constexpr int kLogitCols = 256, kGradCols = 128;  // of launch_grad_gemm's tiles
-// Tiles of bm rows that cover any runs of S rows, and one more that none does.
+// Tiles of bm rows that cover any runs of S rows and one more that none does, in eights.
 inline int64_t grad_gemm_run_tiles(int64_t S, int64_t E, int bm) {
-  return S / bm + (E < S ? E : S) + 1;
+  return (S / bm + (E < S ? E : S) + 8) / 8 * 8;
 }
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
 

@@ -10,7 +10,7 @@
 // buffer_load ... lds; the packed weights go global -> registers some steps ahead, are
 // dequantized there to fmxq_dequantize's bits and written to LDS.  Both stages hold rows of
 // 64 contraction values (128 bytes), so one fragment read serves both forms: where the
-// weights are packed along the outputs (nn), a thread takes 8 rows of half a word column, and
+// weights are packed along the outputs (nn), a thread takes 4 rows of 8 columns, and
 // the transposition costs nothing: the roundings pack any two values.
 //
 // The barrier of a step sits before its last quarter's MFMAs, when every wave has read the
@@ -43,13 +43,13 @@ struct GradCfg {
 // rows and expert, or rows = 0 behind the last tile.  Then *spare is the number of tiles
 // behind the last one up to and with this one, of *spares in all, and rows *lo .. *hi are
 // what the runs cover (nothing where the offsets decrease or leave 0 .. S).  All threads of
-// the block take part, each in a range of experts.
+// the block take part, each in a range of experts; lds: T / 64 + 4 words.
 template <int T>
 __device__ __forceinline__ int64_t run_tile(const GradGemm& g, int64_t mt, int BM, int64_t* m0,
                                             int64_t* expert, int64_t* spare, int64_t* spares,
-                                            int64_t* lo, int64_t* hi) {
-  __shared__ uint32_t wsum[T / 64];
-  __shared__ int found[3], bad;
+                                            int64_t* lo, int64_t* hi, int* lds) {
+  uint32_t* wsum = reinterpret_cast<uint32_t*>(lds);
+  int *found = lds + T / 64, &bad = lds[T / 64 + 3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t* off = g.offsets;
   const int E = (int)g.experts, S = (int)g.M;
@@ -81,7 +81,8 @@ __device__ __forceinline__ int64_t run_tile(const GradGemm& g, int64_t mt, int B
     if (i < wave) at += wsum[i];
     all += wsum[i];
   }
-  if (bad) all = 0;
+  const int wrong = bad;
+  if (wrong) all = 0;
   else if (mt >= at && mt < at + n) {
     for (int e = e0; e < e1; ++e) {
       const int a = off[e], b = off[e + 1], k = (b - a + BM - 1) / BM;
@@ -104,20 +105,21 @@ __device__ __forceinline__ int64_t run_tile(const GradGemm& g, int64_t mt, int B
   *spares = g.max_tiles - all;
   *lo = all ? off[0] : S;
   *hi = all ? off[E] : S;
-  if (bad && blockIdx.x == 0 && tid == 0) atomicOr(g.flag, 1u);
-  return __builtin_amdgcn_readfirstlane(found[1]);
+  const int rows = __builtin_amdgcn_readfirstlane(found[1]);
+  if (wrong && blockIdx.x == 0 && tid == 0) atomicOr(g.flag, 1u);
+  __syncthreads();  // lds may be overwritten
+  return rows;
 }
 
-// Value j (0..3) of 4 packed values as a float: a byte conversion each.
+// Value j of 8 packed values as a float: a byte conversion each, after the masks.
 template <int BITS>
-struct Q4;
+struct Q8;
 template <>
-struct Q4<4> {
+struct Q8<4> {
   uint32_t e, o;
-  __device__ __forceinline__ explicit Q4(uint32_t w, int half) {
-    const uint32_t v = w >> (16 * half);
-    e = v & 0x0F0Fu;
-    o = (v >> 4) & 0x0F0Fu;
+  __device__ __forceinline__ explicit Q8(const uint32_t* w) {
+    e = w[0] & 0x0F0F0F0Fu;
+    o = (w[0] >> 4) & 0x0F0F0F0Fu;
     asm("" : "+v"(e), "+v"(o));
   }
   __device__ __forceinline__ float at(int j) const {
@@ -125,25 +127,30 @@ struct Q4<4> {
   }
 };
 template <>
-struct Q4<8> {
-  uint32_t w;
-  __device__ __forceinline__ explicit Q4(uint32_t v, int) : w(v) {}
-  __device__ __forceinline__ float at(int j) const { return (float)((w >> (8 * j)) & 0xffu); }
+struct Q8<8> {
+  uint32_t w0, w1;
+  __device__ __forceinline__ explicit Q8(const uint32_t* w) : w0(w[0]), w1(w[1]) {}
+  __device__ __forceinline__ float at(int j) const {
+    return (float)(((j < 4 ? w0 : w1) >> (8 * (j & 3))) & 0xffu);
+  }
 };
 
 template <int BM, int BN, int BITS, bool G32, bool NN>
-__global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kernel(GradGemm g) {
+__global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kernel(GradGemm g) {
   using C = GradCfg<BM, BN>;
   constexpr int W = C::W, WN = C::WN, MI = C::MI, NJ = C::NJ, CB = C::CB;
   constexpr int XI = BM / (8 * W);           // A DMA instructions per wave and step
   static_assert(XI * 8 * W == BM, "the waves' DMA instructions fill the rows");
-  constexpr int NSB = NN && G32 ? 4 : 2;     // scale and bias loads per thread and step
-  constexpr int NW = NN ? 8 : 4 * (BITS / 4);  // packed words per thread and step
-  constexpr int NLD = (NN ? 8 : BITS / 4) + NSB;  // loads per thread and step
+  constexpr int WPU = BITS / 4;              // words of 8 values
+  constexpr int NLD = (NN ? 4 : WPU) + 2;    // loads per thread and step
+  // Stages of A, and steps whose packed weights are in registers or on their way.  Three for
+  // the gradients, whose short steps (half the columns) end before memory answers.
+  constexpr int AS = NN ? 3 : 2;
   // Each stage an LDS object of its own, so that the compiler can tell a DMA's target from
   // the reads of another stage.
   __shared__ __attribute__((aligned(1024))) uint8_t as0[BM * 128];
   __shared__ __attribute__((aligned(1024))) uint8_t as1[BM * 128];
+  __shared__ __attribute__((aligned(1024))) uint8_t as2[AS > 2 ? BM * 128 : 16];
   __shared__ __attribute__((aligned(1024))) uint8_t bs0[BN * 128];
   __shared__ __attribute__((aligned(1024))) uint8_t bs1[BN * 128];
 
@@ -152,16 +159,25 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
   const int r32 = lane & 31, h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
 
-  // Tile of this block: row tiles fastest, so that the blocks of one XCD (every eighth)
-  // share weight columns.
-  const int tn = (int)((g.N + BN - 1) / BN);
-  const int tm = (int)(g.offsets ? g.max_tiles : (g.M + BM - 1) / BM);
+  // Tile of this block; every eighth block runs on one XCD.  One matrix: row tiles fastest in
+  // contiguous shares, so that the blocks of an XCD share weight columns.  Expert runs: an
+  // XCD takes every eighth row tile with all its columns, so that its rows are read once
+  // (8192 rows of 64 experts of 512 x 2048, 8 bits: 300 MB past L2 the other way).
+  const uint32_t tn = (uint32_t)((g.N + BN - 1) / BN);
+  const uint32_t tm = (uint32_t)(g.offsets ? g.max_tiles : (g.M + BM - 1) / BM);
   const uint32_t total = gridDim.x;
-  uint32_t b = blockIdx.x;
-  if ((total & 7) == 0) b = (b & 7) * (total >> 3) + (b >> 3);
-  const uint32_t split = b / ((uint32_t)tm * tn);
-  b -= split * ((uint32_t)tm * tn);
-  const int64_t mt = b % (uint32_t)tm, nt = b / (uint32_t)tm;
+  uint32_t b = blockIdx.x, split = 0;
+  int64_t mt, nt;
+  if (NN && g.offsets) {
+    mt = (b & 7) + 8 * ((b >> 3) / tn);
+    nt = (b >> 3) % tn;
+  } else {
+    if ((total & 7) == 0) b = (b & 7) * (total >> 3) + (b >> 3);
+    split = b / (tm * tn);
+    b -= split * (tm * tn);
+    mt = b % tm;
+    nt = b / tm;
+  }
   int64_t m0 = mt * BM, rows = g.M - m0 < BM ? g.M - m0 : BM;
   const int64_t n0 = nt * BN;
   const uint32_t* w = g.w;
@@ -171,7 +187,8 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
   const int64_t wpr = wk * BITS / 32, gpr = wk >> gs;
   if (NN && g.offsets) {
     int64_t e, spare, spares, lo, hi;
-    rows = run_tile<C::W * 64>(g, mt, BM, &m0, &e, &spare, &spares, &lo, &hi);
+    rows = run_tile<C::W * 64>(g, mt, BM, &m0, &e, &spare, &spares, &lo, &hi,
+                                 reinterpret_cast<int*>(as0));
     if (rows == 0) {
       // The tiles behind the last one zero the rows of no expert.
       const int64_t units = (g.N - n0 < BN ? g.N - n0 : BN) / 8;
@@ -192,25 +209,22 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
   const int64_t c1 = c0 + g.c_split < g.C ? c0 + g.c_split : g.C;
   const int nk = c1 > c0 ? (int)((c1 - c0 + kS - 1) / kS) : 0;
 
-  auto as = [&](int st) -> uint8_t* { return st == 0 ? as0 : as1; };
+  auto as = [&](int st) -> uint8_t* { return st == 0 ? as0 : st == 1 ? as1 : as2; };
   auto bs = [&](int st) -> uint8_t* { return st == 0 ? bs0 : bs1; };
 
   // ---- A: instruction i of a wave fills rows 8 (XI wave + i) .. + 8 of the stage.
+  // (Rows past the tile's lie past its buffer.)
   const __amdgpu_buffer_rsrc_t ares = rsrc(g.a + m0 * g.lda, rows * g.lda * 2);
-  uint32_t ao[XI], ac[XI];
-#pragma unroll
-  for (int i = 0; i < XI; ++i) {
-    const int row = 8 * (XI * wave + i) + (lane >> 3);
-    ac[i] = ((lane & 7) ^ swz8(row)) * 8;
-    ao[i] = row < rows ? (uint32_t)(row * g.lda * 2) : 0x7ffffff0u;
-  }
+  const int arow = 8 * XI * wave + (lane >> 3);
+  const uint32_t ao = (uint32_t)(arow * g.lda * 2), a8 = (uint32_t)(8 * g.lda * 2);
+  const uint32_t ac = ((lane & 7) ^ swz8(arow)) * 8;  // the row 8 i further flips i into it
   const uint32_t acols = (uint32_t)g.a_cols;
   auto issue_a = [&](int k, int st) {
-    const uint32_t kc = (uint32_t)c0 + (uint32_t)k * kS;
+    const uint32_t kc = (uint32_t)c0 + (uint32_t)k * kS, end = k < nk ? acols : 0u;
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
-      const uint32_t col = kc + ac[i];
-      const uint32_t off = col < acols && k < nk ? ao[i] + col * 2 : 0x7ffffff0u;
+      const uint32_t col = kc + (ac ^ (8 * ((XI * wave + i) ^ (XI * wave))));
+      const uint32_t off = col < end ? ao + i * a8 + col * 2 : 0x7ffffff0u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lds_t*)(as(st) + 8 * (XI * wave + i) * 128),
                                                16, (int)off, 0, 0, 0);
     }
@@ -218,21 +232,26 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
 
   // ---- B: packed words and scales of a step in registers.
   struct Packed {
-    uint32_t w[NW];
-    uint16_t s[NSB / 2], b[NSB / 2];
+    uint32_t w[4 * WPU];
+    uint16_t s, b;
   };
-  Packed pk[2];
-  // nn: wave (column block, half word); lane: rows 8 q .. + 8, word column c.
+  Packed pk[AS];
+  // nn: wave (column block, half); lane: rows 8 q + 4 half .. + 4, unit c of 8 columns.
   const int cb = wave % CB, half = wave / CB, q = lane >> 3, c = lane & 7;
-  // nt: row (token) tid % BN, its contraction half tid / BN.
-  const int trow = tid % BN, kh = tid / BN;
+  // nt: row (token) tid / 2, its contraction half tid % 2: a load then meets 32 rows' lines, of
+  // which two lanes take their share (half as long in the data path as 64 rows).
+  const int trow = tid >> 1, kh = tid & 1;
   uint32_t wo, so;
   if constexpr (NN) {
     // Columns past the weight's last are clamped into its rows; they are not stored.
     const int64_t u = n0 / 8 + 8 * cb + c;
     const int unit = (int)(u < wk / 8 ? u : wk / 8 - 1);
-    wo = (uint32_t)(8 * q * wpr * 4 + unit * BITS + (BITS == 8 ? 4 * half : 0));
-    so = (uint32_t)(((8 * q + (G32 ? c & 3 : c)) * gpr + (unit * 8 >> gs)) * 2);
+    wo = (uint32_t)((8 * q + 4 * half) * wpr * 4 + unit * BITS);
+    // Lane c of an octet (whose 64 columns share a group; 32 of them in groups of 32) loads a
+    // row's scale and the others take it from there.  A load of 64 rows costs the data path 64
+    // lines whatever it takes of them, so none is repeated within a wave: an octet's upper
+    // half loads the biases where the lower half's scales serve it too.
+    so = (uint32_t)(((8 * q + 4 * half + (c & 3)) * gpr + (unit * 8 >> gs)) * 2);
   } else {
     wo = (uint32_t)(trow * wpr * 4);
     so = (uint32_t)(trow * gpr * 2);
@@ -244,22 +263,27 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
       const int64_t left = k < nk ? (c1 - kc < kS ? c1 - kc : kS) : 0;
       const __amdgpu_buffer_rsrc_t wr = rsrc(w + kc * wpr, left * wpr * 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        p.w[i] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)(wo + (uint32_t)(i * wpr * 4)), 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        const int o = (int)(wo + (uint32_t)(i * wpr * 4));
+        if constexpr (BITS == 8) {
+          const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(wr, o, 0, 0));
+          p.w[2 * i] = v[0];
+          p.w[2 * i + 1] = v[1];
+        } else {
+          p.w[i] = __builtin_amdgcn_raw_buffer_load_b32(wr, o, 0, 0);
+        }
+      }
+      // (Lanes that load nothing here have offsets past the buffer.)
       const __amdgpu_buffer_rsrc_t sr = rsrc(scales + kc * gpr, left * gpr * 2);
       const __amdgpu_buffer_rsrc_t br = rsrc(biases + kc * gpr, left * gpr * 2);
-#pragma unroll
-      for (int i = 0; i < NSB / 2; ++i) {
-        const int o = (int)(so + (uint32_t)(4 * i * gpr * 2));
-        p.s[i] = __builtin_amdgcn_raw_buffer_load_b16(sr, o, 0, 0);
-        p.b[i] = __builtin_amdgcn_raw_buffer_load_b16(br, o, 0, 0);
-      }
+      p.s = __builtin_amdgcn_raw_buffer_load_b16(sr, (int)(G32 || c < 4 ? so : 0x7ffffff0u), 0, 0);
+      p.b = __builtin_amdgcn_raw_buffer_load_b16(br, (int)(G32 || c >= 4 ? so : 0x7ffffff0u), 0, 0);
     } else {
       // A half step past the row's end takes the row's last values against zeros of A.
       const int kq = (int)(kc + 32 * kh < wk ? kc + 32 * kh : wk - 32);
       const __amdgpu_buffer_rsrc_t wr = rsrc(w + n0 * wpr, nrows * wpr * 4);
 #pragma unroll
-      for (int i = 0; i < NW / 4; ++i) {
+      for (int i = 0; i < WPU; ++i) {
         const u32x4 v = __builtin_bit_cast(
             u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, (int)(wo + kq * BITS / 8), 16 * i, 0));
 #pragma unroll
@@ -268,58 +292,54 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
       const __amdgpu_buffer_rsrc_t sr = rsrc(scales + n0 * gpr, nrows * gpr * 2);
       const __amdgpu_buffer_rsrc_t br = rsrc(biases + n0 * gpr, nrows * gpr * 2);
       const int o = (int)(so + 2 * (kq >> gs));
-      p.s[0] = __builtin_amdgcn_raw_buffer_load_b16(sr, o, 0, 0);
-      p.b[0] = __builtin_amdgcn_raw_buffer_load_b16(br, o, 0, 0);
+      p.s = __builtin_amdgcn_raw_buffer_load_b16(sr, o, 0, 0);
+      p.b = __builtin_amdgcn_raw_buffer_load_b16(br, o, 0, 0);
     }
   };
-  // nn: lane c of an octet holds the scale and bias of row 8 q + c (rows c & 3 and + 4 of its
-  // half octet's group in groups of 32) and the others take them from there.
-  uint32_t rs[8];
+  // nn: the scales and biases of the lane's four rows.
+  float rsc[4], rbi[4];
   auto share = [&](const Packed& p) {
     if constexpr (NN) {
-      uint32_t sb[NSB / 2];
-#pragma unroll
-      for (int i = 0; i < NSB / 2; ++i) sb[i] = (uint32_t)p.s[i] | ((uint32_t)p.b[i] << 16);
+      const int sb = (int)((uint32_t)p.s | ((uint32_t)p.b << 16));
       auto from = [&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        constexpr int pattern = G32 ? (0x1c | ((i & 3) << 5)) : (0x18 | (i << 5));
-        rs[i] = (uint32_t)__builtin_amdgcn_ds_swizzle((int)sb[G32 ? i >> 2 : 0], pattern);
+        if constexpr (G32) {  // lane i of the half octet holds both
+          const uint32_t v = (uint32_t)__builtin_amdgcn_ds_swizzle(sb, 0x1c | (i << 5));
+          rsc[i] = bf16_lo(v);
+          rbi[i] = bf16_hi(v);
+        } else {
+          rsc[i] = bf16_lo((uint32_t)__builtin_amdgcn_ds_swizzle(sb, 0x18 | (i << 5)));
+          rbi[i] = bf16_hi((uint32_t)__builtin_amdgcn_ds_swizzle(sb, 0x18 | ((4 + i) << 5)));
+        }
       };
       from(std::integral_constant<int, 0>{});
       from(std::integral_constant<int, 1>{});
       from(std::integral_constant<int, 2>{});
       from(std::integral_constant<int, 3>{});
-      from(std::integral_constant<int, 4>{});
-      from(std::integral_constant<int, 5>{});
-      from(std::integral_constant<int, 6>{});
-      from(std::integral_constant<int, 7>{});
     }
   };
-  // Quarter t of the thread's weights: one 16-byte chunk of the stage.
+  // Quarter t of the thread's weights: 16 bytes of the stage.
   auto dequant = [&](const Packed& p, int st, int t) {
-    u32x4 o;
-    int row, chunk;
     if constexpr (NN) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Q4<BITS> a(p.w[2 * i], half), z(p.w[2 * i + 1], half);
-        o[i] = deq_pair(a.at(t), z.at(t), bf16_lo(rs[2 * i]), bf16_lo(rs[2 * i + 1]),
-                        bf16_hi(rs[2 * i]), bf16_hi(rs[2 * i + 1]));
-      }
-      row = 64 * cb + 8 * c + 4 * half + t;
-      chunk = q;
-    } else {
-      const float s = bf16_bits_to_f32(p.s[0]), bb = bf16_bits_to_f32(p.b[0]);
+      for (int u = 0; u < 2; ++u) {
+        const int j = 2 * t + u, row = 64 * cb + 8 * c + j;
+        u32x2 o;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Q4<BITS> v(BITS == 4 ? p.w[t] : p.w[2 * t + i], i);
-        o[2 * i] = deq_pair(v.at(0), v.at(1), s, s, bb, bb);
-        o[2 * i + 1] = deq_pair(v.at(2), v.at(3), s, s, bb, bb);
+        for (int i = 0; i < 2; ++i) {
+          const Q8<BITS> a(p.w + 2 * i * WPU), z(p.w + (2 * i + 1) * WPU);
+          o[i] = deq_pair(a.at(j), z.at(j), rsc[2 * i], rsc[2 * i + 1], rbi[2 * i], rbi[2 * i + 1]);
+        }
+        *reinterpret_cast<u32x2*>(bs(st) + row * 128 + ((q ^ swz8(row)) << 4) + 8 * half) = o;
       }
-      row = trow;
-      chunk = 4 * kh + t;
+    } else {
+      const float s = bf16_bits_to_f32(p.s), bb = bf16_bits_to_f32(p.b);
+      const Q8<BITS> v(p.w + t * WPU);
+      u32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = deq_pair(v.at(2 * i), v.at(2 * i + 1), s, s, bb, bb);
+      *reinterpret_cast<u32x4*>(bs(st) + trow * 128 + (((4 * kh + t) ^ swz8(trow)) << 4)) = o;
     }
-    *reinterpret_cast<u32x4*>(bs(st) + row * 128 + ((chunk ^ swz8(row)) << 4)) = o;
   };
 
   f32x16 acc[MI][NJ];
@@ -330,24 +350,20 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  // Fragment of sub-step s in a 32-row group: row r32, chunk 2 s + h; the group's parity
-  // flips the position's highest bit.
-  uint32_t fo[2][4];
-#pragma unroll
-  for (int p = 0; p < 2; ++p)
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-      fo[p][s] = r32 * 128 + (((2 * s + h) ^ swz8(32 * p + r32)) << 4);
-  auto frag = [&](const uint8_t* stage, int group0, int i, int s) {
-    const int par = (group0 + i) & 1;  // group0 is even unless a wave has one group
-    return *reinterpret_cast<const bf16x8*>(stage + (group0 + i) * 4096 + fo[par][s]);
+  // Fragment of sub-step s in a 32-row group: row r32, chunk 2 s + h.  The chunk's position is
+  // an exclusive or with the swizzle, which the sub-step and the group's parity enter as
+  // constants: one register an operand (kept from the compiler, which would hold them all).
+  uint32_t fa = (uint32_t)((wm * MI * 32 + r32) * 128 + ((h ^ swz8(wm * MI * 32 + r32)) << 4));
+  uint32_t fb = (uint32_t)((wn * NJ * 32 + r32) * 128 + ((h ^ swz8(wn * NJ * 32 + r32)) << 4));
+  auto frag = [&](const uint8_t* stage, uint32_t f, int i, int s) {
+    return *reinterpret_cast<const bf16x8*>(stage + (f ^ (uint32_t)(64 * (i & 1) ^ 32 * s)) + i * 4096);
   };
   bf16x8 a0[MI], a1[MI], b0[NJ], b1[NJ];
-  auto read = [&](bf16x8 (&af)[MI], bf16x8 (&bf)[NJ], int st, int s) {
+  auto read = [&](bf16x8 (&af)[MI], bf16x8 (&bf)[NJ], int sa, int sb, int s) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) bf[j] = frag(bs(st), wn * NJ, j, s);
+    for (int j = 0; j < NJ; ++j) bf[j] = frag(bs(sb), fb, j, s);
 #pragma unroll
-    for (int i = 0; i < MI; ++i) af[i] = frag(as(st), wm * MI, i, s);
+    for (int i = 0; i < MI; ++i) af[i] = frag(as(sa), fa, i, s);
   };
   auto mfmas = [&](const bf16x8 (&af)[MI], const bf16x8 (&bf)[NJ]) {
 #pragma unroll
@@ -356,54 +372,88 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 128 ? 3 : 2) void grad_gemm_kern
       for (int j = 0; j < NJ; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
   };
-  // Step k, staged in st; the weights of step k + 1 (set st ^ 1) go to the other stage, their
-  // first chunk during the step before.
+  // The dequantization's work in even shares under `quarters` quarters of a step's MFMAs.
+  // (The logits' larger tile has no registers left for it.)
+  auto pace = [&](int quarters) {
+    if constexpr (!NN) return;
+#pragma unroll
+    for (int t = 0; t < quarters * MI * NJ; ++t) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                 // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                 // DS read
+      __builtin_amdgcn_sched_group_barrier(0x002, 56 / (MI * NJ), 0);    // VALU
+      __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);                 // DS write
+    }
+  };
+  // Step k (st = k modulo the stages' common period), its A in stage k % AS, its weights in
+  // stage k % 2; the weights of step k + 1 go to the other stage, their first chunk during the
+  // step before.
   auto step = [&](int k, auto stc) {
-    constexpr int st = decltype(stc)::value;
-    read(a1, b1, st, 1);
+    constexpr int st = decltype(stc)::value, a = st % AS, a1s = (st + 1) % AS, a2s = (st + 2) % AS;
+    constexpr int b = st % 2;
+    asm volatile("" : "+v"(fa), "+v"(fb));
+    read(a1, b1, a, b, 1);
     mfmas(a0, b0);
-    dequant(pk[st ^ 1], st ^ 1, 1);
-    read(a0, b0, st, 2);
+    dequant(pk[a1s], b ^ 1, 1);
+    read(a0, b0, a, b, 2);
     mfmas(a1, b1);
-    dequant(pk[st ^ 1], st ^ 1, 2);
-    read(a1, b1, st, 3);
+    dequant(pk[a1s], b ^ 1, 2);
+    read(a1, b1, a, b, 3);
     mfmas(a0, b0);
-    dequant(pk[st ^ 1], st ^ 1, 3);
-    // Step k + 1's A has landed (only the packed loads of step k + 2 are younger), its weights
-    // are written, and this stage is read.
-    __builtin_amdgcn_s_waitcnt(wait_enc(NLD, 0));
+    dequant(pk[a1s], b ^ 1, 3);
+    pace(3);
+    // Step k + 1's A has landed (younger are the weights of AS - 1 steps and the A of AS - 2),
+    // its weights are written, and this stage is read.
+    __builtin_amdgcn_s_waitcnt(wait_enc(NLD + (AS - 2) * (XI + NLD), 0));
     __builtin_amdgcn_s_barrier();
-    issue_a(k + 2, st);
+    issue_a(k + AS, a);
     __builtin_amdgcn_sched_barrier(0);
-    issue_b(k + 3, pk[st ^ 1]);
+    issue_b(k + 1 + AS, pk[a1s]);
     __builtin_amdgcn_sched_barrier(0);
-    read(a0, b0, st ^ 1, 0);
-    share(pk[st]);
+    read(a0, b0, a1s, b ^ 1, 0);
+    share(pk[a2s]);
     mfmas(a1, b1);
-    dequant(pk[st], st, 0);
+    dequant(pk[a2s], b, 0);
+    pace(1);
   };
   if (nk > 0) {
-    issue_b(0, pk[0]);
-    issue_a(0, 0);
-    __builtin_amdgcn_sched_barrier(0);  // the waits count on this order
-    issue_b(1, pk[1]);
-    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < AS; ++i) {  // the waits count on this order
+      issue_b(i, pk[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      issue_a(i, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     share(pk[0]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) dequant(pk[0], 0, t);
-    __builtin_amdgcn_s_waitcnt(wait_enc(NLD, 0));
+    __builtin_amdgcn_s_waitcnt(wait_enc((AS - 1) * (XI + NLD), 0));
     __builtin_amdgcn_s_barrier();
-    issue_a(1, 1);
+    issue_b(AS, pk[0]);
     __builtin_amdgcn_sched_barrier(0);
-    issue_b(2, pk[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    read(a0, b0, 0, 0);
+    read(a0, b0, 0, 0, 0);
     share(pk[1]);
     dequant(pk[1], 1, 0);
-    // Two steps a turn, the last one on zeros where nk is odd.
-    for (int k = 0; k < nk; k += 2) {
-      step(k, std::integral_constant<int, 0>{});
-      step(k + 1, std::integral_constant<int, 1>{});
+    if constexpr (AS == 2) {
+      // Two steps a turn, the last one on zeros where nk is odd.
+      for (int k = 0; k < nk; k += 2) {
+        step(k, std::integral_constant<int, 0>{});
+        step(k + 1, std::integral_constant<int, 1>{});
+      }
+    } else {
+      for (int k = 0;; k += 6) {
+        step(k, std::integral_constant<int, 0>{});
+        if (k + 1 >= nk) break;
+        step(k + 1, std::integral_constant<int, 1>{});
+        if (k + 2 >= nk) break;
+        step(k + 2, std::integral_constant<int, 2>{});
+        if (k + 3 >= nk) break;
+        step(k + 3, std::integral_constant<int, 3>{});
+        if (k + 4 >= nk) break;
+        step(k + 4, std::integral_constant<int, 4>{});
+        if (k + 5 >= nk) break;
+        step(k + 5, std::integral_constant<int, 5>{});
+        if (k + 6 >= nk) break;
+      }
     }
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
   }
