@@ -21,8 +21,8 @@ struct GradGemm {
   const uint16_t* scales = nullptr;
   const uint16_t* biases = nullptr;
   int group_size = 64, bits = 4;
-  // launch_panel_gemm: the weights as bf16, row n of panel [N][ldp] the C contraction values
-  // of output column n (ldp a multiple of 8; values from C on are not read).
+  // launch_panel_gemm: the weights as bf16 rows of ldp values (a multiple of 8), [N][C] for the
+  // logits and [C][N] for input gradients.
   const uint16_t* panel = nullptr;
   int64_t ldp = 0;
   // launch_skinny_gemm (nt): skinny_pack_bytes of memory for x, or null to read it as it is.
@@ -83,12 +83,6 @@ hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 constexpr int kPanelRows = 256;
 constexpr int kPanelStatWidth = 128;
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream);
-// panel [K][ld] = deq(W)^T for packed rows W [n, K], ld >= n a multiple of 8; columns n .. of
-// the last 8 hold zeros.
-hipError_t launch_dequant_transposed(const uint32_t* w, const uint16_t* scales,
-                                     const uint16_t* biases, uint16_t* panel, int64_t n, int64_t K,
-                                     int64_t ld, int group_size, int bits, hipStream_t stream);
-
 // bf16 y [M, N] = the sum of the slices of out [splits][M][N].
 hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64_t M, int64_t N,
                              hipStream_t stream);
@@ -118,9 +112,8 @@ struct HeadLoss {
 struct HeadPlan {
   int bm, grad_bm, stat_width, pieces, splits;
   int64_t piece, c_split, stat_tiles;
-  // The logits and the gradient run over panels of dequantized weights, or both on the
-  // kernels for few rows.
-  bool panel, grad_panel, skinny;
+  // The products run over panels of dequantized weights, or on the kernels for few rows.
+  bool panel, skinny;
   size_t stats, e, slices, state, factor, sel, panel_at, xp, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);

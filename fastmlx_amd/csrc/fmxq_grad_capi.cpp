@@ -84,7 +84,7 @@ struct GradPlan {
   size_t pad, slices, panel_at, bytes;
 };
 // Rows from which the weights are dequantized to a panel beforehand.
-constexpr int64_t kGradPanelRows = 256;
+constexpr int64_t kGradPanelRows = 1025;
 
 // The rows of dy are copied to a stride of 8 values where N (or the address) is not one.
 int64_t pad_cols(int64_t N) { return up(N, 8); }
@@ -94,18 +94,18 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   p.panel = M >= kGradPanelRows;
   p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M, true);
   p.skinny = fmxq::skinny_gemm_supported(M, pad_cols(N), N + 64, K);
-  const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.panel ? fmxq::kGradTileCols : fmxq::kGradCols;
+  const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.bm > 128 ? fmxq::kGradTileCols : fmxq::kGradCols;
   const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at
   // least.
-  const int64_t want = tiles ? (p.panel ? kCus : 2 * kCus) / tiles : 1;
+  const int64_t want = tiles ? (p.bm > 128 ? kCus : 2 * kCus) / tiles : 1;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, N / 256));
   p.c_split = up((N + p.splits - 1) / p.splits, 64);
   p.splits = (int)std::max<int64_t>(1, (N + p.c_split - 1) / std::max<int64_t>(p.c_split, 1));
   p.pad = 0;
   p.slices = up(M * pad_cols(N) * 2, 256);
   p.panel_at = p.slices + (p.splits > 1 ? up(p.splits * M * K * 4, 256) : 0);
-  p.bytes = p.panel_at + (p.panel ? pad_cols(N) * K * 2 : 0);
+  p.bytes = p.panel_at + (p.panel ? N * K * 2 : 0);
   return p;
 }
 
@@ -235,9 +235,8 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
   if (p.panel) {
     uint16_t* panel = reinterpret_cast<uint16_t*>(ws + p.panel_at);
     g.panel = panel;
-    g.C = g.ldp = pad_cols(N);
-    if (int rc = hip_status(fmxq::launch_dequant_transposed(w, scales, biases, panel, N, K, g.ldp,
-                                                            group_size, bits, s),
+    g.ldp = K;
+    if (int rc = hip_status(fmxq::launch_dequantize(w, scales, biases, panel, N, K, group_size, bits, s),
                             op))
       return rc;
     if (int rc = hip_status(fmxq::launch_panel_gemm(g, true, s), op)) return rc;

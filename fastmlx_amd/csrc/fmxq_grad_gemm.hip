@@ -145,7 +145,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
   constexpr int NLD = (NN ? 4 : WPU) + 2;    // loads per thread and step
   // Stages of A, and steps whose packed weights are in registers or on their way.  Three for
   // the gradients, whose short steps (half the columns) end before memory answers.
-  constexpr int AS = NN ? 3 : 2;
+  constexpr int AS = BN == 128 ? 3 : 2;
   // Each stage an LDS object of its own, so that the compiler can tell a DMA's target from
   // the reads of another stage.
   __shared__ __attribute__((aligned(1024))) uint8_t as0[BM * 128];
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
   // The dequantization's work in even shares under `quarters` quarters of a step's MFMAs.
   // (The logits' larger tile has no registers left for it.)
   auto pace = [&](int quarters) {
-    if constexpr (!NN) return;
+    if constexpr (BN == 256) return;
 #pragma unroll
     for (int t = 0; t < quarters * MI * NJ; ++t) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                 // MFMA
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
 
 template <int BM, bool NN>
 hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
-  constexpr int BN = NN ? kGradCols : kLogitCols;
+  constexpr int BN = NN && BM < 256 ? kGradCols : kLogitCols;
   const int64_t tn = (g.N + BN - 1) / BN, tm = g.offsets ? g.max_tiles : (g.M + BM - 1) / BM;
   const int64_t blocks = tm * tn * g.splits;
   if (blocks < 1) return hipSuccess;
@@ -483,7 +483,7 @@ hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
 
 }  // namespace
 
-int grad_gemm_rows(int64_t M, bool nn) { return M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 || nn ? 128 : 256; }
+int grad_gemm_rows(int64_t M, bool nn) { return M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256; }
 
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream) {
   // Offsets into one tile's rows and into 64 or 256 weight rows are 32 bits.
@@ -495,7 +495,7 @@ hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stre
     case 32: return nn ? launch_bm<32, true>(g, stream) : hipErrorInvalidValue;
     case 64: return nn ? launch_bm<64, true>(g, stream) : hipErrorInvalidValue;
     case 128: return nn ? launch_bm<128, true>(g, stream) : launch_bm<128, false>(g, stream);
-    case 256: return nn ? hipErrorInvalidValue : launch_bm<256, false>(g, stream);
+    case 256: return nn ? launch_bm<256, true>(g, stream) : launch_bm<256, false>(g, stream);
   }
   return hipErrorInvalidValue;
 }

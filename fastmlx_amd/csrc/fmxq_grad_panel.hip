@@ -2,6 +2,11 @@
 // dequantized to a bf16 panel once, and both operands of the product go to LDS without
 // passing through registers.
 //
+// One panel [tokens, width] serves both products.  The logits' contraction runs along its
+// rows: a stage holds 256 rows of 64 values.  The gradient's runs across them: a stage holds
+// 64 rows of 256 columns, and ds_read_b64_tr_b16 turns it on the way to the registers (16 lanes
+// give 4 rows of 16 columns and get 4 rows' values of one column each).
+//
 // Tile: 256 rows by 256 columns, 64 deep steps in two LDS stages, 4 waves of 128 x 128 (one
 // per SIMD, 256 accumulators each).  A step's fragments of 16 contraction values are read
 // while the MFMAs of the 16 before run; the barrier sits before the last quarter's MFMAs,
@@ -17,6 +22,8 @@ namespace {
 
 constexpr int kS = 64;  // contraction values per step
 constexpr int kN = kGradTileCols;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <bool NN>
 __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
@@ -47,7 +54,6 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   auto bs = [&](int st) -> uint8_t* { return st == 0 ? bs0 : bs1; };
 
   const __amdgpu_buffer_rsrc_t ares = rsrc(g.a + m0 * g.lda, rows * g.lda * 2);
-  const __amdgpu_buffer_rsrc_t bres = rsrc(g.panel + n0 * g.ldp, cols * g.ldp * 2);
   // Instruction i of a wave fills rows 8 (8 wave + i) .. + 8 of a stage; lane L lands at row
   // L / 8, chunk position L % 8.
   const int chunk8 = ((lane & 7) ^ swz(lane >> 3)) * 8;  // rows 8 i differ in swz's last bit
@@ -57,10 +63,20 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
     const int row = 8 * (XI * wave + i) + (lane >> 3);
     ao[i] = row < rows ? (uint32_t)(row * g.lda * 2) : 0x7ffffff0u;
   }
+  // nn: instruction i fills rows 2 (8 wave + i) .. + 2 of 512 bytes; the row's 64-byte blocks
+  // sit at block ^ turn(row), so that the 8 rows of a turning read meet 8 different ones.
+  auto turn = [](int row) { return (row & 3) | ((row >> 3) & 1) << 2; };
+  const __amdgpu_buffer_rsrc_t bres = rsrc(g.panel + n0 * g.ldp, cols * g.ldp * 2);  // nt
 #pragma unroll
   for (int i = 0; i < YI; ++i) {
-    const int row = 8 * (YI * wave + i) + (lane >> 3);
-    bo[i] = row < cols ? (uint32_t)(row * g.ldp * 2) : 0x7ffffff0u;
+    if constexpr (NN) {
+      const int row = 2 * (YI * wave + i) + (lane >> 5), at = lane & 31;
+      const int unit = ((at >> 2) ^ turn(row)) * 4 + (at & 3);
+      bo[i] = (uint32_t)(row * g.ldp * 2 + (n0 + 8 * unit) * 2);
+    } else {
+      const int row = 8 * (YI * wave + i) + (lane >> 3);
+      bo[i] = row < cols ? (uint32_t)(row * g.ldp * 2) : 0x7ffffff0u;
+    }
   }
   auto issue = [&](int k, int st) {
     const int64_t kc = c0 + (int64_t)k * kS;
@@ -68,21 +84,37 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
     for (int p = 0; p < 2; ++p) {
       const int64_t col = kc + (chunk8 ^ (8 * p));
       const uint32_t va = k < nk && col < g.a_cols ? (uint32_t)(col * 2) : 0x7ffffff0u;
-      const uint32_t vb = k < nk && col < g.C ? (uint32_t)(col * 2) : 0x7ffffff0u;
 #pragma unroll
       for (int i = p; i < XI; i += 2)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(ares, (lds_t*)(as(st) + 8 * (XI * wave + i) * 128),
                                                  16, (int)__builtin_elementwise_add_sat(ao[i], va), 0, 0, 0);
+      if constexpr (!NN) {
+        const uint32_t vb = k < nk && col < g.C ? (uint32_t)(col * 2) : 0x7ffffff0u;
 #pragma unroll
-      for (int i = p; i < YI; i += 2)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(bres, (lds_t*)(bs(st) + 8 * (YI * wave + i) * 128),
-                                                 16, (int)__builtin_elementwise_add_sat(bo[i], vb), 0, 0, 0);
+        for (int i = p; i < YI; i += 2)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(bres, (lds_t*)(bs(st) + 8 * (YI * wave + i) * 128),
+                                                   16, (int)__builtin_elementwise_add_sat(bo[i], vb), 0, 0, 0);
+      }
+    }
+    if constexpr (NN) {
+      // Rows past the part lie past the buffer; columns past N belong to the next row and to
+      // outputs that are not stored.
+      const int64_t left = k < nk ? (c1 - kc < kS ? c1 - kc : kS) : 0;
+      const __amdgpu_buffer_rsrc_t br = rsrc(g.panel + kc * g.ldp, left * g.ldp * 2);
+#pragma unroll
+      for (int i = 0; i < YI; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(br, (lds_t*)(bs(st) + 2 * (YI * wave + i) * 512), 16,
+                                                 (int)bo[i], 0, 0, 0);
     }
   };
 
   uint32_t fo[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) fo[s] = r32 * 128 + (((2 * s + h) ^ swz(r32)) << 4);
+  // nn: the lane's 8 bytes of row 8 h + lane % 16 / 4, block 4 wn (block j: flipped by j).
+  const int trow = 8 * h + ((lane & 15) >> 2);
+  const uint32_t to = (uint32_t)(trow * 512 + (((4 * wn) ^ turn(trow)) << 6) + ((lane >> 4) & 1) * 32 +
+                                 (lane & 3) * 8);
 
   f32x16 acc[MI][NJ];
 #pragma unroll
@@ -95,8 +127,16 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   bf16x8 a0[MI], a1[MI], b0[NJ], b1[NJ];
   auto read = [&](bf16x8 (&af)[MI], bf16x8 (&bf)[NJ], int st, int s) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      bf[j] = *reinterpret_cast<const bf16x8*>(bs(st) + (wn * NJ + j) * 4096 + fo[s]);
+    for (int j = 0; j < NJ; ++j) {
+      if constexpr (NN) {
+        uint8_t* p = bs(st) + (to ^ (uint32_t)(j << 6)) + s * 8192;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2048));
+        bf[j] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      } else {
+        bf[j] = *reinterpret_cast<const bf16x8*>(bs(st) + (wn * NJ + j) * 4096 + fo[s]);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < MI; ++i)
       af[i] = *reinterpret_cast<const bf16x8*>(as(st) + (wm * MI + i) * 4096 + fo[s]);
@@ -108,12 +148,13 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
       for (int j = 0; j < NJ; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
   };
-  // One fragment read under each of the first MFMAs of a quarter.
+  // The next quarter's fragment reads (two a turned fragment) under the first MFMAs of this.
+  constexpr int RD = MI + (NN ? 2 : 1) * NJ;
   auto pace = [&]() {
 #pragma unroll
     for (int t = 0; t < MI * NJ; ++t) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                     // MFMA
-      if (t < MI + NJ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // DS read
+      if (t < RD) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);         // DS read
     }
   };
   auto step = [&](int k, auto stc) {
@@ -136,7 +177,7 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
 #pragma unroll
     for (int t = 0; t < MI * NJ; ++t) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (t < MI + NJ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (t < RD) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // VMEM (the DMA)
     }
   };
@@ -159,54 +200,11 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   else store_stats<MI, NJ>(g, acc, mw, m0 + rows, nw);
 }
 
-// A thread takes 8 rows of 8 columns: the roundings pack any two values, so the block comes
-// out transposed at no cost.  Lanes 8 c .. 8 c + 7 hold 64 rows of one 8-column unit and
-// store 128 contiguous bytes of a panel row.
-template <int BITS>
-__global__ __launch_bounds__(256) void dequant_transposed_kernel(
-    const uint32_t* __restrict__ w, const uint16_t* __restrict__ scales,
-    const uint16_t* __restrict__ biases, uint16_t* __restrict__ panel, int64_t n, int64_t K,
-    int64_t ld, int group_size) {
-  constexpr int WPU = BITS / 4;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t units = K / 8, gpr = K / group_size;
-  const int64_t r0 = (int64_t)blockIdx.y * 64 + 8 * (lane & 7);
-  const int64_t u = ((int64_t)blockIdx.x * 4 + wave) * 8 + (lane >> 3);
-  if (u >= units || r0 >= ld) return;
-  float q[8][8], s[8], b[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + i;
-    uint32_t x[2] = {0u, 0u};
-    s[i] = b[i] = 0.f;
-    if (r < n) {
-      x[0] = w[(r * units + u) * WPU];
-      if (WPU == 2) x[1] = w[(r * units + u) * WPU + 1];
-      const int64_t grp = r * gpr + u * 8 / group_size;
-      s[i] = bf16_bits_to_f32(scales[grp]);
-      b[i] = bf16_bits_to_f32(biases[grp]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      q[i][j] = BITS == 4 ? (float)((x[0] >> (4 * j)) & 15u)
-                          : (float)((x[j >> 2] >> (8 * (j & 3))) & 255u);
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t m = pack_bf16x2(q[2 * i][j] * s[2 * i], q[2 * i + 1][j] * s[2 * i + 1]);
-      o[i] = pack_bf16x2(bf16_lo(m) + b[2 * i], bf16_hi(m) + b[2 * i + 1]);
-    }
-    *reinterpret_cast<u32x4*>(panel + (u * 8 + j) * ld + r0) = o;
-  }
-}
-
 }  // namespace
 
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats) || kPanelRows * g.lda * 2 >= 0x7ffffff0LL || kN * g.ldp * 2 >= 0x7ffffff0LL || g.c_split % kS ||
+  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats) || 
+      kPanelRows * g.lda * 2 >= 0x7ffffff0LL || (kN + 1) * g.ldp * 2 >= 0x7ffffff0LL || g.c_split % kS ||
       g.lda % 8 || g.a_cols % 8 || g.ldp % 8 || g.offsets)
     return hipErrorInvalidValue;
   const int64_t blocks = (g.M + kPanelRows - 1) / kPanelRows * ((g.N + kN - 1) / kN) * g.splits;
@@ -214,19 +212,6 @@ hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   if (nn) panel_gemm_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(g);
   else panel_gemm_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(g);
-  return hipGetLastError();
-}
-
-hipError_t launch_dequant_transposed(const uint32_t* w, const uint16_t* scales,
-                                     const uint16_t* biases, uint16_t* panel, int64_t n, int64_t K,
-                                     int64_t ld, int group_size, int bits, hipStream_t stream) {
-  const int64_t by = (ld + 63) / 64;
-  if (ld % 8 || by > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)((K / 8 + 31) / 32), (unsigned)by);
-  if (bits == 4)
-    dequant_transposed_kernel<4><<<grid, 256, 0, stream>>>(w, scales, biases, panel, n, K, ld, group_size);
-  else
-    dequant_transposed_kernel<8><<<grid, 256, 0, stream>>>(w, scales, biases, panel, n, K, ld, group_size);
   return hipGetLastError();
 }
 

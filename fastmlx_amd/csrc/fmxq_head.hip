@@ -285,19 +285,16 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // Most bytes of a piece's e, and of its panel of dequantized weights.
 constexpr int64_t kHeadPieceBytes = 256 << 20;
 constexpr int64_t kHeadPanelBytes = 256 << 20;
-// Rows from which the weights are dequantized to panels beforehand, for the logits and for the
-// gradient.
-constexpr int64_t kHeadPanelRows = 1001;
-constexpr int64_t kHeadGradPanelRows = 257;
+// Rows from which the weights are dequantized to a panel beforehand.
+constexpr int64_t kHeadPanelRows = 1025;
 
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
   p.panel = M >= kHeadPanelRows;
-  p.grad_panel = grad && M >= kHeadGradPanelRows;
   p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M, false), 128);
-  p.grad_bm = p.grad_panel ? kPanelRows : std::max(grad_gemm_rows(M, true), 128);
+  p.grad_bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M, true), 128);
   int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
-  if (p.panel || p.grad_panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
+  if (p.panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
   p.pieces = (int)((V + piece - 1) / piece);
   piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
   p.pieces = (int)((V + piece - 1) / piece);
@@ -308,9 +305,9 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   p.stat_tiles = (grad ? piece : up(V, kGradTileCols)) / p.stat_width;
   // Parts of the gradient product's contraction: enough blocks for the chip, each walking
   // 256 tokens at least.
-  const int64_t cols = p.skinny ? kSkinnyCols : p.grad_panel ? kGradTileCols : kGradCols;
+  const int64_t cols = p.skinny ? kSkinnyCols : p.grad_bm > 128 ? kGradTileCols : kGradCols;
   const int64_t tiles = (p.skinny ? 1 : (M + p.grad_bm - 1) / p.grad_bm) * ((K + cols - 1) / cols);
-  const int64_t want = (p.grad_panel ? cus : 2 * cus) / tiles;
+  const int64_t want = (p.grad_bm > 128 ? cus : 2 * cus) / tiles;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, piece / 256));
   p.c_split = up((piece + p.splits - 1) / p.splits, 64);
   size_t at = 0;
@@ -327,7 +324,7 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
     p.e = take(M * piece * 2);
     p.slices = take((int64_t)p.splits * M * K * 4);
   }
-  if (p.panel || p.grad_panel) p.panel_at = take(piece * K * 2);
+  if (p.panel) p.panel_at = take(piece * K * 2);
   if (p.skinny) p.xp = take(skinny_pack_bytes(M, K));
   p.bytes = at;
   return p;
@@ -342,7 +339,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   uint16_t* e = a.dh ? reinterpret_cast<uint16_t*>(base + p.e) : nullptr;
   float* slices = a.dh ? reinterpret_cast<float*>(base + p.slices) : nullptr;
   const float scale = kLog2e / a.temperature;
-  uint16_t* panel = p.panel || p.grad_panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
+  uint16_t* panel = p.panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
   // (in, out): the running state before and after the pieces joined so far.
   auto join = [&](int i, int64_t v0, int64_t n, int64_t lde) {
     const int64_t chunks = (lde + kJoinCols - 1) / kJoinCols, shares = (a.k + 3) / 4;
@@ -397,12 +394,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     d.c_split = p.c_split;
     d.out = slices;
     d.factor = i ? factor : nullptr;
-    if (p.grad_panel) {
-      d.panel = panel;
-      d.C = d.ldp = up(n, 8);
-      if (hipError_t r = launch_dequant_transposed(g.w, g.scales, g.biases, panel, n, a.K, d.ldp,
-                                                   a.group_size, a.bits, stream))
-        return r;
+    if (p.panel) {
       if (hipError_t r = launch_panel_gemm(d, true, stream)) return r;
     } else if (hipError_t r = p.skinny ? launch_skinny_gemm(d, true, stream)
                                        : launch_grad_gemm(d, true, p.grad_bm, stream)) {
