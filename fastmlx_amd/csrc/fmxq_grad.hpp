@@ -65,17 +65,19 @@ inline int64_t grad_gemm_run_tiles(int64_t S, int64_t E, int bm) {
 }
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
 
-// The same products for up to kSkinnyRows rows, where reading the weights is the work
-// (fmxq_grad_skinny.hip).  weight_rows: rows of a part of the contraction (nn).
+// The same products where reading the weights is the work (fmxq_grad_skinny.hip): gradients
+// of up to kSkinnyRows rows, logits of as many or in chunks of as many.  weight_rows: rows of
+// a part of the contraction (nn).
 constexpr int64_t kSkinnyRows = 64;
 constexpr int kSkinnyStatWidth = 32;
 constexpr int kSkinnyCols = 128;  // outputs of a block (nn)
 // Rows from which the logits' x is packed beforehand, and the bytes that takes.
 constexpr int64_t kSkinnyPackRows = 17;
 inline int64_t skinny_pack_bytes(int64_t M, int64_t K) {
-  return M < kSkinnyPackRows ? 0 : (K + 63) / 64 * 4096 * (M <= 32 ? 1 : 2);
+  if (M < kSkinnyPackRows) return 0;
+  return (K + 63) / 64 * 4096 * (M <= 32 ? 1 : 2) * ((M + kSkinnyRows - 1) / kSkinnyRows);
 }
-bool skinny_gemm_supported(int64_t M, int64_t lda, int64_t weight_rows, int64_t weight_cols);
+bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols);
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 
 // The same products over a panel of weights dequantized beforehand (fmxq_grad_panel.hip), in
@@ -112,8 +114,9 @@ struct HeadLoss {
 struct HeadPlan {
   int bm, grad_bm, stat_width, pieces, splits;
   int64_t piece, c_split, stat_tiles;
-  // The products run over panels of dequantized weights, or on the kernels for few rows.
-  bool panel, skinny;
+  // The products run over panels of dequantized weights; the logits, the gradient on the
+  // kernels that read the weights once.
+  bool panel, skinny, grad_skinny;
   size_t stats, e, slices, state, factor, sel, panel_at, xp, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);

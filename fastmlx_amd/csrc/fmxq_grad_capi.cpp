@@ -93,7 +93,7 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
   p.panel = M >= kGradPanelRows;
   p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M, true);
-  p.skinny = fmxq::skinny_gemm_supported(M, pad_cols(N), N + 64, K);
+  p.skinny = M <= fmxq::kSkinnyRows && fmxq::skinny_gemm_supported(pad_cols(N), N + 64, K);
   const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.bm > 128 ? fmxq::kGradTileCols : fmxq::kGradCols;
   const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at

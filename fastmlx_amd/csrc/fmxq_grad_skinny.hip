@@ -2,8 +2,9 @@
 // packed weights are the work: every weight is read and dequantized once, in the registers
 // of the wave that multiplies it, with no stage in LDS and no barrier before the last sum.
 //
-// Logits: a block takes 32 tokens and its 8 waves every eighth 64-deep step of the hidden
-// width; a lane holds 32 values of one token's row.
+// Logits: a block takes 32 tokens and up to 64 rows (more rows in chunks of 64 where the tokens
+// are few), its 8 waves every eighth 64-deep step of the hidden width; a lane holds 32 values
+// of one token's row.
 // Input gradients: a block takes 128 outputs and its waves every eighth step of 32 weight
 // rows; lane r16 of quarter q4 holds the word of outputs 8 r16 .. + 8 in rows 8 q4 .. + 8, and
 // column r16 of v_mfma_f32_16x16x32_bf16's tile j is output 8 r16 + j, so that a word's values
@@ -24,6 +25,9 @@ __global__ __launch_bounds__(256) void pack_x_kernel(const uint16_t* __restrict_
                                                      int mt, int64_t n) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
+  a += (int64_t)blockIdx.y * kSkinnyRows * lda;
+  M -= (int64_t)blockIdx.y * kSkinnyRows;
+  xp += blockIdx.y * n;
   const int lane = (int)i & 63, c = (int)(i >> 6) & 3;
   const int64_t t = i >> 8;  // step mt + row tile
   const int64_t m = t % mt * 32 + (lane & 31), k = t / mt * 64 + 32 * (lane >> 5) + 8 * c;
@@ -39,6 +43,8 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * 32;
+  const int64_t m0 = (int64_t)blockIdx.y * kSkinnyRows;
+  const int64_t M = g.M - m0 < kSkinnyRows ? g.M - m0 : kSkinnyRows;
   const int K = (int)g.C;
   const int gs = __builtin_ctz(g.group_size);
   const int64_t wpr = (int64_t)K * BITS / 32, gpr = K >> gs;
@@ -48,7 +54,9 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   const __amdgpu_buffer_rsrc_t br = rsrc(g.biases + n0 * gpr, rows * gpr * 2);
   const int steps = (K + 63) / 64;
   const __amdgpu_buffer_rsrc_t ar =
-      PACKED ? rsrc(g.xp, (int64_t)steps * MT * 4096) : rsrc(g.a, g.M * g.lda * 2);
+      PACKED ? rsrc(static_cast<const uint8_t*>(g.xp) + blockIdx.y * ((int64_t)steps * MT * 4096),
+                    (int64_t)steps * MT * 4096)
+             : rsrc(g.a + m0 * g.lda, M * g.lda * 2);
   // Rows of x past M lie past its buffer.
   uint32_t ao[MT];
 #pragma unroll
@@ -125,7 +133,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[0][0][4 * q + e] = v[e];
   }
-  store_stats<1, 1>(g, sum, 32 * wave, g.M, n0);
+  store_stats<1, 1>(g, sum, m0 + 32 * wave, g.M, n0);
 }
 
 template <int BITS, int MT, bool G32>
@@ -302,17 +310,18 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void grad_skinny_kernel(GradG
 
 template <int BITS, int MT>
 hipError_t launch_logits(const GradGemm& g, hipStream_t stream) {
-  const int64_t blocks = (g.N + 31) / 32;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  const int64_t blocks = (g.N + 31) / 32, chunks = (g.M + kSkinnyRows - 1) / kSkinnyRows;
+  if (blocks > 0x7fffffff || chunks > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, (unsigned)chunks);
   if (!g.xp) {
-    logits_skinny_kernel<BITS, MT, false><<<(unsigned)blocks, 512, 0, stream>>>(g);
+    logits_skinny_kernel<BITS, MT, false><<<grid, 512, 0, stream>>>(g);
     return hipGetLastError();
   }
   const int64_t n = (g.C + 63) / 64 * MT * 256;
-  pack_x_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(g.a, g.lda, g.M, g.C,
-                                                                 reinterpret_cast<u32x4*>(g.xp), MT, n);
+  pack_x_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)chunks), 256, 0, stream>>>(
+      g.a, g.lda, g.M, g.C, reinterpret_cast<u32x4*>(g.xp), MT, n);
   if (hipError_t e = hipGetLastError()) return e;
-  logits_skinny_kernel<BITS, MT, true><<<(unsigned)blocks, 512, 0, stream>>>(g);
+  logits_skinny_kernel<BITS, MT, true><<<grid, 512, 0, stream>>>(g);
   return hipGetLastError();
 }
 
@@ -327,16 +336,16 @@ hipError_t launch_grad(const GradGemm& g, hipStream_t stream) {
 
 }  // namespace
 
-// Byte offsets of a call's rows are 32 bits: 64 rows of x, 32 weight rows of the logits, a
+// Byte offsets of a block's rows are 32 bits: 64 rows of x, 32 weight rows of the logits, a
 // part's weight rows of the gradient and the steps that are requested past its end.
-bool skinny_gemm_supported(int64_t M, int64_t lda, int64_t weight_rows, int64_t weight_cols) {
-  return M <= kSkinnyRows && 64 * lda * 2 < 0x7ffffff0LL &&
-         (weight_rows + 1024) * weight_cols < 0x7fff0000LL;
+bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols) {
+  return 64 * lda * 2 < 0x7ffffff0LL && (weight_rows + 1024) * weight_cols < 0x7fff0000LL;
 }
 
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
   if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats) ||
-      !skinny_gemm_supported(g.M, g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.offsets || g.lda % 8 ||
+      (nn && g.M > kSkinnyRows) ||
+      !skinny_gemm_supported(g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.offsets || g.lda % 8 ||
       g.a_cols % 8 || g.c_split % 16)
     return hipErrorInvalidValue;
   if (g.M < 1 || g.N < 1 || g.splits < 1) return hipSuccess;

@@ -288,6 +288,17 @@ constexpr int64_t kHeadPanelBytes = 256 << 20;
 // Rows from which the weights are dequantized to a panel beforehand.
 constexpr int64_t kHeadPanelRows = 1025;
 
+// Few tokens for many rows: the tiles of the logits leave most of the chip idle and each walks
+// the whole width, about 2 us a 64-deep step; the kernel for few rows has a block for every
+// 32 tokens of every 64 rows and takes about 1.1 ns a block's step.  (500 rows over 1200
+// tokens, 4096 wide: 130 against 30 us.)
+bool few_tokens(int64_t M, int64_t V, int bm, int cus) {
+  const int64_t tiles = (M + bm - 1) / bm * ((V + kLogitCols - 1) / kLogitCols);
+  const int64_t waves = (tiles + cus - 1) / cus;
+  const int64_t chunks = (M + kSkinnyRows - 1) / kSkinnyRows;
+  return chunks <= 65535 && chunks * ((V + 31) / 32) * 11 < waves * 20000;
+}
+
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
   p.panel = M >= kHeadPanelRows;
@@ -299,14 +310,15 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
   p.pieces = (int)((V + piece - 1) / piece);
   p.piece = piece;
-  p.skinny = skinny_gemm_supported(M, std::max(K, piece), piece, K);
+  p.grad_skinny = M <= kSkinnyRows && skinny_gemm_supported(piece, piece, K);
+  p.skinny = skinny_gemm_supported(K, 32, K) && (M <= kSkinnyRows || few_tokens(M, piece, p.bm, cus));
   p.stat_width = p.skinny ? kSkinnyStatWidth : p.panel ? kPanelStatWidth : kGradStatWidth;
   // Without a gradient the tiles of all pieces are joined at once.
   p.stat_tiles = (grad ? piece : up(V, kGradTileCols)) / p.stat_width;
   // Parts of the gradient product's contraction: enough blocks for the chip, each walking
   // 256 tokens at least.
-  const int64_t cols = p.skinny ? kSkinnyCols : p.grad_bm > 128 ? kGradTileCols : kGradCols;
-  const int64_t tiles = (p.skinny ? 1 : (M + p.grad_bm - 1) / p.grad_bm) * ((K + cols - 1) / cols);
+  const int64_t cols = p.grad_skinny ? kSkinnyCols : p.grad_bm > 128 ? kGradTileCols : kGradCols;
+  const int64_t tiles = (p.grad_skinny ? 1 : (M + p.grad_bm - 1) / p.grad_bm) * ((K + cols - 1) / cols);
   const int64_t want = (p.grad_bm > 128 ? cus : 2 * cus) / tiles;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, piece / 256));
   p.c_split = up((piece + p.splits - 1) / p.splits, 64);
@@ -371,17 +383,17 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     g.lde = up(n, kGradTileCols);
     g.logit_scale = scale;
     if (p.skinny && skinny_pack_bytes(a.M, a.K)) g.xp = base + p.xp;
-    if (p.panel) {
+    if (p.panel && (e || !p.skinny)) {
       if (hipError_t r = launch_dequantize(g.w, g.scales, g.biases, panel, n, a.K, a.group_size, a.bits,
                                            stream))
         return r;
       g.panel = panel;
       g.ldp = a.K;
-      if (hipError_t r = launch_panel_gemm(g, false, stream)) return r;
-    } else if (hipError_t r = p.skinny ? launch_skinny_gemm(g, false, stream)
-                                       : launch_grad_gemm(g, false, p.bm, stream)) {
-      return r;
     }
+    if (hipError_t r = p.skinny  ? launch_skinny_gemm(g, false, stream)
+                       : p.panel ? launch_panel_gemm(g, false, stream)
+                                 : launch_grad_gemm(g, false, p.bm, stream))
+      return r;
     if (!e) continue;
     if (hipError_t r = join(i, v0, n, g.lde)) return r;
     GradGemm d = g;
@@ -394,12 +406,10 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     d.c_split = p.c_split;
     d.out = slices;
     d.factor = i ? factor : nullptr;
-    if (p.panel) {
-      if (hipError_t r = launch_panel_gemm(d, true, stream)) return r;
-    } else if (hipError_t r = p.skinny ? launch_skinny_gemm(d, true, stream)
-                                       : launch_grad_gemm(d, true, p.grad_bm, stream)) {
+    if (hipError_t r = p.panel         ? launch_panel_gemm(d, true, stream)
+                       : p.grad_skinny ? launch_skinny_gemm(d, true, stream)
+                                       : launch_grad_gemm(d, true, p.grad_bm, stream))
       return r;
-    }
   }
   if (!e)
     if (hipError_t r = join(0, 0, a.V, 0)) return r;
