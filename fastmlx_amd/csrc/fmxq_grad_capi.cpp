@@ -26,8 +26,11 @@ constexpr int kCus = 256;
 constexpr int kHeadMaxTopK = 64;
 constexpr int64_t kSortMaxExperts = 2048;
 constexpr int64_t kMaxCount = 0x7fffffff;
+// Rows of a call: a launch has at most 2^32 threads, 256 a row.
+constexpr int64_t kMaxRows = (1 << 24) - 1;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // a * b within 62 bits (a, b >= 0).
@@ -52,7 +55,7 @@ int head_sizes(int64_t M, int64_t V, int64_t K, int k, const char* op) {
   if (k < 1 || k > kHeadMaxTopK)
     return fail(FMXQ_ERR_SHAPE, "%s: top_k=%d outside 1..%d", op, k, kHeadMaxTopK);
   if (M > 0 && V == 0) return fail(FMXQ_ERR_SHAPE, "%s: %lld rows over no tokens", op, (long long)M);
-  if (M > (1 << 24) || V > kMaxCount || K > (1 << 22))
+  if (M > kMaxRows || V > kMaxCount || K > (1 << 22))
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, V=%lld or K=%lld too large", op, (long long)M,
                 (long long)V, (long long)K);
   return FMXQ_OK;
@@ -68,6 +71,9 @@ int head_loss(fmxq::HeadLoss a, void* ws, size_t ws_bytes, void* stream, const c
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
   if (!aligned16(a.h) || !aligned16(a.w) || !aligned16(a.dh))
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: h, w and dh must be 16-byte aligned", op);
+  if (!aligned(a.ids, 4) || !aligned(a.loss, 4) || !aligned(a.lse, 4) || !aligned(a.grad_loss, 4) ||
+      !aligned(a.scales, 2) || !aligned(a.biases, 2))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   const fmxq::HeadPlan p = fmxq::head_plan(a.M, a.V, a.K, a.k, a.dh != nullptr, kCus);
   if (int rc = check_workspace(ws, ws_bytes, p.bytes, op)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -124,7 +130,7 @@ int grad_sizes(int64_t M, int64_t N, int64_t K, const char* op) {
   if (M < 0 || N < 0 || K < 0)
     return fail(FMXQ_ERR_SHAPE, "%s: negative size M=%lld N=%lld K=%lld", op, (long long)M,
                 (long long)N, (long long)K);
-  if (M > kMaxCount || N > (1 << 22) || K > (1 << 22))
+  if (M > kMaxRows || N > (1 << 22) || K > (1 << 22))
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, N=%lld or K=%lld too large", op, (long long)M,
                 (long long)N, (long long)K);
   return FMXQ_OK;
@@ -144,12 +150,10 @@ int row_sizes(int64_t T, int64_t k, int64_t D, const char* op) {
   if (T < 0 || k < 1 || D < 0)
     return fail(FMXQ_ERR_SHAPE, "%s: need T >= 0, top_k >= 1 and D >= 0 (got %lld %lld %lld)", op,
                 (long long)T, (long long)k, (long long)D);
-  if (!product_ok(T, k) || T * k > kMaxCount)
+  if (T > kMaxRows || !product_ok(T, k) || T * k > 4 * kMaxRows)
     return fail(FMXQ_ERR_SHAPE, "%s: %lld x %lld slots are too many", op, (long long)T, (long long)k);
   return FMXQ_OK;
 }
-
-bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 }  // namespace
 
@@ -210,6 +214,8 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
     return hip_status(fmxq::launch_fill_u32(reinterpret_cast<uint32_t*>(dx), 0u, M * K / 2, s), op);
   if (!dy || !w || !scales || !biases) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
   if (!aligned16(w)) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: w must be 16-byte aligned", op);
+  if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   const GradPlan p = grad_plan(M, N, K);
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, op)) return rc;
   char* ws = static_cast<char*>(workspace);
@@ -273,7 +279,11 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
     return hip_status(fmxq::launch_fill_u32(reinterpret_cast<uint32_t*>(dx), 0u, S * K / 2, s), op);
   if (!dy || !w || !scales || !biases || !offsets)
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
+  if (!aligned(offsets, 4))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   if (!aligned16(w)) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: w must be 16-byte aligned", op);
+  if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   if (E > kMaxCount) return fail(FMXQ_ERR_SHAPE, "%s: %lld experts are too many", op, (long long)E);
   if (int rc = check_workspace(workspace, workspace_bytes, S * pad_cols(N) * 2, op)) return rc;
   uint32_t* flag = nullptr;

@@ -468,7 +468,7 @@ hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
   const int64_t tn = (g.N + BN - 1) / BN, tm = g.offsets ? g.max_tiles : (g.M + BM - 1) / BM;
   const int64_t blocks = tm * tn * g.splits;
   if (blocks < 1) return hipSuccess;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  if (blocks >= (int64_t)1 << 23) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks), block(BN * 2);
   const bool g32 = NN && g.group_size == 32;
   if (g.bits == 4) {

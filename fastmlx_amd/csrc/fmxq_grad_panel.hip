@@ -209,7 +209,7 @@ hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
     return hipErrorInvalidValue;
   const int64_t blocks = (g.M + kPanelRows - 1) / kPanelRows * ((g.N + kN - 1) / kN) * g.splits;
   if (blocks < 1) return hipSuccess;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  if (blocks >= (int64_t)1 << 23) return hipErrorInvalidConfiguration;
   if (nn) panel_gemm_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(g);
   else panel_gemm_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(g);
   return hipGetLastError();

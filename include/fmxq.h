@@ -282,7 +282,8 @@ int fmxq_route_group_topk(const void* gates, int gates_bf16, const float* bias, 
  * These calls own no memory: `workspace` holds the bytes that the call's _workspace function
  * reports for the same sizes, is 16-byte aligned, needs no contents and may be reused once
  * the call's work is done.  Calls that may overlap (two streams, two graphs replayed at once)
- * need a workspace each.  They can be captured into a graph at any time. */
+ * need a workspace each.  They can be captured into a graph at any time.  Outputs do not
+ * overlap other operands.  Rows (M, S, T) below 2^24, N and K up to 2^22, 2^26 slots. */
 
 /* Cross entropy of a quantized head: logits l = h . deq(W)^T over V tokens, which are never
  * stored;
@@ -353,8 +354,8 @@ int fmxq_moe_sort_grad(const uint16_t* dxs, const uint32_t* pos, uint16_t* dx, i
  * raises the error flag. */
 int fmxq_moe_unsort(const uint16_t* y, const uint32_t* pos, const void* weights, int weights_bf16,
                     uint16_t* out, int64_t T, int64_t top_k, int64_t D, void* stream);
-/* Its gradients: dy[pos[t, j]] = weights[t, j] dout[t] (rows of dy that no position names are
- * left as they were), dweights[t, j] = <dout[t], y[pos[t, j]]> in the weights' type. */
+/* Its gradients: dy[pos[t, j]] = weights[t, j] dout[t] (positions differ; rows of dy that none
+ * names are left as they were), dweights[t, j] = <dout[t], y[pos[t, j]]> in the weights' type. */
 int fmxq_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t* pos,
                          const void* weights, int weights_bf16, uint16_t* dy, void* dweights,
                          int64_t T, int64_t top_k, int64_t D, void* stream);

@@ -43,7 +43,12 @@ def ce_check(h, w, y, g, bits, group, ignore=-100):
 CE = [(1, 1, 32, 4, 32), (1, 1000, 64, 4, 64), (2, 7, 96, 8, 32), (5, 255, 128, 4, 128),
       (31, 256, 512, 4, 64), (33, 257, 1056, 4, 32), (64, 4099, 256, 8, 64), (65, 300, 192, 4, 64),
       (130, 1025, 384, 8, 128), (300, 2000, 512, 4, 64), (16, 50257, 128, 4, 64),
-      (513, 700, 96, 4, 32), (257, 8192, 1024, 8, 64)]
+      (513, 700, 96, 4, 32), (257, 8192, 1024, 8, 64),
+      # tiles of 128 and 256 rows, with part-full last steps, tiles and tokens
+      (100, 40000, 256, 4, 128), (70, 60001, 96, 8, 32), (300, 20000, 96, 4, 32),
+      (200, 30001, 192, 8, 64), (1000, 9001, 160, 4, 32), (1024, 12800, 320, 4, 64),
+      # panels, the last step of 32 values, widths below a tile
+      (1100, 24001, 96, 4, 32), (1300, 20001, 320, 8, 64), (2050, 10240, 1056, 4, 32)]
 
 
 @pytest.mark.parametrize("M,V,K,bits,group", CE)
@@ -100,17 +105,18 @@ def test_cross_entropy_ignore_index_inside_the_vocabulary(gpu):
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
-def test_cross_entropy_bad_row_stays_alone(gpu, value):
-    announce(f"ce row of {value}")
-    h, w, y, g = ce_case(gpu, 70, 600, 128, ignored=0.0)
-    want = ops.head_cross_entropy(h, *w, y, grad=True)
+@pytest.mark.parametrize("M,V", [(20, 600), (70, 600), (90, 50000), (300, 20000), (1100, 20000)])
+def test_cross_entropy_bad_row_stays_alone(gpu, value, M, V):
+    announce(f"ce row of {value}, {M}x{V}")
+    h, w, y, g = ce_case(gpu, M, V, 96, 4, 32, ignored=0.0)
+    want = ops.head_cross_entropy(h, *w, y, grad=True, group_size=32)
     h2 = h.clone()
-    h2[33, 5] = value
-    got = ops.head_cross_entropy(h2, *w, y, grad=True)
-    rest = torch.arange(70, device=gpu) != 33
+    h2[13, 5] = value
+    got = ops.head_cross_entropy(h2, *w, y, grad=True, group_size=32)
+    rest = torch.arange(M, device=gpu) != 13
     for a, b in zip(got, want):
         assert torch.equal(a[rest], b[rest])
-        assert not torch.isfinite(a[33]).all()
+        assert not torch.isfinite(a[13]).all()
 
 
 def distill_case(gpu, M, V, K, k, bits, group, seed, dtype):
@@ -209,7 +215,11 @@ def test_losses_against_differences(gpu):
 @pytest.mark.parametrize("M,N,K,bits,group", [
     (1, 1, 32, 4, 32), (1, 4096, 512, 4, 64), (3, 7, 96, 8, 32), (32, 64, 128, 4, 128),
     (33, 1000, 320, 4, 64), (64, 2048, 1056, 4, 32), (65, 129, 256, 8, 128), (200, 512, 2048, 8, 64),
-    (129, 4100, 704, 4, 64), (515, 72, 96, 4, 32), (256, 11008, 256, 4, 64)])
+    (129, 4100, 704, 4, 64), (515, 72, 96, 4, 32), (256, 11008, 256, 4, 64),
+    (1000, 333, 1056, 8, 32), (700, 2000, 64, 8, 64),
+    # panels
+    (1025, 37, 96, 4, 32), (1030, 300, 1056, 8, 32), (2001, 129, 320, 4, 64), (1500, 5000, 256, 4, 128),
+    (1026, 64, 2048, 8, 64)])
 def test_quantized_matmul_grad(gpu, M, N, K, bits, group):
     announce(f"grad {M}x{N}x{K} {bits} bits, groups of {group}")
     gen = torch.Generator().manual_seed(M + N)
@@ -252,7 +262,9 @@ def test_quantized_matmul_grad_bad_rows_stay_alone(gpu):
 
 @pytest.mark.parametrize("counts,N,K,bits,group", [
     ([1], 8, 32, 4, 32), ([0, 5, 0, 40, 1], 100, 192, 4, 64), ([33] * 7, 64, 1056, 8, 32),
-    ([200, 0, 0, 130], 512, 384, 4, 128), ([3] * 70, 37, 128, 8, 64), ([0, 0, 900], 256, 512, 4, 64)])
+    ([200, 0, 0, 130], 512, 384, 4, 128), ([3] * 70, 37, 128, 8, 64), ([0, 0, 900], 256, 512, 4, 64),
+    ([700, 300, 0, 513], 130, 1056, 8, 32), ([256, 257], 72, 320, 4, 64), ([1, 0, 2] * 230, 40, 64, 4, 64),
+    ([50, 0, 61, 64], 1000, 96, 4, 32)])
 def test_gather_qmm_grad(gpu, counts, N, K, bits, group):
     announce(f"gather grad {len(counts)} experts {N}x{K}")
     gen = torch.Generator().manual_seed(N)
@@ -285,6 +297,66 @@ def test_gather_qmm_grad_refuses_bad_offsets(gpu):
     dx = ops.gather_qmm_grad(dy, *w, torch.zeros(4, dtype=torch.int32, device=gpu))
     assert not dx.any()
     ops.device_error()
+
+
+@pytest.mark.parametrize("M,N", [(40, 37), (100, 500), (300, 72), (1100, 130)])
+def test_quantized_matmul_grad_bad_row_stays_alone(gpu, M, N):
+    announce(f"grad NaN row, {M}x{N}")
+    gen = torch.Generator().manual_seed(M)
+    w = ref.quant(gen, (N,), 160, 4, 32, gpu)
+    dy = hidden(gen, M, N, gpu)
+    want = ops.quantized_matmul_grad(dy, *w, 32)
+    dy[17, N - 1] = float("inf")
+    got = ops.quantized_matmul_grad(dy, *w, 32)
+    rest = torch.arange(M, device=gpu) != 17
+    assert torch.equal(got[rest], want[rest]) and not torch.isfinite(got[17]).any()
+
+
+def test_results_do_not_depend_on_what_the_workspace_held(gpu):
+    """Workspaces come with whatever was there: the memory is filled with NaN before each call."""
+    announce("dirty workspaces")
+    for M, V, K, group in ((3, 70, 96, 32), (40, 300, 128, 64), (100, 3000, 96, 32), (300, 20001, 96, 32),
+                           (1100, 7001, 96, 32)):
+        h, w, y, g = ce_case(gpu, M, V, K, 4, group, seed=M)
+        dy = hidden(torch.Generator().manual_seed(M), M, V, gpu)
+        off = torch.tensor([0, M // 3, M], dtype=torch.int32, device=gpu)
+        two = tuple(torch.stack([t, t]) for t in w)
+        first = None
+        for fill in (0, 0xFF):
+            junk = [torch.full((n,), fill, dtype=torch.uint8, device=gpu)
+                    for n in (1 << 28, 1 << 26, 1 << 22, 1 << 18, 4096, 512)]
+            torch.cuda.synchronize()
+            del junk
+            got = [*ops.head_cross_entropy(h, *w, y, grad=True, group_size=group),
+                   *ops.head_cross_entropy(h, *w, y, group_size=group),
+                   ops.quantized_matmul_grad(dy, *w, group), ops.gather_qmm_grad(dy, *two, off, group)]
+            assert all(torch.isfinite(t).all() for t in got)
+            first = first or got
+            assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_refuses_strides_and_other_shapes(gpu):
+    h, w, y, g = ce_case(gpu, 8, 64, 64)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.head_cross_entropy(h.t().contiguous().t(), *w, y)
+    with pytest.raises(ValueError, match="shape"):
+        ops.head_cross_entropy(h, *w, y[:5].contiguous())
+    with pytest.raises(ValueError, match="shape"):
+        ops.head_cross_entropy(h, w[0], w[1][:60].contiguous(), w[2], y)
+    with pytest.raises(ValueError, match="grad"):
+        ops.head_cross_entropy(h, *w, y, grad_loss=g)
+    with pytest.raises(TypeError):
+        ops.head_cross_entropy(h, *w, y.long())
+    with pytest.raises(TypeError):
+        ops.head_cross_entropy(h.float(), *w, y)
+    with pytest.raises(FmxqError, match="bits"):
+        ops.head_cross_entropy(h, *w, y, bits=3)
+    with pytest.raises(FmxqError, match="top_k"):
+        ops.head_distill(h, *w, y[:, None].expand(8, 65).contiguous(), torch.zeros(8, 65, device=gpu))
+    with pytest.raises(ValueError, match="columns"):
+        ops.quantized_matmul_grad(h[:, :32].contiguous(), *w)
+    with pytest.raises(ValueError, match="shape"):
+        ops.gather_qmm_grad(h, *(t[None] for t in w), y[:3].contiguous())
 
 
 def run_all(c):

@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1, 1, 8), (1, 8, 256, 64), (16, 10, 512, 2048), (100, 3, 7, 100), (333, 6, 64, 1000),
           (1024, 1, 2, 16), (257, 4, 2048, 24), (700, 8, 5, 33), (3000, 8, 128, 256),
-          (20000, 10, 300, 8)]
+          (20000, 10, 300, 8), (40, 20, 64, 72), (90, 16, 30, 40), (128, 8, 2048, 1), (129, 8, 3, 520)]
 
 
 def case(gpu, T, k, E, D, dtype, seed=0):
