@@ -119,6 +119,34 @@ def test_cross_entropy_bad_row_stays_alone(gpu, value, M, V):
         assert not torch.isfinite(a[13]).all()
 
 
+@pytest.mark.parametrize("off", [0, 1, 2])
+@pytest.mark.parametrize("M,V,K,bits,group", [
+    (3, 100, 192, 4, 32), (20, 300, 384, 8, 64), (1, 70, 640, 4, 128), (40, 700, 576, 4, 32),
+    (9, 500, 896, 8, 128), (64, 99, 1152, 4, 64)])
+def test_cross_entropy_rows_of_few_groups(gpu, M, V, K, bits, group, off):
+    """5 to 18 groups a row, never a multiple of 4, and scales that begin in the middle of
+    a 4-byte word."""
+    announce(f"ce {M}x{V}x{K} {bits} bits, groups of {group}, scales from {off}")
+    h, (w, s, b), y, g = ce_case(gpu, M, V, K, bits, group, seed=M + K)
+
+    def moved(t):
+        buf = torch.empty(t.numel() + off, dtype=t.dtype, device=gpu)
+        return buf[off:].copy_(t.flatten()).view(t.shape)
+
+    ce_check(h, (w, moved(s), moved(b)), y, g, bits, group)
+
+
+def test_cross_entropy_bad_last_row_stays_alone(gpu):
+    """The rows that a tile has past the last one read the last one's values."""
+    announce("ce last row of nan, 5x600")
+    h, w, y, g = ce_case(gpu, 5, 600, 96, 4, 32, ignored=0.0)
+    want = ops.head_cross_entropy(h, *w, y, grad=True, group_size=32)
+    h[4] = float("nan")
+    got = ops.head_cross_entropy(h, *w, y, grad=True, group_size=32)
+    for a, b in zip(got, want):
+        assert torch.equal(a[:4], b[:4]) and torch.isnan(a[4]).all()
+
+
 def distill_case(gpu, M, V, K, k, bits, group, seed, dtype):
     gen = torch.Generator().manual_seed(seed)
     w = ref.quant(gen, (V,), K, bits, group, gpu)
