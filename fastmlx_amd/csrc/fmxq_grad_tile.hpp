@@ -92,7 +92,12 @@ __device__ __forceinline__ void store_grad(const GradGemm& g, const f32x16 (&acc
   }
 }
 
-// The softmax statistics of a tile of 32 NJ columns, and e.
+// The softmax statistics of a tile of 32 NJ columns, and e.  They are relative to the nearest
+// multiple of kStatStep (units of log 2) to the row's largest logit in the tile: bf16 and fp32
+// keep their precision at any exponent, so tiles of a row whose logits reach about as far share
+// one and need no rescaling, and where they differ 2^-kStatStep is still a normal number.
+constexpr float kStatStep = 64.f;
+
 template <int MI, int NJ>
 __device__ __forceinline__ void store_stats(const GradGemm& g, const f32x16 (&acc)[MI][NJ],
                                             int64_t mw, int64_t mend, int64_t nw) {
@@ -121,7 +126,7 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, const f32x16 (&ac
       for (int r = 0; r < 16; ++r)
         if (full || nw + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) < g.N)
           top = fmaxf(top, acc[i][j][r] * g.logit_scale);
-    const float mx = ceilf(fmaxf(top, other_half(top)));
+    const float mx = kStatStep * rintf(fmaxf(top, other_half(top)) * (1.f / kStatStep));
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)

@@ -7,15 +7,17 @@
 //   loss = T^2 sum_j q_j (log q_j - l_j + lse)
 //   dh   = g T (sum_v p_v W_v - sum_j q_j W_j)
 // The vocabulary is walked in pieces.  A piece's product leaves e = 2^(l - m) in bf16 with m
-// the largest l of the row in a tile, rounded up to an integer, and the tile's sum; the join
-// brings the tiles of a row to one m (a power of two: no second rounding), and e . deq(W) is
-// added to fp32 sums that are scaled by the change of m.  The wanted entries' e are zeroed
+// the largest l of the row in a tile, rounded to a multiple of 64, and the tile's sum; the join
+// brings the tiles of a row to one m (a power of two: no second rounding; with m the largest l
+// itself nearly all tiles needed it, which took 50 us of a piece of 2048 rows by 32064 tokens
+// where the join now takes 17), and e . deq(W) is added to fp32 sums that are scaled by the
+// change of m.  The wanted entries' e are zeroed
 // and their share p_j - q_j enters at the end in fp32: where p_j nears q_j the two cancel,
 // and bf16 values of them would leave their rounding.
 #include <algorithm>
 
 #include "fmxq_common.hpp"
-#include "fmxq_grad.hpp"
+#include "fmxq_grad_tile.hpp"
 #include "fmxq_internal.hpp"
 
 namespace fmxq {
@@ -29,29 +31,39 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// 8 dequantized values (fmxq_dequantize's bits) of packed row `row` from column c on.
-__device__ __forceinline__ void deq8(const HeadLoss& a, int64_t row, int64_t c, float* v) {
-  const int64_t grp = (row * a.K + c) >> __builtin_ctz(a.group_size);
-  const float s = bf16_bits_to_f32(a.scales[grp]), b = bf16_bits_to_f32(a.biases[grp]);
-  uint32_t w0, w1 = 0;
-  const int64_t at = (row * a.K + c) >> (a.bits == 4 ? 3 : 2);
-  w0 = a.w[at];
-  if (a.bits == 8) w1 = a.w[at + 1];
+// 8 packed values of row `row`, which is the same in every lane, from column c on.
+struct Packed8 {
+  u32x2 w;
+  uint16_t s, b;
+};
+__device__ __forceinline__ Packed8 load8(const HeadLoss& a, int row, int c) {
+  const int64_t r = __builtin_amdgcn_readfirstlane(row);
+  const int gs = __builtin_ctz(a.group_size);
+  const int64_t g0 = r * (a.K >> gs);
+  Packed8 p;
+  if (a.bits == 4) p.w = u32x2{(a.w + r * (a.K >> 3))[(uint32_t)c >> 3], 0u};
+  else p.w = *reinterpret_cast<const u32x2*>(a.w + r * (a.K >> 2) + ((uint32_t)c >> 2));
+  p.s = (a.scales + g0)[(uint32_t)c >> gs];
+  p.b = (a.biases + g0)[(uint32_t)c >> gs];
+  return p;
+}
+
+// Their dequantized values (fmxq_dequantize's bits).
+__device__ __forceinline__ void deq8(const Packed8& p, int bits, float* v) {
+  const float s = bf16_bits_to_f32(p.s), b = bf16_bits_to_f32(p.b);
+  // Bytes: the even and the odd values.
+  uint32_t lo = p.w[0] & 0x0F0F0F0Fu, hi = (p.w[0] >> 4) & 0x0F0F0F0Fu;
+  if (bits == 8) {
+    lo = __builtin_amdgcn_perm(p.w[1], p.w[0], 0x06040200u);
+    hi = __builtin_amdgcn_perm(p.w[1], p.w[0], 0x07050301u);
+  }
+  asm("" : "+v"(lo), "+v"(hi));
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    float q0, q1;
-    if (a.bits == 4) {
-      q0 = (float)((w0 >> (4 * j)) & 15u);
-      q1 = (float)((w0 >> (4 * j + 4)) & 15u);
-    } else {
-      const uint32_t w = j < 4 ? w0 : w1;
-      q0 = (float)((w >> (8 * (j & 3))) & 255u);
-      q1 = (float)((w >> (8 * (j & 3) + 8)) & 255u);
-    }
-    const uint32_t m = pack_bf16x2(q0 * s, q1 * s);
-    const uint32_t r = pack_bf16x2(bf16_lo(m) + b, bf16_hi(m) + b);
-    v[j] = bf16_lo(r);
-    v[j + 1] = bf16_hi(r);
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t t = deq_pair((float)((lo >> (8 * j)) & 0xffu), (float)((hi >> (8 * j)) & 0xffu), s,
+                                s, b, b);
+    v[2 * j] = bf16_lo(t);
+    v[2 * j + 1] = bf16_hi(t);
   }
 }
 
@@ -68,15 +80,29 @@ __device__ __forceinline__ int64_t token_of(const HeadLoss& a, int64_t m, int j,
 
 // The logit of token v for row m in units of log 2, fp32 sums over the wave.
 __device__ __forceinline__ float logit_of(const HeadLoss& a, int64_t m, int64_t v, float scale) {
+  constexpr int B = 4;  // chunks of 512 columns that are requested together
+  const uint16_t* h = a.h + m * a.K;
+  const int K = (int)a.K;
   float t = 0.f;
-  for (int64_t c = 8 * (threadIdx.x & 63); c < a.K; c += 512) {
-    float wv[8];
-    deq8(a, v, c, wv);
-    const u32x4 x = *reinterpret_cast<const u32x4*>(a.h + m * a.K + c);
+  for (int c0 = 8 * (threadIdx.x & 63); c0 < K; c0 += 512 * B) {
+    Packed8 p[B];
+    u32x4 x[B];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t = __builtin_fmaf(wv[2 * j], bf16_lo(x[j]), t);
-      t = __builtin_fmaf(wv[2 * j + 1], bf16_hi(x[j]), t);
+    for (int i = 0; i < B; ++i) {
+      const int c = c0 + 512 * i < K ? c0 + 512 * i : c0;
+      p[i] = load8(a, (int)v, c);
+      x[i] = *reinterpret_cast<const u32x4*>(h + c);
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (c0 + 512 * i >= K) break;
+      float wv[8];
+      deq8(p[i], a.bits, wv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t = __builtin_fmaf(wv[2 * j], bf16_lo(x[i][j]), t);
+        t = __builtin_fmaf(wv[2 * j + 1], bf16_hi(x[i][j]), t);
+      }
     }
   }
   return wave_sum(t) * scale;
@@ -136,12 +162,13 @@ __device__ __forceinline__ bool finish_row(const HeadLoss& a, int64_t m, float2 
 // writes out and the factor of the earlier pieces' sums and, after the last piece, finishes
 // the row where no gradient follows.  After the last piece the blocks of a row share its
 // wanted entries' logits (sel).
-constexpr int kJoinCols = 8192;
+// A chunk is a multiple of 64 tiles: a wave looks at 64 tiles' exponents at once and, where
+// none differs from the row's, as in most rows, leaves their e alone.
 __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2* __restrict__ stats,
                                                         int64_t stat_tiles, int tw,
                                                         const float2* in, float2* out,
                                                         float* factor, uint16_t* e, int64_t lde,
-                                                        int64_t v0, int64_t tiles, bool last,
+                                                        int64_t v0, int tiles, int chunk, bool last,
                                                         float scale, float* sel) {
   __shared__ float red[4], red2[4], l2s[64];
   const int64_t m = blockIdx.x;
@@ -165,7 +192,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
     if (wave == 0) {
       // The first piece starts from nothing: its factor is never used on anything but zeros.
       const float f = in ? __builtin_amdgcn_exp2f(old.x - top) : 0.f;
-      now = make_float2(top, 
+      now = make_float2(top,
                         (in ? old.y * f : 0.f) + (red2[0] + red2[1]) + (red2[2] + red2[3]));
       if (lane == 0) {
         out[m] = now;
@@ -189,17 +216,20 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
   }
   if (!e) return;
   uint16_t* row = e + m * lde;
-  const int64_t c0 = (int64_t)blockIdx.y * kJoinCols;
-  const int64_t c1 = c0 + kJoinCols < lde ? c0 + kJoinCols : lde;
-  for (int64_t c = c0 + 8 * tid; c < c1; c += 2048) {
-    const int64_t t = c >> __builtin_ctz(tw);
-    if (t >= tiles) break;  // columns past the vocabulary hold zeros
-    const float f = __builtin_amdgcn_exp2f(st[t].x - top);
-    if (f == 1.f) continue;
-    u32x4 v = *reinterpret_cast<u32x4*>(row + c);
+  const int ta = (int)blockIdx.y * chunk, tb = ta + chunk < tiles ? ta + chunk : tiles;
+  const int64_t c0 = (int64_t)ta * tw, c1 = (int64_t)tb * tw;
+  for (int t0 = ta + 64 * wave; t0 < tb; t0 += 256) {
+    const float f = t0 + lane < tb ? __builtin_amdgcn_exp2f(st[t0 + lane].x - top) : 1.f;
+    if (!__any(f != 1.f)) continue;
+    for (int c = 8 * lane; c < 64 * tw; c += 512) {
+      const float ft = __shfl(f, c >> __builtin_ctz(tw), 64);
+      if (ft == 1.f) continue;
+      uint16_t* at = row + (int64_t)t0 * tw + c;
+      u32x4 v = *reinterpret_cast<u32x4*>(at);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2(bf16_lo(v[j]) * f, bf16_hi(v[j]) * f);
-    *reinterpret_cast<u32x4*>(row + c) = v;
+      for (int j = 0; j < 4; ++j) v[j] = pack_bf16x2(bf16_lo(v[j]) * ft, bf16_hi(v[j]) * ft);
+      *reinterpret_cast<u32x4*>(at) = v;
+    }
   }
   __syncthreads();
   for (int j = tid; j < a.k; j += 256) {
@@ -245,15 +275,24 @@ __global__ __launch_bounds__(256) void head_dh_kernel(HeadLoss a, const float* _
   v[0] *= factor;
   v[1] *= factor;
   if (c < a.K) {
-#pragma unroll 4
-    for (int i = WS > 1 ? wave : 0; i < a.k; i += WS) {
-      const int64_t id = token_of(a, m, i, false);
-      const float co = coef[i];
-      float wv[8];
-      deq8(a, id < 0 ? 0 : id, c, wv);
+    constexpr int B = 4;  // entries that are requested together
+    for (int i0 = WS > 1 ? wave : 0; i0 < a.k; i0 += B * WS) {
+      Packed8 p[B];
+      int id[B];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (id >= 0) v[j >> 2][j & 3] = __builtin_fmaf(co, wv[j], v[j >> 2][j & 3]);
+      for (int i = 0; i < B; ++i) {
+        id[i] = i0 + i * WS < a.k ? (int)token_of(a, m, i0 + i * WS, false) : -1;
+        p[i] = load8(a, id[i] < 0 ? 0 : id[i], (int)c);
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (__builtin_amdgcn_readfirstlane(id[i]) < 0) continue;
+        const float co = coef[i0 + i * WS];
+        float wv[8];
+        deq8(p[i], a.bits, wv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j >> 2][j & 3] = __builtin_fmaf(co, wv[j], v[j >> 2][j & 3]);
+      }
     }
   }
   if constexpr (WS > 1) {
@@ -354,13 +393,17 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   uint16_t* panel = p.panel ? reinterpret_cast<uint16_t*>(base + p.panel_at) : nullptr;
   // (in, out): the running state before and after the pieces joined so far.
   auto join = [&](int i, int64_t v0, int64_t n, int64_t lde) {
-    const int64_t chunks = (lde + kJoinCols - 1) / kJoinCols, shares = (a.k + 3) / 4;
-    const dim3 grid((unsigned)a.M, e ? (unsigned)std::max(chunks, v0 + n == a.V ? shares : 1) : 1u);
-    head_join_kernel<<<grid, 256, 0, stream>>>(a, stats, p.stat_tiles, p.stat_width,
-                                               i ? state + (i & 1) * a.M : nullptr,
-                                               state + ((i + 1) & 1) * a.M, factor, e, lde, v0,
-                                               (n + p.stat_width - 1) / p.stat_width,
-                                               v0 + n == a.V, scale, sel);
+    // About 4096 blocks: each reads all statistics of its row, so more of them cost (1000 rows of
+    // 128256 tokens, 64 entries: 148 us with 16 blocks a row, 110 with 4), and fewer leave
+    // compute units idle.
+    const int64_t tiles = (n + p.stat_width - 1) / p.stat_width;
+    const int64_t most = std::max((tiles + 63) / 64, v0 + n == a.V ? (a.k + 3) / 4 : (int64_t)1);
+    const int64_t by = e ? std::max<int64_t>(1, std::min(most, 4096 / a.M)) : 1;
+    const int64_t chunk = up((tiles + by - 1) / by, 64);
+    head_join_kernel<<<dim3((unsigned)a.M, (unsigned)by), 256, 0, stream>>>(
+        a, stats, p.stat_tiles, p.stat_width, i ? state + (i & 1) * a.M : nullptr,
+        state + ((i + 1) & 1) * a.M, factor, e, lde, v0, (int)tiles, (int)chunk, v0 + n == a.V, scale,
+        sel);
     return hipGetLastError();
   };
   for (int i = 0; i < p.pieces; ++i) {

@@ -75,6 +75,19 @@ def test_cross_entropy_wide_and_flat_logits(gpu, scale):
     ce_check(h, w, y, g, 4, 64)
 
 
+@pytest.mark.parametrize("M,V", [(60, 3000), (150, 30000), (1100, 12000)])
+def test_cross_entropy_tiles_of_different_exponents(gpu, M, V):
+    """Rows whose largest logits lie within and beyond +-32 and +-96 units of log 2, so that the
+    statistics of a row's tiles are relative to one power of two, two, or several."""
+    announce(f"ce exponents {M}x{V}")
+    h, w, y, g = ce_case(gpu, M, V, 256)
+    h = (h * torch.linspace(0.5, 40, M, device=gpu)[:, None]).bfloat16()
+    W = ref.values(*w, 4, 64)
+    top = (h.double() @ W.double().t()).amax(1) / 0.6931471805599453
+    assert top.min() < 28 and top.max() > 100
+    ce_check(h, w, y, g, 4, 64)
+
+
 def test_cross_entropy_confident_rows(gpu):
     """Targets that the head is sure of: p - 1 is a small difference of near equals."""
     announce("ce confident")
