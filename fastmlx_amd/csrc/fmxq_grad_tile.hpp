@@ -99,8 +99,11 @@ __device__ __forceinline__ void store_grad(const GradGemm& g, const f32x16 (&acc
 constexpr float kStatStep = 64.f;
 
 template <int MI, int NJ>
-__device__ __forceinline__ void store_stats(const GradGemm& g, const f32x16 (&acc)[MI][NJ],
-                                            int64_t mw, int64_t mend, int64_t nw) {
+__device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI][NJ], int64_t mw,
+                                            int64_t mend, int64_t nw) {
+  // The scaled logits are rounded once and the same values everywhere: an unrounded product
+  // passes the largest one by half a unit, which among logits of 1e10 is no power of two.
+#pragma clang fp contract(off)
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
   if (nw >= g.N) {  // no token here: zeros where a product reads whole tiles
     if (g.e)
@@ -123,9 +126,10 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, const f32x16 (&ac
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (full || nw + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) < g.N)
-          top = fmaxf(top, acc[i][j][r] * g.logit_scale);
+      for (int r = 0; r < 16; ++r) {
+        acc[i][j][r] *= g.logit_scale;
+        if (full || nw + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) < g.N) top = fmaxf(top, acc[i][j][r]);
+      }
     const float mx = kStatStep * rintf(fmaxf(top, other_half(top)) * (1.f / kStatStep));
     float sum = 0.f;
 #pragma unroll
@@ -136,7 +140,7 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, const f32x16 (&ac
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * q + e], g.logit_scale, -mx));
+          v[e] = __builtin_amdgcn_exp2f(acc[i][j][4 * q + e] - mx);
           if (!full && n + e >= g.N) v[e] = 0.f;
           sum += v[e];
         }

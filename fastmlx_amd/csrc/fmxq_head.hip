@@ -144,14 +144,15 @@ __device__ __forceinline__ bool finish_row(const HeadLoss& a, int64_t m, float2 
     a.loss[m] = empty ? 0.f : loss;
   }
   if (!a.dh) return !empty;
-  // p of an id that a row names twice counts once.
+  // p of an id that a row names twice counts once.  Its logit, summed in another order than
+  // those in lse, may pass it by their roundings.
   bool first = v >= 0;
   for (int j = 0; j < a.k; ++j) {
     const int32_t vj = __shfl((int)v, j, 64);
     if (j < lane && vj == (int32_t)v) first = false;
   }
   const float g = (a.grad_loss ? a.grad_loss[m] : 1.f) * T;
-  const float p = first ? __builtin_amdgcn_exp2f(l2 - lse2) : 0.f;
+  const float p = first ? __builtin_amdgcn_exp2f(fminf(l2 - lse2, 0.f)) : 0.f;
   *coef = v >= 0 ? g * (p - q) : 0.f;
   *factor = g / st.y;
   return !empty;

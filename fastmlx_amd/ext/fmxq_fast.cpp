@@ -372,6 +372,7 @@ PyObject* head_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t M = h->size(0), K = h->size(1), V = w->size(0);
     if (!weight_ok(*h, *w, *s, *b, K, group, bits) || (gl && !same(*gl, *h, {M}))) return nullptr;
     const int64_t k = distill ? ids->size(-1) : 1;
+    if (k > 64) return nullptr;  // refused there, before the int below
     if (distill ? ids->dim() != 2 || !same(*ids, *h, {M, k}) || !same(*t, *h, {M, k})
                 : !same(*ids, *h, {M}))
       return nullptr;

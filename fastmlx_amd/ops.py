@@ -419,7 +419,7 @@ def head_distill(h, w, scales, biases, ids, teacher, temperature: float = 1.0, g
     M, V, K, ptrs = _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits)
     if ids.dim() != 2:
         raise ValueError("ids must be [M, k]")
-    k = ids.shape[1]
+    k = min(ids.shape[1], 2**31 - 1)  # more than 64 are refused by the library
     _shape("ids", ids, M, k)
     _shape("teacher", teacher, M, k)
     ip = _dev(ids, "ids", (torch.int32,))

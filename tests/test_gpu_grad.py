@@ -88,6 +88,20 @@ def test_cross_entropy_tiles_of_different_exponents(gpu, M, V):
     ce_check(h, w, y, g, 4, 64)
 
 
+@pytest.mark.parametrize("M,V", [(12, 900), (150, 30000), (1100, 12000)])
+def test_logits_beyond_the_exponents_range(gpu, M, V):
+    """Logits of 1e9 and more, whose roundings are larger than any exponent of a power of two:
+    one token takes everything and the loss is a difference of logits."""
+    announce(f"ce huge logits {M}x{V}")
+    h, w, y, g = ce_case(gpu, M, V, 256)
+    h = (h * torch.logspace(8, 24, M, device=gpu)[:, None]).bfloat16()
+    got = ce_check(h, w, y, g, 4, 64)
+    assert all(torch.isfinite(t).all() for t in got)
+    ids, t = y.clamp(min=0)[:, None], torch.zeros(M, 1, device=gpu)
+    got = ops.head_distill((h * 0 + 1).bfloat16(), *w, ids, t, temperature=1e-10, grad=True)
+    assert all(torch.isfinite(t).all() for t in got)
+
+
 def test_cross_entropy_confident_rows(gpu):
     """Targets that the head is sure of: p - 1 is a small difference of near equals."""
     announce("ce confident")
