@@ -28,6 +28,8 @@ constexpr int64_t kSortMaxExperts = 2048;
 constexpr int64_t kMaxCount = 0x7fffffff;
 // Rows of a call: a launch has at most 2^32 threads, 256 a row.
 constexpr int64_t kMaxRows = (1 << 24) - 1;
+// Widths: the products' offsets into 256 rows of bf16 are 32 bits.
+constexpr int64_t kMaxWidth = (1 << 22) - 8;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -55,7 +57,7 @@ int head_sizes(int64_t M, int64_t V, int64_t K, int k, const char* op) {
   if (k < 1 || k > kHeadMaxTopK)
     return fail(FMXQ_ERR_SHAPE, "%s: top_k=%d outside 1..%d", op, k, kHeadMaxTopK);
   if (M > 0 && V == 0) return fail(FMXQ_ERR_SHAPE, "%s: %lld rows over no tokens", op, (long long)M);
-  if (M > kMaxRows || V > kMaxCount || K > (1 << 22))
+  if (M > kMaxRows || V > kMaxCount || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, V=%lld or K=%lld too large", op, (long long)M,
                 (long long)V, (long long)K);
   return FMXQ_OK;
@@ -89,7 +91,8 @@ struct GradPlan {
   bool panel, skinny;
   size_t pad, slices, panel_at, bytes;
 };
-// Rows from which the weights are dequantized to a panel beforehand.
+// Rows from which the weights are dequantized to a panel beforehand: 14336 x 4096, four tiles of
+// 256 rows take 149 us without, five 175 us with it.
 constexpr int64_t kGradPanelRows = 1025;
 
 // The rows of dy are copied to a stride of 8 values where N (or the address) is not one.
@@ -99,7 +102,7 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
   p.panel = M >= kGradPanelRows;
   p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M, true);
-  p.skinny = M <= fmxq::kSkinnyRows && fmxq::skinny_gemm_supported(pad_cols(N), N + 64, K);
+  p.skinny = M <= fmxq::kGradSkinnyRows && fmxq::skinny_gemm_supported(pad_cols(N), N + 64, K);
   const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.bm > 128 ? fmxq::kGradTileCols : fmxq::kGradCols;
   const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at
@@ -130,7 +133,7 @@ int grad_sizes(int64_t M, int64_t N, int64_t K, const char* op) {
   if (M < 0 || N < 0 || K < 0)
     return fail(FMXQ_ERR_SHAPE, "%s: negative size M=%lld N=%lld K=%lld", op, (long long)M,
                 (long long)N, (long long)K);
-  if (M > kMaxRows || N > (1 << 22) || K > (1 << 22))
+  if (M > kMaxRows || N > kMaxWidth || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, N=%lld or K=%lld too large", op, (long long)M,
                 (long long)N, (long long)K);
   return FMXQ_OK;

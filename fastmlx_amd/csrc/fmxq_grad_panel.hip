@@ -12,6 +12,10 @@
 // while the MFMAs of the 16 before run; the barrier sits before the last quarter's MFMAs,
 // when every wave has read the stage, so the next stage's first fragments and the DMA that
 // refills this one are under way while they run.
+//
+// Bound: MFMAs at the clock that the power limit leaves.  Measured for 2048 rows, 32064 x 4096:
+// the gradient 440 to 455 us, 1.18 to 1.22 PFLOP/s; the logits with their statistics 488 us,
+// 1.10 PFLOP/s (the epilogue's exponentials; a large library product ran at 1.20 there).
 #include <algorithm>
 #include <type_traits>
 

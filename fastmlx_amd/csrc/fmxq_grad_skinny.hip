@@ -1,14 +1,20 @@
-// fmxq_grad_skinny.hip -- the products of fmxq_grad_gemm.hip for up to 64 rows, where the
+// fmxq_grad_skinny.hip -- the products of fmxq_grad_gemm.hip for few rows, where the
 // packed weights are the work: every weight is read and dequantized once, in the registers
 // of the wave that multiplies it, with no stage in LDS and no barrier before the last sum.
 //
 // Logits: a block takes 32 tokens and up to 64 rows (more rows in chunks of 64 where the tokens
 // are few), its 8 waves every eighth 64-deep step of the hidden width; a lane holds 32 values
 // of one token's row.
-// Input gradients: a block takes 128 outputs and its waves every eighth step of 32 weight
+// Input gradients (48 rows at most): a block takes 128 outputs and its waves every eighth step of 32 weight
 // rows; lane r16 of quarter q4 holds the word of outputs 8 r16 .. + 8 in rows 8 q4 .. + 8, and
 // column r16 of v_mfma_f32_16x16x32_bf16's tile j is output 8 r16 + j, so that a word's values
 // go to eight tiles and never have to cross lanes.
+//
+// Bound: the dequantization's VALU instructions (6 a weight, with the roundings that make it
+// exact), and below about 20 us the launch, the first loads and the sum over the waves.
+// Measured: logits of one row, 32000 x 2048, 4 bits: 19.5 us; of 16 rows, 32000 x 2560 in
+// groups of 32: 28.6 us; of 37 rows, 50257 x 1024, 8 bits: 26.8 us; gradients of the last two
+// 28.4 and 31.7 us; of 13 rows, 4096 x 4096: 8.8 us.
 #include <type_traits>
 
 #include "fmxq_grad_tile.hpp"
@@ -367,24 +373,20 @@ bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols
 
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
   if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats) ||
-      (nn && g.M > kSkinnyRows) ||
+      (nn && g.M > kGradSkinnyRows) ||
       !skinny_gemm_supported(g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.offsets || g.lda % 8 ||
       g.a_cols % 8 || g.c_split % 16)
     return hipErrorInvalidValue;
   if (g.M < 1 || g.N < 1 || g.splits < 1) return hipSuccess;
   if (nn) {
-    // Tiles of 48 rows save a quarter of the products of 64 (37 rows through 4096 x 4096: 23.6
-    // against 27.5 us).
     const int mt = (int)(g.M + 15) / 16;
     if (g.bits == 4)
       return mt == 1   ? launch_grad<4, 1>(g, stream)
              : mt == 2 ? launch_grad<4, 2>(g, stream)
-             : mt == 3 ? launch_grad<4, 3>(g, stream)
-                       : launch_grad<4, 4>(g, stream);
+                       : launch_grad<4, 3>(g, stream);
     return mt == 1   ? launch_grad<8, 1>(g, stream)
            : mt == 2 ? launch_grad<8, 2>(g, stream)
-           : mt == 3 ? launch_grad<8, 3>(g, stream)
-                     : launch_grad<8, 4>(g, stream);
+                     : launch_grad<8, 3>(g, stream);
   }
   if (g.bits == 4) return g.M <= 32 ? launch_logits<4, 1>(g, stream) : launch_logits<4, 2>(g, stream);
   return g.M <= 32 ? launch_logits<8, 1>(g, stream) : launch_logits<8, 2>(g, stream);

@@ -11,9 +11,13 @@
 // brings the tiles of a row to one m (a power of two: no second rounding; with m the largest l
 // itself nearly all tiles needed it, which took 50 us of a piece of 2048 rows by 32064 tokens
 // where the join now takes 17), and e . deq(W) is added to fp32 sums that are scaled by the
-// change of m.  The wanted entries' e are zeroed
-// and their share p_j - q_j enters at the end in fp32: where p_j nears q_j the two cancel,
-// and bf16 values of them would leave their rounding.
+// change of m.  The wanted entries' e are zeroed and their share p_j - q_j enters at the end in
+// fp32: where p_j nears q_j the two cancel, and bf16 values of them would leave their rounding.
+//
+// e and the weights' panel pass through memory because a piece of either (256 MB at most) stays
+// in the last-level cache; recomputing the logits for the gradient would cost a third product.
+// Bound: the two products.  2048 rows, 128256 x 4096: 3.96 ms, of them the products 3.75, the
+// panels 0.24 and the kernels here 0.09 ms.
 #include <algorithm>
 
 #include "fmxq_common.hpp"
@@ -325,8 +329,11 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // Most bytes of a piece's e, and of its panel of dequantized weights.
 constexpr int64_t kHeadPieceBytes = 256 << 20;
 constexpr int64_t kHeadPanelBytes = 256 << 20;
-// Rows from which the weights are dequantized to a panel beforehand.
-constexpr int64_t kHeadPanelRows = 1025;
+// Rows from which the weights are dequantized to a panel beforehand: for two products, where
+// five tiles of 256 rows take as long either way (128256 x 4096: 2.75 ms) and eight 4.0 against
+// 4.4 ms; for the logits alone, where the panel's 0.24 ms are won back later (1025 rows 1.34
+// against 1.50 ms, 1700 rows 1.89 against 2.07, 2048 rows 2.13 against 2.09).
+constexpr int64_t kHeadPanelRows = 1025, kScorePanelRows = 1793;
 
 // Few tokens for many rows: the tiles of the logits leave most of the chip idle and each walks
 // the whole width, about 2 us a 64-deep step; the kernel for few rows has a block for every
@@ -341,16 +348,16 @@ bool few_tokens(int64_t M, int64_t V, int bm, int cus) {
 
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
-  p.panel = M >= kHeadPanelRows;
+  p.panel = M >= (grad ? kHeadPanelRows : kScorePanelRows);
   p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M, false), 128);
-  p.grad_bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M, true), 128);
+  p.grad_bm = p.panel ? kPanelRows : grad_gemm_rows(M, true);
   int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
   if (p.panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
   p.pieces = (int)((V + piece - 1) / piece);
   piece = up((V + p.pieces - 1) / p.pieces, kGradTileCols);
   p.pieces = (int)((V + piece - 1) / piece);
   p.piece = piece;
-  p.grad_skinny = M <= kSkinnyRows && skinny_gemm_supported(piece, piece, K);
+  p.grad_skinny = M <= kGradSkinnyRows && skinny_gemm_supported(piece, piece, K);
   p.skinny = skinny_gemm_supported(K, 32, K) && (M <= kSkinnyRows || few_tokens(M, piece, p.bm, cus));
   p.stat_width = p.skinny ? kSkinnyStatWidth : p.panel ? kPanelStatWidth : kGradStatWidth;
   // Without a gradient the tiles of all pieces are joined at once.

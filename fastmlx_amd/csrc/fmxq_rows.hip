@@ -6,6 +6,10 @@
 // e.  Ids >= E sort behind offsets[E]; their rows are zero and they raise the error flag.
 // The row kernels work by token: x (or dout) is read once for its k slots, and the sums of a
 // token are fp32, rounded once.
+//
+// Bound: HBM; a call of few rows by its launch.  Measured for 8192 tokens of 8 slots, 7168 wide:
+// the sort 16 us and its rows 183 us (5.8 TB/s), the sums 246 us (4.3 TB/s), the gradients of
+// rows and weights 375 us (5.3 TB/s); a large copy ran at 4.5 to 5.0 TB/s.
 #include <algorithm>
 
 #include "fmxq_common.hpp"

@@ -48,7 +48,9 @@ CE = [(1, 1, 32, 4, 32), (1, 1000, 64, 4, 64), (2, 7, 96, 8, 32), (5, 255, 128, 
       (100, 40000, 256, 4, 128), (70, 60001, 96, 8, 32), (300, 20000, 96, 4, 32),
       (200, 30001, 192, 8, 64), (1000, 9001, 160, 4, 32), (1024, 12800, 320, 4, 64),
       # panels, the last step of 32 values, widths below a tile
-      (1100, 24001, 96, 4, 32), (1300, 20001, 320, 8, 64), (2050, 10240, 1056, 4, 32)]
+      (1100, 24001, 96, 4, 32), (1300, 20001, 320, 8, 64), (2050, 10240, 1056, 4, 32),
+      # the logits alone on panels too, and gradients in the lowest tiles
+      (2900, 14001, 96, 8, 32), (50, 12345, 1056, 8, 32), (64, 30000, 256, 4, 64)]
 
 
 @pytest.mark.parametrize("M,V,K,bits,group", CE)
@@ -282,6 +284,21 @@ def test_quantized_matmul_grad(gpu, M, N, K, bits, group):
     dy = hidden(gen, M, N, gpu)
     ref.check(ops.quantized_matmul_grad(dy, *w, group, bits),
               *ref.product(dy, ref.values(*w, bits, group)), "dx")
+
+
+@pytest.mark.parametrize("M", [2, 66])
+def test_quantized_matmul_grad_of_the_widest_rows(gpu, M):
+    """2^22 - 8 values a row: 64 and 256 rows of dy end just below 2^29 and 2^31 bytes."""
+    N = (1 << 22) - 8
+    announce(f"grad {M}x{N}x32")
+    gen = torch.Generator().manual_seed(M)
+    w = ref.quant(gen, (N,), 32, 4, 32, gpu)
+    dy = torch.zeros(M, N, device=gpu, dtype=torch.bfloat16)
+    dy[:, -5000:] = torch.randn(M, 5000, generator=gen).bfloat16().to(gpu)
+    dy[:, :700] = torch.randn(M, 700, generator=gen).bfloat16().to(gpu)
+    at = torch.cat([torch.arange(700), torch.arange(N - 5000, N)]).to(gpu)
+    y, e = ref.product(dy[:, at], ref.values(w[0][at], w[1][at], w[2][at], 4, 32))
+    ref.check(ops.quantized_matmul_grad(dy, *w, 32, 4), y, e, "dx")
 
 
 def test_quantized_matmul_grad_takes_batches_and_any_alignment(gpu):

@@ -71,6 +71,12 @@ def test_quantized_matmul_grad_refuses(kw, want):
     assert grad(**kw) == "FMXQ_ERR_" + want
 
 
+def test_widths_past_the_products_offsets_are_refused():
+    n = (1 << 22) - 7
+    assert grad(N=n) == gather(N=n) == "FMXQ_ERR_SHAPE"
+    assert grad(K=1 << 22) == gather(K=1 << 22) == ce(K=1 << 22) == "FMXQ_ERR_SHAPE"
+
+
 @pytest.mark.parametrize("kw,want", [
     (dict(E=0), "SHAPE"), (dict(E=-1), "SHAPE"), (dict(S=-1), "SHAPE"),
     (dict(off=None), "INVALID_ARGUMENT"), (dict(dy=None), "INVALID_ARGUMENT"),
