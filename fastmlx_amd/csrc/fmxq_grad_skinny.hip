@@ -3,12 +3,12 @@
 // of the wave that multiplies it, with no stage in LDS and no barrier before the last sum.
 //
 // Logits: a block takes 32 tokens and up to 64 rows (more rows in chunks of 64 where the tokens
-// are few), its 8 waves every eighth 64-deep step of the hidden width; a lane holds 32 values
-// of one token's row.
-// Input gradients (48 rows at most): a block takes 128 outputs and its waves every eighth step of 32 weight
-// rows; lane r16 of quarter q4 holds the word of outputs 8 r16 .. + 8 in rows 8 q4 .. + 8, and
-// column r16 of v_mfma_f32_16x16x32_bf16's tile j is output 8 r16 + j, so that a word's values
-// go to eight tiles and never have to cross lanes.
+// are few), each of its 8 waves an eighth of the hidden width in 64-deep steps; a lane holds 32
+// values of one token's row.
+// Input gradients (48 rows at most): a block takes 128 outputs and its waves every eighth step
+// of 32 weight rows; lane r16 of quarter q4 holds the word of outputs 8 r16 .. + 8 in rows
+// 8 q4 .. + 8, and column r16 of v_mfma_f32_16x16x32_bf16's tile j is output 8 r16 + j, so that
+// a word's values go to eight tiles and never have to cross lanes.
 //
 // Bound: the dequantization's VALU instructions (6 a weight, with the roundings that make it
 // exact), and below about 20 us the launch, the first loads and the sum over the waves.
