@@ -8,7 +8,7 @@
 // token are fp32, rounded once.
 //
 // Bound: HBM; a call of few rows by its launch.  Measured for 8192 tokens of 8 slots, 7168 wide:
-// the sort 16 us and its rows 183 us (5.8 TB/s), the sums 246 us (4.3 TB/s), the gradients of
+// the sort 16 us and its rows 183 us (5.8 TB/s), the sums 189 us (5.6 TB/s), the gradients of
 // rows and weights 375 us (5.3 TB/s); a large copy ran at 4.5 to 5.0 TB/s.
 #include <algorithm>
 
@@ -146,6 +146,9 @@ struct Row<8> {
   __device__ __forceinline__ static Row load(const uint16_t* p) {
     return {*reinterpret_cast<const u32x4*>(p)};
   }
+  __device__ __forceinline__ static Row stream(const uint16_t* p) {
+    return {__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p))};
+  }
   __device__ __forceinline__ void store(uint16_t* p) const { *reinterpret_cast<u32x4*>(p) = v; }
   __device__ __forceinline__ float at(int i) const {
     return i & 1 ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]);
@@ -159,6 +162,7 @@ template <>
 struct Row<1> {
   uint16_t v;
   __device__ __forceinline__ static Row load(const uint16_t* p) { return {*p}; }
+  __device__ __forceinline__ static Row stream(const uint16_t* p) { return load(p); }
   __device__ __forceinline__ void store(uint16_t* p) const { *p = v; }
   __device__ __forceinline__ float at(int) const { return bf16_bits_to_f32(v); }
   __device__ __forceinline__ static Row of(const float* f) {
@@ -269,9 +273,11 @@ __global__ __launch_bounds__(256) void sort_small_kernel(MoeSort a, int S) {
   }
 }
 
+constexpr int64_t kCacheBytes = 256 << 20;  // the last-level cache
+
 // out[t] = sum_j w[t, j] y[pos[t, j]] in the order of j; a position outside the rows adds
 // nothing.  Eight rows are requested before any is added.
-template <int VEC>
+template <int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void rows_sum_kernel(const uint16_t* __restrict__ y,
                                                        const uint32_t* __restrict__ pos,
                                                        const void* __restrict__ weights,
@@ -296,7 +302,7 @@ __global__ __launch_bounds__(256) void rows_sum_kernel(const uint16_t* __restric
         v[j] = Row<VEC>{};
         w[j] = 0.f;
         if (on[j]) {
-          v[j] = Row<VEC>::load(y + p * D + c);
+          v[j] = STREAM ? Row<VEC>::stream(y + p * D + c) : Row<VEC>::load(y + p * D + c);
           w[j] = weights ? weight_of(weights, wbf16, t * k + j0 + j) : 1.f;
         } else if (in && c == 0) {
           atomicOr(flag, 1u);
@@ -395,12 +401,16 @@ hipError_t launch_moe_sort(const MoeSort& a, hipStream_t stream) {
 hipError_t launch_moe_unsort(const uint16_t* y, const uint32_t* pos, const void* weights,
                              bool weights_bf16, uint16_t* out, int64_t T, int64_t k, int64_t D,
                              uint32_t* flag, hipStream_t stream) {
-  if (vec8(D, y, out, nullptr))
-    rows_sum_kernel<8><<<row_grid(T, D, 8), 256, 0, stream>>>(y, pos, weights, weights_bf16, out,
-                                                              T * k, k, D, flag);
+  // Rows that do not fit the last-level cache are read past it (8192 x 8 rows 7168 wide 189
+  // against 216 us); smaller ones are read again by the gradients (all four calls of 4096 x 4
+  // rows 2048 wide 74 us, 76 with such reads).
+  const dim3 grid = row_grid(T, D, vec8(D, y, out, nullptr) ? 8 : 1);
+  if (!vec8(D, y, out, nullptr))
+    rows_sum_kernel<1, false><<<grid, 256, 0, stream>>>(y, pos, weights, weights_bf16, out, T * k, k, D, flag);
+  else if (T * k * D * 2 > kCacheBytes)
+    rows_sum_kernel<8, true><<<grid, 256, 0, stream>>>(y, pos, weights, weights_bf16, out, T * k, k, D, flag);
   else
-    rows_sum_kernel<1><<<row_grid(T, D, 1), 256, 0, stream>>>(y, pos, weights, weights_bf16, out,
-                                                              T * k, k, D, flag);
+    rows_sum_kernel<8, false><<<grid, 256, 0, stream>>>(y, pos, weights, weights_bf16, out, T * k, k, D, flag);
   return hipGetLastError();
 }
 

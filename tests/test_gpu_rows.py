@@ -64,6 +64,21 @@ def test_unsort_and_gradients(gpu, T, k, E, D, dtype):
     ops.device_error()
 
 
+def test_sums_of_rows_larger_than_the_cache(gpu):
+    T, k, E, D = 4200, 8, 16, 4096
+    announce(f"sums {T}x{k}, {D} wide")
+    x, inds, w, y, _ = case(gpu, T, k, E, D, torch.bfloat16)
+    pos = ops.moe_sort(x, inds, E)[2]
+    half = ref.HALF[torch.bfloat16]
+    for got, weights in ((ops.moe_unsort(y, pos, w), w.double()),
+                         (ops.moe_sort_grad(y, pos), torch.ones_like(w).double())):
+        for t in range(0, T, 700):  # in parts, for the 64-bit copies' memory
+            terms = y[pos[t:t + 700].long()].double() * weights[t:t + 700, :, None]
+            e = (k + 2) * ref.U32 * terms.abs().sum(1)
+            ref.check(got[t:t + 700], terms.sum(1), e + half * (terms.sum(1).abs() + e), "sums")
+    ops.device_error()
+
+
 def test_empty(gpu):
     announce("no tokens")
     x = torch.empty(0, 16, dtype=torch.bfloat16, device=gpu)
