@@ -57,6 +57,7 @@ int head_sizes(int64_t M, int64_t V, int64_t K, int k, const char* op) {
   if (k < 1 || k > kHeadMaxTopK)
     return fail(FMXQ_ERR_SHAPE, "%s: top_k=%d outside 1..%d", op, k, kHeadMaxTopK);
   if (M > 0 && V == 0) return fail(FMXQ_ERR_SHAPE, "%s: %lld rows over no tokens", op, (long long)M);
+  if (M > 0 && K == 0) return fail(FMXQ_ERR_SHAPE, "%s: %lld rows of no width", op, (long long)M);
   if (M > kMaxRows || V > kMaxCount || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, V=%lld or K=%lld too large", op, (long long)M,
                 (long long)V, (long long)K);

@@ -147,3 +147,10 @@ def test_torch_wrappers_refuse_cpu_tensors_and_shapes():
             call()
     with pytest.raises(TypeError):
         ops.moe_sort(None, y, 4)
+
+
+@pytest.mark.parametrize("M", [4, 5000])
+@pytest.mark.parametrize("grad", [False, True])
+def test_head_workspace_refuses_rows_of_no_width(M, grad):
+    assert ws("fmxq_head_workspace", M, 100, 0, 1, grad)[0] == "FMXQ_ERR_SHAPE"
+    assert ws("fmxq_head_workspace", 0, 100, 0, 1, grad) == ("FMXQ_OK", 0)
