@@ -41,8 +41,14 @@ struct GradGemm {
   // tiles of stat_width columns: stats[row][tile] = (m, sum 2^(l - m)) with m the tile's
   // largest l rounded up to an integer, and, with e, e[row][col] = bf16(2^(l - m)) with
   // zeros in columns N .. lde.
+  // The row's wanted tokens take no part (their e is 0): ids wanted[row][0 .. wanted_k] of tokens
+  // counted from -first_token on, other than wanted_none.
   float2* stats = nullptr;
   int64_t stat_tiles = 0;
+  const int32_t* wanted = nullptr;
+  int wanted_k = 0;
+  int32_t wanted_none = -1;
+  int64_t first_token = 0;
   uint16_t* e = nullptr;
   int64_t lde = 0;
   float logit_scale = 1.f;

@@ -160,6 +160,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
   __shared__ __attribute__((aligned(1024))) uint8_t as2[AS > 2 ? BM * 128 : 16];
   __shared__ __attribute__((aligned(1024))) uint8_t bs0[BN * 128];
   __shared__ __attribute__((aligned(1024))) uint8_t bs1[BN * 128];
+  __shared__ int32_t one[NN ? 1 : BM];  // the rows' wanted tokens, where they have one
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -422,6 +423,8 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
     dequant(pk[a2s], b, 0);
     pace(1);
   };
+  int32_t id = -1;
+  if (!NN && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
   if (nk > 0) {
 #pragma unroll
     for (int i = 0; i < AS; ++i) {  // the waits count on this order
@@ -433,6 +436,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
     share(pk[0]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) dequant(pk[0], 0, t);
+    if (!NN && tid < BM) one[tid] = id;  // the loads behind it have landed
     __builtin_amdgcn_s_waitcnt(wait_enc((AS - 1) * (XI + NLD), 0));
     __builtin_amdgcn_s_barrier();
     issue_b(AS, pk[0]);
@@ -466,7 +470,12 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
   }
   const int64_t mw = m0 + wm * MI * 32, nw = n0 + wn * NJ * 32;
   if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
-  else store_stats<MI, NJ>(g, acc, mw, m0 + rows, nw);
+  else {
+    uint32_t out[MI][NJ];
+    find_wanted<BM, BN, W * 64>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
+                                      out);
+    store_stats<MI, NJ>(g, acc, out, mw, m0 + rows, nw);
+  }
 }
 
 template <int BM, bool NN>
@@ -499,7 +508,7 @@ int grad_gemm_rows(int64_t M, bool nn) { return M <= 32 ? 32 : M <= 64 ? 64 : M 
 
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream) {
   // Offsets into one tile's rows and into 64 or 256 weight rows are 32 bits.
-  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats) || 256 * g.lda * 2 >= 0x7ffffff0LL ||
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || 256 * g.lda * 2 >= 0x7ffffff0LL ||
       256 * (nn ? g.N : g.C) >= 0x7ffffff0LL || g.c_split % kS || g.lda % 8 || g.a_cols % 8 ||
       (g.offsets && (!nn || !g.y || !g.flag || g.splits != 1)))
     return hipErrorInvalidValue;

@@ -37,6 +37,7 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   __shared__ __attribute__((aligned(1024))) uint8_t as1[BM * 128];
   __shared__ __attribute__((aligned(1024))) uint8_t bs0[kN * 128];
   __shared__ __attribute__((aligned(1024))) uint8_t bs1[kN * 128];
+  __shared__ int32_t one[NN ? 1 : BM];  // the rows' wanted tokens, where they have one
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
@@ -185,11 +186,14 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // VMEM (the DMA)
     }
   };
+  int32_t id = -1;
+  if (!NN && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
   if (nk > 0) {
     issue(0, 0);
     __builtin_amdgcn_sched_barrier(0);  // the wait counts on this order
     issue(1, 1);
     __builtin_amdgcn_s_waitcnt(wait_enc(XI + YI, 15));
+    if (!NN) one[tid] = id;
     __builtin_amdgcn_s_barrier();
     read(a0, b0, 0, 0);
     // Two steps a turn, the last one on zeros where nk is odd.
@@ -201,13 +205,18 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   }
   const int64_t mw = m0 + wm * MI * 32, nw = n0 + wn * NJ * 32;
   if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
-  else store_stats<MI, NJ>(g, acc, mw, m0 + rows, nw);
+  else {
+    uint32_t out[MI][NJ];
+    find_wanted<BM, kN, 256>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
+                                 out);
+    store_stats<MI, NJ>(g, acc, out, mw, m0 + rows, nw);
+  }
 }
 
 }  // namespace
 
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats) || 
+  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || 
       kPanelRows * g.lda * 2 >= 0x7ffffff0LL || (kN + 1) * g.ldp * 2 >= 0x7ffffff0LL || g.c_split % kS ||
       g.lda % 8 || g.a_cols % 8 || g.ldp % 8 || g.offsets)
     return hipErrorInvalidValue;

@@ -140,6 +140,11 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
                                                          0, 0, 0);
     }
   }
+  // The first id that the lane's row of the tile it finishes wants is on its way while the waves
+  // meet; a row's two lanes share its ids.
+  const bool wanting = wave < MT && 32 * wave + r32 < M;
+  const int32_t* want = g.wanted + (m0 + 32 * wave + r32) * g.wanted_k;
+  const int32_t id0 = wanting && h < g.wanted_k ? want[h] : g.wanted_none;
   // The waves' sums, in the order of the waves; wave m finishes row tile m.
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -149,6 +154,17 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
           f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
   __syncthreads();
   if (wave >= MT) return;
+  uint32_t out[1][1] = {{0u}};
+  auto find = [&](int32_t id) {
+    const uint32_t c = wanted_column(g, id, n0);
+    if (c < 32) out[0][0] |= 1u << c;
+  };
+  find(id0);
+  if (wanting) {
+#pragma unroll 4
+    for (int j = h + 2; j < g.wanted_k; j += 2) find(want[j]);
+  }
+  out[0][0] |= other_half(out[0][0]);
   f32x16 sum[1][1];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -162,7 +178,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[0][0][4 * q + e] = v[e];
   }
-  store_stats<1, 1>(g, sum, m0 + 32 * wave, g.M, n0);
+  store_stats<1, 1>(g, sum, out, m0 + 32 * wave, g.M, n0);
 }
 
 template <int BITS, int MT, bool G32>
@@ -372,7 +388,7 @@ bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols
 }
 
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats) ||
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats || !g.wanted) ||
       (nn && g.M > kGradSkinnyRows) ||
       !skinny_gemm_supported(g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.offsets || g.lda % 8 ||
       g.a_cols % 8 || g.c_split % 16)

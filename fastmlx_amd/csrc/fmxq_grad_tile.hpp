@@ -44,10 +44,12 @@ __device__ __forceinline__ uint32_t deq_pair(float q0, float q1, float s0, float
 }
 
 // The other half of the wave's value.
-__device__ __forceinline__ float other_half(float v) {
-  const uint32_t u = __float_as_uint(v);
+__device__ __forceinline__ uint32_t other_half(uint32_t u) {
   const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
+  return (threadIdx.x & 32) ? p[0] : p[1];
+}
+__device__ __forceinline__ float other_half(float v) {
+  return __uint_as_float(other_half(__float_as_uint(v)));
 }
 
 // Rows mw .. of 32 MI (below mend), columns nw .. of 32 NJ: input gradients.
@@ -92,15 +94,67 @@ __device__ __forceinline__ void store_grad(const GradGemm& g, const f32x16 (&acc
   }
 }
 
+// The column of an id that a row wants, counted from n0; ids of no token land behind the last.
+__device__ __forceinline__ uint32_t wanted_column(const GradGemm& g, int32_t id, int64_t n0) {
+  return id == g.wanted_none ? ~0u : (uint32_t)id - (uint32_t)(g.first_token + n0);
+}
+
+// out[i][j]: a bit for each of the 32 columns from nw + 32 j on that the lane's row of group i (from
+// mw on) of the tile of BM x BN at (m0, n0) wants.  One id a row: the block has read them to `one`.
+// Of more, all T threads of the block read the tile's rows' ids here, and their bits meet in
+// `lds` (BM * BN / 8 bytes that no wave uses any more).
+template <int BM, int BN, int T, int MI, int NJ>
+__device__ __forceinline__ void find_wanted(const GradGemm& g, int64_t m0, int64_t rows, int64_t n0,
+                                            int64_t mw, int64_t nw, const int32_t* one,
+                                            uint32_t* lds, uint32_t (&out)[MI][NJ]) {
+  const int r32 = threadIdx.x & 31;
+  if (g.wanted_k == 1) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const uint32_t c = wanted_column(g, one[mw - m0 + 32 * i + r32], nw);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) out[i][j] = c >> 5 == (uint32_t)j ? 1u << (c & 31) : 0u;
+    }
+    return;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < BM * BN / 32; i += T) lds[i] = 0;
+  __syncthreads();
+  const uint32_t k = (uint32_t)g.wanted_k, n = (uint32_t)rows * k;
+  constexpr int B = 16;  // ids that are requested together
+  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += B * T) {
+    int32_t id[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) id[j] = g.wanted[m0 * k + (i0 + j * T < n ? i0 + j * T : i0)];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const uint32_t i = i0 + j * T, c = wanted_column(g, id[j], n0);
+      if (c < BN && i < n) atomicOr(&lds[i / k * (BN / 32) + (c >> 5)], 1u << (c & 31));
+    }
+  }
+  __syncthreads();
+  const uint32_t* mine = lds + (mw - m0 + r32) * (BN / 32) + (nw - n0) / 32;
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) out[i][j] = mine[i * 32 * (BN / 32) + j];
+}
+
 // The softmax statistics of a tile of 32 NJ columns, and e.  They are relative to the nearest
 // multiple of kStatStep (units of log 2) to the row's largest logit in the tile: bf16 and fp32
 // keep their precision at any exponent, so tiles of a row whose logits reach about as far share
 // one and need no rescaling, and where they differ 2^-kStatStep is still a normal number.
+//
+// The row's wanted tokens are left out, and enter the row's sums with its loss: where one of them
+// takes nearly everything, what the others leave is the loss, and could not be had from a sum
+// that holds both (out: find_wanted's bits).  A tile without other tokens has the sum 0 of kNoStat.
 constexpr float kStatStep = 64.f;
+constexpr float kNoStat = -3.4028234663852886e38f;  // below every tile's; differences stay numbers
 
 template <int MI, int NJ>
-__device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI][NJ], int64_t mw,
-                                            int64_t mend, int64_t nw) {
+__device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI][NJ],
+                                            const uint32_t (&out)[MI][NJ], int64_t mw, int64_t mend,
+                                            int64_t nw) {
   // The scaled logits are rounded once and the same values everywhere: an unrounded product
   // passes the largest one by half a unit, which among logits of 1e10 is no power of two.
 #pragma clang fp contract(off)
@@ -122,6 +176,18 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI]
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int64_t m = mw + 32 * i + r32;
+    uint32_t some = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) some |= out[i][j];
+    if (__any(some != 0))
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if (!__any(out[i][j] != 0)) continue;
+        const uint32_t mine = out[i][j] >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if ((mine >> (8 * (r >> 2) + (r & 3))) & 1u) acc[i][j][r] = -INFINITY;
+      }
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
@@ -130,7 +196,8 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI]
         acc[i][j][r] *= g.logit_scale;
         if (full || nw + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) < g.N) top = fmaxf(top, acc[i][j][r]);
       }
-    const float mx = kStatStep * rintf(fmaxf(top, other_half(top)) * (1.f / kStatStep));
+    top = fmaxf(top, other_half(top));
+    const float mx = top == -INFINITY ? kNoStat : kStatStep * rintf(top * (1.f / kStatStep));
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)

@@ -11,8 +11,9 @@
 // brings the tiles of a row to one m (a power of two: no second rounding; with m the largest l
 // itself nearly all tiles needed it, which took 50 us of a piece of 2048 rows by 32064 tokens
 // where the join now takes 17), and e . deq(W) is added to fp32 sums that are scaled by the
-// change of m.  The wanted entries' e are zeroed and their share p_j - q_j enters at the end in
-// fp32: where p_j nears q_j the two cancel, and bf16 values of them would leave their rounding.
+// change of m.  The wanted entries are left out of e and of the sums.  Their exponentials and their
+// share p_j - q_j enter at the end in fp32: where one of them takes nearly everything, the loss and
+// the gradient are what the other tokens leave, which no sum over all of them holds.
 //
 // e and the weights' panel pass through memory because a piece of either (256 MB at most) stays
 // in the last-level cache; recomputing the logits for the gradient would cost a third product.
@@ -112,58 +113,142 @@ __device__ __forceinline__ float logit_of(const HeadLoss& a, int64_t m, int64_t 
   return wave_sum(t) * scale;
 }
 
-// One wave: lse and the loss (stored where `store`) from the row's final (m, sum) and lane j's
-// logit l2 of entry j; the lane's coefficient of W_id and the factor of the sums over e.
-// False for a row without a wanted entry, whose loss and gradient are 0.
-__device__ __forceinline__ bool finish_row(const HeadLoss& a, int64_t m, float2 st, float l2,
-                                           bool store, float* coef, float* factor) {
+// d - 1 + exp(-d) for |d| < 1/2, where it nears d^2 / 2: its series, cut off below 1e-7 of it.
+__device__ __forceinline__ float excess(float d) {
+  float s = 1.f / 40320;
+  s = __builtin_fmaf(s, d, -1.f / 5040);
+  s = __builtin_fmaf(s, d, 1.f / 720);
+  s = __builtin_fmaf(s, d, -1.f / 120);
+  s = __builtin_fmaf(s, d, 1.f / 24);
+  s = __builtin_fmaf(s, d, -1.f / 6);
+  s = __builtin_fmaf(s, d, 0.5f);
+  return s * (d * d);
+}
+
+// A row's tokens, lane j's entry among them, from the row's final (m, sum over the tokens that are
+// not wanted) and the entry's logit l2: exponentials relative to 2^top.
+//
+// Nothing in it is the difference of near equals, which a row that is sure of what it wants would
+// make of log q - log p and of p - q (a loss of 1e-6 came out as one of -3e-6): 1 - p of the likeliest
+// entry is what the others leave, and its -log p is log1p of their ratio; q alike.
+struct HeadRow {
+  int v;                // the lane's token, or -1
+  bool first, twice;    // an id that a row names twice is one token
+  bool led, t_led;      // the likeliest entry, of the row's and of the teacher's
+  bool empty;           // no wanted entry: loss and gradient are 0
+  float l, e, p;
+  float top, rest, rest_scale;  // rest: the tokens that are not wanted
+  float others, z;              // all tokens but the likeliest entry; all
+  float t, t_top, t_others, q;  // cross entropy: a teacher with one entry
+};
+// An entry's logit, and whether the row names its token in an earlier entry or in another one.
+struct Entry {
+  float l2;
+  uint32_t again, twice;
+};
+__device__ __forceinline__ HeadRow read_row(const HeadLoss& a, int64_t m, float2 st, Entry en) {
   const int lane = threadIdx.x & 63;
-  const float lse2 = st.x + __builtin_amdgcn_logf(st.y);  // in units of log 2
-  const float T = a.temperature;
-  const bool on = lane < a.k;
-  const int64_t v = on ? token_of(a, m, lane, false) : -1;
-  float q = v >= 0 ? 1.f : 0.f, logq = 0.f;
-  bool empty;
-  if (a.teacher) {
-    float t = -INFINITY;
-    if (v >= 0)
-      t = (a.teacher_bf16
-               ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.teacher)[m * a.k + lane])
-               : reinterpret_cast<const float*>(a.teacher)[m * a.k + lane]) * (kLog2e / T);
-    const float top = wave_max(t);
-    const bool nan = __any(t != t);
-    empty = top == -INFINITY && !nan;
-    q = empty ? 0.f : __builtin_amdgcn_exp2f(t - top);
-    const float s = wave_sum(q);
-    logq = (t - top) - __builtin_amdgcn_logf(s);
-    q = empty ? 0.f : q / s;
+  HeadRow r;
+  r.v = -1;
+  r.t = -INFINITY;
+  if (lane < a.k) {
+    if (!a.teacher) r.t = 0.f;
+    else if (a.teacher_bf16) r.t = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(a.teacher)[m * a.k + lane]);
+    else r.t = reinterpret_cast<const float*>(a.teacher)[m * a.k + lane];
+    r.v = (int)token_of(a, m, lane, false);
+  }
+  r.first = r.v >= 0 && !en.again;
+  r.twice = r.v >= 0 && en.twice;
+  r.l = r.v >= 0 ? en.l2 : -INFINITY;
+  r.t = r.v >= 0 ? r.t * (kLog2e / a.temperature) : -INFINITY;
+  float most = r.l;
+  r.t_top = r.t;
+  if (a.k > 1) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      most = fmaxf(most, __shfl_xor(most, o, 64));
+      r.t_top = fmaxf(r.t_top, __shfl_xor(r.t_top, o, 64));
+    }
   } else {
-    empty = !__any(v >= 0);
+    most = __shfl(most, 0, 64);
+    r.t_top = __shfl(r.t_top, 0, 64);
   }
-  // Entries of no weight add nothing (0 log 0 = 0); NaN stays.
-  const float term = v >= 0 && q != 0.f ? q * (logq - l2 + lse2) : 0.f;
-  const float loss = wave_sum(term) * (T * T * kLn2);
-  if (store && lane == 0) {
-    a.lse[m] = lse2 * kLn2;
-    a.loss[m] = empty ? 0.f : loss;
+  r.empty = r.t_top == -INFINITY && !__any(r.t != r.t);
+  r.top = fmaxf(st.x, most);
+  r.rest_scale = __builtin_amdgcn_exp2f(st.x - r.top);
+  r.rest = st.y * r.rest_scale;
+  r.e = __builtin_amdgcn_exp2f(r.l - r.top);
+  const float w = r.empty ? 0.f : __builtin_amdgcn_exp2f(r.t - r.t_top);
+  const uint64_t at = __ballot(r.first && r.l == most), t_at = __ballot(r.t == r.t_top);
+  const int lead = at ? __builtin_ctzll(at) : -1, v_lead = __shfl(r.v, lead & 63, 64);
+  r.led = at && r.v == v_lead;
+  r.t_led = t_at && lane == __builtin_ctzll(t_at);
+  float others = r.first && lane != lead ? r.e : 0.f;
+  r.t_others = r.t_led ? 0.f : w;
+  if (a.k > 1) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      others += __shfl_xor(others, o, 64);
+      r.t_others += __shfl_xor(r.t_others, o, 64);
+    }
+  } else {
+    others = __shfl(others, 0, 64);
+    r.t_others = __shfl(r.t_others, 0, 64);
   }
-  if (!a.dh) return !empty;
-  // p of an id that a row names twice counts once.  Its logit, summed in another order than
-  // those in lse, may pass it by their roundings.
-  bool first = v >= 0;
-  for (int j = 0; j < a.k; ++j) {
-    const int32_t vj = __shfl((int)v, j, 64);
-    if (j < lane && vj == (int32_t)v) first = false;
+  r.others = r.rest + others;
+  r.z = r.others + (at ? __builtin_amdgcn_exp2f(most - r.top) : 0.f);
+  r.p = r.e / r.z;
+  r.q = w / (1.f + r.t_others);
+  return r;
+}
+
+// lse and the loss.  With d_j = log q_j - log p_j and p_rest the share of the tokens that are not
+// wanted,
+//   sum_j q_j d_j = sum_j q_j (d_j - 1 + exp(-d_j)) + p_rest,
+// because the q_j add up to 1 and the p_j = q_j exp(-d_j) to 1 - p_rest.  No term is negative.
+// (Of an id named twice the terms are not, and its p counts once.)
+__device__ __forceinline__ void store_loss(const HeadLoss& a, int64_t m, const HeadRow& r) {
+  const float log2_z = __builtin_amdgcn_logf(r.z);
+  const float neg_log_p = r.led && r.others < r.e ? log1pf(r.others / r.e)
+                                                  : (r.top - r.l + log2_z) * kLn2;
+  float neg_log_q = 0.f;
+  if (a.k > 1)
+    neg_log_q = r.t_led ? log1pf(r.t_others)
+                        : (r.t_top - r.t + __builtin_amdgcn_logf(1.f + r.t_others)) * kLn2;
+  const float d = neg_log_p - neg_log_q, p_once = r.first ? r.p : 0.f;
+  // Entries of no weight (q = 0) add their p; NaN stays.
+  float term = !r.twice && fabsf(d) < 0.5f ? r.q * excess(d) : r.q * (d - 1.f) + p_once;
+  if (r.q == 0.f) term = p_once;
+  if (r.v < 0) term = 0.f;
+  term = a.k > 1 ? wave_sum(term) : term;
+  if ((threadIdx.x & 63) != 0) return;
+  a.lse[m] = (r.top + log2_z) * kLn2;
+  a.loss[m] = r.empty ? 0.f : (term + r.rest / r.z) * (a.temperature * a.temperature);
+}
+
+// The lane's coefficient of W_id, and the factor of the sums over e.
+__device__ __forceinline__ float row_coef(const HeadLoss& a, int64_t m, const HeadRow& r,
+                                          float* factor) {
+  float q = r.q, not_q = r.t_led ? r.t_others / (1.f + r.t_others) : 1.f - r.q;
+  if (__any(r.twice)) {
+    float all = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+      const float qj = __shfl(q, j, 64);
+      if (__builtin_amdgcn_readlane(r.v, j) == r.v) all += qj;
+    }
+    if (r.twice) {
+      q = all;
+      not_q = 1.f - q;
+    }
   }
-  const float g = (a.grad_loss ? a.grad_loss[m] : 1.f) * T;
-  const float p = first ? __builtin_amdgcn_exp2f(fminf(l2 - lse2, 0.f)) : 0.f;
-  *coef = v >= 0 ? g * (p - q) : 0.f;
-  *factor = g / st.y;
-  return !empty;
+  const float g = (a.grad_loss ? a.grad_loss[m] : 1.f) * a.temperature;
+  *factor = g * r.rest_scale / r.z;
+  if (!r.first) return 0.f;
+  return g * (q > 0.5f ? not_q - (r.led ? r.others / r.z : 1.f - r.p) : r.p - q);
 }
 
 // Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought
-// to it with the wanted entries zeroed.  in / out are the states before and after; chunk 0
+// to it.  in / out are the states before and after; chunk 0
 // writes out and the factor of the earlier pieces' sums and, after the last piece, finishes
 // the row where no gradient follows.  After the last piece the blocks of a row share its
 // wanted entries' logits (sel).
@@ -173,9 +258,10 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
                                                         int64_t stat_tiles, int tw,
                                                         const float2* in, float2* out,
                                                         float* factor, uint16_t* e, int64_t lde,
-                                                        int64_t v0, int tiles, int chunk, bool last,
-                                                        float scale, float* sel) {
-  __shared__ float red[4], red2[4], l2s[64];
+                                                        int tiles, int chunk, bool last, float scale,
+                                                        Entry* sel) {
+  __shared__ float red[4], red2[4];
+  __shared__ Entry entries[64];
   const int64_t m = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float2* st = stats + m * stat_tiles;
@@ -208,21 +294,19 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
   if (last)
     for (int j = 4 * blockIdx.y + wave; j < a.k; j += 4 * gridDim.y) {
       const int64_t v = token_of(a, m, j, lane == 0);
-      const float l2 = v >= 0 ? logit_of(a, m, v, scale) : 0.f;
-      if (lane == 0) {
-        if (e) sel[m * a.k + j] = l2;
-        else l2s[j] = l2;
-      }
+      uint64_t same = 1;
+      if (a.k > 1) same = __ballot(lane < a.k && a.ids[m * a.k + lane] == (int32_t)v);
+      const Entry en = {v >= 0 ? logit_of(a, m, v, scale) : 0.f, (same & ((1ull << j) - 1)) != 0,
+                        (same & (same - 1)) != 0};
+      if (lane == 0) (e ? sel + m * a.k : entries)[j] = en;
     }
   if (last && !e) {
     __syncthreads();
-    if (wave == 0)
-      finish_row(a, m, now, lane < a.k ? l2s[lane] : 0.f, true, nullptr, nullptr);
+    if (wave == 0) store_loss(a, m, read_row(a, m, now, lane < a.k ? entries[lane] : Entry{}));
   }
   if (!e) return;
   uint16_t* row = e + m * lde;
   const int ta = (int)blockIdx.y * chunk, tb = ta + chunk < tiles ? ta + chunk : tiles;
-  const int64_t c0 = (int64_t)ta * tw, c1 = (int64_t)tb * tw;
   for (int t0 = ta + 64 * wave; t0 < tb; t0 += 256) {
     const float f = t0 + lane < tb ? __builtin_amdgcn_exp2f(st[t0 + lane].x - top) : 1.f;
     if (!__any(f != 1.f)) continue;
@@ -236,11 +320,6 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
       *reinterpret_cast<u32x4*>(at) = v;
     }
   }
-  __syncthreads();
-  for (int j = tid; j < a.k; j += 256) {
-    const int64_t v = token_of(a, m, j, false) - v0;
-    if (v >= c0 && v < c1) row[v] = 0;
-  }
 }
 
 // A row's loss and gradient: the slices' sum times the row's factor, plus the wanted entries'
@@ -249,7 +328,7 @@ __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2
 template <int WS>
 __global__ __launch_bounds__(256) void head_dh_kernel(HeadLoss a, const float* __restrict__ slices,
                                                       int splits, const float2* __restrict__ state,
-                                                      const float* __restrict__ sel) {
+                                                      const Entry* __restrict__ sel) {
   __shared__ float coef[64], factor;
   __shared__ int any;
   __shared__ f32x4 part[WS > 1 ? 2 * 256 : 1];
@@ -258,13 +337,13 @@ __global__ __launch_bounds__(256) void head_dh_kernel(HeadLoss a, const float* _
   const int64_t c0 = (int64_t)blockIdx.y * (WS > 1 ? 512 : 2048);
   const int64_t c = c0 + 8 * (WS > 1 ? lane : (int)threadIdx.x);
   if (wave == 0) {
-    float co = 0.f, f = 0.f;
-    const bool on = finish_row(a, m, state[m], lane < a.k ? sel[m * a.k + lane] : 0.f,
-                               blockIdx.y == 0, &co, &f);
-    coef[lane] = co;
+    const HeadRow r = read_row(a, m, state[m], lane < a.k ? sel[m * a.k + lane] : Entry{});
+    if (blockIdx.y == 0) store_loss(a, m, r);
+    float f;
+    coef[lane] = row_coef(a, m, r, &f);
     if (lane == 0) {
       factor = f;
-      any = on;
+      any = !r.empty;
     }
   }
   f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -377,7 +456,7 @@ HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   };
   p.stats = take(M * p.stat_tiles * 8);
   p.state = take(2 * M * 8);
-  p.sel = take(M * k * 4);
+  p.sel = take(M * k * (int64_t)sizeof(Entry));
   p.factor = take(M * 4);
   if (grad) {
     p.e = take(M * piece * 2);
@@ -393,7 +472,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
   char* base = static_cast<char*>(ws);
   float2* stats = reinterpret_cast<float2*>(base + p.stats);
   float2* state = reinterpret_cast<float2*>(base + p.state);
-  float* sel = reinterpret_cast<float*>(base + p.sel);
+  Entry* sel = reinterpret_cast<Entry*>(base + p.sel);
   float* factor = reinterpret_cast<float*>(base + p.factor);
   uint16_t* e = a.dh ? reinterpret_cast<uint16_t*>(base + p.e) : nullptr;
   float* slices = a.dh ? reinterpret_cast<float*>(base + p.slices) : nullptr;
@@ -410,8 +489,7 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     const int64_t chunk = up((tiles + by - 1) / by, 64);
     head_join_kernel<<<dim3((unsigned)a.M, (unsigned)by), 256, 0, stream>>>(
         a, stats, p.stat_tiles, p.stat_width, i ? state + (i & 1) * a.M : nullptr,
-        state + ((i + 1) & 1) * a.M, factor, e, lde, v0, (int)tiles, (int)chunk, v0 + n == a.V, scale,
-        sel);
+        state + ((i + 1) & 1) * a.M, factor, e, lde, (int)tiles, (int)chunk, v0 + n == a.V, scale, sel);
     return hipGetLastError();
   };
   for (int i = 0; i < p.pieces; ++i) {
@@ -433,6 +511,10 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     g.e = e;
     g.lde = up(n, kGradTileCols);
     g.logit_scale = scale;
+    g.wanted = a.ids;
+    g.wanted_k = a.k;
+    g.wanted_none = a.teacher ? -1 : a.ignore;
+    g.first_token = v0;
     if (p.skinny && skinny_pack_bytes(a.M, a.K)) g.xp = base + p.xp;
     if (p.panel && (e || !p.skinny)) {
       if (hipError_t r = launch_dequantize(g.w, g.scales, g.biases, panel, n, a.K, a.group_size, a.bits,
