@@ -139,7 +139,8 @@ struct HeadRow {
   float l, e, p;
   float top, rest, rest_scale;  // rest: the tokens that are not wanted
   float others, z;              // all tokens but the likeliest entry; all
-  float t, t_top, t_others, q;  // cross entropy: a teacher with one entry
+  float t, t_others, q;  // the teacher's logit less the row's largest, in units of log 2
+                         // (cross entropy: a teacher with one entry)
 };
 // An entry's logit, and whether the row names its token in an earlier entry or in another one.
 struct Entry {
@@ -160,29 +161,31 @@ __device__ __forceinline__ HeadRow read_row(const HeadLoss& a, int64_t m, float2
   r.first = r.v >= 0 && !en.again;
   r.twice = r.v >= 0 && en.twice;
   r.l = r.v >= 0 ? en.l2 : -INFINITY;
-  r.t = r.v >= 0 ? r.t * (kLog2e / a.temperature) : -INFINITY;
-  float most = r.l;
-  r.t_top = r.t;
+  if (r.v < 0) r.t = -INFINITY;
+  float most = r.l, t_top = r.t;
   if (a.k > 1) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
       most = fmaxf(most, __shfl_xor(most, o, 64));
-      r.t_top = fmaxf(r.t_top, __shfl_xor(r.t_top, o, 64));
+      t_top = fmaxf(t_top, __shfl_xor(t_top, o, 64));
     }
   } else {
     most = __shfl(most, 0, 64);
-    r.t_top = __shfl(r.t_top, 0, 64);
+    t_top = __shfl(t_top, 0, 64);
   }
-  r.empty = r.t_top == -INFINITY && !__any(r.t != r.t);
+  r.empty = t_top == -INFINITY && !__any(r.t != r.t);
+  const uint64_t t_at = __ballot(r.t == t_top);
+  r.t_led = t_at && lane == __builtin_ctzll(t_at);
+  // The difference first: a logit of the type's lowest value times log2 e would be -infinity.
+  r.t = (r.t - t_top) * (kLog2e / a.temperature);
   r.top = fmaxf(st.x, most);
   r.rest_scale = __builtin_amdgcn_exp2f(st.x - r.top);
   r.rest = st.y * r.rest_scale;
   r.e = __builtin_amdgcn_exp2f(r.l - r.top);
-  const float w = r.empty ? 0.f : __builtin_amdgcn_exp2f(r.t - r.t_top);
-  const uint64_t at = __ballot(r.first && r.l == most), t_at = __ballot(r.t == r.t_top);
+  const float w = r.empty ? 0.f : __builtin_amdgcn_exp2f(r.t);
+  const uint64_t at = __ballot(r.first && r.l == most);
   const int lead = at ? __builtin_ctzll(at) : -1, v_lead = __shfl(r.v, lead & 63, 64);
   r.led = at && r.v == v_lead;
-  r.t_led = t_at && lane == __builtin_ctzll(t_at);
   float others = r.first && lane != lead ? r.e : 0.f;
   r.t_others = r.t_led ? 0.f : w;
   if (a.k > 1) {
@@ -213,8 +216,7 @@ __device__ __forceinline__ void store_loss(const HeadLoss& a, int64_t m, const H
                                                   : (r.top - r.l + log2_z) * kLn2;
   float neg_log_q = 0.f;
   if (a.k > 1)
-    neg_log_q = r.t_led ? log1pf(r.t_others)
-                        : (r.t_top - r.t + __builtin_amdgcn_logf(1.f + r.t_others)) * kLn2;
+    neg_log_q = r.t_led ? log1pf(r.t_others) : (__builtin_amdgcn_logf(1.f + r.t_others) - r.t) * kLn2;
   const float d = neg_log_p - neg_log_q, p_once = r.first ? r.p : 0.f;
   // Entries of no weight (q = 0) add their p; NaN stays.
   float term = !r.twice && fabsf(d) < 0.5f ? r.q * excess(d) : r.q * (d - 1.f) + p_once;
