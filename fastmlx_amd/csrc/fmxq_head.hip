@@ -225,7 +225,8 @@ __device__ __forceinline__ void store_loss(const HeadLoss& a, int64_t m, const H
   term = a.k > 1 ? wave_sum(term) : term;
   if ((threadIdx.x & 63) != 0) return;
   a.lse[m] = (r.top + log2_z) * kLn2;
-  a.loss[m] = r.empty ? 0.f : (term + r.rest / r.z) * (a.temperature * a.temperature);
+  // One factor T at a time: T T alone leaves fp32's range where the loss need not.
+  a.loss[m] = r.empty ? 0.f : (term + r.rest / r.z) * a.temperature * a.temperature;
 }
 
 // The lane's coefficient of W_id, and the factor of the sums over e.

@@ -46,3 +46,13 @@ def test_teacher_rows_of_the_types_lowest_value(gpu, dtype):
     assert loss[0] > 1 and loss[2] == 0
     check(h, w, ids, t, T=0.25)
     ops.device_error()
+
+
+@pytest.mark.parametrize("T", [1e-25, 1e-15, 1e15])
+def test_temperatures_whose_square_leaves_the_range(gpu, T):
+    """T^2 = 1e-50 is no fp32 number, the loss (the divergence is near a logit / T) is one."""
+    announce(f"temperature {T}")
+    h, w, ids, gen = case(gpu)
+    t = torch.randn(ids.shape, generator=gen).to(gpu)
+    loss = check(h, w, ids, t, T)[0]
+    assert (loss > 0).all()
