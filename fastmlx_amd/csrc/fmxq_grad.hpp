@@ -31,9 +31,10 @@ struct GradGemm {
   // slice p of out.
   int splits = 1;
   int64_t c_split = 0;
-  // nn: fp32 slices out [splits][M][N], added to what is there times factor[row] when
-  // factor is given; or, with y, bf16 rows y [M][ldy] (one part only).
+  // nn: fp32 slices out [splits][M][N], added to what is there (with add) times factor[row] (where
+  // it is given); or, with y, bf16 rows y [M][ldy] (one part only).
   float* out = nullptr;
+  bool add = false;
   const float* factor = nullptr;
   uint16_t* y = nullptr;
   int64_t ldy = 0;

@@ -88,13 +88,17 @@ int head_loss(fmxq::HeadLoss a, void* ws, size_t ws_bytes, void* stream, const c
 
 struct GradPlan {
   int bm, splits;
-  int64_t c_split;
+  int64_t c_split, piece;  // piece: rows of the weight of one panel (N without panels)
   bool panel, skinny;
   size_t pad, slices, panel_at, bytes;
 };
 // Rows from which the weights are dequantized to a panel beforehand: 14336 x 4096, four tiles of
 // 256 rows take 149 us without, five 175 us with it.
 constexpr int64_t kGradPanelRows = 1025;
+// Most bytes of a panel: a larger weight is walked in pieces whose products are added in fp32, so
+// that a call needs no bf16 copy of it.  (2048 rows, 128256 x 4096, in one panel of 1 GB 1.94 ms, in two
+// pieces 1.97, in four of 256 MB 2.05: each piece reads the sums again and ends in a tail.)
+constexpr int64_t kGradPanelBytes = 512 << 20;
 
 // The rows of dy are copied to a stride of 8 values where N (or the address) is not one.
 int64_t pad_cols(int64_t N) { return up(N, 8); }
@@ -102,6 +106,12 @@ int64_t pad_cols(int64_t N) { return up(N, 8); }
 GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
   p.panel = M >= kGradPanelRows;
+  p.piece = N;
+  if (p.panel) {
+    const int64_t most = std::max<int64_t>(kGradPanelBytes / 2 / std::max<int64_t>(K, 1), 256);
+    const int64_t pieces = std::max<int64_t>(1, (N + most - 1) / most);
+    p.piece = up((N + pieces - 1) / pieces, 64);
+  }
   p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M, true);
   p.skinny = M <= fmxq::kGradSkinnyRows && fmxq::skinny_gemm_supported(pad_cols(N), N + 64, K);
   const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.bm > 128 ? fmxq::kGradTileCols : fmxq::kGradCols;
@@ -109,13 +119,13 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at
   // least.
   const int64_t want = tiles ? (p.bm > 128 ? kCus : 2 * kCus) / tiles : 1;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, N / 256));
-  p.c_split = up((N + p.splits - 1) / p.splits, 64);
-  p.splits = (int)std::max<int64_t>(1, (N + p.c_split - 1) / std::max<int64_t>(p.c_split, 1));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, p.piece / 256));
+  p.c_split = up((p.piece + p.splits - 1) / p.splits, 64);
+  p.splits = (int)std::max<int64_t>(1, (p.piece + p.c_split - 1) / std::max<int64_t>(p.c_split, 1));
   p.pad = 0;
   p.slices = up(M * pad_cols(N) * 2, 256);
-  p.panel_at = p.slices + (p.splits > 1 ? up(p.splits * M * K * 4, 256) : 0);
-  p.bytes = p.panel_at + (p.panel ? N * K * 2 : 0);
+  p.panel_at = p.slices + (p.splits > 1 || p.piece < N ? up(p.splits * M * K * 4, 256) : 0);
+  p.bytes = p.panel_at + (p.panel ? std::min(p.piece, N) * K * 2 : 0);
   return p;
 }
 
@@ -236,7 +246,7 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
   g.splits = p.splits;
   g.c_split = p.c_split;
   float* slices = reinterpret_cast<float*>(ws + p.slices);
-  if (p.splits > 1) {
+  if (p.splits > 1 || p.piece < N) {
     g.out = slices;
   } else {
     g.y = dx;
@@ -246,16 +256,25 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
     uint16_t* panel = reinterpret_cast<uint16_t*>(ws + p.panel_at);
     g.panel = panel;
     g.ldp = K;
-    if (int rc = hip_status(fmxq::launch_dequantize(w, scales, biases, panel, N, K, group_size, bits, s),
-                            op))
-      return rc;
-    if (int rc = hip_status(fmxq::launch_panel_gemm(g, true, s), op)) return rc;
+    for (int64_t n0 = 0; n0 < N; n0 += p.piece) {
+      fmxq::GradGemm d = g;
+      d.C = std::min(p.piece, N - n0);
+      d.a = g.a + n0;
+      d.a_cols = std::min(p.piece, g.a_cols - n0);
+      d.add = n0 > 0;
+      const int64_t at = n0 * (K / group_size);
+      if (int rc = hip_status(fmxq::launch_dequantize(w + n0 * (K * bits / 32), scales + at, biases + at,
+                                                      panel, d.C, K, group_size, bits, s),
+                              op))
+        return rc;
+      if (int rc = hip_status(fmxq::launch_panel_gemm(d, true, s), op)) return rc;
+    }
   } else if (int rc = hip_status(p.skinny ? fmxq::launch_skinny_gemm(g, true, s)
                                           : fmxq::launch_grad_gemm(g, true, p.bm, s),
                                  op)) {
     return rc;
   }
-  if (p.splits == 1) return FMXQ_OK;
+  if (!g.out) return FMXQ_OK;
   return hip_status(fmxq::launch_sum_slices(slices, p.splits, dx, M, K, s), op);
 }
 

@@ -342,9 +342,9 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void grad_skinny_kernel(GradG
       *reinterpret_cast<u32x2*>(g.y + row * g.ldy + n) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     } else {
       float* o = g.out + (split * g.M + row) * g.N + n;
-      if (g.factor) {
+      if (g.add) {
         const f32x4 old = *reinterpret_cast<const f32x4*>(o);
-        const float f = g.factor[row];
+        const float f = g.factor ? g.factor[row] : 1.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(old[e], f, v[e]);
       }

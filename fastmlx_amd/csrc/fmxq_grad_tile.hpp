@@ -74,7 +74,7 @@ __device__ __forceinline__ void store_grad(const GradGemm& g, const f32x16 (&acc
         }
     } else {
       float* o = g.out + (split * g.M + m) * g.N;
-      const float f = g.factor ? g.factor[m] : 0.f;
+      const float f = g.factor ? g.factor[m] : 1.f;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -83,7 +83,7 @@ __device__ __forceinline__ void store_grad(const GradGemm& g, const f32x16 (&acc
           if (n >= g.N) continue;
           f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                      acc[i][j][4 * q + 3]};
-          if (g.factor) {
+          if (g.add) {
             const f32x4 old = *reinterpret_cast<const f32x4*>(o + n);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(old[e], f, v[e]);

@@ -541,7 +541,8 @@ hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipS
     d.splits = p.splits;
     d.c_split = p.c_split;
     d.out = slices;
-    d.factor = i ? factor : nullptr;
+    d.add = i > 0;
+    d.factor = factor;
     if (hipError_t r = p.panel         ? launch_panel_gemm(d, true, stream)
                        : p.grad_skinny ? launch_skinny_gemm(d, true, stream)
                                        : launch_grad_gemm(d, true, p.grad_bm, stream))

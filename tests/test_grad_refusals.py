@@ -154,3 +154,12 @@ def test_torch_wrappers_refuse_cpu_tensors_and_shapes():
 def test_head_workspace_refuses_rows_of_no_width(M, grad):
     assert ws("fmxq_head_workspace", M, 100, 0, 1, grad)[0] == "FMXQ_ERR_SHAPE"
     assert ws("fmxq_head_workspace", 0, 100, 0, 1, grad) == ("FMXQ_OK", 0)
+
+
+def test_a_gradient_needs_no_copy_of_a_large_weight():
+    """The panel of dequantized weights is bounded, whatever their number."""
+    for M, N, K in ((2048, 128256, 4096), (1025, 500000, 8192), (4096, 28672, 8192)):
+        rc, n = ws("fmxq_quantized_matmul_grad_workspace", M, N, K)
+        # A copy of dy, two parts of fp32 sums at most for that many tiles (three below 2048 rows
+        # of 4096), and the panel.
+        assert rc == "FMXQ_OK" and n <= 2 * M * (N + 8) + 3 * 4 * M * K + (513 << 20)
