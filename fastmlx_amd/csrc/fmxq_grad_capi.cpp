@@ -90,7 +90,7 @@ struct GradPlan {
   int bm, splits;
   int64_t c_split, piece;  // piece: rows of the weight of one panel (N without panels)
   bool panel, skinny;
-  size_t pad, slices, panel_at, bytes;
+  size_t slices, panel_at, bytes;
 };
 // Rows from which the weights are dequantized to a panel beforehand: 14336 x 4096, four tiles of
 // 256 rows take 149 us without, five 175 us with it.
@@ -100,8 +100,16 @@ constexpr int64_t kGradPanelRows = 1025;
 // pieces 1.97, in four of 256 MB 2.05: each piece reads the sums again and ends in a tail.)
 constexpr int64_t kGradPanelBytes = 512 << 20;
 
-// The rows of dy are copied to a stride of 8 values where N (or the address) is not one.
+// The rows of dy are copied to a stride of 8 values where N is not one, and where dy's address is
+// not 16-byte aligned: for that, which the sizes do not show, a call takes moved_bytes more.
 int64_t pad_cols(int64_t N) { return up(N, 8); }
+size_t pad_bytes(int64_t M, int64_t N) { return N % 8 ? (size_t)up(M * pad_cols(N) * 2, 256) : 0; }
+size_t moved_bytes(const void* dy, int64_t M, int64_t N) {
+  return N % 8 == 0 && !aligned16(dy) ? (size_t)(M * N * 2) : 0;
+}
+// A call with rows needs some workspace at any size, so that a missing one is an error at every
+// size and not at some.
+constexpr size_t kLeastBytes = 256;
 
 GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
@@ -122,10 +130,9 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, p.piece / 256));
   p.c_split = up((p.piece + p.splits - 1) / p.splits, 64);
   p.splits = (int)std::max<int64_t>(1, (p.piece + p.c_split - 1) / std::max<int64_t>(p.c_split, 1));
-  p.pad = 0;
-  p.slices = up(M * pad_cols(N) * 2, 256);
+  p.slices = pad_bytes(M, N);
   p.panel_at = p.slices + (p.splits > 1 || p.piece < N ? up(p.splits * M * K * 4, 256) : 0);
-  p.bytes = p.panel_at + (p.panel ? std::min(p.piece, N) * K * 2 : 0);
+  p.bytes = M == 0 ? 0 : std::max(p.panel_at + (p.panel ? std::min(p.piece, N) * K * 2 : 0), kLeastBytes);
   return p;
 }
 
@@ -231,10 +238,12 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
   if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   const GradPlan p = grad_plan(M, N, K);
-  if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, op)) return rc;
+  const size_t moved = moved_bytes(dy, M, N), moved_at = moved ? up(p.bytes, 256) : 0;
+  if (int rc = check_workspace(workspace, workspace_bytes, moved ? moved_at + moved : p.bytes, op))
+    return rc;
   char* ws = static_cast<char*>(workspace);
   fmxq::GradGemm g;
-  if (int rc = grad_operand(dy, ws + p.pad, M, N, s, &g, op)) return rc;
+  if (int rc = grad_operand(dy, ws + moved_at, M, N, s, &g, op)) return rc;
   g.M = M;
   g.N = K;
   g.C = N;
@@ -282,7 +291,7 @@ int fmxq_gather_qmm_grad_workspace(int64_t S, int64_t E, int64_t N, int64_t K, s
   const char* op = "gather_qmm_grad_workspace";
   if (int rc = grad_sizes(S, N, K, op)) return rc;
   if (E < 0) return fail(FMXQ_ERR_SHAPE, "%s: negative size E=%lld", op, (long long)E);
-  return bytes_out(S * pad_cols(N) * 2, bytes, op);
+  return bytes_out(S == 0 ? 0 : std::max(pad_bytes(S, N), kLeastBytes), bytes, op);
 }
 
 int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
@@ -308,7 +317,8 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
   if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   if (E > kMaxCount) return fail(FMXQ_ERR_SHAPE, "%s: %lld experts are too many", op, (long long)E);
-  if (int rc = check_workspace(workspace, workspace_bytes, S * pad_cols(N) * 2, op)) return rc;
+  const size_t need = std::max(pad_bytes(S, N), kLeastBytes) + moved_bytes(dy, S, N);
+  if (int rc = check_workspace(workspace, workspace_bytes, need, op)) return rc;
   uint32_t* flag = nullptr;
   if (int rc = device_flag(s, &flag)) return rc;
   fmxq::GradGemm g;

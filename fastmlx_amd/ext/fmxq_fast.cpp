@@ -431,10 +431,14 @@ PyObject* qmm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     size_t bytes = 0;
     at::Tensor ws;
+    // Rows that do not begin at 16 bytes are moved.
+    const bool moved = N % 8 == 0 && reinterpret_cast<uintptr_t>(dy->data_ptr()) % 16 != 0;
     if (!workspace(*dy,
                    [&](size_t* o) {
-                     return runs ? fmxq_gather_qmm_grad_workspace(M, E, N, K, o)
-                                 : fmxq_quantized_matmul_grad_workspace(M, N, K, o);
+                     const int rc = runs ? fmxq_gather_qmm_grad_workspace(M, E, N, K, o)
+                                         : fmxq_quantized_matmul_grad_workspace(M, N, K, o);
+                     if (moved) *o += 256 + (size_t)dy->numel() * 2;
+                     return rc;
                    },
                    &ws, &bytes))
       return nullptr;

@@ -333,15 +333,21 @@ def _quant_shapes(w, scales, biases, lead, K, group_size, bits):
     _shape("biases", biases, *lead, K // group_size)
 
 
-def _workspace(fn, dev, *sizes):
-    """A workspace for a call with these sizes, from torch's allocator: its own in every
-    call, stream and captured graph.  (pointer, bytes, the tensor that keeps it)"""
+def _workspace(fn, dev, *sizes, more=0):
+    """A workspace for a call with these sizes (and `more` bytes), from torch's allocator: its own
+    in every call, stream and captured graph.  (pointer, bytes, the tensor that keeps it)"""
     import ctypes
 
     n = ctypes.c_size_t()
     check(fn(*sizes, ctypes.byref(n)))
-    t = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    return (t.data_ptr() if n.value else None), n.value, t
+    bytes_ = n.value + more
+    t = torch.empty(bytes_, dtype=torch.uint8, device=dev)
+    return (t.data_ptr() if bytes_ else None), bytes_, t
+
+
+def _moved(dy):
+    """The bytes that a gradient takes to move rows that do not begin at 16 bytes."""
+    return 256 + dy.numel() * 2 if dy.data_ptr() % 16 and dy.shape[-1] % 8 == 0 else 0
 
 
 def _head_operands(h, w, scales, biases, grad, grad_loss, group_size, bits):
@@ -456,7 +462,8 @@ def quantized_matmul_grad(dy, w, scales, biases, group_size: int = 64, bits: int
     lib = load()
     with torch.cuda.device(dev):
         dx = torch.empty(*dy.shape[:-1], K, dtype=torch.bfloat16, device=dev)
-        ws, n, keep = _workspace(lib.fmxq_quantized_matmul_grad_workspace, dev, M, N, K)
+        ws, n, keep = _workspace(lib.fmxq_quantized_matmul_grad_workspace, dev, M, N, K,
+                                 more=_moved(dy))
         check(lib.fmxq_quantized_matmul_grad(*args, dx.data_ptr(), M, N, K, group_size, bits, ws,
                                              n, _stream(dy)))
     return dx
@@ -485,7 +492,8 @@ def gather_qmm_grad(dy, w, scales, biases, offsets, group_size: int = 64, bits: 
     lib = load()
     with torch.cuda.device(dev):
         dx = torch.empty(S, K, dtype=torch.bfloat16, device=dev)
-        ws, n, keep = _workspace(lib.fmxq_gather_qmm_grad_workspace, dev, S, E, N, K)
+        ws, n, keep = _workspace(lib.fmxq_gather_qmm_grad_workspace, dev, S, E, N, K,
+                                 more=_moved(dy))
         check(lib.fmxq_gather_qmm_grad(*args, dx.data_ptr(), S, E, N, K, group_size, bits, ws, n,
                                        _stream(dy)))
     return dx

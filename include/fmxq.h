@@ -323,6 +323,8 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
                                const uint16_t* biases, uint16_t* dx, int64_t M, int64_t N,
                                int64_t K, int group_size, int bits, void* workspace,
                                size_t workspace_bytes, void* stream);
+/* (Where N is a multiple of 8 but dy is not 16-byte aligned, 256 + M N 2 bytes more; so for
+ * gather_qmm_grad with S.) */
 int fmxq_quantized_matmul_grad_workspace(int64_t M, int64_t N, int64_t K, size_t* bytes);
 
 /* The same for gather_qmm over rows sorted by expert: row r of dx [S, K] is dy[r] . deq(W[e])

@@ -37,3 +37,25 @@ def test_quantized_matmul_grad_in_pieces(gpu, M, N, K, bits, group):
     # Rows do not depend on the other rows' number of tiles or parts by more than their sums' errors.
     one = ops.quantized_matmul_grad(dy[:7].contiguous(), *w, group, bits)
     ref.check(one, y[:7], (e + ref.HALF[torch.bfloat16] * (y.abs() + e) + ref.TINY)[:7], "seven rows")
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 16, 64), (40, 512, 256), (300, 4096, 128), (1100, 72, 128)])
+@pytest.mark.parametrize("off", [1, 4, 7])
+def test_rows_at_any_address(gpu, M, N, K, off):
+    """Rows that begin between 16-byte addresses are moved to a workspace, and all the results are
+    those of rows that do not."""
+    announce(f"rows {off} values further, {M}x{N}x{K}")
+    gen = torch.Generator().manual_seed(M)
+    w = ref.quant(gen, (N,), K, 4, 64, gpu)
+    dy = torch.randn(M, N, generator=gen).bfloat16().to(gpu)
+    odd = torch.empty(M * N + off, dtype=torch.bfloat16, device=gpu)[off:].view(M, N).copy_(dy)
+    two = tuple(torch.stack([t, t]) for t in w)
+    ends = torch.tensor([0, M // 3, M], dtype=torch.int32, device=gpu)
+    for path in (ops._fast, None):
+        ops_fast, ops._fast = ops._fast, path
+        try:
+            assert torch.equal(ops.quantized_matmul_grad(odd, *w), ops.quantized_matmul_grad(dy, *w))
+            assert torch.equal(ops.gather_qmm_grad(odd, *two, ends), ops.gather_qmm_grad(dy, *two, ends))
+        finally:
+            ops._fast = ops_fast
+    ops.device_error()

@@ -163,3 +163,24 @@ def test_a_gradient_needs_no_copy_of_a_large_weight():
         # A copy of dy, two parts of fp32 sums at most for that many tiles (three below 2048 rows
         # of 4096), and the panel.
         assert rc == "FMXQ_OK" and n <= 2 * M * (N + 8) + 3 * 4 * M * K + (513 << 20)
+
+
+def test_gradients_reserve_no_copy_of_rows_that_are_read_as_they_are():
+    rc, n = ws("fmxq_gather_qmm_grad_workspace", 65536, 64, 7168, 2048)
+    assert rc == "FMXQ_OK" and n <= 4096
+    rc, n = ws("fmxq_quantized_matmul_grad_workspace", 4096, 28672, 4096)
+    assert rc == "FMXQ_OK" and n <= 28672 * 4096 * 2 + 4096
+    # Rows of 7 values are copied to 8.
+    assert ws("fmxq_gather_qmm_grad_workspace", 1000, 4, 7, 64)[1] >= 1000 * 8 * 2
+    for name, sizes in (("fmxq_gather_qmm_grad_workspace", (0, 4, 7, 64)),
+                        ("fmxq_quantized_matmul_grad_workspace", (0, 7, 64))):
+        assert ws(name, *sizes) == ("FMXQ_OK", 0)
+
+
+def test_moved_rows_need_their_bytes():
+    """dy at an odd address: what the query reports does not do, and nothing is enqueued."""
+    for M, N in ((4, 16), (40, 512)):
+        n = ws("fmxq_quantized_matmul_grad_workspace", M, N, 64)[1]
+        assert grad(dy=P + 2, M=M, N=N, n=n + M * N * 2 - 1) == "FMXQ_ERR_INVALID_ARGUMENT"
+        n = ws("fmxq_gather_qmm_grad_workspace", M, 3, N, 64)[1]
+        assert gather(dy=P + 2, S=M, N=N, n=n + M * N * 2 - 1) == "FMXQ_ERR_INVALID_ARGUMENT"
