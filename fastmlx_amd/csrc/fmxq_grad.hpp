@@ -61,6 +61,8 @@ struct GradGemm {
   uint32_t* flag = nullptr;
 };
 
+// A launch has fewer blocks of these products: 2^32 threads.
+constexpr int64_t kMaxBlocks = 1 << 23;
 // Rows of a block's tile, for M rows (or expert runs of about that many).
 int grad_gemm_rows(int64_t M, bool nn);
 constexpr int kGradStatWidth = 64;  // columns of a tile of the statistics (128 rows and more)
@@ -70,6 +72,13 @@ constexpr int kLogitCols = 256, kGradCols = 128;  // of launch_grad_gemm's tiles
 inline int64_t grad_gemm_run_tiles(int64_t S, int64_t E, int bm) {
   return (S / bm + (E < S ? E : S) + 8) / 8 * 8;
 }
+// Blocks of the gradient of `tiles` row tiles of bm rows, N columns.
+inline int64_t grad_gemm_blocks(int64_t tiles, int bm, int64_t N) {
+  const int64_t bn = bm < 256 ? kGradCols : kLogitCols;
+  return tiles * ((N + bn - 1) / bn);
+}
+// What a tile's 32-bit offsets into its rows of A hold: lda of launch_grad_gemm and launch_panel_gemm.
+constexpr int64_t kMaxLda = 0x7ffffff0LL / 512 - 1;
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream);
 
 // The same products where reading the weights is the work (fmxq_grad_skinny.hip): logits
@@ -93,6 +102,8 @@ hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 // tiles of kPanelRows rows.
 constexpr int kPanelRows = 256;
 constexpr int kPanelStatWidth = 128;
+// Whether a tile's 32-bit offsets into a panel of rows of ld values hold it.
+inline bool panel_gemm_supported(int64_t ld) { return (kGradTileCols + 1) * ld * 2 < 0x7ffffff0LL; }
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 // bf16 y [M, N] = the sum of the slices of out [splits][M][N].
 hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64_t M, int64_t N,

@@ -35,6 +35,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// The gradient of M rows, K wide, in one launch.
+bool outputs_ok(int64_t M, int64_t K) {
+  return fmxq::grad_gemm_blocks((M + fmxq::kPanelRows - 1) / fmxq::kPanelRows, fmxq::kPanelRows, K) <
+         fmxq::kMaxBlocks;
+}
+
 // a * b within 62 bits (a, b >= 0).
 bool product_ok(int64_t a, int64_t b) { return a == 0 || b <= ((int64_t)1 << 62) / a; }
 
@@ -50,7 +56,7 @@ int check_workspace(const void* ws, size_t have, size_t need, const char* op) {
 
 // ---- losses ---------------------------------------------------------------------
 
-int head_sizes(int64_t M, int64_t V, int64_t K, int k, const char* op) {
+int head_sizes(int64_t M, int64_t V, int64_t K, int k, bool grad, const char* op) {
   if (M < 0 || V < 0 || K < 0)
     return fail(FMXQ_ERR_SHAPE, "%s: negative size M=%lld V=%lld K=%lld", op, (long long)M,
                 (long long)V, (long long)K);
@@ -61,12 +67,14 @@ int head_sizes(int64_t M, int64_t V, int64_t K, int k, const char* op) {
   if (M > kMaxRows || V > kMaxCount || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, V=%lld or K=%lld too large", op, (long long)M,
                 (long long)V, (long long)K);
+  if (grad && !outputs_ok(M, K))
+    return fail(FMXQ_ERR_SHAPE, "%s: %lld rows of %lld are too many", op, (long long)M, (long long)K);
   return FMXQ_OK;
 }
 
 int head_loss(fmxq::HeadLoss a, void* ws, size_t ws_bytes, void* stream, const char* op) {
   if (int rc = check_quant(a.group_size, a.bits, a.K, true, op)) return rc;
-  if (int rc = head_sizes(a.M, a.V, a.K, a.k, op)) return rc;
+  if (int rc = head_sizes(a.M, a.V, a.K, a.k, a.dh != nullptr, op)) return rc;
   if (a.grad_loss && !a.dh)
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: grad_loss without dh", op);
   if (a.M == 0) return FMXQ_OK;
@@ -113,7 +121,7 @@ constexpr size_t kLeastBytes = 256;
 
 GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   GradPlan p{};
-  p.panel = M >= kGradPanelRows;
+  p.panel = M >= kGradPanelRows && fmxq::panel_gemm_supported(K);
   p.piece = N;
   if (p.panel) {
     const int64_t most = std::max<int64_t>(kGradPanelBytes / 2 / std::max<int64_t>(K, 1), 256);
@@ -154,6 +162,8 @@ int grad_sizes(int64_t M, int64_t N, int64_t K, const char* op) {
   if (M > kMaxRows || N > kMaxWidth || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, N=%lld or K=%lld too large", op, (long long)M,
                 (long long)N, (long long)K);
+  if (!outputs_ok(M, K))
+    return fail(FMXQ_ERR_SHAPE, "%s: %lld rows of %lld are too many", op, (long long)M, (long long)K);
   return FMXQ_OK;
 }
 
@@ -164,6 +174,17 @@ int bytes_out(size_t v, size_t* out, const char* op) {
 }
 
 int run_rows(int64_t S, int64_t E) { return fmxq::grad_gemm_rows(E > 0 ? (S + E - 1) / E : S, true); }
+
+int run_sizes(int64_t S, int64_t E, int64_t N, int64_t K, const char* op) {
+  if (int rc = grad_sizes(S, N, K, op)) return rc;
+  if (E < 0) return fail(FMXQ_ERR_SHAPE, "%s: negative size E=%lld", op, (long long)E);
+  if (E > kMaxCount) return fail(FMXQ_ERR_SHAPE, "%s: %lld experts are too many", op, (long long)E);
+  const int bm = run_rows(S, E);
+  if (fmxq::grad_gemm_blocks(fmxq::grad_gemm_run_tiles(S, E, bm), bm, K) >= fmxq::kMaxBlocks)
+    return fail(FMXQ_ERR_SHAPE, "%s: %lld rows of %lld in %lld runs are too many", op, (long long)S,
+                (long long)K, (long long)E);
+  return FMXQ_OK;
+}
 
 // ---- sorted rows --------------------------------------------------------------------
 
@@ -182,7 +203,7 @@ extern "C" {
 
 int fmxq_head_workspace(int64_t M, int64_t V, int64_t K, int top_k, bool with_grad, size_t* bytes) {
   const char* op = "head_workspace";
-  if (int rc = head_sizes(M, V, K, top_k, op)) return rc;
+  if (int rc = head_sizes(M, V, K, top_k, with_grad, op)) return rc;
   return bytes_out(M == 0 ? 0 : fmxq::head_plan(M, V, K, top_k, with_grad, kCus).bytes, bytes, op);
 }
 
@@ -289,8 +310,7 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
 
 int fmxq_gather_qmm_grad_workspace(int64_t S, int64_t E, int64_t N, int64_t K, size_t* bytes) {
   const char* op = "gather_qmm_grad_workspace";
-  if (int rc = grad_sizes(S, N, K, op)) return rc;
-  if (E < 0) return fail(FMXQ_ERR_SHAPE, "%s: negative size E=%lld", op, (long long)E);
+  if (int rc = run_sizes(S, E, N, K, op)) return rc;
   return bytes_out(S == 0 ? 0 : std::max(pad_bytes(S, N), kLeastBytes), bytes, op);
 }
 
@@ -300,8 +320,7 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
                          void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "gather_qmm_grad";
   if (int rc = check_quant(group_size, bits, K, true, op)) return rc;
-  if (int rc = grad_sizes(S, N, K, op)) return rc;
-  if (E < 0) return fail(FMXQ_ERR_SHAPE, "%s: negative size E=%lld", op, (long long)E);
+  if (int rc = run_sizes(S, E, N, K, op)) return rc;
   if (S == 0) return FMXQ_OK;
   if (E == 0) return fail(FMXQ_ERR_SHAPE, "%s: %lld rows but no experts", op, (long long)S);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -316,7 +335,6 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
   if (!aligned16(w)) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: w must be 16-byte aligned", op);
   if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
-  if (E > kMaxCount) return fail(FMXQ_ERR_SHAPE, "%s: %lld experts are too many", op, (long long)E);
   const size_t need = std::max(pad_bytes(S, N), kLeastBytes) + moved_bytes(dy, S, N);
   if (int rc = check_workspace(workspace, workspace_bytes, need, op)) return rc;
   uint32_t* flag = nullptr;

@@ -484,7 +484,7 @@ hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
   const int64_t tn = (g.N + BN - 1) / BN, tm = g.offsets ? g.max_tiles : (g.M + BM - 1) / BM;
   const int64_t blocks = tm * tn * g.splits;
   if (blocks < 1) return hipSuccess;
-  if (blocks >= (int64_t)1 << 23) return hipErrorInvalidConfiguration;
+  if (blocks >= kMaxBlocks) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks), block(BN * 2);
   const bool g32 = NN && g.group_size == 32;
   if (g.bits == 4) {
@@ -508,7 +508,7 @@ int grad_gemm_rows(int64_t M, bool nn) { return M <= 32 ? 32 : M <= 64 ? 64 : M 
 
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream) {
   // Offsets into one tile's rows and into 64 or 256 weight rows are 32 bits.
-  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || 256 * g.lda * 2 >= 0x7ffffff0LL ||
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || g.lda > kMaxLda ||
       256 * (nn ? g.N : g.C) >= 0x7ffffff0LL || g.c_split % kS || g.lda % 8 || g.a_cols % 8 ||
       (g.offsets && (!nn || !g.y || !g.flag || g.splits != 1)))
     return hipErrorInvalidValue;

@@ -216,13 +216,13 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
 }  // namespace
 
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || 
-      kPanelRows * g.lda * 2 >= 0x7ffffff0LL || (kN + 1) * g.ldp * 2 >= 0x7ffffff0LL || g.c_split % kS ||
+  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || g.lda > kMaxLda ||
+      !panel_gemm_supported(g.ldp) || g.c_split % kS ||
       g.lda % 8 || g.a_cols % 8 || g.ldp % 8 || g.offsets)
     return hipErrorInvalidValue;
   const int64_t blocks = (g.M + kPanelRows - 1) / kPanelRows * ((g.N + kN - 1) / kN) * g.splits;
   if (blocks < 1) return hipSuccess;
-  if (blocks >= (int64_t)1 << 23) return hipErrorInvalidConfiguration;
+  if (blocks >= kMaxBlocks) return hipErrorInvalidConfiguration;
   if (nn) panel_gemm_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(g);
   else panel_gemm_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(g);
   return hipGetLastError();

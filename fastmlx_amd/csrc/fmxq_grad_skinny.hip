@@ -356,7 +356,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void grad_skinny_kernel(GradG
 template <int BITS, int MT>
 hipError_t launch_logits(const GradGemm& g, hipStream_t stream) {
   const int64_t blocks = (g.N + 31) / 32, chunks = (g.M + kSkinnyRows - 1) / kSkinnyRows;
-  if (blocks >= (int64_t)1 << 23 || chunks > 65535) return hipErrorInvalidConfiguration;
+  if (blocks >= kMaxBlocks || chunks > 65535) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks, (unsigned)chunks);
   if (!g.xp) {
     logits_skinny_kernel<BITS, MT, false><<<grid, 512, 0, stream>>>(g);
@@ -373,7 +373,7 @@ hipError_t launch_logits(const GradGemm& g, hipStream_t stream) {
 template <int BITS, int MT>
 hipError_t launch_grad(const GradGemm& g, hipStream_t stream) {
   const int64_t blocks = (g.N + kSkinnyCols - 1) / kSkinnyCols * g.splits;
-  if (blocks >= (int64_t)1 << 23) return hipErrorInvalidConfiguration;
+  if (blocks >= kMaxBlocks) return hipErrorInvalidConfiguration;
   if (g.group_size == 32) grad_skinny_kernel<BITS, MT, true><<<(unsigned)blocks, 512, 0, stream>>>(g);
   else grad_skinny_kernel<BITS, MT, false><<<(unsigned)blocks, 512, 0, stream>>>(g);
   return hipGetLastError();

@@ -283,7 +283,9 @@ int fmxq_route_group_topk(const void* gates, int gates_bf16, const float* bias, 
  * reports for the same sizes, is 16-byte aligned, needs no contents and may be reused once
  * the call's work is done.  Calls that may overlap (two streams, two graphs replayed at once)
  * need a workspace each.  They can be captured into a graph at any time.  Outputs do not
- * overlap other operands.  Rows (M, S, T) below 2^24, N and K up to 2^22 - 8, below 2^26 slots. */
+ * overlap other operands.  Rows (M, S, T) below 2^24, N and K up to 2^22 - 8, V below 2^31, below
+ * 2^26 slots; gradients of fewer than 2^23 tiles of 256 rows by 256 columns (gather_qmm_grad: in
+ * its runs' tiles of 32 to 256 rows by 128 or 256). */
 
 /* Cross entropy of a quantized head: logits l = h . deq(W)^T over V tokens, which are never
  * stored;

@@ -184,3 +184,24 @@ def test_moved_rows_need_their_bytes():
         assert grad(dy=P + 2, M=M, N=N, n=n + M * N * 2 - 1) == "FMXQ_ERR_INVALID_ARGUMENT"
         n = ws("fmxq_gather_qmm_grad_workspace", M, 3, N, 64)[1]
         assert gather(dy=P + 2, S=M, N=N, n=n + M * N * 2 - 1) == "FMXQ_ERR_INVALID_ARGUMENT"
+
+
+def test_sizes_that_no_launch_takes_are_refused_first():
+    """More blocks than a launch has, with or without a workspace (its address is never used)."""
+    M, K = (1 << 24) - 1, 1 << 21
+    assert grad(M=M, K=K) == gather(S=M, K=K) == ce(M=M, K=K) == "FMXQ_ERR_SHAPE"
+    assert gather(S=(1 << 24) - 1, E=1 << 22, K=4096) == "FMXQ_ERR_SHAPE"
+    assert ws("fmxq_quantized_matmul_grad_workspace", M, 16, K)[0] == "FMXQ_ERR_SHAPE"
+    assert ws("fmxq_gather_qmm_grad_workspace", M, 3, 16, K)[0] == "FMXQ_ERR_SHAPE"
+    assert ws("fmxq_head_workspace", M, 100, K, 1, True)[0] == "FMXQ_ERR_SHAPE"
+    # The loss alone has no such outputs.
+    assert ws("fmxq_head_workspace", M, 100, K, 1, False)[0] == "FMXQ_OK"
+
+
+def test_no_panel_where_its_offsets_do_not_fit():
+    """K past what the panel's 32-bit offsets hold: tiles without a panel, which need no memory."""
+    wide = 4180000
+    rc, n = ws("fmxq_quantized_matmul_grad_workspace", 1025, 16, wide)
+    assert rc == "FMXQ_OK" and n < 16 * wide * 2
+    rc, n = ws("fmxq_head_workspace", 2000, 64, wide, 1, False)
+    assert rc == "FMXQ_OK" and n < 64 * wide * 2
