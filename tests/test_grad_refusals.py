@@ -205,3 +205,10 @@ def test_no_panel_where_its_offsets_do_not_fit():
     assert rc == "FMXQ_OK" and n < 16 * wide * 2
     rc, n = ws("fmxq_head_workspace", 2000, 64, wide, 1, False)
     assert rc == "FMXQ_OK" and n < 64 * wide * 2
+
+
+def test_the_sorts_histograms_do_not_grow_with_the_slots():
+    """Every block reads all of them."""
+    assert ws("fmxq_moe_sort_workspace", 1 << 23, 7, 2048) == ("FMXQ_OK", 512 * 2049 * 4)
+    assert ws("fmxq_moe_sort_workspace", (1 << 24) - 1, 3, 8)[1] <= 512 * 9 * 4
+    assert ws("fmxq_moe_sort_workspace", 0, 4, 8) == ("FMXQ_OK", 0)
