@@ -56,3 +56,44 @@ def test_temperatures_whose_square_leaves_the_range(gpu, T):
     t = torch.randn(ids.shape, generator=gen).to(gpu)
     loss = check(h, w, ids, t, T)[0]
     assert (loss > 0).all()
+
+
+@pytest.mark.parametrize("M,V", [(12, 900), (150, 30000), (1100, 12000)])
+def test_gradients_of_logits_beyond_the_exponents_range(gpu, M, V):
+    """Logits of 1e9 and more, the largest of a row further from the others than any error of
+    theirs: one token takes everything, and dh is the difference of two rows of the weights."""
+    announce(f"gradients of huge logits {M}x{V}")
+    gen = torch.Generator().manual_seed(M)
+    K = 256
+    w = ref.quant(gen, (V,), K, 4, 64, gpu)
+    W = ref.values(*w, 4, 64)
+    h = torch.randn(M, K, generator=gen).to(gpu)
+    h = (h * torch.logspace(8, 24, M, device=gpu)[:, None]).bfloat16()
+    logits = h.double() @ W.T
+    (first, second), ids = (lambda t: (t.values.T, t.indices))(logits.topk(2, -1))
+    error = (K + 16) * ref.U32 * (h.double().abs() @ W.abs().T).amax(-1)
+    apart = first - second > 4 * error
+    assert apart.double().mean() > 0.9
+    y = torch.randint(0, V, (M,), generator=gen).to(gpu)
+    y[::3] = ids[::3, 0]          # some rows want the token that they take
+    g = (torch.rand(M, generator=gen) + 0.5).to(gpu)
+    dh = g.double()[:, None] * (W[ids[:, 0]] - W[y])
+    # The taken token's share is a power of two in bf16, half a step off at most; the wanted one's
+    # and the sums are fp32.
+    size = g.double()[:, None] * (W[ids[:, 0]].abs() + W[y].abs())
+    e = (ref.HALF[torch.bfloat16] + 64 * ref.U32) * size
+    e = e + ref.HALF[torch.bfloat16] * (dh.abs() + e)
+    got = ops.head_cross_entropy(h, *w, y.int(), grad=True, grad_loss=g)
+    ref.check(got[2][apart], dh[apart], e[apart], "dh")
+    same = apart & (y == ids[:, 0])
+    assert same.any() and not got[2][same].any() and not got[0][same].any()
+    # One entry of a teacher is the same, at any temperature.
+    got = ops.head_distill((h * 0 + 1).bfloat16(), *w, y.int()[:, None].contiguous(),
+                           torch.zeros(M, 1, device=gpu), temperature=1e-10, grad=True)
+    top = W.sum(-1).topk(2)
+    assert top.values[0] - top.values[1] > 4 * (K + 16) * ref.U32 * W.abs().sum(-1).max()
+    at = int(top.indices[0])
+    dh = 1e-10 * (W[at] - W[y])
+    size = 1e-10 * (W[at].abs() + W[y].abs())
+    e = (ref.HALF[torch.bfloat16] + 64 * ref.U32) * size
+    ref.check(got[2], dh, e + ref.HALF[torch.bfloat16] * (dh.abs() + e), "dh at 1e-10")
