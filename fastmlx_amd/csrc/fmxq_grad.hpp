@@ -39,9 +39,10 @@ struct GradGemm {
   uint16_t* y = nullptr;
   int64_t ldy = 0;
   // nt: what a softmax needs of the logits l = D * logit_scale (in units of log 2) by
-  // tiles of stat_width columns: stats[row][tile] = (m, sum 2^(l - m)) with m the tile's
-  // largest l rounded up to an integer, and, with e, e[row][col] = bf16(2^(l - m)) with
-  // zeros in columns N .. lde.
+  // tiles of the kernel's stat width: stats[row][tile] = (m, sum 2^(l - m)) with m the multiple of
+  // 64 nearest to the tile's largest l, and, with e, e[row][col] = bf16(2^(l - m)), which reaches
+  // 2^32; zeros from column N to the next multiple of the stat width (what lies behind, up to
+  // lde, may be anything: a product over e reads a_cols of it).
   // The row's wanted tokens take no part (their e is 0): ids wanted[row][0 .. wanted_k] of tokens
   // counted from -first_token on, other than wanted_none.
   float2* stats = nullptr;
@@ -64,7 +65,7 @@ struct GradGemm {
 // A launch has fewer blocks of these products: 2^32 threads.
 constexpr int64_t kMaxBlocks = 1 << 23;
 // Rows of a block's tile, for M rows (or expert runs of about that many).
-int grad_gemm_rows(int64_t M, bool nn);
+int grad_gemm_rows(int64_t M);
 constexpr int kGradStatWidth = 64;  // columns of a tile of the statistics (128 rows and more)
 constexpr int kGradTileCols = 256;
 constexpr int kLogitCols = 256, kGradCols = 128;  // of launch_grad_gemm's tiles

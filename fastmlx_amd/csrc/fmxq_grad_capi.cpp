@@ -128,7 +128,7 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t pieces = std::max<int64_t>(1, (N + most - 1) / most);
     p.piece = up((N + pieces - 1) / pieces, 64);
   }
-  p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M, true);
+  p.bm = p.panel ? fmxq::kPanelRows : fmxq::grad_gemm_rows(M);
   p.skinny = M <= fmxq::kGradSkinnyRows && fmxq::skinny_gemm_supported(pad_cols(N), N + 64, K);
   const int64_t cols = p.skinny ? fmxq::kSkinnyCols : p.bm > 128 ? fmxq::kGradTileCols : fmxq::kGradCols;
   const int64_t tiles = (p.skinny ? M > 0 : (M + p.bm - 1) / p.bm) * ((K + cols - 1) / cols);
@@ -173,7 +173,7 @@ int bytes_out(size_t v, size_t* out, const char* op) {
   return FMXQ_OK;
 }
 
-int run_rows(int64_t S, int64_t E) { return fmxq::grad_gemm_rows(E > 0 ? (S + E - 1) / E : S, true); }
+int run_rows(int64_t S, int64_t E) { return fmxq::grad_gemm_rows(E > 0 ? (S + E - 1) / E : S); }
 
 int run_sizes(int64_t S, int64_t E, int64_t N, int64_t K, const char* op) {
   if (int rc = grad_sizes(S, N, K, op)) return rc;

@@ -504,7 +504,7 @@ hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
 // expert runs of 128 rows, 512 x 2048, 47 us in 128-row tiles and 62 in 256-row ones, of 129 rows
 // 87 and 64; runs of 128 in the mean with Zipf-like lengths 69 and 81, of 256 and more the higher
 // tile takes 0.74 to 0.87 of the time.
-int grad_gemm_rows(int64_t M, bool nn) { return M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256; }
+int grad_gemm_rows(int64_t M) { return M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256; }
 
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream) {
   // Offsets into one tile's rows and into 64 or 256 weight rows are 32 bits.

@@ -109,6 +109,7 @@ __device__ __forceinline__ void find_wanted(const GradGemm& g, int64_t m0, int64
                                             uint32_t* lds, uint32_t (&out)[MI][NJ]) {
   const int r32 = threadIdx.x & 31;
   if (g.wanted_k == 1) {
+    asm volatile("" ::: "memory");  // written before the steps' barriers
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const uint32_t c = wanted_column(g, one[mw - m0 + 32 * i + r32], nw);

@@ -431,8 +431,8 @@ bool few_tokens(int64_t M, int64_t V, int bm, int cus) {
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus) {
   HeadPlan p{};
   p.panel = M >= (grad ? kHeadPanelRows : kScorePanelRows) && panel_gemm_supported(K);
-  p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M, false), 128);
-  p.grad_bm = p.panel ? kPanelRows : grad_gemm_rows(M, true);
+  p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M), 128);
+  p.grad_bm = p.panel ? kPanelRows : grad_gemm_rows(M);
   int64_t piece = grad ? std::max<int64_t>(kHeadPieceBytes / 2 / M, 2048) : V;
   if (p.panel) piece = std::min(piece, std::max<int64_t>(kHeadPanelBytes / 2 / K, 2048));
   // What the launches take: blocks of 256 tokens by bm rows, or 32 by 64, and e's rows as an operand.
