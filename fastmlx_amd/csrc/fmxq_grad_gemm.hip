@@ -3,10 +3,9 @@
 // dx = dy . deq(W) of a quantized product (nn), of one matrix or of expert runs.
 //
 // Tile: BM rows by BN columns, 64 deep contraction steps in two LDS stages, a wave for every 32
-// columns; two waves on a SIMD, so that one's dequantization runs under the other's MFMAs: of
-// one block for the logits (BN = 256), of two for the gradients (BN = 128), whose
-// contraction is often short and whose first loads and last stores then run under the other
-// block's steps.  A goes global -> LDS with
+// columns; two waves on a SIMD: of one block for the logits (BN = 256), of two for the
+// gradients (BN = 128), whose contraction is often short and whose first loads and last stores
+// then run under the other block's steps.  A goes global -> LDS with
 // buffer_load ... lds; the packed weights go global -> registers some steps ahead, are
 // dequantized there to fmxq_dequantize's bits and written to LDS.  Both stages hold rows of
 // 64 contraction values (128 bytes), so one fragment read serves both forms: where the
@@ -17,11 +16,13 @@
 // stage: the next fragments, the DMA that refills this stage and the first share of its
 // weights' dequantization run under them.
 //
-// Bound: MFMAs and dequantization together (a weight is dequantized once for every BM rows);
-// short contractions and expert runs of few rows by the latency of the weights instead.
-// Measured: logits of 509 rows, 151936 x 2048, 4 bits: 335 us, 0.95 PFLOP/s; gradients of 1000
-// rows, 128256 x 4096: 1.13 ms, 0.93 PFLOP/s; of 256 / 512 / 1024 rows, 14336 x 4096: 0.53 /
-// 0.71 / 0.84 PFLOP/s; of 8192 rows in 64 expert runs, 512 x 2048, 8 bits: 67 us, 0.26
+// Bound: MFMAs and dequantization in turn (a weight is dequantized once for every BM rows).  In the
+// 256-row tiles the two waves of a SIMD hardly overlap them: 45% of the cycles are MFMAs and 50%
+// VALU, 509 rows over 151936 x 2048.  Short contractions and expert runs of few rows are bound by
+// the latency of the weights instead.
+// Measured: logits of 509 rows, 151936 x 2048, 4 bits: 335 to 355 us, 0.89 to 0.95 PFLOP/s; gradients
+// of 1000 rows, 128256 x 4096: 1.13 to 1.2 ms, 0.88 to 0.93 PFLOP/s; of 256 / 512 / 1024 rows, 14336 x
+// 4096: 0.55 / 0.72 / 0.83 PFLOP/s; of 8192 rows in 64 expert runs, 512 x 2048, 8 bits: 67 us, 0.26
 // PFLOP/s and 1.7 TB/s.
 #include <type_traits>
 

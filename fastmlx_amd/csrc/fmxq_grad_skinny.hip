@@ -10,11 +10,13 @@
 // 8 q4 .. + 8, and column r16 of v_mfma_f32_16x16x32_bf16's tile j is output 8 r16 + j, so that
 // a word's values go to eight tiles and never have to cross lanes.
 //
-// Bound: the dequantization's VALU instructions (6 a weight, with the roundings that make it
-// exact), and below about 20 us the launch, the first loads and the sum over the waves.
-// Measured: logits of one row, 32000 x 2048, 4 bits: 19.5 us; of 16 rows, 32000 x 2560 in
-// groups of 32: 28.6 us; of 37 rows, 50257 x 1024, 8 bits: 26.8 us; gradients of the last two
-// 28.4 and 31.7 us; of 13 rows, 4096 x 4096: 8.8 us.
+// Bound: waiting for loads.  A wave requests a step's weights, scales and x and uses them at once;
+// the other waves hide a part of it.  31 to 45% of the wave cycles wait, and the dequantization's
+// VALU instructions (6 a weight, with the roundings that make it exact) fill 34 to 49% of the
+// SIMDs' cycles, the MFMAs 3 to 8%.  Below about 20 us also the launch and the sum over the waves.
+// Measured: logits of one row, 32000 x 2048, 4 bits: 19 us; of 16 rows, 32000 x 2560 in
+// groups of 32: 29 us; of 37 rows, 50257 x 1024, 8 bits: 27 us; gradients of the last two
+// 28 and 32 us; of 13 rows, 4096 x 4096: 9 us; logits of one row, 128256 x 4096: 131 us.
 #include <type_traits>
 
 #include "fmxq_grad_tile.hpp"

@@ -17,8 +17,8 @@
 //
 // e and the weights' panel pass through memory because a piece of either (256 MB at most) stays
 // in the last-level cache; recomputing the logits for the gradient would cost a third product.
-// Bound: the two products.  2048 rows, 128256 x 4096: 3.96 ms, of them the products 3.75, the
-// panels 0.24 and the kernels here 0.09 ms.
+// Bound: the two products.  2048 rows, 128256 x 4096: 4.07 to 4.16 ms, of them the products 3.75 to
+// 3.9, the panels 0.24 and the kernels here 0.07 ms.
 #include <algorithm>
 
 #include "fmxq_common.hpp"
@@ -250,11 +250,10 @@ __device__ __forceinline__ float row_coef(const HeadLoss& a, int64_t m, const He
   return g * (q > 0.5f ? not_q - (r.led ? r.others / r.z : 1.f - r.p) : r.p - q);
 }
 
-// Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought
-// to it.  in / out are the states before and after; chunk 0
-// writes out and the factor of the earlier pieces' sums and, after the last piece, finishes
-// the row where no gradient follows.  After the last piece the blocks of a row share its
-// wanted entries' logits (sel).
+// Block (row, chunk): the row's running (m, sum) after this piece, and the chunk's e brought to it.
+// in / out are the states before and after; chunk 0 writes out and the factor of the earlier
+// pieces' sums and, after the last piece, finishes the row where no gradient follows.  After the
+// last piece the blocks of a row share its wanted entries (sel).
 // A chunk is a multiple of 64 tiles: a wave looks at 64 tiles' exponents at once and, where
 // none differs from the row's, as in most rows, leaves their e alone.
 __global__ __launch_bounds__(256) void head_join_kernel(HeadLoss a, const float2* __restrict__ stats,

@@ -576,7 +576,8 @@ def moe_unsort(y, pos, weights):
 
 def moe_unsort_grad(dout, y, pos, weights):
     """Gradients of moe_unsort: dout [T, D] bf16 -> (dy [T k, D] bf16, dweights [T, k] in the
-    weights' type)."""
+    weights' type).  The positions are those of moe_sort, all different: rows of dy that none names
+    (where one is out of range, which device_error reports) are not written."""
     if _fast is not None:
         r = _fast.moe_unsort_grad(dout, y, pos, weights)
         if r is not None:
