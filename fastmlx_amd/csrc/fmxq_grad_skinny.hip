@@ -48,6 +48,7 @@ template <int BITS, int MT, bool PACKED>
 __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(GradGemm g) {
   constexpr int NW = BITS / 4;  // 16-byte weight loads per lane and step
   __shared__ __attribute__((aligned(16))) float part[8 * MT * 1024];
+  __shared__ uint32_t want[16 * 32];
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = (int64_t)blockIdx.x * 32;
@@ -142,11 +143,16 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
                                                          0, 0, 0);
     }
   }
-  // The first id that the lane's row of the tile it finishes wants is on its way while the waves
-  // meet; a row's two lanes share its ids.
-  const bool wanting = wave < MT && 32 * wave + r32 < M;
-  const int32_t* want = g.wanted + (m0 + 32 * wave + r32) * g.wanted_k;
-  const int32_t id0 = wanting && h < g.wanted_k ? want[h] : g.wanted_none;
+  // The columns that the rows want: wave m, m + MT, ... share the ids of row tile m, two lanes a wave.
+  constexpr int SH = 16 / MT;
+  const int row = 32 * (wave % MT) + r32, share = 2 * (wave / MT) + h;
+  uint32_t some = 0;
+  if (row < M)
+    for (int j = share; j < g.wanted_k; j += SH) {
+      const uint32_t c = wanted_column(g, g.wanted[(m0 + row) * g.wanted_k + j], n0);
+      if (c < 32) some |= 1u << c;
+    }
+  want[share * (MT * 32) + row] = some;
   // The waves' sums, in the order of the waves; wave m finishes row tile m.
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -157,16 +163,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   __syncthreads();
   if (wave >= MT) return;
   uint32_t out[1][1] = {{0u}};
-  auto find = [&](int32_t id) {
-    const uint32_t c = wanted_column(g, id, n0);
-    if (c < 32) out[0][0] |= 1u << c;
-  };
-  find(id0);
-  if (wanting) {
-#pragma unroll 4
-    for (int j = h + 2; j < g.wanted_k; j += 2) find(want[j]);
-  }
-  out[0][0] |= other_half(out[0][0]);
+  for (int i = 0; i < SH && i < g.wanted_k; ++i) out[0][0] |= want[i * (MT * 32) + row];
   f32x16 sum[1][1];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {

@@ -118,19 +118,24 @@ __device__ __forceinline__ void find_wanted(const GradGemm& g, int64_t m0, int64
     }
     return;
   }
+  const uint32_t k = (uint32_t)g.wanted_k, n = (uint32_t)rows * k;
+  const uint32_t per_k = 0xffffffffu / k + 1;  // i / k as the high half of a product (i < 2^14)
+  constexpr int B = 32;  // ids that are requested together
+  int32_t id[B];
+  auto load = [&](uint32_t i0) {
+#pragma unroll
+    for (int j = 0; j < B; ++j) id[j] = g.wanted[m0 * k + (i0 + j * T < n ? i0 + j * T : 0)];
+  };
+  load(threadIdx.x);
   __syncthreads();
   for (int i = threadIdx.x; i < BM * BN / 32; i += T) lds[i] = 0;
   __syncthreads();
-  const uint32_t k = (uint32_t)g.wanted_k, n = (uint32_t)rows * k;
-  constexpr int B = 16;  // ids that are requested together
   for (uint32_t i0 = threadIdx.x; i0 < n; i0 += B * T) {
-    int32_t id[B];
-#pragma unroll
-    for (int j = 0; j < B; ++j) id[j] = g.wanted[m0 * k + (i0 + j * T < n ? i0 + j * T : i0)];
+    if (i0 >= B * T) load(i0);
 #pragma unroll
     for (int j = 0; j < B; ++j) {
       const uint32_t i = i0 + j * T, c = wanted_column(g, id[j], n0);
-      if (c < BN && i < n) atomicOr(&lds[i / k * (BN / 32) + (c >> 5)], 1u << (c & 31));
+      if (c < BN && i < n) atomicOr(&lds[__umulhi(i, per_k) * (BN / 32) + (c >> 5)], 1u << (c & 31));
     }
   }
   __syncthreads();

@@ -125,6 +125,21 @@ __device__ __forceinline__ float excess(float d) {
   return s * (d * d);
 }
 
+// log(1 + a / b) for 0 <= a <= b, relative to itself: 2 atanh(a / (2 b + a)), whose series over at most
+// 1/3 is cut off below 1e-8 of it.
+__device__ __forceinline__ float log1p_ratio(float a, float b) {
+  const float t = a / (2.f * b + a), u = t * t;
+  float s = 1.f / 15;
+  s = __builtin_fmaf(s, u, 1.f / 13);
+  s = __builtin_fmaf(s, u, 1.f / 11);
+  s = __builtin_fmaf(s, u, 1.f / 9);
+  s = __builtin_fmaf(s, u, 1.f / 7);
+  s = __builtin_fmaf(s, u, 1.f / 5);
+  s = __builtin_fmaf(s, u, 1.f / 3);
+  s = __builtin_fmaf(s, u, 1.f);
+  return 2.f * t * s;
+}
+
 // A row's tokens, lane j's entry among them, from the row's final (m, sum over the tokens that are
 // not wanted) and the entry's logit l2: exponentials relative to 2^top.
 //
@@ -212,11 +227,12 @@ __device__ __forceinline__ HeadRow read_row(const HeadLoss& a, int64_t m, float2
 // (Of an id named twice the terms are not, and its p counts once.)
 __device__ __forceinline__ void store_loss(const HeadLoss& a, int64_t m, const HeadRow& r) {
   const float log2_z = __builtin_amdgcn_logf(r.z);
-  const float neg_log_p = r.led && r.others < r.e ? log1pf(r.others / r.e)
+  const float neg_log_p = r.led && r.others < r.e ? log1p_ratio(r.others, r.e)
                                                   : (r.top - r.l + log2_z) * kLn2;
   float neg_log_q = 0.f;
   if (a.k > 1)
-    neg_log_q = r.t_led ? log1pf(r.t_others) : (__builtin_amdgcn_logf(1.f + r.t_others) - r.t) * kLn2;
+    neg_log_q = r.t_led && r.t_others < 1.f ? log1p_ratio(r.t_others, 1.f)
+                                            : (__builtin_amdgcn_logf(1.f + r.t_others) - r.t) * kLn2;
   const float d = neg_log_p - neg_log_q, p_once = r.first ? r.p : 0.f;
   // Entries of no weight (q = 0) add their p; NaN stays.
   float term = !r.twice && fabsf(d) < 0.5f ? r.q * excess(d) : r.q * (d - 1.f) + p_once;
