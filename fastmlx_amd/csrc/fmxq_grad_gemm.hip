@@ -20,9 +20,9 @@
 // 256-row tiles the two waves of a SIMD hardly overlap them: 45% of the cycles are MFMAs and 50%
 // VALU, 509 rows over 151936 x 2048.  Short contractions and expert runs of few rows are bound by
 // the latency of the weights instead.
-// Measured: logits of 509 rows, 151936 x 2048, 4 bits: 335 to 355 us, 0.89 to 0.95 PFLOP/s; gradients
+// Measured: logits of 509 rows, 151936 x 2048, 4 bits: 329 to 357 us, 0.89 to 0.96 PFLOP/s; gradients
 // of 1000 rows, 128256 x 4096: 1.13 to 1.2 ms, 0.88 to 0.93 PFLOP/s; of 256 / 512 / 1024 rows, 14336 x
-// 4096: 0.55 / 0.72 / 0.83 PFLOP/s; of 8192 rows in 64 expert runs, 512 x 2048, 8 bits: 67 us, 0.26
+// 4096: 0.56 / 0.75 / 0.88 PFLOP/s; of 8192 rows in 64 expert runs, 512 x 2048, 8 bits: 67 us, 0.26
 // PFLOP/s and 1.7 TB/s.
 #include <type_traits>
 

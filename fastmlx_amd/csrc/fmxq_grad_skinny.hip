@@ -12,7 +12,7 @@
 //
 // Bound: waiting for loads.  A wave requests a step's weights, scales and x and uses them at once;
 // the other waves hide a part of it.  31 to 45% of the wave cycles wait, and the dequantization's
-// VALU instructions (6 a weight, with the roundings that make it exact) fill 34 to 49% of the
+// VALU instructions (6 a weight, with the roundings that make it exact) fill 34 to 50% of the
 // SIMDs' cycles, the MFMAs 3 to 8%.  Below about 20 us also the launch and the sum over the waves.
 // Measured: logits of one row, 32000 x 2048, 4 bits: 19 us; of 16 rows, 32000 x 2560 in
 // groups of 32: 29 us; of 37 rows, 50257 x 1024, 8 bits: 27 us; gradients of the last two
