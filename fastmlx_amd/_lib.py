@@ -55,6 +55,14 @@ FMXQ_SYMBOLS = {
     "fmxq_moe_sort_grad": (_int, [_p] * 3 + [_i64] * 3 + [_p]),
     "fmxq_moe_unsort": (_int, [_p] * 3 + [_int, _p] + [_i64] * 3 + [_p]),
     "fmxq_moe_unsort_grad": (_int, [_p] * 4 + [_int, _p, _p] + [_i64] * 3 + [_p]),
+    "fmxq_quantized_matmul_lora": (_int, [_p] * 9 + [_i64] * 4 + [_int] * 3 + [_p, ctypes.c_size_t, _p]),
+    "fmxq_quantized_matmul_lora_workspace": (_int, [_i64] * 4 + [_int, _p]),
+    "fmxq_quantized_matmul_lora_grad": (_int, [_p] * 12 + [_i64] * 4 + [_int] * 3 +
+                                        [_p, ctypes.c_size_t, _p]),
+    "fmxq_quantized_matmul_lora_grad_workspace": (_int, [_i64] * 4 + [_int, _p]),
+    "fmxq_grad_norm": (_int, [_p] * 3 + [_i64, _p, _p, ctypes.c_size_t, _p]),
+    "fmxq_clip_grad_norm": (_int, [_p] * 4 + [_i64, ctypes.c_float, _p, _p, ctypes.c_size_t, _p]),
+    "fmxq_grad_norm_workspace": (_int, [_p]),
 }
 
 

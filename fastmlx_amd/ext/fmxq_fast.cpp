@@ -15,6 +15,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <vector>
+
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -546,11 +548,159 @@ PyObject* moe_unsort_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The operands that quantized_matmul_lora and its gradients share.
+struct Lora {
+  const at::Tensor *x, *w, *s, *b, *la, *lb, *ids, *ls;
+  int64_t M, N, K, E, r;
+};
+bool lora_operands(Call& c, PyObject* const* a, int64_t group, int64_t bits, Lora* l) {
+  l->x = c.tensor(a[0], kBf16Like);
+  l->w = c.tensor(a[1], kU32Like);
+  l->s = c.tensor(a[2], kBf16Like);
+  l->b = c.tensor(a[3], kBf16Like);
+  l->la = c.tensor(a[4], kBf16Like);
+  l->lb = c.tensor(a[5], kBf16Like);
+  l->ids = c.tensor(a[6], kU32Like);
+  l->ls = c.tensor(a[7], kF32);
+  if (!c.ok || l->x->dim() < 1 || l->w->dim() != 2 || l->la->dim() != 3 || l->lb->dim() != 3 ||
+      l->ids->scalar_type() != at::kInt || !on_current(*l->x))
+    return false;
+  l->K = l->x->size(-1);
+  l->N = l->w->size(0);
+  l->E = l->la->size(0);
+  l->r = l->la->size(1);
+  l->M = l->ids->numel();
+  return l->r <= 128 && weight_ok(*l->x, *l->w, *l->s, *l->b, l->K, group, bits) &&
+         same(*l->la, *l->x, {l->E, l->r, l->K}) && same(*l->lb, *l->x, {l->E, l->N, l->r}) &&
+         same(*l->ls, *l->x, {l->E}) && same(*l->ids, *l->x, l->x->sizes().slice(0, l->x->dim() - 1));
+}
+template <class T = uint16_t>
+T* at_of(const at::Tensor* t) {
+  return static_cast<T*>(t->data_ptr());
+}
+
+// (x, w, scales, biases, a, b, adapters, lora_scales, group_size, bits) -> y
+PyObject* qmm_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 10) return nullptr;
+    Call c;
+    int64_t group, bits;
+    Lora l;
+    if (!c.format(a[8], a[9], &group, &bits) || !lora_operands(c, a, group, bits, &l)) return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*l.x,
+                   [&](size_t* o) {
+                     return fmxq_quantized_matmul_lora_workspace(l.M, l.N, l.K, l.E, (int)l.r, o);
+                   },
+                   &ws, &bytes))
+      return nullptr;
+    at::DimVector sizes(l.x->sizes());
+    sizes.back() = l.N;
+    at::Tensor y = make(*l.x, sizes, at::kBFloat16);
+    void* st = stream_of(*l.x);
+    if (!enqueue([&] {
+          return fmxq_quantized_matmul_lora(
+              at_of(l.x), at_of<uint32_t>(l.w), at_of(l.s), at_of(l.b), at_of(l.la), at_of(l.lb),
+              at_of<int32_t>(l.ids), at_of<float>(l.ls), at_of(&y), l.M, l.N, l.K, l.E, (int)l.r,
+              (int)group, (int)bits, ws.data_ptr(), bytes, st);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// (dy, x, w, scales, biases, a, b, adapters, lora_scales, group_size, bits) -> (dx, da, db)
+PyObject* qmm_lora_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 11) return nullptr;
+    Call c;
+    int64_t group, bits;
+    Lora l;
+    const at::Tensor* dy = c.tensor(a[0], kBf16Like);
+    if (!c.format(a[9], a[10], &group, &bits) || !lora_operands(c, a + 1, group, bits, &l)) return nullptr;
+    at::DimVector sizes(l.x->sizes());
+    sizes.back() = l.N;
+    // Rows that do not begin at 16 bytes are moved, which takes memory that ops.py adds.
+    if (!same(*dy, *l.x, sizes) ||
+        (l.N % 8 == 0 && reinterpret_cast<uintptr_t>(dy->data_ptr()) % 16 != 0))
+      return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*l.x,
+                   [&](size_t* o) {
+                     return fmxq_quantized_matmul_lora_grad_workspace(l.M, l.N, l.K, l.E, (int)l.r, o);
+                   },
+                   &ws, &bytes))
+      return nullptr;
+    at::Tensor dx = make(*l.x, l.x->sizes(), at::kBFloat16), da = make(*l.x, {l.E, l.r, l.K}, at::kFloat),
+               db = make(*l.x, {l.E, l.N, l.r}, at::kFloat);
+    void* st = stream_of(*l.x);
+    if (!enqueue([&] {
+          return fmxq_quantized_matmul_lora_grad(
+              at_of(dy), at_of(l.x), at_of<uint32_t>(l.w), at_of(l.s), at_of(l.b), at_of(l.la),
+              at_of(l.lb), at_of<int32_t>(l.ids), at_of<float>(l.ls), at_of(&dx), at_of<float>(&da),
+              at_of<float>(&db), l.M, l.N, l.K, l.E, (int)l.r, (int)group, (int)bits, ws.data_ptr(),
+              bytes, st);
+        }))
+      return nullptr;
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(dx)), THPVariable_Wrap(std::move(da)),
+                         THPVariable_Wrap(std::move(db)));
+  });
+}
+
+// (grads, outs | None, max_norm) -> norm: lists (or tuples) of tensors.
+PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    auto list = [](PyObject* o) { return PyTuple_CheckExact(o) || PyList_CheckExact(o); };
+    const bool outs = n == 3 && a[1] != Py_None;
+    if (n != 3 || !list(a[0]) || (outs && !list(a[1])) || !PyFloat_CheckExact(a[2])) return nullptr;
+    const Py_ssize_t k = PySequence_Fast_GET_SIZE(a[0]);
+    if (k < 1 || (outs && PySequence_Fast_GET_SIZE(a[1]) != k)) return nullptr;
+    Call c;
+    std::vector<const void*> src(k);
+    std::vector<void*> dst(outs ? k : 0);
+    std::vector<int64_t> counts(k);
+    std::vector<int> bf16(k);
+    const at::Tensor* first = nullptr;
+    for (Py_ssize_t i = 0; i < k; ++i) {
+      const at::Tensor* g = c.tensor(PySequence_Fast_GET_ITEM(a[0], i), kBf16 | kF32);
+      if (!g) return nullptr;
+      if (!first) first = g;
+      if (g->device() != first->device()) return nullptr;
+      src[i] = g->data_ptr();
+      counts[i] = g->numel();
+      bf16[i] = g->scalar_type() == at::kBFloat16;
+      if (!outs) continue;
+      const at::Tensor* o = c.tensor(PySequence_Fast_GET_ITEM(a[1], i), kBf16 | kF32);
+      if (!o || o->scalar_type() != g->scalar_type() || !same(*o, *g, g->sizes())) return nullptr;
+      dst[i] = o->data_ptr();
+    }
+    if (!on_current(*first)) return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*first, [&](size_t* o) { return fmxq_grad_norm_workspace(o); }, &ws, &bytes))
+      return nullptr;
+    at::Tensor norm = make(*first, {}, at::kFloat);
+    void* st = stream_of(*first);
+    const float most = (float)PyFloat_AS_DOUBLE(a[2]);
+    if (!enqueue([&] {
+          return outs ? fmxq_clip_grad_norm(src.data(), dst.data(), counts.data(), bf16.data(), k, most,
+                                            at_of<float>(&norm), ws.data_ptr(), bytes, st)
+                      : fmxq_grad_norm(src.data(), counts.data(), bf16.data(), k, at_of<float>(&norm),
+                                       ws.data_ptr(), bytes, st);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(std::move(norm));
+  });
+}
+
 #define FMXQ_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FMXQ_FAST(quantized_matmul), FMXQ_FAST(dequantize),       FMXQ_FAST(quantize),
                          FMXQ_FAST(moe_layer),        FMXQ_FAST(route_softmax_topk), FMXQ_FAST(route_group_topk),
                          FMXQ_FAST(head_loss),        FMXQ_FAST(qmm_grad),           FMXQ_FAST(moe_sort),
                          FMXQ_FAST(moe_unsort),       FMXQ_FAST(moe_unsort_grad),
+                         FMXQ_FAST(qmm_lora),         FMXQ_FAST(qmm_lora_grad),      FMXQ_FAST(clip),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

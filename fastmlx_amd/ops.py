@@ -595,6 +595,143 @@ def moe_unsort_grad(dout, y, pos, weights):
     return dy, dw
 
 
+# ---- adapters beside quantized weights, and clipped gradients ---------------------
+
+
+def _lora_operands(x, N, w, scales, biases, a, b, adapters, lora_scales, group_size, bits):
+    if w.dim() != 2 or a.dim() != 3 or b.dim() != 3 or x.dim() < 1:
+        raise ValueError("x must be [..., K], w [N, K*bits/32], a [E, r, K] and b [E, N, r]")
+    K = x.shape[-1]
+    E, r = a.shape[0], min(a.shape[1], 2**31 - 1)  # more than 128 are refused by the library
+    _quant_shapes(w, scales, biases, (N,), K, group_size, bits)
+    _shape("a", a, E, r, K)
+    _shape("b", b, E, N, r)
+    _shape("adapters", adapters, *x.shape[:-1])
+    _shape("lora_scales", lora_scales, E)
+    M = adapters.numel()
+    ptrs = (_dev(x, "x", _BF16_LIKE), _dev(w, "w", _U32_LIKE), _dev(scales, "scales", _BF16_LIKE),
+            _dev(biases, "biases", _BF16_LIKE), _dev(a, "a", _BF16_LIKE), _dev(b, "b", _BF16_LIKE),
+            _dev(adapters, "adapters", (torch.int32,)),
+            _dev(lora_scales, "lora_scales", (torch.float32,)))
+    return M, K, E, r, ptrs
+
+
+def quantized_matmul_lora(x, w, scales, biases, a, b, adapters, lora_scales, group_size: int = 64,
+                          bits: int = 4):
+    """quantized_matmul with a low-rank adapter for each row:
+    y[m] = x[m] @ deq(W)^T + lora_scales[e] (x[m] @ A[e]^T) @ B[e]^T with e = adapters[m].
+
+    x [..., K] bf16; w [N, K*bits/32]; a [E, r, K] and b [E, N, r] bf16, r a multiple of 8 up to
+    128 (zeros fill smaller ranks); adapters [...] int32, below zero for a row without one;
+    lora_scales [E] float32.  Returns y [..., N] bf16: quantized_matmul's, and the adapter's part
+    added to its bf16 values.  An adapter past the last counts as none, and device_error reports it."""
+    if _fast is not None:
+        r = _fast.qmm_lora(x, w, scales, biases, a, b, adapters, lora_scales, group_size, bits)
+        if r is not None:
+            return r
+    dev = _same_device(x=x, w=w, scales=scales, biases=biases, a=a, b=b, adapters=adapters,
+                       lora_scales=lora_scales)
+    N = w.shape[0] if w.dim() else 0
+    M, K, E, r, ptrs = _lora_operands(x, N, w, scales, biases, a, b, adapters, lora_scales,
+                                      group_size, bits)
+    lib = load()
+    with torch.cuda.device(dev):
+        y = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=dev)
+        ws, n, keep = _workspace(lib.fmxq_quantized_matmul_lora_workspace, dev, M, N, K, E, r)
+        check(lib.fmxq_quantized_matmul_lora(*ptrs, y.data_ptr(), M, N, K, E, r, group_size, bits, ws,
+                                             n, _stream(x)))
+    return y
+
+
+def quantized_matmul_lora_grad(dy, x, w, scales, biases, a, b, adapters, lora_scales,
+                               group_size: int = 64, bits: int = 4):
+    """Gradients of quantized_matmul_lora, W frozen: dy [..., N] bf16 and its operands ->
+    (dx [..., K] bf16, da [E, r, K] float32, db [E, N, r] float32), the adapters' sums over their
+    rows and zeros for one without."""
+    if _fast is not None:
+        r = _fast.qmm_lora_grad(dy, x, w, scales, biases, a, b, adapters, lora_scales, group_size,
+                                bits)
+        if r is not None:
+            return r
+    dev = _same_device(dy=dy, x=x, w=w, scales=scales, biases=biases, a=a, b=b, adapters=adapters,
+                       lora_scales=lora_scales)
+    N = w.shape[0] if w.dim() else 0
+    M, K, E, r, ptrs = _lora_operands(x, N, w, scales, biases, a, b, adapters, lora_scales,
+                                      group_size, bits)
+    _shape("dy", dy, *x.shape[:-1], N)
+    dyp = _dev(dy, "dy", _BF16_LIKE)
+    lib = load()
+    with torch.cuda.device(dev):
+        dx = torch.empty(*x.shape, dtype=torch.bfloat16, device=dev)
+        da = torch.empty(E, r, K, dtype=torch.float32, device=dev)
+        db = torch.empty(E, N, r, dtype=torch.float32, device=dev)
+        ws, n, keep = _workspace(lib.fmxq_quantized_matmul_lora_grad_workspace, dev, M, N, K, E, r,
+                                 more=_moved(dy) if N else 0)
+        check(lib.fmxq_quantized_matmul_lora_grad(dyp, *ptrs, dx.data_ptr(), da.data_ptr(),
+                                                  db.data_ptr(), M, N, K, E, r, group_size, bits, ws,
+                                                  n, _stream(dy)))
+    return dx, da, db
+
+
+def _clip_call(grads, outs, max_norm):
+    """grad_norm (outs None) or clip_grad_norm of lists of tensors."""
+    import ctypes
+
+    types = (torch.float32, torch.bfloat16)
+    if not grads:
+        raise ValueError("no gradients")
+    dev = _same_device(**{f"grads[{i}]": g for i, g in enumerate(grads)})
+    ptrs = [_dev(g, f"grads[{i}]", types) for i, g in enumerate(grads)]
+    n = len(grads)
+    if outs is not None:
+        if len(outs) != n:
+            raise ValueError(f"{len(outs)} results for {n} gradients")
+        _same_device(**{"grads[0]": grads[0]}, **{f"outs[{i}]": o for i, o in enumerate(outs)})
+        for i, (g, o) in enumerate(zip(grads, outs)):
+            _shape(f"outs[{i}]", o, *g.shape)
+            _dev(o, f"outs[{i}]", (g.dtype,))
+    P = ctypes.c_void_p * n
+    counts = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
+    bf16 = (ctypes.c_int * n)(*[int(g.dtype is torch.bfloat16) for g in grads])
+    lib = load()
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws, size, keep = _workspace(lib.fmxq_grad_norm_workspace, dev)
+        if outs is None:
+            check(lib.fmxq_grad_norm(P(*ptrs), counts, bf16, n, norm.data_ptr(), ws, size,
+                                     _stream(grads[0])))
+        else:
+            check(lib.fmxq_clip_grad_norm(P(*ptrs), P(*[o.data_ptr() for o in outs]), counts, bf16, n,
+                                          max_norm, norm.data_ptr(), ws, size, _stream(grads[0])))
+    return norm
+
+
+def grad_norm(grads):
+    """The norm over many gradients: the root of the sum of all their squares, summed in 64 bits.
+    grads: a list of float32 or bfloat16 tensors of one device.  Returns a float32 scalar tensor,
+    without waiting for it."""
+    if _fast is not None:
+        r = _fast.clip(grads, None, 0.0)
+        if r is not None:
+            return r
+    return _clip_call(list(grads), None, 0.0)
+
+
+def clip_grad_norm(grads, max_norm: float, outs=None):
+    """Gradients scaled by min(1, max_norm / norm), norm as grad_norm has it -> (outs, norm).
+
+    outs: the results' tensors, of the gradients' shapes and types (new ones without); they may
+    be the gradients themselves.  A norm that is zero, infinite or NaN leaves the values as they
+    are, so a step can be skipped by the norm alone."""
+    if outs is None:
+        outs = [torch.empty_like(g) for g in grads]
+    if _fast is not None:
+        r = _fast.clip(grads, outs, float(max_norm))
+        if r is not None:
+            return outs, r
+    return outs, _clip_call(list(grads), list(outs), float(max_norm))
+
+
 def device_error(device=None) -> None:
     """Raise FmxqError(FMXQ_ERR_INDEX) if a gather met an out-of-range index."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device

@@ -364,6 +364,54 @@ int fmxq_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t
                          const void* weights, int weights_bf16, uint16_t* dy, void* dweights,
                          int64_t T, int64_t top_k, int64_t D, void* stream);
 
+/* ---- adapters beside quantized weights, and clipped gradients ----
+ * No counterpart in the reference.  Workspaces as above. */
+
+/* Low-rank adapters of many requests beside quantized_matmul: with e = adapters[m],
+ *     y[m] = x[m] . deq(W)^T + lora_scales[e] (x[m] . A_e^T) . B_e^T.
+ * x [M, K] and y [M, N] bf16; a [E, r, K] and b [E, N, r] bf16, r a multiple of 8 up to 128 (adapters of
+ * several ranks share the largest: rows of zeros in a, columns of zeros in b); adapters [M]
+ * int32, below zero for a row without one; lora_scales [E] fp32; E <= 2048.  The first product is
+ * fmxq_quantized_matmul's, bf16 values included, so a row without adapter holds its bits; the
+ * adapter's part is summed in fp32 and added before the row's second rounding.  An adapter of E or
+ * more counts as none and raises the error flag.  a and b are 16-byte aligned.  As
+ * quantized_matmul the call may use the library's memory of its stream: run a shape once before it is
+ * captured. */
+int fmxq_quantized_matmul_lora(const uint16_t* x, const uint32_t* w, const uint16_t* scales,
+                               const uint16_t* biases, const uint16_t* a, const uint16_t* b,
+                               const int32_t* adapters, const float* lora_scales, uint16_t* y, int64_t M,
+                               int64_t N, int64_t K, int64_t E, int r, int group_size, int bits,
+                               void* workspace, size_t workspace_bytes, void* stream);
+int fmxq_quantized_matmul_lora_workspace(int64_t M, int64_t N, int64_t K, int64_t E, int r, size_t* bytes);
+
+/* Its gradients, W frozen: with t = x . A_e^T and dt = lora_scales[e] dy . B_e,
+ *     dx = dy . deq(W) + dt . A_e  [M, K] bf16,
+ *     da [E, r, K] = sum over e's rows of dt^T . x,  db [E, N, r] = lora_scales[e] times that of dy^T . t,
+ * both fp32, zero for an adapter without rows.  dy [M, N] bf16; dx, da and db 16-byte aligned.  Where N is a
+ * multiple of 8 but dy is not 16-byte aligned, 256 + M N 2 bytes more of workspace. */
+int fmxq_quantized_matmul_lora_grad(const uint16_t* dy, const uint16_t* x, const uint32_t* w,
+                                    const uint16_t* scales, const uint16_t* biases, const uint16_t* a,
+                                    const uint16_t* b, const int32_t* adapters, const float* lora_scales,
+                                    uint16_t* dx, float* da, float* db, int64_t M, int64_t N, int64_t K,
+                                    int64_t E, int r, int group_size, int bits, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+int fmxq_quantized_matmul_lora_grad_workspace(int64_t M, int64_t N, int64_t K, int64_t E, int r,
+                                              size_t* bytes);
+
+/* The norm over many gradients: norm [1] fp32 = sqrt(sum over all tensors of g^2), summed in 64 bits.
+ * grads[i]: device address of counts[i] values, bf16 where bf16[i], else fp32, aligned to their
+ * size; the four arrays are the host's and are read before the call returns. */
+int fmxq_grad_norm(const void* const* grads, const int64_t* counts, const int* bf16, int64_t n,
+                   float* norm, void* workspace, size_t workspace_bytes, void* stream);
+/* ... and the gradients scaled to a norm of max_norm >= 0 at most:
+ *     outs[i] = grads[i] min(1, max_norm / norm),
+ * in grads[i]'s type.  outs[i] may be grads[i]; otherwise no result may share memory with another or
+ * with a gradient.  A norm that is zero, infinite or NaN leaves the values as they are. */
+int fmxq_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* counts,
+                        const int* bf16, int64_t n, float max_norm, float* norm, void* workspace,
+                        size_t workspace_bytes, void* stream);
+int fmxq_grad_norm_workspace(size_t* bytes);
+
 /* Synchronizes `stream`, then reports (and clears) the device-side error flags
  * that gather kernels raise on an out-of-range index: returns FMXQ_OK or
  * FMXQ_ERR_INDEX (FMXQ_ERR_DEVICE if a wide-GEMM block gave up waiting).  Two
