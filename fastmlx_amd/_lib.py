@@ -45,6 +45,12 @@ FMXQ_SYMBOLS = {
     "fmxq_head_distill": (_int, [_p] * 6 + [_int] + [_p] * 4 + [_i64] * 3 +
                           [_int, ctypes.c_float, _int, _int, _p, ctypes.c_size_t, _p]),
     "fmxq_head_workspace": (_int, [_i64] * 3 + [_int, _bool, _p]),
+    "fmxq_head_logprobs": (_int, [_p] * 10 + [_i64] * 3 + [_int, _int, ctypes.c_float, _int, _int, _p,
+                                                         ctypes.c_size_t, _p]),
+    "fmxq_head_logprobs_workspace": (_int, [_i64] * 3 + [_int, _int, _p]),
+    "fmxq_head_logprobs_grad": (_int, [_p] * 11 + [_i64] * 3 + [_int, ctypes.c_float, _int, _int, _p,
+                                                              ctypes.c_size_t, _p]),
+    "fmxq_head_logprobs_grad_workspace": (_int, [_i64] * 3 + [_int, _p]),
     "fmxq_quantized_matmul_grad": (_int, [_p] * 5 + [_i64] * 3 + [_int, _int, _p, ctypes.c_size_t,
                                                                   _p]),
     "fmxq_quantized_matmul_grad_workspace": (_int, [_i64] * 3 + [_p]),

@@ -7,6 +7,15 @@
 
 namespace fmxq {
 
+// What a product of logits leaves (nt): the softmax statistics of the losses, those of log
+// probabilities, or the logits' gradient.
+enum Epilogue { kEpiStats = 0, kEpiScores = 1, kEpiCoef = 2 };
+// A tile of a row's logits for log probabilities (store_scores).
+struct HeadTile {
+  float top, sum, low;
+  uint32_t first;
+};
+
 // One product D [M, N] = A [M, C] . B with B the dequantized weights (the bits of
 // fmxq_dequantize):
 //   nn = false: B = deq(W)^T, W [N, C] packed along the contraction (logits);
@@ -54,6 +63,11 @@ struct GradGemm {
   uint16_t* e = nullptr;
   int64_t lde = 0;
   float logit_scale = 1.f;
+  // epi: kEpiScores writes score[row][tile] in place of stats (no wanted tokens); kEpiCoef writes e
+  // from rows[row] = (lse, a, c, -) in units of log 2 (store_coef).
+  Epilogue epi = kEpiStats;
+  HeadTile* score = nullptr;
+  const float* rows = nullptr;
   // Expert runs (nn only, into y): rows offsets[e] .. offsets[e + 1] of M take expert e, whose
   // weights are C rows into w; other rows get zeros.  max_tiles: grad_gemm_run_tiles.  *flag
   // is raised where the offsets decrease or leave 0 .. M (all rows are zero then).
@@ -141,7 +155,51 @@ struct HeadPlan {
   size_t stats, e, slices, state, factor, sel, panel_at, xp, bytes;  // in the workspace
 };
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);
+// Whether the operands of a product's logits are there.
+inline bool logits_operands(const GradGemm& g) {
+  switch (g.epi) {
+    case kEpiStats: return g.stats && g.wanted;
+    case kEpiScores: return g.score != nullptr;
+    case kEpiCoef: return g.rows && g.wanted && g.e;
+  }
+  return false;
+}
 hipError_t launch_head_loss(const HeadLoss& a, const HeadPlan& p, void* ws, hipStream_t stream);
+
+// Log probabilities through a quantized head (fmxq_logprobs.hip).
+struct HeadScore {
+  const uint16_t* h;
+  const uint32_t* w;
+  const uint16_t *scales, *biases;
+  const int32_t* ids;  // [M, k], below zero for an absent entry
+  float *logp, *entropy, *lse;
+  int32_t* top_ids;  // [M, top]
+  float* top_logp;
+  int64_t M, V, K;
+  int k, top;
+  float temperature;
+  int group_size, bits;
+  uint32_t* flag;
+};
+size_t head_score_bytes(int64_t M, int64_t V, int64_t K, int k, int top, int cus);
+hipError_t launch_head_score(const HeadScore& a, int cus, void* ws, hipStream_t stream);
+// Their gradient: dh from grad_logp [M, k] and grad_entropy [M] (or null), with the logp, entropy
+// and lse that the scores gave.
+struct HeadScoreGrad {
+  const uint16_t* h;
+  const uint32_t* w;
+  const uint16_t *scales, *biases;
+  const int32_t* ids;
+  const float *logp, *entropy, *lse, *grad_logp, *grad_entropy;
+  uint16_t* dh;
+  int64_t M, V, K;
+  int k;
+  float temperature;
+  int group_size, bits;
+  uint32_t* flag;
+};
+size_t head_score_grad_bytes(int64_t M, int64_t V, int64_t K, int k, int cus);
+hipError_t launch_head_score_grad(const HeadScoreGrad& a, int cus, void* ws, hipStream_t stream);
 
 // Rows sorted by expert and back (fmxq_rows.hip); S = T k slots, slot s of token s / k.
 struct MoeSort {

@@ -92,6 +92,16 @@ int head_loss(fmxq::HeadLoss a, void* ws, size_t ws_bytes, void* stream, const c
   return hip_status(fmxq::launch_head_loss(a, p, ws, s), op);
 }
 
+int score_sizes(int64_t M, int64_t V, int64_t K, int k, int top, const char* op) {
+  if (int rc = head_sizes(M, V, K, std::max(k, 1), false, op)) return rc;
+  if (k < 0) return fail(FMXQ_ERR_SHAPE, "%s: k=%d outside 0..%d", op, k, kHeadMaxTopK);
+  if (top < 0 || top > kHeadMaxTopK || (M > 0 && top > V))
+    return fail(FMXQ_ERR_SHAPE, "%s: top=%d outside 0..%d, or of %lld tokens", op, top, kHeadMaxTopK,
+                (long long)V);
+  return FMXQ_OK;
+}
+bool temperature_ok(float t) { return t >= 1e-30f && t <= 1e30f; }
+
 // ---- input gradients --------------------------------------------------------------
 
 struct GradPlan {
@@ -233,6 +243,76 @@ int fmxq_head_distill(const uint16_t* h, const uint32_t* w, const uint16_t* scal
   fmxq::HeadLoss a{h, w, scales, biases, ids, teacher, teacher_bf16 != 0, grad_loss, loss, lse, dh, M,
                    V, K, top_k, 0, temperature, group_size, bits, nullptr};
   return head_loss(a, workspace, workspace_bytes, stream, op);
+}
+
+int fmxq_head_logprobs_workspace(int64_t M, int64_t V, int64_t K, int k, int top, size_t* bytes) {
+  const char* op = "head_logprobs_workspace";
+  if (int rc = score_sizes(M, V, K, k, top, op)) return rc;
+  return bytes_out(M == 0 ? 0 : fmxq::head_score_bytes(M, V, K, k, top, kCus), bytes, op);
+}
+
+int fmxq_head_logprobs(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
+                       const uint16_t* biases, const int32_t* ids, float* logp, float* entropy, float* lse,
+                       int32_t* top_ids, float* top_logp, int64_t M, int64_t V, int64_t K, int k, int top,
+                       float temperature, int group_size, int bits, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  const char* op = "head_logprobs";
+  if (int rc = check_quant(group_size, bits, K, true, op)) return rc;
+  if (int rc = score_sizes(M, V, K, k, top, op)) return rc;
+  if (!temperature_ok(temperature))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: temperature %g must be a positive number", op,
+                (double)temperature);
+  if (M == 0) return FMXQ_OK;
+  if (!h || !w || !scales || !biases || !entropy || !lse || (k > 0 && (!ids || !logp)) ||
+      (top > 0 && (!top_ids || !top_logp)))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
+  if (!aligned16(h) || !aligned16(w))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: h and w must be 16-byte aligned", op);
+  if (!aligned(ids, 4) || !aligned(logp, 4) || !aligned(entropy, 4) || !aligned(lse, 4) ||
+      !aligned(top_ids, 4) || !aligned(top_logp, 4) || !aligned(scales, 2) || !aligned(biases, 2))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
+  if (int rc = check_workspace(workspace, workspace_bytes, fmxq::head_score_bytes(M, V, K, k, top, kCus), op))
+    return rc;
+  fmxq::HeadScore a{h, w, scales, biases, ids, logp, entropy, lse, top_ids, top_logp, M, V, K, k, top,
+                    temperature, group_size, bits, nullptr};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (int rc = device_flag(s, &a.flag)) return rc;
+  return hip_status(fmxq::launch_head_score(a, kCus, workspace, s), op);
+}
+
+int fmxq_head_logprobs_grad_workspace(int64_t M, int64_t V, int64_t K, int k, size_t* bytes) {
+  const char* op = "head_logprobs_grad_workspace";
+  if (int rc = head_sizes(M, V, K, k, true, op)) return rc;
+  return bytes_out(M == 0 ? 0 : fmxq::head_score_grad_bytes(M, V, K, k, kCus), bytes, op);
+}
+
+int fmxq_head_logprobs_grad(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
+                            const uint16_t* biases, const int32_t* ids, const float* logp,
+                            const float* entropy, const float* lse, const float* grad_logp,
+                            const float* grad_entropy, uint16_t* dh, int64_t M, int64_t V, int64_t K, int k,
+                            float temperature, int group_size, int bits, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const char* op = "head_logprobs_grad";
+  if (int rc = check_quant(group_size, bits, K, true, op)) return rc;
+  if (int rc = head_sizes(M, V, K, k, true, op)) return rc;
+  if (!temperature_ok(temperature))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: temperature %g must be a positive number", op,
+                (double)temperature);
+  if (M == 0) return FMXQ_OK;
+  if (!h || !w || !scales || !biases || !ids || !logp || !entropy || !lse || !grad_logp || !dh)
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
+  if (!aligned16(h) || !aligned16(w) || !aligned16(dh))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: h, w and dh must be 16-byte aligned", op);
+  if (!aligned(ids, 4) || !aligned(logp, 4) || !aligned(entropy, 4) || !aligned(lse, 4) ||
+      !aligned(grad_logp, 4) || !aligned(grad_entropy, 4) || !aligned(scales, 2) || !aligned(biases, 2))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
+  if (int rc = check_workspace(workspace, workspace_bytes, fmxq::head_score_grad_bytes(M, V, K, k, kCus), op))
+    return rc;
+  fmxq::HeadScoreGrad a{h, w, scales, biases, ids, logp, entropy, lse, grad_logp, grad_entropy, dh, M, V, K,
+                        k, temperature, group_size, bits, nullptr};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (int rc = device_flag(s, &a.flag)) return rc;
+  return hip_status(fmxq::launch_head_score_grad(a, kCus, workspace, s), op);
 }
 
 int fmxq_quantized_matmul_grad_workspace(int64_t M, int64_t N, int64_t K, size_t* bytes) {

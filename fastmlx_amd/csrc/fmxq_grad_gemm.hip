@@ -143,7 +143,7 @@ struct Q8<8> {
   }
 };
 
-template <int BM, int BN, int BITS, bool G32, bool NN>
+template <int BM, int BN, int BITS, bool G32, bool NN, int EPI = kEpiStats>
 __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kernel(GradGemm g) {
   using C = GradCfg<BM, BN>;
   constexpr int W = C::W, WN = C::WN, MI = C::MI, NJ = C::NJ, CB = C::CB;
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
     pace(1);
   };
   int32_t id = -1;
-  if (!NN && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
+  if (!NN && EPI != kEpiScores && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
   if (nk > 0) {
 #pragma unroll
     for (int i = 0; i < AS; ++i) {  // the waits count on this order
@@ -473,13 +473,14 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
   if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
   else {
     uint32_t out[MI][NJ];
-    find_wanted<BM, BN, W * 64>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
-                                      out);
-    store_stats<MI, NJ>(g, acc, out, mw, m0 + rows, nw);
+    if constexpr (EPI != kEpiScores)
+      find_wanted<BM, BN, W * 64>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
+                                  out);
+    store_logits<EPI>(g, acc, out, mw, m0 + rows, nw);
   }
 }
 
-template <int BM, bool NN>
+template <int BM, bool NN, int EPI = kEpiStats>
 hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
   constexpr int BN = NN && BM < 256 ? kGradCols : kLogitCols;
   const int64_t tn = (g.N + BN - 1) / BN, tm = g.offsets ? g.max_tiles : (g.M + BM - 1) / BM;
@@ -489,13 +490,20 @@ hipError_t launch_bm(const GradGemm& g, hipStream_t stream) {
   const dim3 grid((unsigned)blocks), block(BN * 2);
   const bool g32 = NN && g.group_size == 32;
   if (g.bits == 4) {
-    if (g32) grad_gemm_kernel<BM, BN, 4, NN, NN><<<grid, block, 0, stream>>>(g);
-    else grad_gemm_kernel<BM, BN, 4, false, NN><<<grid, block, 0, stream>>>(g);
+    if (g32) grad_gemm_kernel<BM, BN, 4, NN, NN, EPI><<<grid, block, 0, stream>>>(g);
+    else grad_gemm_kernel<BM, BN, 4, false, NN, EPI><<<grid, block, 0, stream>>>(g);
   } else {
-    if (g32) grad_gemm_kernel<BM, BN, 8, NN, NN><<<grid, block, 0, stream>>>(g);
-    else grad_gemm_kernel<BM, BN, 8, false, NN><<<grid, block, 0, stream>>>(g);
+    if (g32) grad_gemm_kernel<BM, BN, 8, NN, NN, EPI><<<grid, block, 0, stream>>>(g);
+    else grad_gemm_kernel<BM, BN, 8, false, NN, EPI><<<grid, block, 0, stream>>>(g);
   }
   return hipGetLastError();
+}
+
+template <int BM>
+hipError_t launch_logits(const GradGemm& g, hipStream_t stream) {
+  return g.epi == kEpiStats    ? launch_bm<BM, false, kEpiStats>(g, stream)
+         : g.epi == kEpiScores ? launch_bm<BM, false, kEpiScores>(g, stream)
+                               : launch_bm<BM, false, kEpiCoef>(g, stream);
 }
 
 }  // namespace
@@ -509,15 +517,15 @@ int grad_gemm_rows(int64_t M) { return M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 
 
 hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stream) {
   // Offsets into one tile's rows and into 64 or 256 weight rows are 32 bits.
-  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || g.lda > kMaxLda ||
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !logits_operands(g)) || g.lda > kMaxLda ||
       256 * (nn ? g.N : g.C) >= 0x7ffffff0LL || g.c_split % kS || g.lda % 8 || g.a_cols % 8 ||
       (g.offsets && (!nn || !g.y || !g.flag || g.splits != 1)))
     return hipErrorInvalidValue;
   switch (bm) {
     case 32: return nn ? launch_bm<32, true>(g, stream) : hipErrorInvalidValue;
     case 64: return nn ? launch_bm<64, true>(g, stream) : hipErrorInvalidValue;
-    case 128: return nn ? launch_bm<128, true>(g, stream) : launch_bm<128, false>(g, stream);
-    case 256: return nn ? launch_bm<256, true>(g, stream) : launch_bm<256, false>(g, stream);
+    case 128: return nn ? launch_bm<128, true>(g, stream) : launch_logits<128>(g, stream);
+    case 256: return nn ? launch_bm<256, true>(g, stream) : launch_logits<256>(g, stream);
   }
   return hipErrorInvalidValue;
 }

@@ -29,7 +29,7 @@ constexpr int kN = kGradTileCols;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-template <bool NN>
+template <bool NN, int EPI = kEpiStats>
 __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   constexpr int BM = kPanelRows, MI = 4, NJ = 4;
   constexpr int XI = BM / 32, YI = kN / 32;  // DMA instructions per wave and step
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
     }
   };
   int32_t id = -1;
-  if (!NN && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
+  if (!NN && EPI != kEpiScores && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
   if (nk > 0) {
     issue(0, 0);
     __builtin_amdgcn_sched_barrier(0);  // the wait counts on this order
@@ -207,16 +207,17 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
   if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
   else {
     uint32_t out[MI][NJ];
-    find_wanted<BM, kN, 256>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
-                                 out);
-    store_stats<MI, NJ>(g, acc, out, mw, m0 + rows, nw);
+    if constexpr (EPI != kEpiScores)
+      find_wanted<BM, kN, 256>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
+                               out);
+    store_logits<EPI>(g, acc, out, mw, m0 + rows, nw);
   }
 }
 
 }  // namespace
 
 hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !g.stats || !g.wanted) || g.lda > kMaxLda ||
+  if (!g.a || !g.panel || (nn ? !g.out && !g.y : !logits_operands(g)) || g.lda > kMaxLda ||
       !panel_gemm_supported(g.ldp) || g.c_split % kS ||
       g.lda % 8 || g.a_cols % 8 || g.ldp % 8 || g.offsets)
     return hipErrorInvalidValue;
@@ -224,7 +225,9 @@ hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
   if (blocks < 1) return hipSuccess;
   if (blocks >= kMaxBlocks) return hipErrorInvalidConfiguration;
   if (nn) panel_gemm_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(g);
-  else panel_gemm_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(g);
+  else if (g.epi == kEpiStats) panel_gemm_kernel<false, kEpiStats><<<(unsigned)blocks, 256, 0, stream>>>(g);
+  else if (g.epi == kEpiScores) panel_gemm_kernel<false, kEpiScores><<<(unsigned)blocks, 256, 0, stream>>>(g);
+  else panel_gemm_kernel<false, kEpiCoef><<<(unsigned)blocks, 256, 0, stream>>>(g);
   return hipGetLastError();
 }
 

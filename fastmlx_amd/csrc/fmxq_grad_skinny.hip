@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void pack_x_kernel(const uint16_t* __restrict_
   xp[i] = v;
 }
 
-template <int BITS, int MT, bool PACKED>
+template <int BITS, int MT, bool PACKED, int EPI>
 __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(GradGemm g) {
   constexpr int NW = BITS / 4;  // 16-byte weight loads per lane and step
   __shared__ __attribute__((aligned(16))) float part[8 * MT * 1024];
@@ -147,12 +147,12 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   constexpr int SH = 16 / MT;
   const int row = 32 * (wave % MT) + r32, share = 2 * (wave / MT) + h;
   uint32_t some = 0;
-  if (row < M)
+  if (EPI != kEpiScores && row < M)
     for (int j = share; j < g.wanted_k; j += SH) {
       const uint32_t c = wanted_column(g, g.wanted[(m0 + row) * g.wanted_k + j], n0);
       if (c < 32) some |= 1u << c;
     }
-  want[share * (MT * 32) + row] = some;
+  if (EPI != kEpiScores) want[share * (MT * 32) + row] = some;
   // The waves' sums, in the order of the waves; wave m finishes row tile m.
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -163,7 +163,8 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   __syncthreads();
   if (wave >= MT) return;
   uint32_t out[1][1] = {{0u}};
-  for (int i = 0; i < SH && i < g.wanted_k; ++i) out[0][0] |= want[i * (MT * 32) + row];
+  if (EPI != kEpiScores)
+    for (int i = 0; i < SH && i < g.wanted_k; ++i) out[0][0] |= want[i * (MT * 32) + row];
   f32x16 sum[1][1];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[0][0][4 * q + e] = v[e];
   }
-  store_stats<1, 1>(g, sum, out, m0 + 32 * wave, g.M, n0);
+  store_logits<EPI>(g, sum, out, m0 + 32 * wave, g.M, n0);
 }
 
 template <int BITS, int MT, bool G32>
@@ -352,21 +353,28 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void grad_skinny_kernel(GradG
   }
 }
 
-template <int BITS, int MT>
+template <int BITS, int MT, int EPI>
 hipError_t launch_logits(const GradGemm& g, hipStream_t stream) {
   const int64_t blocks = (g.N + 31) / 32, chunks = (g.M + kSkinnyRows - 1) / kSkinnyRows;
   if (blocks >= kMaxBlocks || chunks > 65535) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks, (unsigned)chunks);
   if (!g.xp) {
-    logits_skinny_kernel<BITS, MT, false><<<grid, 512, 0, stream>>>(g);
+    logits_skinny_kernel<BITS, MT, false, EPI><<<grid, 512, 0, stream>>>(g);
     return hipGetLastError();
   }
   const int64_t n = (g.C + 63) / 64 * MT * 256;
   pack_x_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)chunks), 256, 0, stream>>>(
       g.a, g.lda, g.M, g.C, reinterpret_cast<u32x4*>(g.xp), MT, n);
   if (hipError_t e = hipGetLastError()) return e;
-  logits_skinny_kernel<BITS, MT, true><<<grid, 512, 0, stream>>>(g);
+  logits_skinny_kernel<BITS, MT, true, EPI><<<grid, 512, 0, stream>>>(g);
   return hipGetLastError();
+}
+
+template <int EPI>
+hipError_t launch_logits_of(const GradGemm& g, hipStream_t stream) {
+  if (g.bits == 4)
+    return g.M <= 32 ? launch_logits<4, 1, EPI>(g, stream) : launch_logits<4, 2, EPI>(g, stream);
+  return g.M <= 32 ? launch_logits<8, 1, EPI>(g, stream) : launch_logits<8, 2, EPI>(g, stream);
 }
 
 template <int BITS, int MT>
@@ -387,7 +395,7 @@ bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols
 }
 
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
-  if (!g.a || !g.w || (nn ? !g.out && !g.y : !g.stats || !g.wanted) ||
+  if (!g.a || !g.w || (nn ? !g.out && !g.y : !logits_operands(g)) ||
       (nn && g.M > kGradSkinnyRows) ||
       !skinny_gemm_supported(g.lda, nn ? g.c_split : 32, nn ? g.N : g.C) || g.offsets || g.lda % 8 ||
       g.a_cols % 8 || g.c_split % 16)
@@ -403,8 +411,9 @@ hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
            : mt == 2 ? launch_grad<8, 2>(g, stream)
                      : launch_grad<8, 3>(g, stream);
   }
-  if (g.bits == 4) return g.M <= 32 ? launch_logits<4, 1>(g, stream) : launch_logits<4, 2>(g, stream);
-  return g.M <= 32 ? launch_logits<8, 1>(g, stream) : launch_logits<8, 2>(g, stream);
+  return g.epi == kEpiStats    ? launch_logits_of<kEpiStats>(g, stream)
+         : g.epi == kEpiScores ? launch_logits_of<kEpiScores>(g, stream)
+                               : launch_logits_of<kEpiCoef>(g, stream);
 }
 
 }  // namespace fmxq

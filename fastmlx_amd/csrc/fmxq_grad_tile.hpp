@@ -226,4 +226,112 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI]
   }
 }
 
+// What log probabilities need of a tile of 32 NJ columns (HeadTile), in units of log 2: its largest
+// logit m and the first column that has it, and of the other columns the sums of 2^(l - m) and of
+// 2^(l - m) (m - l).  That column takes no part in the sums, so that where one token takes nearly
+// everything, what the others leave is not the difference of near equals.  With e, also bf16(2^(l - m)),
+// zeros from column N to the tile's end.
+template <int MI, int NJ>
+__device__ __forceinline__ void store_scores(const GradGemm& g, f32x16 (&acc)[MI][NJ], int64_t mw,
+                                             int64_t mend, int64_t nw) {
+#pragma clang fp contract(off)
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  if (nw >= g.N) return;
+  const int left = g.N - nw < 32 * NJ ? (int)(g.N - nw) : 32 * NJ;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = mw + 32 * i + r32;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        acc[i][j][r] *= g.logit_scale;
+        if (32 * j + 8 * (r >> 2) + 4 * h + (r & 3) < left) top = fmaxf(top, acc[i][j][r]);
+      }
+    top = fmaxf(top, other_half(top));
+    uint32_t first = 32 * NJ;
+#pragma unroll
+    for (int j = NJ - 1; j >= 0; --j)
+#pragma unroll
+      for (int r = 15; r >= 0; --r) {
+        const uint32_t c = 32 * j + 8 * (r >> 2) + 4 * h + (r & 3);
+        if (acc[i][j][r] == top && (int)c < left) first = c;
+      }
+    const uint32_t theirs = other_half(first);
+    first = first < theirs ? first : theirs;
+    float sum = 0.f, low = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * j + 8 * q + 4 * h;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d = top - acc[i][j][4 * q + e];
+          v[e] = c + e < left ? __builtin_amdgcn_exp2f(-d) : 0.f;
+          const float w = (uint32_t)(c + e) == first || c + e >= left ? 0.f : v[e];
+          sum += w;
+          low = __builtin_fmaf(w, w == 0.f ? 0.f : d, low);
+        }
+        if (g.e && m < mend)
+          *reinterpret_cast<u32x2*>(g.e + m * g.lde + nw + c) =
+              u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      }
+    sum += other_half(sum);
+    low += other_half(low);
+    if (h == 0 && m < mend)
+      g.score[m * g.stat_tiles + nw / (32 * NJ)] = HeadTile{top, sum, low, first};
+  }
+}
+
+// The gradient of log probabilities and entropy for the logits of a tile:
+//   d = -p (a + c (log p + entropy)),  p = 2^(l - lse),
+// as bf16 in e, zeros for the row's wanted tokens (whose share enters later) and from column N to
+// the tile's end.
+template <int MI, int NJ>
+__device__ __forceinline__ void store_coef(const GradGemm& g, const f32x16 (&acc)[MI][NJ],
+                                           const uint32_t (&out)[MI][NJ], int64_t mw, int64_t mend,
+                                           int64_t nw) {
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const int64_t ln = g.N - nw;
+  const int left = ln < 0 ? 0 : ln < 32 * NJ ? (int)ln : 32 * NJ;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = mw + 32 * i + r32;
+    const f32x4 row = reinterpret_cast<const f32x4*>(g.rows)[m < mend ? m : mend - 1];
+    const float lse = row[0], a = row[1], c2 = row[2];  // c in units of log 2, c entropy in a
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const uint32_t mine = out[i][j] >> (4 * h);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * j + 8 * q + 4 * h;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lp = __builtin_fmaf(acc[i][j][4 * q + e], g.logit_scale, -lse);
+          const float p = __builtin_amdgcn_exp2f(lp);
+          v[e] = -p * __builtin_fmaf(c2, lp, a);
+          if (p == 0.f || c + e >= left || ((mine >> (8 * q + e)) & 1u)) v[e] = 0.f;
+        }
+        if (m < mend && nw + c < g.lde)
+          *reinterpret_cast<u32x2*>(g.e + m * g.lde + nw + c) =
+              u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      }
+    }
+  }
+}
+
+// A tile's epilogue of logits.
+template <int EPI, int MI, int NJ>
+__device__ __forceinline__ void store_logits(const GradGemm& g, f32x16 (&acc)[MI][NJ],
+                                             const uint32_t (&out)[MI][NJ], int64_t mw, int64_t mend,
+                                             int64_t nw) {
+  if constexpr (EPI == kEpiStats) store_stats<MI, NJ>(g, acc, out, mw, mend, nw);
+  else if constexpr (EPI == kEpiScores) store_scores<MI, NJ>(g, acc, mw, mend, nw);
+  else store_coef<MI, NJ>(g, acc, out, mw, mend, nw);
+}
+
 }  // namespace fmxq

@@ -412,6 +412,111 @@ PyObject* head_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The operands that head_logprobs and its gradient share.
+struct Head {
+  const at::Tensor *h, *w, *s, *b, *ids;
+  int64_t M, V, K, k;
+};
+bool head_operands(Call& c, PyObject* const* a, int64_t group, int64_t bits, Head* o) {
+  o->h = c.tensor(a[0], kBf16Like);
+  o->w = c.tensor(a[1], kU32Like);
+  o->s = c.tensor(a[2], kBf16Like);
+  o->b = c.tensor(a[3], kBf16Like);
+  o->ids = c.tensor(a[4], kU32Like);
+  if (!c.ok || o->h->dim() != 2 || o->w->dim() != 2 || o->ids->dim() != 2 ||
+      o->ids->scalar_type() != at::kInt || !on_current(*o->h))
+    return false;
+  o->M = o->h->size(0);
+  o->K = o->h->size(1);
+  o->V = o->w->size(0);
+  o->k = o->ids->size(1);
+  return o->k <= 64 && weight_ok(*o->h, *o->w, *o->s, *o->b, o->K, group, bits) &&
+         same(*o->ids, *o->h, {o->M, o->k});
+}
+template <class T = uint16_t>
+T* at_of(const at::Tensor* t) {
+  return static_cast<T*>(t->data_ptr());
+}
+
+// (h, w, scales, biases, ids, top, temperature, group_size, bits) -> (logp, entropy, lse) and, with
+// top, (top_ids, top_logp)
+PyObject* head_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 9 || !PyFloat_CheckExact(a[6])) return nullptr;
+    Call c;
+    int64_t group, bits, top;
+    Head o;
+    if (!c.integer(a[5], &top) || !c.format(a[7], a[8], &group, &bits) ||
+        !head_operands(c, a, group, bits, &o) || top < 0 || top > 64)
+      return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*o.h,
+                   [&](size_t* out) {
+                     return fmxq_head_logprobs_workspace(o.M, o.V, o.K, (int)o.k, (int)top, out);
+                   },
+                   &ws, &bytes))
+      return nullptr;
+    at::Tensor logp = make(*o.h, {o.M, o.k}, at::kFloat), ent = make(*o.h, {o.M}, at::kFloat),
+               lse = make(*o.h, {o.M}, at::kFloat), ti, tl;
+    if (top) {
+      ti = make(*o.h, {o.M, top}, at::kInt);
+      tl = make(*o.h, {o.M, top}, at::kFloat);
+    }
+    void* st = stream_of(*o.h);
+    const float temperature = (float)PyFloat_AS_DOUBLE(a[6]);
+    if (!enqueue([&] {
+          return fmxq_head_logprobs(at_of(o.h), at_of<uint32_t>(o.w), at_of(o.s), at_of(o.b),
+                                    at_of<int32_t>(o.ids), at_of<float>(&logp), at_of<float>(&ent),
+                                    at_of<float>(&lse), top ? at_of<int32_t>(&ti) : nullptr,
+                                    top ? at_of<float>(&tl) : nullptr, o.M, o.V, o.K, (int)o.k, (int)top,
+                                    temperature, (int)group, (int)bits, ws.data_ptr(), bytes, st);
+        }))
+      return nullptr;
+    if (!top)
+      return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(logp)), THPVariable_Wrap(std::move(ent)),
+                           THPVariable_Wrap(std::move(lse)));
+    return Py_BuildValue("(NNNNN)", THPVariable_Wrap(std::move(logp)), THPVariable_Wrap(std::move(ent)),
+                         THPVariable_Wrap(std::move(lse)), THPVariable_Wrap(std::move(ti)),
+                         THPVariable_Wrap(std::move(tl)));
+  });
+}
+
+// (h, w, scales, biases, ids, logp, entropy, lse, grad_logp, grad_entropy | None, temperature,
+// group_size, bits) -> dh
+PyObject* head_logprobs_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 13 || !PyFloat_CheckExact(a[10])) return nullptr;
+    Call c;
+    int64_t group, bits;
+    Head o;
+    const at::Tensor *logp = c.tensor(a[5], kF32), *ent = c.tensor(a[6], kF32), *lse = c.tensor(a[7], kF32),
+                     *gl = c.tensor(a[8], kF32), *ge = a[9] == Py_None ? nullptr : c.tensor(a[9], kF32);
+    if (!c.format(a[11], a[12], &group, &bits) || !head_operands(c, a, group, bits, &o) ||
+        !same(*logp, *o.h, {o.M, o.k}) || !same(*gl, *o.h, {o.M, o.k}) || !same(*ent, *o.h, {o.M}) ||
+        !same(*lse, *o.h, {o.M}) || (ge && !same(*ge, *o.h, {o.M})))
+      return nullptr;
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (!workspace(*o.h,
+                   [&](size_t* out) { return fmxq_head_logprobs_grad_workspace(o.M, o.V, o.K, (int)o.k, out); },
+                   &ws, &bytes))
+      return nullptr;
+    at::Tensor dh = make(*o.h, {o.M, o.K}, at::kBFloat16);
+    void* st = stream_of(*o.h);
+    const float temperature = (float)PyFloat_AS_DOUBLE(a[10]);
+    if (!enqueue([&] {
+          return fmxq_head_logprobs_grad(at_of(o.h), at_of<uint32_t>(o.w), at_of(o.s), at_of(o.b),
+                                         at_of<int32_t>(o.ids), at_of<float>(logp), at_of<float>(ent),
+                                         at_of<float>(lse), at_of<float>(gl), ge ? at_of<float>(ge) : nullptr,
+                                         at_of(&dh), o.M, o.V, o.K, (int)o.k, temperature, (int)group,
+                                         (int)bits, ws.data_ptr(), bytes, st);
+        }))
+      return nullptr;
+    return THPVariable_Wrap(std::move(dh));
+  });
+}
+
 // (dy, w, scales, biases, offsets | None, group_size, bits): quantized_matmul_grad, or
 // gather_qmm_grad with offsets.
 PyObject* qmm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -574,11 +679,6 @@ bool lora_operands(Call& c, PyObject* const* a, int64_t group, int64_t bits, Lor
          same(*l->la, *l->x, {l->E, l->r, l->K}) && same(*l->lb, *l->x, {l->E, l->N, l->r}) &&
          same(*l->ls, *l->x, {l->E}) && same(*l->ids, *l->x, l->x->sizes().slice(0, l->x->dim() - 1));
 }
-template <class T = uint16_t>
-T* at_of(const at::Tensor* t) {
-  return static_cast<T*>(t->data_ptr());
-}
-
 // (x, w, scales, biases, a, b, adapters, lora_scales, group_size, bits) -> y
 PyObject* qmm_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -701,6 +801,7 @@ PyMethodDef methods[] = {FMXQ_FAST(quantized_matmul), FMXQ_FAST(dequantize),    
                          FMXQ_FAST(head_loss),        FMXQ_FAST(qmm_grad),           FMXQ_FAST(moe_sort),
                          FMXQ_FAST(moe_unsort),       FMXQ_FAST(moe_unsort_grad),
                          FMXQ_FAST(qmm_lora),         FMXQ_FAST(qmm_lora_grad),      FMXQ_FAST(clip),
+                         FMXQ_FAST(head_logprobs),    FMXQ_FAST(head_logprobs_grad),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -440,6 +440,80 @@ def head_distill(h, w, scales, biases, ids, teacher, temperature: float = 1.0, g
     return (loss, lse, dh) if grad else (loss, lse)
 
 
+def _score_operands(h, w, scales, biases, ids, group_size, bits):
+    M, V, K, ptrs = _head_operands(h, w, scales, biases, False, None, group_size, bits)
+    if ids.dim() != 2:
+        raise ValueError("ids must be [M, k]")
+    k = min(ids.shape[1], 2**31 - 1)  # more than 64 are refused by the library
+    _shape("ids", ids, M, k)
+    return M, V, K, k, (*ptrs, _dev(ids, "ids", (torch.int32,)))
+
+
+def head_logprobs(h, w, scales, biases, ids, top: int = 0, temperature: float = 1.0,
+                  group_size: int = 64, bits: int = 4):
+    """Log probabilities of given tokens through a quantized vocabulary head, its logits never
+    returned, with the entropy and the likeliest tokens.
+
+    h [M, K] bf16; w [V, K*bits/32] with scales and biases [V, K/group]; ids [M, k] int32, k <= 64,
+    an id below zero for an absent entry (0 in logp).  With l = logits / temperature and p =
+    softmax(l): (logp [M, k], entropy [M], lse [M]) float32, and with ``top`` (up to 64) also
+    (top_ids [M, top] int32, top_logp [M, top]), likeliest first, equal ones to the lower token.
+    An id past the vocabulary counts as absent, and device_error reports it.  A row whose logits are
+    not finite gives NaN and top_ids -1."""
+    if _fast is not None:
+        r = _fast.head_logprobs(h, w, scales, biases, ids, top, float(temperature), group_size, bits)
+        if r is not None:
+            return r
+    dev = _same_device(h=h, w=w, scales=scales, biases=biases, ids=ids)
+    M, V, K, k, ptrs = _score_operands(h, w, scales, biases, ids, group_size, bits)
+    top = min(max(int(top), -1), 2**31 - 1)  # outside 0 .. 64 the library refuses
+    lib = load()
+    with torch.cuda.device(dev):
+        ws, n, keep = _workspace(lib.fmxq_head_logprobs_workspace, dev, M, V, K, k, top)
+        logp = torch.empty(M, k, dtype=torch.float32, device=dev)
+        entropy = torch.empty(M, dtype=torch.float32, device=dev)
+        lse = torch.empty(M, dtype=torch.float32, device=dev)
+        top_ids = torch.empty(M, top, dtype=torch.int32, device=dev)
+        top_logp = torch.empty(M, top, dtype=torch.float32, device=dev)
+        check(lib.fmxq_head_logprobs(*ptrs, logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+                                     top_ids.data_ptr(), top_logp.data_ptr(), M, V, K, k, top,
+                                     temperature, group_size, bits, ws, n, _stream(h)))
+    return (logp, entropy, lse, top_ids, top_logp) if top else (logp, entropy, lse)
+
+
+def head_logprobs_grad(h, w, scales, biases, ids, logp, entropy, lse, grad_logp, grad_entropy=None,
+                       temperature: float = 1.0, group_size: int = 64, bits: int = 4):
+    """Gradient of h in head_logprobs: from those of logp [M, k] (k >= 1) and entropy [M] (None: no
+    gradient), float32, and the logp, entropy and lse that head_logprobs returned for the same
+    operands.  Returns dh [M, K] bf16; absent entries pass nothing back."""
+    if _fast is not None:
+        r = _fast.head_logprobs_grad(h, w, scales, biases, ids, logp, entropy, lse, grad_logp,
+                                     grad_entropy, float(temperature), group_size, bits)
+        if r is not None:
+            return r
+    more = {} if grad_entropy is None else {"grad_entropy": grad_entropy}
+    dev = _same_device(h=h, w=w, scales=scales, biases=biases, ids=ids, logp=logp, entropy=entropy,
+                       lse=lse, grad_logp=grad_logp, **more)
+    M, V, K, k, ptrs = _score_operands(h, w, scales, biases, ids, group_size, bits)
+    f32 = (torch.float32,)
+    _shape("logp", logp, M, k)
+    _shape("grad_logp", grad_logp, M, k)
+    _shape("entropy", entropy, M)
+    _shape("lse", lse, M)
+    if grad_entropy is not None:
+        _shape("grad_entropy", grad_entropy, M)
+        _dev(grad_entropy, "grad_entropy", f32)
+    ptrs += (_dev(logp, "logp", f32), _dev(entropy, "entropy", f32), _dev(lse, "lse", f32),
+             _dev(grad_logp, "grad_logp", f32), _ptr(grad_entropy))
+    lib = load()
+    with torch.cuda.device(dev):
+        ws, n, keep = _workspace(lib.fmxq_head_logprobs_grad_workspace, dev, M, V, K, k)
+        dh = torch.empty(M, K, dtype=torch.bfloat16, device=dev)
+        check(lib.fmxq_head_logprobs_grad(*ptrs, dh.data_ptr(), M, V, K, k, temperature, group_size,
+                                          bits, ws, n, _stream(h)))
+    return dh
+
+
 def quantized_matmul_grad(dy, w, scales, biases, group_size: int = 64, bits: int = 4):
     """Gradient of x in quantized_matmul: dx = dy @ deq(W), dy [..., N] bf16, w [N, K*bits/32];
     dx [..., K] bf16."""

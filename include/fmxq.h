@@ -319,6 +319,34 @@ int fmxq_head_distill(const uint16_t* h, const uint32_t* w, const uint16_t* scal
 /* Workspace of the two losses (top_k = 1 for cross entropy). */
 int fmxq_head_workspace(int64_t M, int64_t V, int64_t K, int top_k, bool with_grad, size_t* bytes);
 
+/* Log probabilities of given tokens through the same head, for scoring, sampling with alternatives and
+ * policy training.  With T = temperature > 0, l = h . deq(W)^T / T and p = softmax(l):
+ *     lse[t] = log sum_v exp(l[t, v]),  logp[t, j] = l[t, ids[t, j]] - lse[t],
+ *     entropy[t] = -sum_v p_v log p_v,
+ * and the `top` tokens of the largest l with their log probabilities, in falling order: top_ids and
+ * top_logp [M, top], 0 <= top <= min(64, V).  ids and logp [M, k], 0 <= k <= 64; an id below zero is
+ * absent (logp 0), one of V or more too, which raises the error flag.  The order of the top tokens is
+ * that of logits summed in 64 bits, equal ones to the lower token.  A row with logits that are not finite
+ * gives NaN and top_ids -1. */
+int fmxq_head_logprobs(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
+                       const uint16_t* biases, const int32_t* ids, float* logp, float* entropy, float* lse,
+                       int32_t* top_ids, float* top_logp, int64_t M, int64_t V, int64_t K, int k, int top,
+                       float temperature, int group_size, int bits, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int fmxq_head_logprobs_workspace(int64_t M, int64_t V, int64_t K, int k, int top, size_t* bytes);
+/* Its gradient of the hidden states, from those of logp [M, k] (1 <= k <= 64) and entropy [M] (NULL:
+ * none) and the logp, entropy and lse that fmxq_head_logprobs gave for the same operands:
+ *     dh[t] = 1/T sum_v W_v (sum_j grad_logp[t, j] [ids[t, j] = v]
+ *                            - p_v (sum_j grad_logp[t, j] + grad_entropy[t] (log p_v + entropy[t]))).
+ * Absent entries' gradients are not read into it; a row whose gradients are all 0 gives zeros. */
+int fmxq_head_logprobs_grad(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
+                            const uint16_t* biases, const int32_t* ids, const float* logp,
+                            const float* entropy, const float* lse, const float* grad_logp,
+                            const float* grad_entropy, uint16_t* dh, int64_t M, int64_t V, int64_t K, int k,
+                            float temperature, int group_size, int bits, void* workspace,
+                            size_t workspace_bytes, void* stream);
+int fmxq_head_logprobs_grad_workspace(int64_t M, int64_t V, int64_t K, int k, size_t* bytes);
+
 /* Gradient of x in quantized_matmul's y = x . deq(W)^T:
  *     dx [M, K] = dy [M, N] . deq(W),  dy and dx bf16, N any size. */
 int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
