@@ -7,9 +7,20 @@
 
 namespace fmxq {
 
-// What a product of logits leaves (nt): the softmax statistics of the losses, those of log
-// probabilities, or the logits' gradient.
-enum Epilogue { kEpiStats = 0, kEpiScores = 1, kEpiCoef = 2 };
+// What a product leaves.  Logits (nt): the softmax statistics of the losses, those of log
+// probabilities, the logits' gradient, or itself.  Input gradients (nn): itself.  The product
+// itself (kEpiOut) takes a low-rank adapter's part.
+enum Epilogue { kEpiStats = 0, kEpiScores = 1, kEpiCoef = 2, kEpiOut = 3 };
+// The adapter's part of row m, output n: sum_j (u0 + u1)[m][j] v[e][n][j] with e = ids[m], none
+// where it is outside 0 .. E - 1.  u: `parts` rows of r bf16 values for each m, of which the first two
+// are taken (their sum holds the value to 16 bits); v [E][n][r].
+struct LoraAdd {
+  const uint16_t* u = nullptr;
+  const uint16_t* v = nullptr;
+  const int32_t* ids = nullptr;
+  int64_t E = 0, n = 0;  // n: rows of v an adapter (N, or of more outputs than this product's)
+  int r = 0, parts = 0;
+};
 // A tile of a row's logits for log probabilities (store_scores).
 struct HeadTile {
   float top, sum, low;
@@ -68,6 +79,8 @@ struct GradGemm {
   Epilogue epi = kEpiStats;
   HeadTile* score = nullptr;
   const float* rows = nullptr;
+  // kEpiOut: as nn into y or out (of one part y, any N), with the adapter's part in the first.
+  LoraAdd lora;
   // Expert runs (nn only, into y): rows offsets[e] .. offsets[e + 1] of M take expert e, whose
   // weights are C rows into w; other rows get zeros.  max_tiles: grad_gemm_run_tiles.  *flag
   // is raised where the offsets decrease or leave 0 .. M (all rows are zero then).
@@ -126,6 +139,10 @@ hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64
 // dst [M, ld] = src [M, N] with zeros in columns N .. ld.
 hipError_t launch_pad_rows(const uint16_t* src, uint16_t* dst, int64_t M, int64_t N, int64_t ld,
                            hipStream_t stream);
+// fmxq_quantized_matmul_grad, its checks included, with an adapter's part (fmxq_grad_capi.cpp).
+int input_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
+               const LoraAdd& lora, uint16_t* dx, int64_t M, int64_t N, int64_t K, int group_size, int bits,
+               void* workspace, size_t workspace_bytes, void* stream, const char* op);
 // A loss over a quantized head (fmxq_head.hip).  ids [M, k]: the targets (k = 1, teacher
 // null) or the teacher's entries.  An id that names no token: `ignore` for targets, below
 // zero for a teacher.
@@ -154,6 +171,8 @@ struct HeadPlan {
   bool panel, skinny, grad_skinny;
   size_t stats, e, slices, state, factor, sel, panel_at, xp, bytes;  // in the workspace
 };
+// Few tokens for many rows: launch_skinny_gemm takes them in chunks.
+bool few_tokens(int64_t M, int64_t V, int bm, int cus);
 HeadPlan head_plan(int64_t M, int64_t V, int64_t K, int k, bool grad, int cus);
 // Whether the operands of a product's logits are there.
 inline bool logits_operands(const GradGemm& g) {
@@ -161,6 +180,7 @@ inline bool logits_operands(const GradGemm& g) {
     case kEpiStats: return g.stats && g.wanted;
     case kEpiScores: return g.score != nullptr;
     case kEpiCoef: return g.rows && g.wanted && g.e;
+    case kEpiOut: return g.y || g.out;
   }
   return false;
 }

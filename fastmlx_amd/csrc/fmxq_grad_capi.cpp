@@ -209,6 +209,74 @@ int row_sizes(int64_t T, int64_t k, int64_t D, const char* op) {
 
 }  // namespace
 
+int fmxq::input_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
+                     const uint16_t* biases, const LoraAdd& lora, uint16_t* dx, int64_t M, int64_t N,
+                     int64_t K, int group_size, int bits, void* workspace, size_t workspace_bytes,
+                     void* stream, const char* op) {
+  if (int rc = check_quant(group_size, bits, K, true, op)) return rc;
+  if (int rc = grad_sizes(M, N, K, op)) return rc;
+  if (M == 0) return FMXQ_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!dx || !aligned16(dx))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: dx must be 16-byte aligned", op);
+  if (N == 0)
+    return hip_status(fmxq::launch_fill_u32(reinterpret_cast<uint32_t*>(dx), 0u, M * K / 2, s), op);
+  if (!dy || !w || !scales || !biases) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
+  if (!aligned16(w)) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: w must be 16-byte aligned", op);
+  if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
+  const GradPlan p = grad_plan(M, N, K);
+  const size_t moved = moved_bytes(dy, M, N), moved_at = moved ? up(p.bytes, 256) : 0;
+  if (int rc = check_workspace(workspace, workspace_bytes, moved ? moved_at + moved : p.bytes, op))
+    return rc;
+  char* ws = static_cast<char*>(workspace);
+  fmxq::GradGemm g;
+  if (int rc = grad_operand(dy, ws + moved_at, M, N, s, &g, op)) return rc;
+  g.M = M;
+  g.N = K;
+  g.C = N;
+  g.w = w;
+  g.scales = scales;
+  g.biases = biases;
+  g.group_size = group_size;
+  g.bits = bits;
+  g.splits = p.splits;
+  g.lora = lora;
+  g.c_split = p.c_split;
+  float* slices = reinterpret_cast<float*>(ws + p.slices);
+  if (p.splits > 1 || p.piece < N) {
+    g.out = slices;
+  } else {
+    g.y = dx;
+    g.ldy = K;
+  }
+  if (p.panel) {
+    uint16_t* panel = reinterpret_cast<uint16_t*>(ws + p.panel_at);
+    g.panel = panel;
+    g.ldp = K;
+    for (int64_t n0 = 0; n0 < N; n0 += p.piece) {
+      fmxq::GradGemm d = g;
+      d.C = std::min(p.piece, N - n0);
+      d.a = g.a + n0;
+      d.a_cols = std::min(p.piece, g.a_cols - n0);
+      d.add = n0 > 0;
+      if (d.add) d.lora = fmxq::LoraAdd{};
+      const int64_t at = n0 * (K / group_size);
+      if (int rc = hip_status(fmxq::launch_dequantize(w + n0 * (K * bits / 32), scales + at, biases + at,
+                                                      panel, d.C, K, group_size, bits, s),
+                              op))
+        return rc;
+      if (int rc = hip_status(fmxq::launch_panel_gemm(d, true, s), op)) return rc;
+    }
+  } else if (int rc = hip_status(p.skinny ? fmxq::launch_skinny_gemm(g, true, s)
+                                          : fmxq::launch_grad_gemm(g, true, p.bm, s),
+                                 op)) {
+    return rc;
+  }
+  if (!g.out) return FMXQ_OK;
+  return hip_status(fmxq::launch_sum_slices(slices, p.splits, dx, M, K, s), op);
+}
+
 extern "C" {
 
 int fmxq_head_workspace(int64_t M, int64_t V, int64_t K, int top_k, bool with_grad, size_t* bytes) {
@@ -325,67 +393,8 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
                                const uint16_t* biases, uint16_t* dx, int64_t M, int64_t N,
                                int64_t K, int group_size, int bits, void* workspace,
                                size_t workspace_bytes, void* stream) {
-  const char* op = "quantized_matmul_grad";
-  if (int rc = check_quant(group_size, bits, K, true, op)) return rc;
-  if (int rc = grad_sizes(M, N, K, op)) return rc;
-  if (M == 0) return FMXQ_OK;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!dx || !aligned16(dx))
-    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: dx must be 16-byte aligned", op);
-  if (N == 0)
-    return hip_status(fmxq::launch_fill_u32(reinterpret_cast<uint32_t*>(dx), 0u, M * K / 2, s), op);
-  if (!dy || !w || !scales || !biases) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
-  if (!aligned16(w)) return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: w must be 16-byte aligned", op);
-  if (!aligned(dy, 2) || !aligned(scales, 2) || !aligned(biases, 2))
-    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
-  const GradPlan p = grad_plan(M, N, K);
-  const size_t moved = moved_bytes(dy, M, N), moved_at = moved ? up(p.bytes, 256) : 0;
-  if (int rc = check_workspace(workspace, workspace_bytes, moved ? moved_at + moved : p.bytes, op))
-    return rc;
-  char* ws = static_cast<char*>(workspace);
-  fmxq::GradGemm g;
-  if (int rc = grad_operand(dy, ws + moved_at, M, N, s, &g, op)) return rc;
-  g.M = M;
-  g.N = K;
-  g.C = N;
-  g.w = w;
-  g.scales = scales;
-  g.biases = biases;
-  g.group_size = group_size;
-  g.bits = bits;
-  g.splits = p.splits;
-  g.c_split = p.c_split;
-  float* slices = reinterpret_cast<float*>(ws + p.slices);
-  if (p.splits > 1 || p.piece < N) {
-    g.out = slices;
-  } else {
-    g.y = dx;
-    g.ldy = K;
-  }
-  if (p.panel) {
-    uint16_t* panel = reinterpret_cast<uint16_t*>(ws + p.panel_at);
-    g.panel = panel;
-    g.ldp = K;
-    for (int64_t n0 = 0; n0 < N; n0 += p.piece) {
-      fmxq::GradGemm d = g;
-      d.C = std::min(p.piece, N - n0);
-      d.a = g.a + n0;
-      d.a_cols = std::min(p.piece, g.a_cols - n0);
-      d.add = n0 > 0;
-      const int64_t at = n0 * (K / group_size);
-      if (int rc = hip_status(fmxq::launch_dequantize(w + n0 * (K * bits / 32), scales + at, biases + at,
-                                                      panel, d.C, K, group_size, bits, s),
-                              op))
-        return rc;
-      if (int rc = hip_status(fmxq::launch_panel_gemm(d, true, s), op)) return rc;
-    }
-  } else if (int rc = hip_status(p.skinny ? fmxq::launch_skinny_gemm(g, true, s)
-                                          : fmxq::launch_grad_gemm(g, true, p.bm, s),
-                                 op)) {
-    return rc;
-  }
-  if (!g.out) return FMXQ_OK;
-  return hip_status(fmxq::launch_sum_slices(slices, p.splits, dx, M, K, s), op);
+  return fmxq::input_grad(dy, w, scales, biases, fmxq::LoraAdd{}, dx, M, N, K, group_size, bits, workspace,
+                          workspace_bytes, stream, "quantized_matmul_grad");
 }
 
 int fmxq_gather_qmm_grad_workspace(int64_t S, int64_t E, int64_t N, int64_t K, size_t* bytes) {

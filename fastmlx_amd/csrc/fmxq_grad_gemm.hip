@@ -425,7 +425,7 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
     pace(1);
   };
   int32_t id = -1;
-  if (!NN && EPI != kEpiScores && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
+  if (!NN && epi_wants(EPI) && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
   if (nk > 0) {
 #pragma unroll
     for (int i = 0; i < AS; ++i) {  // the waits count on this order
@@ -470,13 +470,14 @@ __global__ __launch_bounds__(BN * 2, NN && BM < 64 ? 3 : 2) void grad_gemm_kerne
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
   }
   const int64_t mw = m0 + wm * MI * 32, nw = n0 + wn * NJ * 32;
-  if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
+  if constexpr (NN && EPI == kEpiOut) store_out<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
+  else if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
   else {
     uint32_t out[MI][NJ];
-    if constexpr (EPI != kEpiScores)
+    if constexpr (epi_wants(EPI))
       find_wanted<BM, BN, W * 64>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
                                   out);
-    store_logits<EPI>(g, acc, out, mw, m0 + rows, nw);
+    store_logits<EPI>(g, acc, out, mw, m0 + rows, nw, split);
   }
 }
 
@@ -503,7 +504,13 @@ template <int BM>
 hipError_t launch_logits(const GradGemm& g, hipStream_t stream) {
   return g.epi == kEpiStats    ? launch_bm<BM, false, kEpiStats>(g, stream)
          : g.epi == kEpiScores ? launch_bm<BM, false, kEpiScores>(g, stream)
-                               : launch_bm<BM, false, kEpiCoef>(g, stream);
+         : g.epi == kEpiCoef   ? launch_bm<BM, false, kEpiCoef>(g, stream)
+                               : launch_bm<BM, false, kEpiOut>(g, stream);
+}
+
+template <int BM>
+hipError_t launch_grads(const GradGemm& g, hipStream_t stream) {
+  return g.lora.u ? launch_bm<BM, true, kEpiOut>(g, stream) : launch_bm<BM, true>(g, stream);
 }
 
 }  // namespace
@@ -522,10 +529,10 @@ hipError_t launch_grad_gemm(const GradGemm& g, bool nn, int bm, hipStream_t stre
       (g.offsets && (!nn || !g.y || !g.flag || g.splits != 1)))
     return hipErrorInvalidValue;
   switch (bm) {
-    case 32: return nn ? launch_bm<32, true>(g, stream) : hipErrorInvalidValue;
-    case 64: return nn ? launch_bm<64, true>(g, stream) : hipErrorInvalidValue;
-    case 128: return nn ? launch_bm<128, true>(g, stream) : launch_logits<128>(g, stream);
-    case 256: return nn ? launch_bm<256, true>(g, stream) : launch_logits<256>(g, stream);
+    case 32: return nn ? launch_grads<32>(g, stream) : hipErrorInvalidValue;
+    case 64: return nn ? launch_grads<64>(g, stream) : hipErrorInvalidValue;
+    case 128: return nn ? launch_grads<128>(g, stream) : launch_logits<128>(g, stream);
+    case 256: return nn ? launch_grads<256>(g, stream) : launch_logits<256>(g, stream);
   }
   return hipErrorInvalidValue;
 }

@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
     }
   };
   int32_t id = -1;
-  if (!NN && EPI != kEpiScores && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
+  if (!NN && epi_wants(EPI) && g.wanted_k == 1 && tid < rows) id = g.wanted[m0 + tid];
   if (nk > 0) {
     issue(0, 0);
     __builtin_amdgcn_sched_barrier(0);  // the wait counts on this order
@@ -204,13 +204,14 @@ __global__ __launch_bounds__(256, 1) void panel_gemm_kernel(GradGemm g) {
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
   }
   const int64_t mw = m0 + wm * MI * 32, nw = n0 + wn * NJ * 32;
-  if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
+  if constexpr (NN && EPI == kEpiOut) store_out<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
+  else if constexpr (NN) store_grad<MI, NJ>(g, acc, mw, m0 + rows, nw, split);
   else {
     uint32_t out[MI][NJ];
-    if constexpr (EPI != kEpiScores)
+    if constexpr (epi_wants(EPI))
       find_wanted<BM, kN, 256>(g, m0, rows, n0, mw, nw, one, reinterpret_cast<uint32_t*>(as0),
                                out);
-    store_logits<EPI>(g, acc, out, mw, m0 + rows, nw);
+    store_logits<EPI>(g, acc, out, mw, m0 + rows, nw, split);
   }
 }
 
@@ -224,7 +225,9 @@ hipError_t launch_panel_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
   const int64_t blocks = (g.M + kPanelRows - 1) / kPanelRows * ((g.N + kN - 1) / kN) * g.splits;
   if (blocks < 1) return hipSuccess;
   if (blocks >= kMaxBlocks) return hipErrorInvalidConfiguration;
-  if (nn) panel_gemm_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(g);
+  if (nn && g.lora.u) panel_gemm_kernel<true, kEpiOut><<<(unsigned)blocks, 256, 0, stream>>>(g);
+  else if (nn) panel_gemm_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(g);
+  else if (g.epi == kEpiOut) panel_gemm_kernel<false, kEpiOut><<<(unsigned)blocks, 256, 0, stream>>>(g);
   else if (g.epi == kEpiStats) panel_gemm_kernel<false, kEpiStats><<<(unsigned)blocks, 256, 0, stream>>>(g);
   else if (g.epi == kEpiScores) panel_gemm_kernel<false, kEpiScores><<<(unsigned)blocks, 256, 0, stream>>>(g);
   else panel_gemm_kernel<false, kEpiCoef><<<(unsigned)blocks, 256, 0, stream>>>(g);

@@ -147,12 +147,12 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   constexpr int SH = 16 / MT;
   const int row = 32 * (wave % MT) + r32, share = 2 * (wave / MT) + h;
   uint32_t some = 0;
-  if (EPI != kEpiScores && row < M)
+  if (epi_wants(EPI) && row < M)
     for (int j = share; j < g.wanted_k; j += SH) {
       const uint32_t c = wanted_column(g, g.wanted[(m0 + row) * g.wanted_k + j], n0);
       if (c < 32) some |= 1u << c;
     }
-  if (EPI != kEpiScores) want[share * (MT * 32) + row] = some;
+  if (epi_wants(EPI)) want[share * (MT * 32) + row] = some;
   // The waves' sums, in the order of the waves; wave m finishes row tile m.
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
   __syncthreads();
   if (wave >= MT) return;
   uint32_t out[1][1] = {{0u}};
-  if (EPI != kEpiScores)
+  if (epi_wants(EPI))
     for (int i = 0; i < SH && i < g.wanted_k; ++i) out[0][0] |= want[i * (MT * 32) + row];
   f32x16 sum[1][1];
 #pragma unroll
@@ -178,10 +178,10 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[0][0][4 * q + e] = v[e];
   }
-  store_logits<EPI>(g, sum, out, m0 + 32 * wave, g.M, n0);
+  store_logits<EPI>(g, sum, out, m0 + 32 * wave, g.M, n0, 0);
 }
 
-template <int BITS, int MT, bool G32>
+template <int BITS, int MT, bool G32, bool LORA>
 __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void grad_skinny_kernel(GradGemm g) {
   constexpr int NG = G32 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) float part[8 * 2048];
@@ -338,6 +338,26 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void grad_skinny_kernel(GradG
     const int64_t row = (ln & 15) + 16 * m;
     const int64_t n = n0 + 8 * (4 * (ln >> 4) + (un >> 1)) + 4 * (un & 1);
     if (row >= g.M || n >= g.N) continue;
+    if constexpr (LORA) {
+      const int e = split == 0 ? adapter_of(g.lora, row) : -1;
+      if (e >= 0) {
+        const uint16_t* u = g.lora.u + row * g.lora.parts * g.lora.r;
+        const uint16_t* b = g.lora.v + ((int64_t)e * g.lora.n + n) * g.lora.r;
+        for (int j = 0; j < g.lora.r; j += 8) {
+          const u32x4 u0 = *reinterpret_cast<const u32x4*>(u + j);
+          const u32x4 u1 = *reinterpret_cast<const u32x4*>(u + g.lora.r + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(b + i * g.lora.r + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[i] = __builtin_fmaf(bf16_lo(w[k]), bf16_lo(u0[k]) + bf16_lo(u1[k]), v[i]);
+              v[i] = __builtin_fmaf(bf16_hi(w[k]), bf16_hi(u0[k]) + bf16_hi(u1[k]), v[i]);
+            }
+          }
+        }
+      }
+    }
     if (g.y) {
       *reinterpret_cast<u32x2*>(g.y + row * g.ldy + n) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     } else {
@@ -381,8 +401,14 @@ template <int BITS, int MT>
 hipError_t launch_grad(const GradGemm& g, hipStream_t stream) {
   const int64_t blocks = (g.N + kSkinnyCols - 1) / kSkinnyCols * g.splits;
   if (blocks >= kMaxBlocks) return hipErrorInvalidConfiguration;
-  if (g.group_size == 32) grad_skinny_kernel<BITS, MT, true><<<(unsigned)blocks, 512, 0, stream>>>(g);
-  else grad_skinny_kernel<BITS, MT, false><<<(unsigned)blocks, 512, 0, stream>>>(g);
+  const unsigned n = (unsigned)blocks;
+  if (g.lora.u) {
+    if (g.group_size == 32) grad_skinny_kernel<BITS, MT, true, true><<<n, 512, 0, stream>>>(g);
+    else grad_skinny_kernel<BITS, MT, false, true><<<n, 512, 0, stream>>>(g);
+  } else {
+    if (g.group_size == 32) grad_skinny_kernel<BITS, MT, true, false><<<n, 512, 0, stream>>>(g);
+    else grad_skinny_kernel<BITS, MT, false, false><<<n, 512, 0, stream>>>(g);
+  }
   return hipGetLastError();
 }
 
@@ -413,7 +439,8 @@ hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream) {
   }
   return g.epi == kEpiStats    ? launch_logits_of<kEpiStats>(g, stream)
          : g.epi == kEpiScores ? launch_logits_of<kEpiScores>(g, stream)
-                               : launch_logits_of<kEpiCoef>(g, stream);
+         : g.epi == kEpiCoef   ? launch_logits_of<kEpiCoef>(g, stream)
+                               : launch_logits_of<kEpiOut>(g, stream);
 }
 
 }  // namespace fmxq

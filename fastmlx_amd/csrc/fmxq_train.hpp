@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fmxq_grad.hpp"
+
 namespace fmxq {
 
 // ---- the norm over many tensors ----
@@ -47,30 +49,59 @@ struct LoraRows {
 constexpr int kLoraMaxRank = 128;
 constexpr int64_t kLoraMaxAdapters = 2048;
 constexpr int64_t kLoraMaxBlocks = 1 << 23;  // of a launch
-// Parts of the shrink's contraction of C values, for M rows in tiles.
-int lora_splits(int64_t M, int64_t C);
+// u rows: the bf16 parts whose sum stands for a value of t (LoraAdd takes two, products of
+// fp32 results three).
+constexpr int kLoraParts = 3;
+
 // t [splits][M][r] = P . V_e^T by position: P [M, C] (rows of ldp values), V [E][r] rows of ldv
 // values; C, ldp and ldv multiples of 8.  Positions without adapter are not written.
-hipError_t launch_lora_shrink(const LoraRows& l, const uint16_t* p, int64_t ldp, const uint16_t* v,
-                              int64_t ldv, int64_t C, int splits, float* t, hipStream_t stream);
-// The same a row at a time (order null, one part).
-hipError_t launch_lora_shrink_rows(const LoraRows& l, const uint16_t* p, int64_t ldp, const uint16_t* v,
-                                   int64_t ldv, int64_t C, float* t, hipStream_t stream);
-// y [M, N] += scales[e] t . V_e^T, V [E][N][r].
-hipError_t launch_lora_expand(const LoraRows& l, const float* t, int splits, const float* scales,
-                              const uint16_t* v, uint16_t* y, int64_t N, hipStream_t stream);
-hipError_t launch_lora_expand_rows(const LoraRows& l, const float* t, const float* scales,
-                                   const uint16_t* v, uint16_t* y, int64_t N, hipStream_t stream);
-// g [E][C][r] (or [E][r][C] with rows_r) = scales[e] sum over e's rows of P^T t; P's rows of ldp
-// values, C of them used.  part: lora_outer_floats of scratch.
-int64_t lora_outer_chunk(int64_t M, int64_t C);
+struct LoraShrink {
+  const uint16_t* p;
+  int64_t ldp;
+  const uint16_t* v;
+  int64_t ldv, C;
+  int splits;
+  float* t;
+  uint16_t* u;  // launch_lora_parts: [M][parts][r] by row, lora_scales[e] t
+};
+int lora_splits(int64_t M, int64_t C);
+// One or two at once, then their parts.
+hipError_t launch_lora_shrink(const LoraRows& l, const LoraShrink* s, int n, hipStream_t stream);
+hipError_t launch_lora_parts(const LoraRows& l, const LoraShrink* s, int n, int parts, const float* scales,
+                             hipStream_t stream);
+// Few rows: u (two parts) of one shrink at once, in any order (l.order null).
+hipError_t launch_lora_shrink_rows(const LoraRows& l, const LoraShrink& s, const float* scales,
+                                   hipStream_t stream);
+// g [E][C][r] (or [E][r][C] with rows_r) = sum over e's rows of P^T u, u in kLoraParts parts.  part:
+// lora_outer_floats of scratch.
+struct LoraOuter {
+  const uint16_t* p;
+  int64_t ldp, C;
+  const uint16_t* u;
+  bool rows_r;
+  float *g, *part;
+};
 int64_t lora_outer_floats(int64_t M, int64_t C, int r);
 int64_t lora_outer_blocks(int64_t M, int64_t C, int64_t E);
-hipError_t launch_lora_outer(const LoraRows& l, const uint16_t* p, int64_t ldp, int64_t C, const float* t,
-                             int splits, const float* scales, bool rows_r, float* g, float* part,
-                             hipStream_t stream);
+hipError_t launch_lora_outer(const LoraRows& l, const LoraOuter* o, int n, hipStream_t stream);
 // out [E][C][ldo] = in [E][R][C] turned, zeros from R to ldo; adapters without rows are left out.
-hipError_t launch_lora_turn(const LoraRows& l, const uint16_t* in, uint16_t* out, int64_t R, int64_t C,
-                            int64_t ldo, hipStream_t stream);
+struct LoraTurn {
+  const uint16_t* in;
+  uint16_t* out;
+  int64_t R, C, ldo;
+};
+hipError_t launch_lora_turn(const LoraRows& l, const LoraTurn* t, int n, hipStream_t stream);
+
+// y [M, N] = x [M, K] . deq(W)^T with fmxq_dequantize's bits and an adapter's part, rounded once.
+struct OutPlan {
+  bool skinny, panel;
+  int bm, splits;
+  int64_t c_split, piece;  // piece: outputs of one panel
+  size_t slices, panel_at, xp, bytes;
+};
+OutPlan out_plan(int64_t M, int64_t N, int64_t K, int cus);
+hipError_t launch_out(const uint16_t* x, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
+                      const LoraAdd& lora, uint16_t* y, int64_t M, int64_t N, int64_t K, int group_size,
+                      int bits, const OutPlan& p, void* ws, hipStream_t stream);
 
 }  // namespace fmxq

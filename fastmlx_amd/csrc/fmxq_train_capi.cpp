@@ -130,20 +130,22 @@ int clip(const void* const* grads, void* const* outs, const int64_t* counts, con
 // ---- adapters -----------------------------------------------------------------------
 
 constexpr int64_t kMaxRows = (1 << 24) - 1, kMaxWidth = (1 << 22) - 8;
-// Up to here the rows are taken one at a time, in any order.
+constexpr int kCus = 256;  // compute units that plans are made for, so that they need no device
+// Up to here the rows' shrinks are taken one at a time, in any order.
 constexpr int64_t kLoraFewRows = 128;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 struct LoraPlan {
   bool few, sort;
-  int splits, splits_dy;
   int64_t n8;
-  size_t t, dt, order, pos, offsets, hist, none, at, bt, part, pad, base, bytes;
+  int splits, splits_dy;
+  fmxq::OutPlan out;
+  size_t u, t, order, pos, offsets, hist, none, du, dt, at, bt, part_a, part_b, product, pad, bytes;
 };
 
-// Workspace of the forward pass or of the gradients (base: of the input gradient's product).
-LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad, size_t base) {
+// Workspace of the forward pass (product: that of x . deq(W)^T) or of the gradients (of dy . deq(W)).
+LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad, size_t product) {
   LoraPlan p{};
   size_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -154,9 +156,10 @@ LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad,
   p.n8 = up(N, 8);
   p.few = !grad && M <= kLoraFewRows;
   p.sort = !p.few && E > 1;
-  p.splits = p.few ? 1 : fmxq::lora_splits(M, K);
+  p.splits = fmxq::lora_splits(M, K);
   p.splits_dy = fmxq::lora_splits(M, p.n8);
-  p.t = take(p.splits * M * r * 4);
+  p.u = take(M * (grad ? fmxq::kLoraParts : 2) * r * 2);
+  p.t = take(p.few ? 0 : p.splits * M * r * 4);
   if (p.sort) {
     p.order = take(M * 4);
     p.pos = take(M * 4);
@@ -165,13 +168,18 @@ LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad,
     p.none = take(16);
   }
   if (grad) {
+    p.du = take(M * fmxq::kLoraParts * r * 2);
     p.dt = take(p.splits_dy * M * r * 4);
     p.at = take(E * K * r * 2);
     p.bt = take(E * r * p.n8 * 2);
-    p.part = take(std::max(fmxq::lora_outer_floats(M, K, r), fmxq::lora_outer_floats(M, N, r)) * 4);
-    p.base = take((int64_t)base);
-    p.pad = take(N % 8 ? M * p.n8 * 2 : 0);  // at the end: an aligned copy of dy may follow
+    p.part_a = take(fmxq::lora_outer_floats(M, K, r) * 4);
+    p.part_b = take(fmxq::lora_outer_floats(M, N, r) * 4);
+  } else {
+    p.out = fmxq::out_plan(M, N, K, kCus);
+    product = p.out.bytes;
   }
+  p.product = take((int64_t)product);
+  p.pad = take(grad && N % 8 ? M * p.n8 * 2 : 0);  // at the end: an aligned copy of dy may follow
   p.bytes = at;
   return p;
 }
@@ -189,7 +197,7 @@ int lora_sizes(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad, con
   if (M > kMaxRows || N > kMaxWidth || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, N=%lld or K=%lld too large", op, (long long)M,
                 (long long)N, (long long)K);
-  const int64_t rows = (M + 31) / 32, cols = (std::max(N, K) + 511) / 512;
+  const int64_t rows = (M + 127) / 128, cols = (std::max(N, K) + 255) / 256;
   const int64_t turned = (std::max(N, K) / 32 + 1) * (fmxq::kLoraMaxRank / 32) * E;
   if (rows * cols >= fmxq::kLoraMaxBlocks ||
       (grad && (turned >= fmxq::kLoraMaxBlocks ||
@@ -244,27 +252,29 @@ int fmxq_quantized_matmul_lora(const uint16_t* x, const uint32_t* w, const uint1
   if (M == 0 || N == 0) return FMXQ_OK;
   if (!x || !w || !scales || !biases || !a || !b || !adapters || !lora_scales || !y)
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: null operand", op);
-  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(a, 16) || !aligned(b, 16))
-    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: x, w, a and b must be 16-byte aligned", op);
-  if (!aligned(scales, 2) || !aligned(biases, 2) || !aligned(y, 2) || !aligned(adapters, 4) ||
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(y, 16))
+    return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: x, w, a, b and y must be 16-byte aligned", op);
+  if (!aligned(scales, 2) || !aligned(biases, 2) || !aligned(adapters, 4) ||
       !aligned(lora_scales, 4))
     return fail(FMXQ_ERR_INVALID_ARGUMENT, "%s: operands must be aligned to their element size", op);
   const LoraPlan p = lora_plan(M, N, K, E, r, false, 0);
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, op)) return rc;
-  // The base product first: it alone can refuse (memory of the library's own, under capture).
-  if (int rc = fmxq_quantized_matmul(x, w, scales, biases, y, M, N, K, true, group_size, bits, stream))
-    return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   fmxq::LoraRows l;
   if (int rc = lora_rows(p, ws, adapters, M, E, r, s, &l, op)) return rc;
-  float* t = reinterpret_cast<float*>(ws + p.t);
+  const fmxq::LoraShrink xa{x, K, a, K, K, p.splits, reinterpret_cast<float*>(ws + p.t),
+                            reinterpret_cast<uint16_t*>(ws + p.u)};
   if (p.few) {
-    if (int rc = hip_status(fmxq::launch_lora_shrink_rows(l, x, K, a, K, K, t, s), op)) return rc;
-    return hip_status(fmxq::launch_lora_expand_rows(l, t, lora_scales, b, y, N, s), op);
+    if (int rc = hip_status(fmxq::launch_lora_shrink_rows(l, xa, lora_scales, s), op)) return rc;
+  } else {
+    if (int rc = hip_status(fmxq::launch_lora_shrink(l, &xa, 1, s), op)) return rc;
+    if (int rc = hip_status(fmxq::launch_lora_parts(l, &xa, 1, 2, lora_scales, s), op)) return rc;
   }
-  if (int rc = hip_status(fmxq::launch_lora_shrink(l, x, K, a, K, K, p.splits, t, s), op)) return rc;
-  return hip_status(fmxq::launch_lora_expand(l, t, p.splits, lora_scales, b, y, N, s), op);
+  const fmxq::LoraAdd add{xa.u, b, adapters, E, N, r, 2};
+  return hip_status(fmxq::launch_out(x, w, scales, biases, add, y, M, N, K, group_size, bits, p.out,
+                                     ws + p.product, s),
+                    op);
 }
 
 int fmxq_quantized_matmul_lora_grad_workspace(int64_t M, int64_t N, int64_t K, int64_t E, int r,
@@ -327,24 +337,25 @@ int fmxq_quantized_matmul_lora_grad(const uint16_t* dy, const uint16_t* x, const
     if (int rc = hip_status(fmxq::launch_pad_rows(dy, pad, M, N, p.n8, s), op)) return rc;
     g = pad;
   }
-  if (int rc = fmxq_quantized_matmul_grad(moved ? g : dy, w, scales, biases, dx, M, N, K, group_size, bits,
-                                          ws + p.base, base, stream))
-    return rc;
   fmxq::LoraRows l;
   if (int rc = lora_rows(p, ws, adapters, M, E, r, s, &l, op)) return rc;
-  float *t = reinterpret_cast<float*>(ws + p.t), *dt = reinterpret_cast<float*>(ws + p.dt);
   uint16_t *at = reinterpret_cast<uint16_t*>(ws + p.at), *bt = reinterpret_cast<uint16_t*>(ws + p.bt);
-  float* part = reinterpret_cast<float*>(ws + p.part);
-  auto run = [&](hipError_t e) { return hip_status(e, op); };
-  if (int rc = run(fmxq::launch_lora_turn(l, a, at, r, K, r, s))) return rc;
-  if (int rc = run(fmxq::launch_lora_turn(l, b, bt, N, r, p.n8, s))) return rc;
-  if (int rc = run(fmxq::launch_lora_shrink(l, x, K, a, K, K, p.splits, t, s))) return rc;
-  if (int rc = run(fmxq::launch_lora_shrink(l, g, p.n8, bt, p.n8, p.n8, p.splits_dy, dt, s))) return rc;
-  if (int rc = run(fmxq::launch_lora_outer(l, g, p.n8, N, t, p.splits, lora_scales, false, db, part, s)))
+  const fmxq::LoraTurn turns[2] = {{a, at, r, K, r}, {b, bt, N, r, p.n8}};
+  const fmxq::LoraShrink shrinks[2] = {
+      {x, K, a, K, K, p.splits, reinterpret_cast<float*>(ws + p.t), reinterpret_cast<uint16_t*>(ws + p.u)},
+      {g, p.n8, bt, p.n8, p.n8, p.splits_dy, reinterpret_cast<float*>(ws + p.dt),
+       reinterpret_cast<uint16_t*>(ws + p.du)}};
+  const fmxq::LoraOuter outers[2] = {
+      {g, p.n8, N, shrinks[0].u, false, db, reinterpret_cast<float*>(ws + p.part_b)},
+      {x, K, K, shrinks[1].u, true, da, reinterpret_cast<float*>(ws + p.part_a)}};
+  if (int rc = hip_status(fmxq::launch_lora_turn(l, turns, 2, s), op)) return rc;
+  if (int rc = hip_status(fmxq::launch_lora_shrink(l, shrinks, 2, s), op)) return rc;
+  if (int rc = hip_status(fmxq::launch_lora_parts(l, shrinks, 2, fmxq::kLoraParts, lora_scales, s), op))
     return rc;
-  if (int rc = run(fmxq::launch_lora_outer(l, x, K, K, dt, p.splits_dy, lora_scales, true, da, part, s)))
-    return rc;
-  return run(fmxq::launch_lora_expand(l, dt, p.splits_dy, lora_scales, at, dx, K, s));
+  if (int rc = hip_status(fmxq::launch_lora_outer(l, outers, 2, s), op)) return rc;
+  const fmxq::LoraAdd add{shrinks[1].u, at, adapters, E, K, r, fmxq::kLoraParts};
+  return fmxq::input_grad(moved ? g : dy, w, scales, biases, add, dx, M, N, K, group_size, bits,
+                          ws + p.product, base, stream, op);
 }
 
 int fmxq_grad_norm_workspace(size_t* bytes) {

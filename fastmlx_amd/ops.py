@@ -697,8 +697,8 @@ def quantized_matmul_lora(x, w, scales, biases, a, b, adapters, lora_scales, gro
 
     x [..., K] bf16; w [N, K*bits/32]; a [E, r, K] and b [E, N, r] bf16, r a multiple of 8 up to
     128 (zeros fill smaller ranks); adapters [...] int32, below zero for a row without one;
-    lora_scales [E] float32.  Returns y [..., N] bf16: quantized_matmul's, and the adapter's part
-    added to its bf16 values.  An adapter past the last counts as none, and device_error reports it."""
+    lora_scales [E] float32.  Returns y [..., N] bf16, summed in float32 and rounded once.  An adapter
+    past the last counts as none, and device_error reports it."""
     if _fast is not None:
         r = _fast.qmm_lora(x, w, scales, biases, a, b, adapters, lora_scales, group_size, bits)
         if r is not None:

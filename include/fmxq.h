@@ -399,12 +399,10 @@ int fmxq_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t
  *     y[m] = x[m] . deq(W)^T + lora_scales[e] (x[m] . A_e^T) . B_e^T.
  * x [M, K] and y [M, N] bf16; a [E, r, K] and b [E, N, r] bf16, r a multiple of 8 up to 128 (adapters of
  * several ranks share the largest: rows of zeros in a, columns of zeros in b); adapters [M]
- * int32, below zero for a row without one; lora_scales [E] fp32; E <= 2048.  The first product is
- * fmxq_quantized_matmul's, bf16 values included, so a row without adapter holds its bits; the
- * adapter's part is summed in fp32 and added before the row's second rounding.  An adapter of E or
- * more counts as none and raises the error flag.  a and b are 16-byte aligned.  As
- * quantized_matmul the call may use the library's memory of its stream: run a shape once before it is
- * captured. */
+ * int32, below zero for a row without one; lora_scales [E] fp32; E <= 2048.  deq(W) is
+ * fmxq_dequantize's, bit for bit; everything is summed in fp32 and y rounded to bf16 once (so a row
+ * without adapter may differ from fmxq_quantized_matmul's in its last bit).  An adapter of E or more
+ * counts as none and raises the error flag.  x, w, a, b and y are 16-byte aligned. */
 int fmxq_quantized_matmul_lora(const uint16_t* x, const uint32_t* w, const uint16_t* scales,
                                const uint16_t* biases, const uint16_t* a, const uint16_t* b,
                                const int32_t* adapters, const float* lora_scales, uint16_t* y, int64_t M,

@@ -10,6 +10,9 @@ import torch
 import grad_ref as R
 
 SPLIT = 2.0 ** -17
+# The third of three values holds what the first two leave to 2^-9 of it: all bits, but for a
+# last unit.
+SPLIT3 = 2.0 ** -24
 
 
 def make(gen, M, N, K, E, r, bits, group, dev, adapters="runs"):
@@ -27,6 +30,12 @@ def make(gen, M, N, K, E, r, bits, group, dev, adapters="runs"):
     else:
         ids = torch.full((M,), adapters)
     return x, w, a, b, ids.int().to(dev), s
+
+
+def product(x, W):
+    """x @ W^T in 64 bits and the bound of its fp32 sum."""
+    x = x.double()
+    return x @ W.T, (W.shape[1] + 64) * R.U32 * (x.abs() @ W.abs().T)
 
 
 def _shrink(p, v):
@@ -63,8 +72,8 @@ def outer(p, q, ids, v, s, E):
         t, et = _shrink(q[on].double(), v[e].double())
         P, se = p[on].double(), float(s[e])
         g[e] = se * (t.T @ P)
-        err[e] = abs(se) * ((et + (SPLIT + 2 * R.U32) * t.abs()).T @ P.abs() +
-                            (2 * len(on) + 64) * R.U32 * (t.abs().T @ P.abs()))
+        err[e] = abs(se) * ((et + (SPLIT3 + 2 * R.U32) * t.abs()).T @ P.abs() +
+                            (3 * len(on) + 64) * R.U32 * (t.abs().T @ P.abs()))
     return g, err + R.TINY
 
 
