@@ -7,6 +7,7 @@
 #pragma once
 #include "fmxq_common.hpp"
 #include "fmxq_grad.hpp"
+#include "fmxq_lora_tile.hpp"
 
 namespace fmxq {
 
@@ -324,81 +325,12 @@ __device__ __forceinline__ void store_coef(const GradGemm& g, const f32x16 (&acc
   }
 }
 
-// A row's adapter, or -1.
-__device__ __forceinline__ int adapter_of(const LoraAdd& l, int64_t m) {
-  const int e = l.ids[m];
-  return e >= 0 && e < l.E ? e : -1;
-}
-
-// The adapters' part of a tile.  Rows of 32 that share an adapter add it to the sums; others take the
-// adapters in turn, each apart, so that one's infinities reach its own rows only.
-template <int MI, int NJ>
-__device__ __forceinline__ void add_lora(const GradGemm& g, f32x16 (&acc)[MI][NJ], int64_t mw,
-                                         int64_t mend, int64_t nw) {
-  const LoraAdd& l = g.lora;
-  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
-  const int chunks = l.r / 8, steps = (chunks + 1) / 2;
-  if (nw >= g.N) return;
-  int64_t n[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) n[j] = nw + 32 * j + r32 < g.N ? nw + 32 * j + r32 : g.N - 1;
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  auto load = [&](const uint16_t* p, int c) {
-    return __builtin_bit_cast(bf16x8, c < chunks ? *reinterpret_cast<const u32x4*>(p + 8 * c) : zero);
-  };
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int64_t m = mw + 32 * i + r32;
-    const bool in = m < mend;
-    int e = in ? adapter_of(l, m) : -1;
-    uint64_t some = __ballot(e >= 0);
-    if (!some) continue;
-    const uint16_t* u = l.u + (in ? m : mend - 1) * l.parts * l.r;
-    const int first = __builtin_amdgcn_readlane(e, __builtin_ctzll(some));
-    if (__ballot(!in || e == first) == ~0ull) {
-      const uint16_t* v = l.v + (int64_t)first * l.n * l.r;
-      for (int s = 0; s < steps; ++s) {
-        const bf16x8 u0 = load(u, 2 * s + h), u1 = load(u + l.r, 2 * s + h);
-        bf16x8 b[NJ];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) b[j] = load(v + n[j] * l.r, 2 * s + h);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], u0, acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], u1, acc[i][j], 0, 0, 0);
-        }
-      }
-      continue;
-    }
-    while (some) {
-      const int cur = __builtin_amdgcn_readlane(e, __builtin_ctzll(some));
-      const uint16_t* v = l.v + (int64_t)cur * l.n * l.r;
-      const bool mine = e == cur;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        f32x16 t;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) t[x] = 0.f;
-        for (int s = 0; s < steps; ++s) {
-          const bf16x8 u0 = load(u, 2 * s + h), u1 = load(u + l.r, 2 * s + h);
-          const bf16x8 b = load(v + n[j] * l.r, 2 * s + h);
-          t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, u0, t, 0, 0, 0);
-          t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, u1, t, 0, 0, 0);
-        }
-#pragma unroll
-        for (int x = 0; x < 16; ++x) acc[i][j][x] += mine ? t[x] : 0.f;
-      }
-      if (mine) e = -1;
-      some = __ballot(e >= 0);
-    }
-  }
-}
-
 // The product itself: rows of y, of any width, or a part's fp32 slice (N a multiple of 4).
 template <int MI, int NJ>
 __device__ __forceinline__ void store_out(const GradGemm& g, f32x16 (&acc)[MI][NJ], int64_t mw,
                                           int64_t mend, int64_t nw, int64_t split) {
-  if (g.lora.u && split == 0) add_lora<MI, NJ>(g, acc, mw, mend, nw);
+  if (g.lora.u && split == 0)
+    add_lora<MI, NJ>(g.lora, [&](int i, int j) -> f32x16& { return acc[i][j]; }, mw, mend, nw, g.N);
   if (!g.y || ((g.N | g.ldy) & 3) == 0) {
     store_grad<MI, NJ>(g, acc, mw, mend, nw, split);
     return;

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fmxq_grad.hpp"
+
 namespace fmxq {
 
 // Arguments common to every dense quantized product y = x . deq(W)^T.
@@ -180,13 +182,17 @@ struct WideArgs {
   int tm, nk, dp, sk_len;
   int64_t sk_iters;
   uint32_t* err;  // raised (bit 2) when a wait for another block's partial gives up
+  LoraAdd lora;
 };
 WidePlan qmm_wide_plan(int64_t M, int64_t N, int64_t K, int cus);
 // Groups of 32 and 128, which the prefill GEMM takes otherwise: whether the wide GEMM's
 // plan is the quicker one.
 bool qmm_wide_pays(const QmmArgs& a, const WidePlan& p, int cus);
 bool qmm_wide_supported(const QmmArgs& a);
-hipError_t launch_qmm_wide(const QmmArgs& a, const WidePlan& p, uint32_t* err, hipStream_t stream);
+// With `lora` the weights are fmxq_dequantize's bits, and the adapter's part (where it has one) is
+// added before the rounding.
+hipError_t launch_qmm_wide(const QmmArgs& a, const WidePlan& p, uint32_t* err, hipStream_t stream,
+                           const LoraAdd* lora = nullptr);
 // Grouped form (QmmArgs::g_*): grid = N tiles x max_tiles work-list entries.
 constexpr int kGroupedTileRows = 128;
 bool qmm_grouped_supported(int64_t N, int64_t K, int64_t x_rows, int bits, int group_size);

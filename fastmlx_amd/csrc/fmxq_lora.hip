@@ -15,6 +15,7 @@
 // Of v_mfma_f32_16x16x32_bf16 the second operand gives a lane its row, so a lane holds 4
 // neighbouring values of the first operand's index.
 #include <algorithm>
+#include <cstdlib>
 
 #include "fmxq_common.hpp"
 #include "fmxq_internal.hpp"
@@ -502,20 +503,31 @@ namespace {
 // Rows from which the weights are dequantized to a panel beforehand, and most bytes of one.
 constexpr int64_t kOutPanelRows = 1793;
 constexpr int64_t kOutPanelBytes = 512 << 20;
+constexpr int kOutCus = 256;  // compute units that plans are made for
 }  // namespace
 
-OutPlan out_plan(int64_t M, int64_t N, int64_t K, int cus) {
+OutPlan out_plan(int64_t M, int64_t N, int64_t K) {
+  constexpr int cus = kOutCus;
   OutPlan p{};
-  p.panel = M >= kOutPanelRows && panel_gemm_supported(K);
+  alignas(16) static uint16_t any;  // an aligned address
+  // The largest format's limits, so that a plan goes by the sizes alone.
+  const QmmArgs q{&any, reinterpret_cast<const uint32_t*>(&any), &any, &any, nullptr, &any, M, N, K, K, N, 32, 8};
+  const char* lab = getenv("FMXQ_LAB");
+  p.wide = M > kSkinnyRows && qmm_wide_supported(q);
+  if (lab && lab[0] == 'd') p.wide = false;
+  p.panel = !p.wide && M >= kOutPanelRows && panel_gemm_supported(K);
+  if (lab && lab[0] == 'p') p.wide = false, p.panel = true;
   p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M), 128);
-  p.skinny = skinny_gemm_supported(K, 32, K) && (M <= kSkinnyRows || few_tokens(M, N, p.bm, cus));
+  p.skinny = !p.wide && skinny_gemm_supported(K, 32, K) && (M <= kSkinnyRows || few_tokens(M, N, p.bm, cus));
+  if (lab && lab[0] == 's') p.wide = false, p.skinny = true;
   if (p.skinny) p.panel = false;
   p.piece = N;
-  if (p.panel) p.piece = std::min<int64_t>(N, std::max<int64_t>(kOutPanelBytes / 2 / K / kLogitCols * kLogitCols, kLogitCols));
+  if (p.panel)
+    p.piece = std::min<int64_t>(N, std::max<int64_t>(kOutPanelBytes / 2 / K / kLogitCols * kLogitCols, kLogitCols));
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at least.
   p.splits = 1;
   const int64_t tiles = div_up(M, p.bm) * div_up(N, kLogitCols);
-  if (!p.skinny && N % 4 == 0 && p.piece == N)
+  if (!p.skinny && !p.wide && N % 4 == 0 && p.piece == N)
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(tiles, 1), K / 256));
   p.c_split = up(div_up(K, p.splits), 64);
   p.splits = (int)std::max<int64_t>(1, div_up(K, p.c_split));
@@ -525,7 +537,14 @@ OutPlan out_plan(int64_t M, int64_t N, int64_t K, int cus) {
     at += (size_t)up(bytes, 256);
     return o;
   };
-  p.slices = take(p.splits > 1 ? p.splits * M * N * 4 : 0);
+  if (p.wide) {
+    const WidePlan w = qmm_wide_plan(M, N, K, cus);
+    p.slices = take(w.ws_floats * 4);
+    p.counters = w.sk_len > 0 ? w.tiles : 0;
+    p.count_at = take(p.counters * 4);
+  } else {
+    p.slices = take(p.splits > 1 ? p.splits * M * N * 4 : 0);
+  }
   p.panel_at = take(p.panel ? p.piece * K * 2 : 0);
   p.xp = take(p.skinny ? skinny_pack_bytes(M, K) : 0);
   p.bytes = at;
@@ -534,8 +553,15 @@ OutPlan out_plan(int64_t M, int64_t N, int64_t K, int cus) {
 
 hipError_t launch_out(const uint16_t* x, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
                       const LoraAdd& lora, uint16_t* y, int64_t M, int64_t N, int64_t K, int group_size,
-                      int bits, const OutPlan& p, void* ws, hipStream_t stream) {
+                      int bits, const OutPlan& p, void* ws, uint32_t* flag, hipStream_t stream) {
   char* base = static_cast<char*>(ws);
+  if (p.wide) {
+    QmmArgs q{x, w, scales, biases, nullptr, y, M, N, K, K, N, group_size, bits};
+    q.ws = reinterpret_cast<float*>(base + p.slices);
+    q.tile_count = reinterpret_cast<uint32_t*>(base + p.count_at);
+    if (hipError_t r = launch_fill_u32(q.tile_count, 0u, p.counters, stream)) return r;
+    return launch_qmm_wide(q, qmm_wide_plan(M, N, K, kOutCus), flag, stream, &lora);
+  }
   uint16_t* panel = reinterpret_cast<uint16_t*>(base + p.panel_at);
   float* slices = reinterpret_cast<float*>(base + p.slices);
   for (int64_t n0 = 0; n0 < N; n0 += p.piece) {

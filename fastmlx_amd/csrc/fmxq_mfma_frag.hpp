@@ -88,6 +88,29 @@ __device__ __forceinline__ bf16x8 deq_frag8(uint32_t w0, uint32_t w1, float s, f
   return __builtin_bit_cast(bf16x8, r);
 }
 
+// The same with fmxq_dequantize's two roundings, bf16(bf16(q s) + b).  The empty asm hides where a pair
+// comes from: the compiler takes a pack whose halves are used apart for two conversions.
+__device__ __forceinline__ uint32_t add_pair(uint32_t m, float b) {
+  asm("" : "+v"(m));
+  return pack_bf16x2(bf16_lo(m) + b, bf16_hi(m) + b);
+}
+__device__ __forceinline__ bf16x8 deq_exact4(uint32_t w, float s, float s16, float b) {
+  uint32_t e = w & 0x0F0F0F0Fu, o = w & 0xF0F0F0F0u;
+  asm("" : "+v"(e), "+v"(o));
+  const u32x4 r = {add_pair(pack_bf16x2(s * (float)(e & 0xffu), s16 * (float)(o & 0xffu)), b),
+                   add_pair(pack_bf16x2(s * (float)((e >> 8) & 0xffu), s16 * (float)((o >> 8) & 0xffu)), b),
+                   add_pair(pack_bf16x2(s * (float)((e >> 16) & 0xffu), s16 * (float)((o >> 16) & 0xffu)), b),
+                   add_pair(pack_bf16x2(s * (float)(e >> 24), s16 * (float)(o >> 24)), b)};
+  return __builtin_bit_cast(bf16x8, r);
+}
+__device__ __forceinline__ bf16x8 deq_exact8(uint32_t w0, uint32_t w1, float s, float b) {
+  const u32x4 r = {add_pair(pack_bf16x2(s * (float)(w0 & 0xffu), s * (float)((w0 >> 8) & 0xffu)), b),
+                   add_pair(pack_bf16x2(s * (float)((w0 >> 16) & 0xffu), s * (float)(w0 >> 24)), b),
+                   add_pair(pack_bf16x2(s * (float)(w1 & 0xffu), s * (float)((w1 >> 8) & 0xffu)), b),
+                   add_pair(pack_bf16x2(s * (float)((w1 >> 16) & 0xffu), s * (float)(w1 >> 24)), b)};
+  return __builtin_bit_cast(bf16x8, r);
+}
+
 // Two 8-bit words as bf16(q) in natural order: integers up to 255 are exact in bf16.
 __device__ __forceinline__ bf16x8 cvt_frag8(uint32_t w0, uint32_t w1) {
   return as_bf16x8(pack_bf16x2((float)(w0 & 0xffu), (float)((w0 >> 8) & 0xffu)),

@@ -38,6 +38,7 @@
 
 #include "fmxq_common.hpp"
 #include "fmxq_internal.hpp"
+#include "fmxq_lora_tile.hpp"
 #include "fmxq_mfma_frag.hpp"
 
 namespace fmxq {
@@ -74,7 +75,9 @@ struct WideCfg {
 
 enum Role { kFull = 0, kContrib = 1, kFinal = 2 };
 
-template <int BITS, int WAVES, int BM, int GS>
+// EXACT: the weights are fmxq_dequantize's bits (two roundings, twice the VALU work), and the epilogue
+// adds an adapter's part.
+template <int BITS, int WAVES, int BM, int GS, bool EXACT>
 __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
   using C = WideCfg<BITS, WAVES, BM>;
   static_assert(WAVES == 8, "the output staging gives each of 8 waves 4 rows of a 32-row group");
@@ -252,7 +255,12 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
     auto dequant = [&](bf16x8 (&af)[JT][4], int set, const SB& sb, int s) {
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
-        if constexpr (BITS == 4) {
+        if constexpr (BITS == 4 && EXACT) {
+          af[j][s] = deq_exact4(wq[set][j][0][s], sb.s[j], sb.s[j] * 0.0625f, sb.b[j]);
+        } else if constexpr (EXACT) {
+          const u32x4 v = wq[set][j][s >> 1];
+          af[j][s] = deq_exact8(v[(s & 1) * 2], v[(s & 1) * 2 + 1], sb.s[j], sb.b[j]);
+        } else if constexpr (BITS == 4) {
           af[j][s] = deq_frag4(wq[set][j][0][s], sb.s[j], sb.s[j] * 0.0625f, sb.b[j]);
         } else {
           const u32x4 v = wq[set][j][s >> 1];
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
         if (t < NV + 2) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // VMEM read
         if ((t % (RT * JT)) < RT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
-        __builtin_amdgcn_sched_group_barrier(0x002, 3 * 8 / RT, 0);   // VALU
+        __builtin_amdgcn_sched_group_barrier(0x002, (EXACT ? 6 : 3) * 8 / RT, 0);   // VALU
       }
       __builtin_amdgcn_s_waitcnt(wait_enc(wait_x, 0));
       __builtin_amdgcn_s_barrier();
@@ -347,7 +355,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
       for (int t = 0; t < RT * JT; ++t) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         if (t < RT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 3 * 8 / RT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (EXACT ? 6 : 3) * 8 / RT, 0);
       }
     };
     // Piece lengths are multiples of 4 steps (qmm_wide_plan), so the stages and
@@ -446,6 +454,12 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[j][i][4 * g + e] += part[j][g][e];
       }
+      // One row group at a time, as the partials (all of them at once took 130 registers that are not
+      // there).
+      if constexpr (EXACT)
+        if (wa.lora.u)
+          add_lora<1, JT>(wa.lora, [&](int, int j) -> f32x16& { return acc[j][i]; }, m0 + 32 * i, a.M, n0 + wcol,
+                          a.N);
       uint8_t* chunk = stage(i & 1);
 #pragma unroll
       for (int j = 0; j < JT; ++j)
@@ -481,16 +495,16 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
   }
 }
 
-template <int GS>
+template <int GS, bool EXACT>
 hipError_t launch_wide_gs(const WideArgs& wa, const WidePlan& p, hipStream_t stream) {
   constexpr int W = kWideWaves;
   const dim3 grid((unsigned)p.blocks), block(W * 64);
   if (p.bm == 256) {
-    if (wa.q.bits == 4) qmm_wide_kernel<4, W, 256, GS><<<grid, block, 0, stream>>>(wa);
-    else qmm_wide_kernel<8, W, 256, GS><<<grid, block, 0, stream>>>(wa);
+    if (wa.q.bits == 4) qmm_wide_kernel<4, W, 256, GS, EXACT><<<grid, block, 0, stream>>>(wa);
+    else qmm_wide_kernel<8, W, 256, GS, EXACT><<<grid, block, 0, stream>>>(wa);
   } else {
-    if (wa.q.bits == 4) qmm_wide_kernel<4, W, 128, GS><<<grid, block, 0, stream>>>(wa);
-    else qmm_wide_kernel<8, W, 128, GS><<<grid, block, 0, stream>>>(wa);
+    if (wa.q.bits == 4) qmm_wide_kernel<4, W, 128, GS, EXACT><<<grid, block, 0, stream>>>(wa);
+    else qmm_wide_kernel<8, W, 128, GS, EXACT><<<grid, block, 0, stream>>>(wa);
   }
   return hipGetLastError();
 }
@@ -573,15 +587,16 @@ bool qmm_wide_supported(const QmmArgs& a) {
          a.N * (a.K / a.group_size) * 2 < ((int64_t)1 << 31);
 }
 
-hipError_t launch_qmm_wide(const QmmArgs& a, const WidePlan& p, uint32_t* err, hipStream_t stream) {
+hipError_t launch_qmm_wide(const QmmArgs& a, const WidePlan& p, uint32_t* err, hipStream_t stream,
+                           const LoraAdd* lora) {
   if (!qmm_wide_supported(a) || p.blocks < 1 || (p.bm != 128 && p.bm != 256))
     return hipErrorInvalidValue;
   if (p.sk_len > 0 && (!a.ws || !a.tile_count || !err)) return hipErrorInvalidValue;
-  WideArgs wa{a, p.tm, p.nk, p.dp, p.sk_len, p.sk_iters, err};
+  WideArgs wa{a, p.tm, p.nk, p.dp, p.sk_len, p.sk_iters, err, lora ? *lora : LoraAdd{}};
   switch (a.group_size) {
-    case 32: return launch_wide_gs<32>(wa, p, stream);
-    case 64: return launch_wide_gs<64>(wa, p, stream);
-    default: return launch_wide_gs<128>(wa, p, stream);
+    case 32: return lora ? launch_wide_gs<32, true>(wa, p, stream) : launch_wide_gs<32, false>(wa, p, stream);
+    case 64: return lora ? launch_wide_gs<64, true>(wa, p, stream) : launch_wide_gs<64, false>(wa, p, stream);
+    default: return lora ? launch_wide_gs<128, true>(wa, p, stream) : launch_wide_gs<128, false>(wa, p, stream);
   }
 }
 

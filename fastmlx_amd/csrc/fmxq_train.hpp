@@ -94,14 +94,15 @@ hipError_t launch_lora_turn(const LoraRows& l, const LoraTurn* t, int n, hipStre
 
 // y [M, N] = x [M, K] . deq(W)^T with fmxq_dequantize's bits and an adapter's part, rounded once.
 struct OutPlan {
-  bool skinny, panel;
+  bool skinny, wide, panel;
   int bm, splits;
   int64_t c_split, piece;  // piece: outputs of one panel
-  size_t slices, panel_at, xp, bytes;
+  int64_t counters;        // wide: words that are zero when it begins
+  size_t slices, count_at, panel_at, xp, bytes;
 };
-OutPlan out_plan(int64_t M, int64_t N, int64_t K, int cus);
+OutPlan out_plan(int64_t M, int64_t N, int64_t K);
 hipError_t launch_out(const uint16_t* x, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
                       const LoraAdd& lora, uint16_t* y, int64_t M, int64_t N, int64_t K, int group_size,
-                      int bits, const OutPlan& p, void* ws, hipStream_t stream);
+                      int bits, const OutPlan& p, void* ws, uint32_t* flag, hipStream_t stream);
 
 }  // namespace fmxq

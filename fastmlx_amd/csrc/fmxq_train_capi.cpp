@@ -130,7 +130,6 @@ int clip(const void* const* grads, void* const* outs, const int64_t* counts, con
 // ---- adapters -----------------------------------------------------------------------
 
 constexpr int64_t kMaxRows = (1 << 24) - 1, kMaxWidth = (1 << 22) - 8;
-constexpr int kCus = 256;  // compute units that plans are made for, so that they need no device
 // Up to here the rows' shrinks are taken one at a time, in any order.
 constexpr int64_t kLoraFewRows = 128;
 
@@ -175,7 +174,7 @@ LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad,
     p.part_a = take(fmxq::lora_outer_floats(M, K, r) * 4);
     p.part_b = take(fmxq::lora_outer_floats(M, N, r) * 4);
   } else {
-    p.out = fmxq::out_plan(M, N, K, kCus);
+    p.out = fmxq::out_plan(M, N, K);
     product = p.out.bytes;
   }
   p.product = take((int64_t)product);
@@ -273,7 +272,7 @@ int fmxq_quantized_matmul_lora(const uint16_t* x, const uint32_t* w, const uint1
   }
   const fmxq::LoraAdd add{xa.u, b, adapters, E, N, r, 2};
   return hip_status(fmxq::launch_out(x, w, scales, biases, add, y, M, N, K, group_size, bits, p.out,
-                                     ws + p.product, s),
+                                     ws + p.product, l.flag, s),
                     op);
 }
 
