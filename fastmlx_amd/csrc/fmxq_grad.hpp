@@ -126,6 +126,13 @@ inline int64_t skinny_pack_bytes(int64_t M, int64_t K) {
 bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols);
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 
+// Logits or outputs (kEpiScores in tiles of kThinStatWidth, kEpiOut) of up to kThinRows rows, where every
+// load of the weights is whole lines (fmxq_thin.hip).
+constexpr int64_t kThinRows = 16;
+constexpr int kThinStatWidth = 16;
+bool thin_supported(int64_t K);
+hipError_t launch_thin_gemm(const GradGemm& g, hipStream_t stream);
+
 // The same products over a panel of weights dequantized beforehand (fmxq_grad_panel.hip), in
 // tiles of kPanelRows rows.
 constexpr int kPanelRows = 256;

@@ -181,13 +181,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 8 : 4) void logits_skinny_kernel(Gra
       return;
     }
     for (int i = 0; i < 4 && n + i < g.N; ++i) {
-      float s = v[i];
-      if (e >= 0) {
-        const uint16_t* u = g.lora.u + m * g.lora.parts * g.lora.r;
-        const uint16_t* b = g.lora.v + ((int64_t)e * g.lora.n + n + i) * g.lora.r;
-        for (int j = 0; j < g.lora.r; ++j)
-          s = __builtin_fmaf(bf16_bits_to_f32(b[j]), bf16_bits_to_f32(u[j]) + bf16_bits_to_f32(u[g.lora.r + j]), s);
-      }
+      const float s = v[i] + (e >= 0 ? lora_value(g.lora, e, m, n + i) : 0.f);
       y[i] = (uint16_t)f32_to_bf16_rne(s);
     }
     return;

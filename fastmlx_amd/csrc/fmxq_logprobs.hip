@@ -35,7 +35,7 @@ constexpr int kSpareTiles = 8;
 constexpr float kNear = 0.0225f;
 // Exponentials below 2^-kLost are taken as lost.
 constexpr float kLost = 120.f, kLostBelow = 0x1p-120f;
-constexpr int kCandidates = 1024;
+constexpr int kCandidates = 2048;
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -46,18 +46,29 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // The logit of token v for row m in units of log 2, summed in 64 bits (its products are exact
 // there); NaN counts as the lowest.
 __device__ __forceinline__ double logit64(const HeadScore& a, int64_t m, int v) {
+  constexpr int B = 4;  // chunks of 512 columns that are requested together
   const uint16_t* h = a.h + m * a.K;
   const int K = (int)a.K;
   double t = 0.;
-  for (int c = 8 * (threadIdx.x & 63); c < K; c += 512) {
-    const Packed8 p = load8(a, v, c);
-    const u32x4 x = *reinterpret_cast<const u32x4*>(h + c);
-    float wv[8];
-    deq8(p, a.bits, wv);
+  for (int c0 = 8 * (threadIdx.x & 63); c0 < K; c0 += 512 * B) {
+    Packed8 p[B];
+    u32x4 x[B];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t = __builtin_fma((double)wv[2 * j], (double)bf16_lo(x[j]), t);
-      t = __builtin_fma((double)wv[2 * j + 1], (double)bf16_hi(x[j]), t);
+    for (int i = 0; i < B; ++i) {
+      const int c = c0 + 512 * i < K ? c0 + 512 * i : c0;
+      p[i] = load8(a, v, c);
+      x[i] = *reinterpret_cast<const u32x4*>(h + c);
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (c0 + 512 * i >= K) break;
+      float wv[8];
+      deq8(p[i], a.bits, wv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t = __builtin_fma((double)wv[2 * j], (double)bf16_lo(x[i][j]), t);
+        t = __builtin_fma((double)wv[2 * j + 1], (double)bf16_hi(x[i][j]), t);
+      }
     }
   }
   t = wave_sum64(t) * (1.4426950408889634 / (double)a.temperature);
@@ -132,6 +143,7 @@ struct ScoreShared {
   uint64_t red[T / 64];
   float sum[2][T / 64];
   uint32_t tiles[kMaxTop + kSpareTiles];
+  float tops[kMaxTop + kSpareTiles], least;
   uint32_t ntiles, ncand, nbest;
   uint32_t scan[T / 64];
   double bl[2][kMaxTop], cl[kCandidates];
@@ -295,16 +307,28 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
     return st[t].top - (x < kLostBelow ? lost : -__builtin_amdgcn_logf(x));
   };
   // A logit that n columns reach: the n-th highest tile's largest, or of few tiles the n-th column's.
-  uint32_t equal;
-  uint32_t floor_key;
-  if (L >= (uint32_t)n)
-    floor_key = select_key<T>(L, n, [&](uint32_t i) { return tile_key(s.tiles[i]); }, s.sel, &equal);
-  else
-    floor_key = select_key<T>(cols, n, [&](uint32_t i) {
-      int id;
-      return order_key(column(i, &id, INFINITY));
-    }, s.sel, &equal);
-  const float least = key_value(floor_key) - kNear;
+  float least;
+  if (L >= (uint32_t)n) {
+    if ((uint32_t)tid < L) s.tops[tid] = st[s.tiles[tid]].top;
+    __syncthreads();
+    if ((uint32_t)tid < L) {
+      const float mine = s.tops[tid];
+      int above = 0, alike = 0;
+      for (uint32_t i = 0; i < L; ++i) {
+        above += s.tops[i] > mine;
+        alike += s.tops[i] == mine;
+      }
+      if (above < n && n <= above + alike) s.least = mine;  // the same value from every such thread
+    }
+    __syncthreads();
+    least = s.least - kNear;
+  } else {
+    uint32_t equal;
+    least = key_value(select_key<T>(cols, n, [&](uint32_t i) {
+              int id;
+              return order_key(column(i, &id, INFINITY));
+            }, s.sel, &equal)) - kNear;
+  }
   int set = 0;
   for (uint32_t i0 = 0; i0 < cols; i0 += T) {
     int id;
@@ -464,20 +488,26 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // Rows are scored in chunks whose tiles and exponentials take about this much.
 constexpr int64_t kScoreBytes = (int64_t)1 << 30;
 
+constexpr int64_t kFewRows = 512;
 struct ScorePlan {
   HeadPlan p;
-  int64_t lde;
+  bool thin;
+  int stat_width;
+  int64_t stat_tiles, lde;
   size_t e, panel, xp, bytes;  // the tiles' numbers begin the workspace
 };
 int64_t score_rows(int64_t M, int64_t V, int top) {
-  const int64_t row = up(V, kGradTileCols) * (top ? 2 : 0) + up(V, kGradTileCols) / kSkinnyStatWidth * 16;
+  const int64_t row = up(V, kGradTileCols) * (top ? 2 : 0) + up(V, kGradTileCols) / kThinStatWidth * 16;
   return std::min(M, std::max<int64_t>(kScoreBytes / row / 256 * 256, 256));
 }
 ScorePlan score_plan(int64_t M, int64_t V, int64_t K, int k, int top, int cus) {
   ScorePlan s{};
   s.p = head_plan(M, V, K, std::max(k, 1), false, cus);
   s.lde = up(V, kGradTileCols);
-  size_t at = (size_t)up(M * s.p.stat_tiles * (int64_t)sizeof(HeadTile), 256);
+  s.thin = M <= kThinRows && thin_supported(K);
+  s.stat_width = s.thin ? kThinStatWidth : s.p.stat_width;
+  s.stat_tiles = s.lde / s.stat_width;
+  size_t at = (size_t)up(M * s.stat_tiles * (int64_t)sizeof(HeadTile), 256);
   auto take = [&](int64_t bytes) {
     const size_t o = at;
     at += (size_t)up(bytes, 256);
@@ -554,15 +584,21 @@ hipError_t launch_head_score(const HeadScore& all, int cus, void* ws, hipStream_
     for (int64_t v0 = 0; v0 < a.V; v0 += s.p.piece) {
       GradGemm g = logits_gemm(a, v0, std::min(a.V - v0, s.p.piece));
       g.epi = kEpiScores;
-      g.score = score + v0 / s.p.stat_width;
-      g.stat_tiles = s.p.stat_tiles;
+      g.score = score + v0 / s.stat_width;
+      g.stat_tiles = s.stat_tiles;
       g.e = e ? e + v0 : nullptr;
       g.lde = s.lde;
-      if (hipError_t r = launch_logits(g, s.p, reinterpret_cast<uint16_t*>(base + s.panel), base + s.xp, false,
-                                       stream))
+      if (hipError_t r = s.thin ? launch_thin_gemm(g, stream)
+                                : launch_logits(g, s.p, reinterpret_cast<uint16_t*>(base + s.panel), base + s.xp,
+                                                false, stream))
         return r;
     }
-    head_score_kernel<256><<<(unsigned)a.M, 256, 0, stream>>>(a, score, s.p.stat_tiles, s.p.stat_width, e, s.lde);
+    // Few rows: more threads each, where the latency of one row is what counts.
+    const unsigned n = (unsigned)a.M;
+    if (a.M <= kFewRows)
+      head_score_kernel<1024><<<n, 1024, 0, stream>>>(a, score, s.stat_tiles, s.stat_width, e, s.lde);
+    else
+      head_score_kernel<256><<<n, 256, 0, stream>>>(a, score, s.stat_tiles, s.stat_width, e, s.lde);
     if (hipError_t r = hipGetLastError()) return r;
   }
   return hipSuccess;

@@ -15,7 +15,6 @@
 // Of v_mfma_f32_16x16x32_bf16 the second operand gives a lane its row, so a lane holds 4
 // neighbouring values of the first operand's index.
 #include <algorithm>
-#include <cstdlib>
 
 #include "fmxq_common.hpp"
 #include "fmxq_internal.hpp"
@@ -61,10 +60,75 @@ __device__ __forceinline__ int next_adapter(int e0, int e1) {
   return -1;
 }
 
+// ---- order ------------------------------------------------------------------------
+
+// A stable counting sort of up to kSortRows rows by adapter in one block (rows without one last): its
+// 16 waves take consecutive rows.  (2048 rows of 8 adapters: the two launches of the sort for any number
+// 10.5 us.)
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortBuckets = 512;
+__global__ __launch_bounds__(kSortThreads) void lora_sort_kernel(const int32_t* __restrict__ adapters, int M, int E,
+                                                                 int bits, uint32_t* __restrict__ order,
+                                                                 uint32_t* __restrict__ offsets) {
+  __shared__ uint32_t cur[kSortWaves][kSortBuckets], sums[kSortWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < kSortWaves * kSortBuckets; i += kSortThreads) cur[i / kSortBuckets][i % kSortBuckets] = 0;
+  __syncthreads();
+  const int per = (M + kSortThreads - 1) / kSortThreads * 64;
+  const int r0 = wave * per < M ? wave * per : M, r1 = r0 + per < M ? r0 + per : M;
+  auto bucket = [&](int m) {
+    const int e = adapters[m];
+    return e >= 0 && e < E ? e : E;
+  };
+  for (int m = r0 + lane; m < r1; m += 64) atomicAdd(&cur[wave][bucket(m)], 1u);
+  __syncthreads();
+  // Bucket tid's rows, those of the buckets before it, and each wave's first position in it.
+  uint32_t n = 0;
+  if (tid <= E)
+    for (int w = 0; w < kSortWaves; ++w) n += cur[w][tid];
+  uint32_t at = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t u = (uint32_t)__shfl_up((int)at, o, 64);
+    if (lane >= o) at += u;
+  }
+  if (lane == 63) sums[wave] = at;
+  __syncthreads();
+  at -= n;
+  for (int w = 0; w < wave; ++w) at += sums[w];
+  if (tid <= E) {
+    offsets[tid] = at;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = cur[w][tid];
+      cur[w][tid] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (int m = r0 + lane; m - lane < r1; m += 64) {
+    const bool on = m < r1;
+    const uint32_t b = on ? (uint32_t)bucket(m) : 0u;
+    uint64_t same = __ballot(on);
+    for (int i = 0; i < bits; ++i) {
+      const uint64_t set = __ballot((b >> i) & 1u);
+      same &= (b >> i) & 1u ? set : ~set;
+    }
+    const uint64_t before = same & ((1ull << lane) - 1);
+    if (on) order[cur[wave][b] + (uint32_t)__popcll(before)] = (uint32_t)m;
+    // The wave's own LDS accesses, in order.
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (on && before == 0) cur[wave][b] += (uint32_t)__popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
 // ---- t = P . V_e^T ----------------------------------------------------------------
 
-// Block: 32 positions and a part of the contraction, whose 32-deep steps its 8 waves take in turn,
-// four at once (the loads of all are under way before the first is used).
+// Block: 32 positions and a part of the contraction, of whose 32-deep steps its 8 waves take two in turn
+// (a line of each row), the next two's loads under way.
 template <int RT>
 __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraShrink> jobs) {
   __shared__ __attribute__((aligned(16))) f32x4 part[8][2][64];
@@ -74,18 +138,18 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraS
   const LoraShrink& a = jobs.job[second];
   const int split = (int)blockIdx.y - (second ? jobs.job[0].splits : 0);
   const int64_t p0 = (int64_t)blockIdx.x * kTile;
-  const RowOf w0 = row_of(l, p0 + r16), w1 = row_of(l, p0 + 16 + r16);
-  if (wave == 0 && blockIdx.y == 0 && q4 == 0) {
-    const bool bad = (p0 + r16 < l.M && l.adapters[w0.m] >= l.E) ||
-                     (p0 + 16 + r16 < l.M && l.adapters[w1.m] >= l.E);
-    if (bad) atomicOr(l.flag, 1u);
-  }
+  // (Positions past the last take its row's values and no part.)
+  const int64_t q0 = p0 + r16 < l.M ? p0 + r16 : l.M - 1, q1 = p0 + 16 + r16 < l.M ? p0 + 16 + r16 : l.M - 1;
+  const int64_t m0 = l.order ? l.order[q0] : q0, m1 = l.order ? l.order[q1] : q1;
+  int e0 = l.adapters[m0], e1 = l.adapters[m1];
+  if (wave == 0 && blockIdx.y == 0 && (e0 >= l.E || e1 >= l.E)) atomicOr(l.flag, 1u);
+  if (e0 >= l.E || p0 + r16 >= l.M) e0 = -1;
+  if (e1 >= l.E || p0 + 16 + r16 >= l.M) e1 = -1;
   const int steps = (int)((a.C + 31) / 32);
   const int s0 = (int)((int64_t)steps * split / a.splits);
   const int s1 = (int)((int64_t)steps * (split + 1) / a.splits);
-  const uint16_t *x0 = a.p + w0.m * a.ldp, *x1 = a.p + w1.m * a.ldp;
+  const uint16_t *x0 = a.p + m0 * a.ldp, *x1 = a.p + m1 * a.ldp;
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  int e0 = w0.e, e1 = w1.e;
   for (int cur; (cur = next_adapter(e0, e1)) >= 0;) {
     const uint16_t* vr[RT];
 #pragma unroll
@@ -98,25 +162,38 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraS
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = RT > 4 ? 2 : 4;
-    for (int s = s0 + wave; s < s1; s += 8 * U) {
+    constexpr int U = RT > 4 ? 1 : 2;  // steps that are loaded together (2: a line of each row)
+    struct Steps {
       u32x4 x[U][2], b[U][RT];
+    };
+    auto load = [&](int s, Steps& v) {
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int64_t c = 32 * (int64_t)(s + 8 * k) + 8 * q4;
-        const bool in = s + 8 * k < s1 && c < a.C;
-        x[k][0] = in ? *reinterpret_cast<const u32x4*>(x0 + c) : zero;
-        x[k][1] = in ? *reinterpret_cast<const u32x4*>(x1 + c) : zero;
+        const int64_t c = 32 * (int64_t)(s + k) + 8 * q4;
+        const bool in = s + k < s1 && c < a.C;
+        v.x[k][0] = in ? *reinterpret_cast<const u32x4*>(x0 + c) : zero;
+        v.x[k][1] = in ? *reinterpret_cast<const u32x4*>(x1 + c) : zero;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) b[k][i] = in ? *reinterpret_cast<const u32x4*>(vr[i] + c) : zero;
+        for (int i = 0; i < RT; ++i) v.b[k][i] = in ? *reinterpret_cast<const u32x4*>(vr[i] + c) : zero;
       }
+    };
+    auto multiply = [&](const Steps& v) {
 #pragma unroll
       for (int k = 0; k < U; ++k)
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-          acc[0][i] = mfma(b[k][i], x[k][0], acc[0][i]);
-          acc[1][i] = mfma(b[k][i], x[k][1], acc[1][i]);
+          acc[0][i] = mfma(v.b[k][i], v.x[k][0], acc[0][i]);
+          acc[1][i] = mfma(v.b[k][i], v.x[k][1], acc[1][i]);
         }
+    };
+    Steps v0, v1;
+    const int s = s0 + U * wave;
+    load(s, v0);
+    for (int k = s; k < s1; k += 16 * U) {
+      load(k + 8 * U, v1);
+      multiply(v0);
+      load(k + 16 * U, v0);
+      multiply(v1);
     }
     // The waves' sums, in their order.
 #pragma unroll
@@ -139,6 +216,12 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraS
   }
 }
 
+// Words that a product behind this launch wants zero.
+__device__ __forceinline__ void clear(const Zeros& z) {
+  if (blockIdx.y) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < z.n; i += (int64_t)gridDim.x * 256) z.p[i] = 0u;
+}
+
 // A value as the bf16 values that add up to it.
 template <int PARTS>
 __device__ __forceinline__ void store_parts(uint16_t* u, int r, float v) {
@@ -152,7 +235,8 @@ __device__ __forceinline__ void store_parts(uint16_t* u, int r, float v) {
 
 // A thread for 8 values of a row: the sum of the shrink's parts, scaled, in bf16 parts.
 __global__ __launch_bounds__(256) void lora_parts_kernel(LoraRows l, Pair<LoraShrink> jobs, int parts,
-                                                         const float* __restrict__ scales) {
+                                                         const float* __restrict__ scales, Zeros z) {
+  clear(z);
   const LoraShrink& a = jobs.job[blockIdx.y];
   const int chunks = l.r / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, p = i / chunks;
@@ -187,7 +271,8 @@ __global__ __launch_bounds__(256) void lora_parts_kernel(LoraRows l, Pair<LoraSh
 
 // A wave for every value.
 __global__ __launch_bounds__(256) void lora_shrink_rows_kernel(LoraRows l, LoraShrink a,
-                                                               const float* __restrict__ scales) {
+                                                               const float* __restrict__ scales, Zeros z) {
+  clear(z);
   const int64_t m = blockIdx.x;
   const int lane = threadIdx.x & 63, j = 4 * blockIdx.y + (threadIdx.x >> 6);
   const int e = l.adapters[m];
@@ -226,7 +311,8 @@ __global__ __launch_bounds__(256) void lora_shrink_rows_kernel(LoraRows l, LoraS
 // Byte offset of a row of P's tile in LDS: 16 columns of the 16 rows that the quarters of a wave read at
 // once (rows 8 q .. + 4) fall into all banks twice, the least that 512 bytes take.
 __device__ __forceinline__ int tile_row(int row) { return row * 288 + (row >> 3) * 128; }
-constexpr int kOuterRows = 64;  // of a step
+constexpr int kOuterRows = 64;      // of a step
+constexpr int kOuterStretch = 256;  // whose rows are found together
 constexpr int kTileBytes = kOuterRows * 288 + kOuterRows / 8 * 128;
 
 // A lane's 8 values of one column in rows 8 q4 .. + 8: p is the address of 8 bytes of row 8 q4 +
@@ -254,7 +340,8 @@ struct OuterGrid {
 };
 
 // Block: 128 columns of P and all of the rank, over a part of adapter e's rows in steps of 64.  A step's
-// rows are loaded while the one before is multiplied.
+// rows are loaded while the one before is multiplied; which rows they are is found beforehand, so that
+// no load waits for another.
 template <int RT>
 __global__ __launch_bounds__(256) void lora_outer_kernel(LoraRows l, Pair<LoraOuter> jobs, OuterGrid grid) {
   constexpr int UP = RT * 32 + 32;                 // bytes of a row of u in LDS
@@ -262,6 +349,7 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraRows l, Pair<LoraOu
   constexpr int TU = kOuterRows * UC * kLoraParts, NU = (TU + 255) / 256;  // ... of a step, and a thread's
   __shared__ __attribute__((aligned(16))) uint8_t ps[kTileBytes];
   __shared__ __attribute__((aligned(16))) uint8_t us[kLoraParts][kOuterRows * UP];
+  __shared__ int row_of_pos[kOuterStretch + kOuterRows];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool second = blockIdx.x >= grid.blocks;
@@ -281,40 +369,47 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraRows l, Pair<LoraOu
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  u32x4 pv[4], uv[NU];
-  // A position's row, or -1.  (Without an order the one adapter's rows are those that name it.)
-  auto row_at = [&](int64_t pos) -> int64_t {
-    if (pos >= end) return -1;
-    if (l.order) return l.order[pos];
-    return l.adapters[pos] == 0 ? pos : -1;
+  // Rows of a stretch of kOuterStretch positions, or -1.  (Without an order the one adapter's rows are
+  // those that name it.)
+  auto find_rows = [&](int64_t p0) {
+    for (int i = tid; i < kOuterStretch; i += 256) {
+      const int64_t pos = p0 + i;
+      int m = -1;
+      if (pos < end) {
+        if (l.order) m = (int)l.order[pos];
+        else if (l.adapters[pos] == 0) m = (int)pos;
+      }
+      row_of_pos[i] = m;
+    }
   };
-  auto load = [&](int64_t p0) {
+  struct Step {
+    u32x4 p[4], u[NU];
+  };
+  auto load = [&](int at, Step& v) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int64_t m = row_at(p0 + (tid >> 4) + 16 * k), c = c0 + 8 * (tid & 15);
-      pv[k] = m >= 0 && c < o.C ? *reinterpret_cast<const u32x4*>(o.p + m * o.ldp + c) : zero;
+      const int64_t m = row_of_pos[at + (tid >> 4) + 16 * k], c = c0 + 8 * (tid & 15);
+      v.p[k] = m >= 0 && c < o.C ? *reinterpret_cast<const u32x4*>(o.p + m * o.ldp + c) : zero;
     }
 #pragma unroll
     for (int k = 0; k < NU; ++k) {
       const int i = tid + 256 * k, row = i / (UC * kLoraParts), c = i % (UC * kLoraParts);
       const int part = c / UC, j = c % UC * 8;
-      const int64_t m = i < TU ? row_at(p0 + row) : -1;
-      uv[k] = m >= 0 && j < l.r ? *reinterpret_cast<const u32x4*>(o.u + (m * kLoraParts + part) * l.r + j) : zero;
+      const int64_t m = i < TU ? row_of_pos[at + row] : -1;
+      v.u[k] = m >= 0 && j < l.r ? *reinterpret_cast<const u32x4*>(o.u + (m * kLoraParts + part) * l.r + j) : zero;
     }
   };
-  if (begin < end) load(begin);
-  for (int64_t p0 = begin; p0 < end; p0 += kOuterRows) {
+  auto multiply = [&](const Step& v) {
     __syncthreads();  // the step before has been read
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      *reinterpret_cast<u32x4*>(ps + tile_row((tid >> 4) + 16 * k) + 16 * (tid & 15)) = pv[k];
+      *reinterpret_cast<u32x4*>(ps + tile_row((tid >> 4) + 16 * k) + 16 * (tid & 15)) = v.p[k];
 #pragma unroll
     for (int k = 0; k < NU; ++k) {
       const int i = tid + 256 * k, row = i / (UC * kLoraParts), c = i % (UC * kLoraParts);
-      if (i < TU) *reinterpret_cast<u32x4*>(us[c / UC] + row * UP + c % UC * 16) = uv[k];
+      if (i < TU) *reinterpret_cast<u32x4*>(us[c / UC] + row * UP + c % UC * 16) = v.u[k];
     }
     __syncthreads();
-    if (p0 + kOuterRows < end) load(p0 + kOuterRows);
 #pragma unroll
     for (int kk = 0; kk < kOuterRows / 32; ++kk) {
       const int tr = 32 * kk + 8 * q4 + (r16 >> 2), at = 8 * (r16 & 3);
@@ -333,6 +428,21 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraRows l, Pair<LoraOu
           acc[0][i] = mfma(uf, pf[0], acc[0][i]);
           acc[1][i] = mfma(uf, pf[1], acc[1][i]);
         }
+    }
+  };
+  for (int64_t p0 = begin; p0 < end; p0 += kOuterStretch) {
+    __syncthreads();  // the stretch before is done with its rows
+    find_rows(p0);
+    __syncthreads();
+    const int n = end - p0 < kOuterStretch ? (int)(end - p0) : kOuterStretch;
+    Step a, b;
+    load(0, a);
+    for (int at = 0; at < n; at += 2 * kOuterRows) {
+      load(at + kOuterRows, b);
+      multiply(a);
+      if (at + kOuterRows >= n) break;
+      if (at + 2 * kOuterRows < n) load(at + 2 * kOuterRows, a);
+      multiply(b);
     }
   }
 #pragma unroll
@@ -407,11 +517,21 @@ int64_t outer_parts(int64_t M, int64_t C) { return std::max<int64_t>(div_up(M, o
 
 }  // namespace
 
-// Parts that leave each of a block's 8 waves the 4 steps it loads at once, while the blocks are fewer
-// than four for each of 256 compute units.
+bool lora_sort_supported(int64_t M, int64_t E) { return M <= 16 * kSortThreads && E < kSortBuckets; }
+hipError_t launch_lora_sort(const int32_t* adapters, int64_t M, int64_t E, uint32_t* order, uint32_t* offsets,
+                            hipStream_t stream) {
+  if (M < 1 || !lora_sort_supported(M, E)) return hipErrorInvalidValue;
+  int bits = 1;
+  while (E >= ((int64_t)1 << bits)) ++bits;
+  lora_sort_kernel<<<1, kSortThreads, 0, stream>>>(adapters, (int)M, (int)E, bits, order, offsets);
+  return hipGetLastError();
+}
+
+// Parts that leave each of a block's 8 waves 4 steps, while the blocks are no more than two for each of
+// 256 compute units.
 int lora_splits(int64_t M, int64_t C) {
   const int64_t tiles = std::max<int64_t>(div_up(M, kTile), 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / tiles, C / (32 * 8 * 4), 16}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, C / (32 * 8 * 4), 16}));
 }
 
 hipError_t launch_lora_shrink(const LoraRows& l, const LoraShrink* s, int n, hipStream_t stream) {
@@ -432,19 +552,19 @@ hipError_t launch_lora_shrink(const LoraRows& l, const LoraShrink* s, int n, hip
 }
 
 hipError_t launch_lora_parts(const LoraRows& l, const LoraShrink* s, int n, int parts, const float* scales,
-                             hipStream_t stream) {
+                             const Zeros& z, hipStream_t stream) {
   if (!rank_ok(l.r) || n < 1 || n > 2) return hipErrorInvalidValue;
   if (l.M < 1) return hipSuccess;
   const dim3 grid((unsigned)div_up(l.M * (l.r / 8), 256), (unsigned)n);
-  lora_parts_kernel<<<grid, 256, 0, stream>>>(l, pair_of(s, n), parts, scales);
+  lora_parts_kernel<<<grid, 256, 0, stream>>>(l, pair_of(s, n), parts, scales, z);
   return hipGetLastError();
 }
 
 hipError_t launch_lora_shrink_rows(const LoraRows& l, const LoraShrink& s, const float* scales,
-                                   hipStream_t stream) {
+                                   const Zeros& z, hipStream_t stream) {
   if (!rank_ok(l.r) || s.ldp % 8 || s.ldv % 8 || s.C % 8 || l.order) return hipErrorInvalidValue;
   if (l.M < 1) return hipSuccess;
-  lora_shrink_rows_kernel<<<dim3((unsigned)l.M, (unsigned)(l.r / 4)), 256, 0, stream>>>(l, s, scales);
+  lora_shrink_rows_kernel<<<dim3((unsigned)l.M, (unsigned)(l.r / 4)), 256, 0, stream>>>(l, s, scales, z);
   return hipGetLastError();
 }
 
@@ -506,28 +626,47 @@ constexpr int64_t kOutPanelBytes = 512 << 20;
 constexpr int kOutCus = 256;  // compute units that plans are made for
 }  // namespace
 
+// Times of the three kernels that take more than 64 rows, in us.  Chunks of 64 rows on the kernel for
+// few rows: 0.8 ns a 64-deep step of a block of 32 outputs (65 to 128 rows, 4096 x 4096: 18 us, 256 rows
+// 33; 512 rows, 1024 x 4096: 29).  The wide product: 1 PFLOP/s, 20 us of ends, and 0.8 us for each part of a cut
+// tile, which its last block adds up (128 rows 4096 x 4096 33 us, 14336 x 4096 42, 4096 x 14336 56; 256
+// rows, 14336 x 4096: 62; 512 rows, 1024 x 4096: 40).
+static double few_rows_us(int64_t M, int64_t N, int64_t K) {
+  return 4. + 0.8e-3 * (double)(div_up(M, kSkinnyRows) * div_up(N, 32) * div_up(K, 64));
+}
+static double wide_us(int64_t M, int64_t N, int64_t K, const WidePlan& w) {
+  const double parts = w.sk_len > 0 ? (double)w.nk / w.sk_len : 0.;
+  return 20. + 2e-9 * (double)(up(M, w.bm) * N) * (double)K + 0.8 * parts;
+}
+
 OutPlan out_plan(int64_t M, int64_t N, int64_t K) {
   constexpr int cus = kOutCus;
   OutPlan p{};
-  alignas(16) static uint16_t any;  // an aligned address
   // The largest format's limits, so that a plan goes by the sizes alone.
+  alignas(16) static uint16_t any;  // an aligned address
   const QmmArgs q{&any, reinterpret_cast<const uint32_t*>(&any), &any, &any, nullptr, &any, M, N, K, K, N, 32, 8};
-  const char* lab = getenv("FMXQ_LAB");
-  p.wide = M > kSkinnyRows && qmm_wide_supported(q);
-  if (lab && lab[0] == 'd') p.wide = false;
-  p.panel = !p.wide && M >= kOutPanelRows && panel_gemm_supported(K);
-  if (lab && lab[0] == 'p') p.wide = false, p.panel = true;
+  p.thin = M <= kThinRows && thin_supported(K);
+  const bool chunks = skinny_gemm_supported(K, 32, K) && div_up(M, kSkinnyRows) <= 65535;
+  p.skinny = !p.thin && chunks && M <= kSkinnyRows;
+  if (!p.thin && !p.skinny && qmm_wide_supported(q)) {
+    p.wide = !chunks || wide_us(M, N, K, qmm_wide_plan(M, N, K, cus)) < few_rows_us(M, N, K);
+    p.skinny = !p.wide;
+  }
+  // What the wide product does not take: widths that are no multiple of 256, outputs of 8.
+  const bool rest = !p.thin && !p.skinny && !p.wide;
+  p.panel = rest && M >= kOutPanelRows && panel_gemm_supported(K);
   p.bm = p.panel ? kPanelRows : std::max(grad_gemm_rows(M), 128);
-  p.skinny = !p.wide && skinny_gemm_supported(K, 32, K) && (M <= kSkinnyRows || few_tokens(M, N, p.bm, cus));
-  if (lab && lab[0] == 's') p.wide = false, p.skinny = true;
-  if (p.skinny) p.panel = false;
+  if (rest && chunks && few_tokens(M, N, p.bm, cus)) {
+    p.skinny = true;
+    p.panel = false;
+  }
   p.piece = N;
   if (p.panel)
     p.piece = std::min<int64_t>(N, std::max<int64_t>(kOutPanelBytes / 2 / K / kLogitCols * kLogitCols, kLogitCols));
   // Parts of the contraction where the tiles leave compute units idle, of 256 values at least.
   p.splits = 1;
   const int64_t tiles = div_up(M, p.bm) * div_up(N, kLogitCols);
-  if (!p.skinny && !p.wide && N % 4 == 0 && p.piece == N)
+  if (rest && !p.skinny && N % 4 == 0 && p.piece == N)
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(tiles, 1), K / 256));
   p.c_split = up(div_up(K, p.splits), 64);
   p.splits = (int)std::max<int64_t>(1, div_up(K, p.c_split));
@@ -559,7 +698,6 @@ hipError_t launch_out(const uint16_t* x, const uint32_t* w, const uint16_t* scal
     QmmArgs q{x, w, scales, biases, nullptr, y, M, N, K, K, N, group_size, bits};
     q.ws = reinterpret_cast<float*>(base + p.slices);
     q.tile_count = reinterpret_cast<uint32_t*>(base + p.count_at);
-    if (hipError_t r = launch_fill_u32(q.tile_count, 0u, p.counters, stream)) return r;
     return launch_qmm_wide(q, qmm_wide_plan(M, N, K, kOutCus), flag, stream, &lora);
   }
   uint16_t* panel = reinterpret_cast<uint16_t*>(base + p.panel_at);
@@ -594,9 +732,10 @@ hipError_t launch_out(const uint16_t* x, const uint32_t* w, const uint16_t* scal
       g.panel = panel;
       g.ldp = K;
     }
-    if (hipError_t r = p.skinny  ? launch_skinny_gemm(g, false, stream)
-                       : p.panel ? launch_panel_gemm(g, false, stream)
-                                 : launch_grad_gemm(g, false, p.bm, stream))
+    if (hipError_t r = p.thin    ? launch_thin_gemm(g, stream)
+                       : p.skinny ? launch_skinny_gemm(g, false, stream)
+                       : p.panel  ? launch_panel_gemm(g, false, stream)
+                                  : launch_grad_gemm(g, false, p.bm, stream))
       return r;
   }
   return p.splits > 1 ? launch_sum_slices(slices, p.splits, y, M, N, stream) : hipSuccess;

@@ -80,6 +80,7 @@ enum Role { kFull = 0, kContrib = 1, kFinal = 2 };
 template <int BITS, int WAVES, int BM, int GS, bool EXACT>
 __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
   using C = WideCfg<BITS, WAVES, BM>;
+  static_assert(!EXACT || WideCfg<BITS, WAVES, BM>::JT == 1, "the adapters' part takes one group of weights a wave");
   static_assert(WAVES == 8, "the output staging gives each of 8 waves 4 rows of a 32-row group");
   constexpr int T = C::T, JT = C::JT, RT = C::RT, XI = C::XI, NLD = C::NLD, NV = C::NV,
                 NV0 = C::NV0, kStage = C::STAGE;
@@ -433,6 +434,26 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
     // waves' last fragment reads and DMA before the first chunk write.
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
     __builtin_amdgcn_s_barrier();
+    if constexpr (EXACT) {
+      // The adapters' part takes u of the tile's rows from the stages that the output does not use, as it
+      // takes x: the first 64 ranks of its two parts.
+      if (wa.lora.u) {
+        const LoraAdd& lo = wa.lora;
+        const __amdgpu_buffer_rsrc_t ures = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(lo.u + m0 * lo.parts * lo.r), (short)0, (int)(rows_here * lo.parts * lo.r * 2), 0x00020000);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int i = 0; i < XI; ++i) {
+            const int row = 8 * (XI * wave + i) + (lane >> 3), c = (lane & 7) ^ swz(row);
+            const int off = 8 * c < lo.r ? ((row * lo.parts + q) * lo.r + 8 * c) * 2 : 0x7ffffff0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ures, (lds_t*)(stage(2 + q) + 8 * (XI * wave + i) * 128), 16,
+                                                     off, 0, 0, 0);
+          }
+        __builtin_amdgcn_s_waitcnt(wait_enc(0, 0));
+        __builtin_amdgcn_s_barrier();
+      }
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       // Partials of the FINAL piece, one row group at a time (a whole slot's
@@ -454,12 +475,56 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[j][i][4 * g + e] += part[j][g][e];
       }
-      // One row group at a time, as the partials (all of them at once took 130 registers that are not
-      // there).
-      if constexpr (EXACT)
-        if (wa.lora.u)
-          add_lora<1, JT>(wa.lora, [&](int, int j) -> f32x16& { return acc[j][i]; }, m0 + 32 * i, a.M, n0 + wcol,
-                          a.N);
+      if constexpr (EXACT) {
+        // ... a row group at a time, its adapters in turn; a row keeps its own one's part, so that another's
+        // infinities do not reach it.  (2048 rows, 14336 x 4096, rank 64: 325 us with u from global memory,
+        // whose latency each group then waits for.)
+        const LoraAdd& lo = wa.lora;
+        const int64_t m = m0 + 32 * i + r32;
+        int e = lo.u ? adapter_of(lo, m < a.M ? m : a.M - 1) : -1;
+        if (m >= a.M) e = -1;
+        int64_t n = n0 + wcol + r32;
+        if (n > a.N - 1) n = a.N - 1;
+        const u32x4 zero = {0u, 0u, 0u, 0u};
+        for (uint64_t some; (some = __ballot(e >= 0)) != 0;) {
+          const int cur = __builtin_amdgcn_readlane(e, __builtin_ctzll(some));
+          const uint16_t* v = lo.v + ((int64_t)cur * lo.n + n) * lo.r;
+          f32x16 t;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[r] = 0.f;
+          bf16x8 vf[4];
+          auto load_v = [&](int b) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              const int c = 8 * b + 4 * h + s;
+              vf[s] = __builtin_bit_cast(bf16x8, 8 * c < lo.r ? *reinterpret_cast<const u32x4*>(v + 8 * c) : zero);
+            }
+          };
+          load_v(0);
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  vf[s], *reinterpret_cast<const bf16x8*>(stage(2 + q) + xfo[s] + i * 4096), t, 0, 0, 0);
+          if (lo.r > 64) {
+            const uint16_t* u = lo.u + (m < a.M ? m : a.M - 1) * lo.parts * lo.r;
+            load_v(1);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const int c = 8 + 4 * h + s;
+                const u32x4 uv = 8 * c < lo.r ? *reinterpret_cast<const u32x4*>(u + q * lo.r + 8 * c) : zero;
+                t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s], __builtin_bit_cast(bf16x8, uv), t, 0, 0, 0);
+              }
+          }
+          const bool mine = e == cur;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[0][i][r] += mine ? t[r] : 0.f;
+          if (mine) e = -1;
+        }
+      }
       uint8_t* chunk = stage(i & 1);
 #pragma unroll
       for (int j = 0; j < JT; ++j)

@@ -65,13 +65,22 @@ struct LoraShrink {
   uint16_t* u;  // launch_lora_parts: [M][parts][r] by row, lora_scales[e] t
 };
 int lora_splits(int64_t M, int64_t C);
+// order [M] and offsets [E + 1] of up to 16384 rows and 511 adapters.
+bool lora_sort_supported(int64_t M, int64_t E);
+hipError_t launch_lora_sort(const int32_t* adapters, int64_t M, int64_t E, uint32_t* order, uint32_t* offsets,
+                            hipStream_t stream);
+// Words that the last launch before a product clears for it.
+struct Zeros {
+  uint32_t* p;
+  int64_t n;
+};
 // One or two at once, then their parts.
 hipError_t launch_lora_shrink(const LoraRows& l, const LoraShrink* s, int n, hipStream_t stream);
 hipError_t launch_lora_parts(const LoraRows& l, const LoraShrink* s, int n, int parts, const float* scales,
-                             hipStream_t stream);
+                             const Zeros& z, hipStream_t stream);
 // Few rows: u (two parts) of one shrink at once, in any order (l.order null).
 hipError_t launch_lora_shrink_rows(const LoraRows& l, const LoraShrink& s, const float* scales,
-                                   hipStream_t stream);
+                                   const Zeros& z, hipStream_t stream);
 // g [E][C][r] (or [E][r][C] with rows_r) = sum over e's rows of P^T u, u in kLoraParts parts.  part:
 // lora_outer_floats of scratch.
 struct LoraOuter {
@@ -94,10 +103,10 @@ hipError_t launch_lora_turn(const LoraRows& l, const LoraTurn* t, int n, hipStre
 
 // y [M, N] = x [M, K] . deq(W)^T with fmxq_dequantize's bits and an adapter's part, rounded once.
 struct OutPlan {
-  bool skinny, wide, panel;
+  bool thin, skinny, wide, panel;
   int bm, splits;
   int64_t c_split, piece;  // piece: outputs of one panel
-  int64_t counters;        // wide: words that are zero when it begins
+  int64_t counters;        // wide: words at count_at that have to be zero
   size_t slices, count_at, panel_at, xp, bytes;
 };
 OutPlan out_plan(int64_t M, int64_t N, int64_t K);

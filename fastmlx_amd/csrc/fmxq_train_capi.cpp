@@ -213,6 +213,12 @@ int lora_rows(const LoraPlan& p, char* ws, const int32_t* adapters, int64_t M, i
   *l = fmxq::LoraRows{adapters, nullptr, nullptr, M, E, r, nullptr};
   if (int rc = fmxq::device_flag(s, &l->flag)) return rc;
   if (!p.sort) return FMXQ_OK;
+  l->order = reinterpret_cast<uint32_t*>(ws + p.order);
+  l->offsets = reinterpret_cast<uint32_t*>(ws + p.offsets);
+  if (fmxq::lora_sort_supported(M, E))
+    return hip_status(fmxq::launch_lora_sort(adapters, M, E, reinterpret_cast<uint32_t*>(ws + p.order),
+                                             reinterpret_cast<uint32_t*>(ws + p.offsets), s),
+                      op);
   fmxq::MoeSort m{};
   m.inds = reinterpret_cast<const uint32_t*>(adapters);
   m.order = reinterpret_cast<uint32_t*>(ws + p.order);
@@ -223,8 +229,6 @@ int lora_rows(const LoraPlan& p, char* ws, const int32_t* adapters, int64_t M, i
   m.E = E;
   m.hist = reinterpret_cast<uint32_t*>(ws + p.hist);
   m.flag = reinterpret_cast<uint32_t*>(ws + p.none);  // rows without adapter are no error
-  l->order = m.order;
-  l->offsets = m.offsets;
   return hip_status(fmxq::launch_moe_sort(m, s), op);
 }
 
@@ -264,11 +268,12 @@ int fmxq_quantized_matmul_lora(const uint16_t* x, const uint32_t* w, const uint1
   if (int rc = lora_rows(p, ws, adapters, M, E, r, s, &l, op)) return rc;
   const fmxq::LoraShrink xa{x, K, a, K, K, p.splits, reinterpret_cast<float*>(ws + p.t),
                             reinterpret_cast<uint16_t*>(ws + p.u)};
+  const fmxq::Zeros zeros{reinterpret_cast<uint32_t*>(ws + p.product + p.out.count_at), p.out.counters};
   if (p.few) {
-    if (int rc = hip_status(fmxq::launch_lora_shrink_rows(l, xa, lora_scales, s), op)) return rc;
+    if (int rc = hip_status(fmxq::launch_lora_shrink_rows(l, xa, lora_scales, zeros, s), op)) return rc;
   } else {
     if (int rc = hip_status(fmxq::launch_lora_shrink(l, &xa, 1, s), op)) return rc;
-    if (int rc = hip_status(fmxq::launch_lora_parts(l, &xa, 1, 2, lora_scales, s), op)) return rc;
+    if (int rc = hip_status(fmxq::launch_lora_parts(l, &xa, 1, 2, lora_scales, zeros, s), op)) return rc;
   }
   const fmxq::LoraAdd add{xa.u, b, adapters, E, N, r, 2};
   return hip_status(fmxq::launch_out(x, w, scales, biases, add, y, M, N, K, group_size, bits, p.out,
@@ -349,7 +354,7 @@ int fmxq_quantized_matmul_lora_grad(const uint16_t* dy, const uint16_t* x, const
       {x, K, K, shrinks[1].u, true, da, reinterpret_cast<float*>(ws + p.part_a)}};
   if (int rc = hip_status(fmxq::launch_lora_turn(l, turns, 2, s), op)) return rc;
   if (int rc = hip_status(fmxq::launch_lora_shrink(l, shrinks, 2, s), op)) return rc;
-  if (int rc = hip_status(fmxq::launch_lora_parts(l, shrinks, 2, fmxq::kLoraParts, lora_scales, s), op))
+  if (int rc = hip_status(fmxq::launch_lora_parts(l, shrinks, 2, fmxq::kLoraParts, lora_scales, fmxq::Zeros{}, s), op))
     return rc;
   if (int rc = hip_status(fmxq::launch_lora_outer(l, outers, 2, s), op)) return rc;
   const fmxq::LoraAdd add{shrinks[1].u, at, adapters, E, K, r, fmxq::kLoraParts};

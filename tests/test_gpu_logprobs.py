@@ -106,7 +106,7 @@ def test_scores_without_tokens(gpu):
 
 
 def test_scores_in_chunks_of_rows(gpu):
-    """More rows than a chunk's exponentials: 130000 tokens take chunks of 3328."""
+    """More rows than a chunk's exponentials: 130000 tokens take chunks of 2560."""
     M, V = 3400, 130000
     h, w, W, ids, _ = case(gpu, M, V, 64, 1)
     got = ops.head_logprobs(h, *w, ids, top=3)
