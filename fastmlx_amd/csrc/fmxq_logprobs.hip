@@ -36,6 +36,7 @@ constexpr float kNear = 0.0225f;
 // Exponentials below 2^-kLost are taken as lost.
 constexpr float kLost = 120.f, kLostBelow = 0x1p-120f;
 constexpr int kCandidates = 2048;
+constexpr uint32_t kKeptTiles = 4096;
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -139,7 +140,7 @@ __device__ __forceinline__ bool before(double l, int id, double l2, int id2) {
 
 template <int T>
 struct ScoreShared {
-  uint32_t sel[258];
+  uint32_t sel[258], keys[kKeptTiles];
   uint64_t red[T / 64];
   float sum[2][T / 64];
   uint32_t tiles[kMaxTop + kSpareTiles];
@@ -192,9 +193,14 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   const uint32_t nt = (uint32_t)((a.V + tw - 1) / tw);
   const HeadTile* st = score + m * stat_tiles;
   // The largest logit and the first tile that has it.
+  // (The order of the tiles' tops stays in LDS where it has room.)
   uint64_t lead = 0;
+  const bool kept = nt <= kKeptTiles;
+#pragma unroll 4
   for (uint32_t t = tid; t < nt; t += T) {
-    const uint64_t k = (uint64_t)order_key(st[t].top) << 32 | (0xffffffffu - t);
+    const uint32_t o = order_key(st[t].top);
+    if (kept) s.keys[t] = o;
+    const uint64_t k = (uint64_t)o << 32 | (0xffffffffu - t);
     lead = k > lead ? k : lead;
   }
 #pragma unroll
@@ -210,6 +216,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   const float top = key_value((uint32_t)(lead >> 32));
   const int first = (int)((int64_t)lt * tw + st[lt].first);
   float others = 0.f, low = 0.f;
+#pragma unroll 4
   for (uint32_t t = tid; t < nt; t += T) {
     const HeadTile h = st[t];
     const float d = top - h.top, f = __builtin_amdgcn_exp2f(-d);
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   if (tid == 0) s.ntiles = s.ncand = s.nbest = 0;
   __syncthreads();
   const uint32_t want = (uint32_t)(n + kSpareTiles);
-  auto tile_key = [&](uint32_t t) { return order_key(st[t].top); };
+  auto tile_key = [&](uint32_t t) { return kept ? s.keys[t] : order_key(st[t].top); };
   if (nt <= want) {
     for (uint32_t t = tid; t < nt; t += T) s.tiles[t] = t;
     if (tid == 0) s.ntiles = nt;
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   // A logit that n columns reach: the n-th highest tile's largest, or of few tiles the n-th column's.
   float least;
   if (L >= (uint32_t)n) {
-    if ((uint32_t)tid < L) s.tops[tid] = st[s.tiles[tid]].top;
+    if ((uint32_t)tid < L) s.tops[tid] = key_value(tile_key(s.tiles[tid]));
     __syncthreads();
     if ((uint32_t)tid < L) {
       const float mine = s.tops[tid];

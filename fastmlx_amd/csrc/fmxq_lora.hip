@@ -127,11 +127,12 @@ __global__ __launch_bounds__(kSortThreads) void lora_sort_kernel(const int32_t* 
 
 // ---- t = P . V_e^T ----------------------------------------------------------------
 
-// Block: 32 positions and a part of the contraction, of whose 32-deep steps its 8 waves take two in turn
-// (a line of each row), the next two's loads under way.
+// Block: 32 positions and a part of the contraction, whose 32-deep steps its 8 waves take in turn, the
+// next ones' loads under way.
 template <int RT>
 __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraShrink> jobs) {
-  __shared__ __attribute__((aligned(16))) f32x4 part[8][2][64];
+  constexpr int R = RT < 4 ? 2 * RT : 8;  // the sums that meet in LDS at once
+  __shared__ __attribute__((aligned(16))) f32x4 part[8][R][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool second = (int)blockIdx.y >= jobs.job[0].splits;
@@ -162,7 +163,9 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraS
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[m][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = RT > 4 ? 1 : 2;  // steps that are loaded together (2: a line of each row)
+    // Steps that are loaded together: more only where one alone leaves a wave waiting between its products
+    // (2048 rows of 4096 and 14336 values, us with 1 and 2: rank 32 20, 25; rank 64 64.6, 63.4).
+    constexpr int U = RT == 4 ? 2 : 1;
     struct Steps {
       u32x4 x[U][2], b[U][RT];
     };
@@ -197,17 +200,20 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraRows l, Pair<LoraS
     }
     // The waves' sums, in their order.
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      part[wave][0][lane] = acc[0][i];
-      part[wave][1][lane] = acc[1][i];
+    for (int i0 = 0; i0 < RT; i0 += R / 2) {
+#pragma unroll
+      for (int i = 0; i < R / 2; ++i) {
+        part[wave][2 * i][lane] = acc[0][i0 + i];
+        part[wave][2 * i + 1][lane] = acc[1][i0 + i];
+      }
       __syncthreads();
-      if (wave < 2) {
+      if (wave < R) {
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum += part[k][wave][lane];
-        const int j = 16 * i + 4 * q4;
-        if ((wave ? e1 : e0) == cur && j < l.r)
-          *reinterpret_cast<f32x4*>(a.t + ((int64_t)split * l.M + p0 + 16 * wave + r16) * l.r + j) = sum;
+        const int j = 16 * (i0 + (wave >> 1)) + 4 * q4, half = wave & 1;
+        if ((half ? e1 : e0) == cur && j < l.r)
+          *reinterpret_cast<f32x4*>(a.t + ((int64_t)split * l.M + p0 + 16 * half + r16) * l.r + j) = sum;
       }
       __syncthreads();
     }
@@ -645,7 +651,10 @@ OutPlan out_plan(int64_t M, int64_t N, int64_t K) {
   // The largest format's limits, so that a plan goes by the sizes alone.
   alignas(16) static uint16_t any;  // an aligned address
   const QmmArgs q{&any, reinterpret_cast<const uint32_t*>(&any), &any, &any, nullptr, &any, M, N, K, K, N, 32, 8};
-  p.thin = M <= kThinRows && thin_supported(K);
+  // The thin product reads x once for every 16 outputs, the one for few rows packs it first and works on
+  // whole 64-row steps (us, with the adapters: 4096 x 4096, 16 rows 14.5, 17 rows on the other 19;
+  // 14336 x 4096: 8 rows 28.4, 16 rows 41, 17 rows 30).
+  p.thin = M <= kThinRows && thin_supported(K) && (M <= kThinRows / 2 || N <= ((int64_t)1 << 25) / std::max<int64_t>(K, 1));
   const bool chunks = skinny_gemm_supported(K, 32, K) && div_up(M, kSkinnyRows) <= 65535;
   p.skinny = !p.thin && chunks && M <= kSkinnyRows;
   if (!p.thin && !p.skinny && qmm_wide_supported(q)) {

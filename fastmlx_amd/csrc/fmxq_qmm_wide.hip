@@ -374,10 +374,18 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
     pass(k, std::true_type{});
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 15));
 
+    // (A thread's place anew: what is derived from it behind the loop would else be kept in registers from
+    // the kernel's start, through the loop that has none to spare.)
     // Partial slots hold a tile's fp32 sums in register order: 16-byte piece
     // (j, i, g) of thread t at ((j 8 + i) 4 + g) T + t, so every store and load
     // instruction of a wave covers 1 KiB.
-    auto piece = [&](int j, int i, int g) { return ((((j * RT + i) * 4 + g) * T) + tid) * 16; };
+    auto piece = [&](int j, int i, int g) { return ((j * RT + i) * 4 + g) * T * 16; };
+    int et = tid;
+    asm volatile("" : "+v"(et));
+    const int e32 = et & 31, eh = (et >> 5) & 1, piece_at = et * 16;
+    uint32_t efo[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) efo[s] = e32 * 128 + (((4 * eh + s) ^ swz(e32)) << 4);
     if (role == kContrib) {
       // fp32 partial to this block's slot with agent-coherent stores (sc1), then
       // bump the tile's counter.
@@ -391,8 +399,8 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
           for (int g = 0; g < 4; ++g) {
             const f32x4 v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2],
                              acc[j][i][4 * g + 3]};
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), pres, piece(j, i, g),
-                                                   0, 16 /* sc1 */);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), pres, piece_at,
+                                                   piece(j, i, g), 16 /* sc1 */);
           }
       __builtin_amdgcn_s_waitcnt(wait_enc(0, 15));
       __syncthreads();
@@ -427,7 +435,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
     // qlinear-then-add chain, compute/models/quant.go:105-111).  The tile goes
     // out through LDS one 32-row group at a time, so that every store instruction
     // writes whole 512-byte row segments (a lane's own outputs are 4 values on
-    // each of 32 rows).  Lane values: x row m0 + 32 i + r32, outputs
+    // each of 32 rows).  Lane values: x row m0 + 32 i + e32, outputs
     // n0 + wcol + 32 j + 8 g + 4 h .. + 3.  Chunk rows are 512 bytes of 16-byte
     // units, unit u of row r at position u ^ r.  The stages are free: every wave
     // has drained its DMA (vmcnt(0) above), and the barrier orders the other
@@ -445,7 +453,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
         for (int q = 0; q < 2; ++q)
 #pragma unroll
           for (int i = 0; i < XI; ++i) {
-            const int row = 8 * (XI * wave + i) + (lane >> 3), c = (lane & 7) ^ swz(row);
+            const int row = 8 * (XI * wave + i) + ((et & 63) >> 3), c = (et & 7) ^ swz(row);
             const int off = 8 * c < lo.r ? ((row * lo.parts + q) * lo.r + 8 * c) * 2 : 0x7ffffff0;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ures, (lds_t*)(stage(2 + q) + 8 * (XI * wave + i) * 128), 16,
                                                      off, 0, 0, 0);
@@ -467,7 +475,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             part[j][g] = __builtin_bit_cast(
-                f32x4, __builtin_amdgcn_raw_buffer_load_b128(pres, piece(j, i, g), 0, 16 /* sc1 */));
+                f32x4, __builtin_amdgcn_raw_buffer_load_b128(pres, piece_at, piece(j, i, g), 16 /* sc1 */));
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
@@ -477,13 +485,15 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
       }
       if constexpr (EXACT) {
         // ... a row group at a time, its adapters in turn; a row keeps its own one's part, so that another's
-        // infinities do not reach it.  (2048 rows, 14336 x 4096, rank 64: 325 us with u from global memory,
-        // whose latency each group then waits for.)
+        // infinities do not reach it.  (2048 rows, 14336 x 4096: 262 us without an adapter, 275 with rank 16, and
+        // with rank 64 of 8 adapters in any order 286 with what comes before; u from global memory, whose
+        // latency each group then waits for, 325.  The sums started from the adapters' part: 326, the loop
+        // then spills.)
         const LoraAdd& lo = wa.lora;
-        const int64_t m = m0 + 32 * i + r32;
+        const int64_t m = m0 + 32 * i + e32;
         int e = lo.u ? adapter_of(lo, m < a.M ? m : a.M - 1) : -1;
         if (m >= a.M) e = -1;
-        int64_t n = n0 + wcol + r32;
+        int64_t n = n0 + wcol + e32;
         if (n > a.N - 1) n = a.N - 1;
         const u32x4 zero = {0u, 0u, 0u, 0u};
         for (uint64_t some; (some = __ballot(e >= 0)) != 0;) {
@@ -496,7 +506,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
           auto load_v = [&](int b) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-              const int c = 8 * b + 4 * h + s;
+              const int c = 8 * b + 4 * eh + s;
               vf[s] = __builtin_bit_cast(bf16x8, 8 * c < lo.r ? *reinterpret_cast<const u32x4*>(v + 8 * c) : zero);
             }
           };
@@ -506,7 +516,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
 #pragma unroll
             for (int q = 0; q < 2; ++q)
               t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  vf[s], *reinterpret_cast<const bf16x8*>(stage(2 + q) + xfo[s] + i * 4096), t, 0, 0, 0);
+                  vf[s], *reinterpret_cast<const bf16x8*>(stage(2 + q) + efo[s] + i * 4096), t, 0, 0, 0);
           if (lo.r > 64) {
             const uint16_t* u = lo.u + (m < a.M ? m : a.M - 1) * lo.parts * lo.r;
             load_v(1);
@@ -514,7 +524,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
             for (int s = 0; s < 4; ++s)
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const int c = 8 + 4 * h + s;
+                const int c = 8 + 4 * eh + s;
                 const u32x4 uv = 8 * c < lo.r ? *reinterpret_cast<const u32x4*>(u + q * lo.r + 8 * c) : zero;
                 t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s], __builtin_bit_cast(bf16x8, uv), t, 0, 0, 0);
               }
@@ -531,19 +541,19 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int u = wcol / 8 + 4 * j + g;
-          *reinterpret_cast<u32x2*>(chunk + r32 * 512 + ((u ^ r32) << 4) + 8 * h) =
+          *reinterpret_cast<u32x2*>(chunk + e32 * 512 + ((u ^ e32) << 4) + 8 * eh) =
               u32x2{pack_bf16x2(acc[j][i][4 * g], acc[j][i][4 * g + 1]),
                     pack_bf16x2(acc[j][i][4 * g + 2], acc[j][i][4 * g + 3])};
         }
       __syncthreads();
-      // Rows 4 wave + 2 q + h of the chunk, lane r32 taking outputs n0 + 8 r32 ..
+      // Rows 4 wave + 2 q + h of the chunk, lane e32 taking outputs n0 + 8 e32 ..
       // + 7.  (The next write to this buffer comes after the next chunk's
       // barrier, which every wave reaches only after these reads.)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const int R = 4 * (wave & 7) + 2 * q + h;
-        u32x4 v = *reinterpret_cast<const u32x4*>(chunk + R * 512 + ((r32 ^ R) << 4));
-        const int64_t m = m0 + 32 * i + R, n = n0 + 8 * r32;
+        const int R = 4 * (wave & 7) + 2 * q + eh;
+        u32x4 v = *reinterpret_cast<const u32x4*>(chunk + R * 512 + ((e32 ^ R) << 4));
+        const int64_t m = m0 + 32 * i + R, n = n0 + 8 * e32;
         if (m < a.M && n < a.N) {
           if (a.bias) {
 #pragma unroll

@@ -19,7 +19,7 @@ constexpr int kStep = 256;  // values of a wave's step
 constexpr uint32_t kOut = 0x7ffffff0u;  // an offset past every buffer: loads give zero
 
 template <int BITS, int GS, int EPI>
-__global__ __launch_bounds__(512, 4) void thin_kernel(GradGemm g) {
+__global__ __launch_bounds__(512, 8) void thin_kernel(GradGemm g) {
   constexpr int NW = BITS / 2;             // 16-byte loads of a lane's weights in a step
   constexpr int NG = GS < 64 ? 64 / GS : 1;  // groups of a lane's 64 values
   __shared__ f32x4 part[8][64];
