@@ -127,10 +127,13 @@ bool skinny_gemm_supported(int64_t lda, int64_t weight_rows, int64_t weight_cols
 hipError_t launch_skinny_gemm(const GradGemm& g, bool nn, hipStream_t stream);
 
 // Logits or outputs (kEpiScores in tiles of kThinStatWidth, kEpiOut) of up to kThinRows rows, where every
-// load of the weights is whole lines (fmxq_thin.hip).
+// load of the weights is whole lines (fmxq_thin.hip), and where that is the quicker product: it reads x
+// once for every 16 outputs, the one for few rows packs it first and works on 64 of them (us, outputs with
+// an adapter's part: 4096 x 4096, 16 rows 14.5, on the other 17 rows 19; 14336 x 4096, 8 rows 28.4, 16 rows
+// 41, on the other 17 rows 30.  Scores of 128256 x 4096: 1 row 124 on either, 16 rows 284 and 146).
 constexpr int64_t kThinRows = 16;
 constexpr int kThinStatWidth = 16;
-bool thin_supported(int64_t K);
+bool thin_supported(int64_t M, int64_t N, int64_t K);
 hipError_t launch_thin_gemm(const GradGemm& g, hipStream_t stream);
 
 // The same products over a panel of weights dequantized beforehand (fmxq_grad_panel.hip), in

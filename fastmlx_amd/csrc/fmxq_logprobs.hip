@@ -35,8 +35,6 @@ constexpr int kSpareTiles = 8;
 constexpr float kNear = 0.0225f;
 // Exponentials below 2^-kLost are taken as lost.
 constexpr float kLost = 120.f, kLostBelow = 0x1p-120f;
-constexpr int kCandidates = 2048;
-constexpr uint32_t kKeptTiles = 4096;
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -138,8 +136,12 @@ __device__ __forceinline__ bool before(double l, int id, double l2, int id2) {
   return l > l2 || (l == l2 && id < id2);
 }
 
+// (Blocks for few rows take more of LDS; of the others several share it: with 4096 and 2048 there too, 2048
+// rows of 1002 tiles took 212 us in place of 159.)
 template <int T>
 struct ScoreShared {
+  static constexpr uint32_t kKeptTiles = T > 256 ? 4096 : 1280;
+  static constexpr int kCandidates = T > 256 ? 2048 : 1024;
   uint32_t sel[258], keys[kKeptTiles];
   uint64_t red[T / 64];
   float sum[2][T / 64];
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   // The largest logit and the first tile that has it.
   // (The order of the tiles' tops stays in LDS where it has room.)
   uint64_t lead = 0;
-  const bool kept = nt <= kKeptTiles;
+  const bool kept = nt <= s.kKeptTiles;
 #pragma unroll 4
   for (uint32_t t = tid; t < nt; t += T) {
     const uint32_t o = order_key(st[t].top);
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
     const uint32_t i = i0 + tid;
     if (i < cols && column(i, &id, kLost) >= least && id < a.V) s.ci[atomicAdd(&s.ncand, 1u)] = id;
     __syncthreads();
-    const bool full = s.ncand > kCandidates - T;
+    const bool full = s.ncand > s.kCandidates - T;
     __syncthreads();
     if (full) {
       join_candidates<T>(a, m, n, set, set ^ 1, s);
@@ -511,7 +513,7 @@ ScorePlan score_plan(int64_t M, int64_t V, int64_t K, int k, int top, int cus) {
   ScorePlan s{};
   s.p = head_plan(M, V, K, std::max(k, 1), false, cus);
   s.lde = up(V, kGradTileCols);
-  s.thin = M <= kThinRows && thin_supported(K);
+  s.thin = thin_supported(M, V, K);
   s.stat_width = s.thin ? kThinStatWidth : s.p.stat_width;
   s.stat_tiles = s.lde / s.stat_width;
   size_t at = (size_t)up(M * s.stat_tiles * (int64_t)sizeof(HeadTile), 256);

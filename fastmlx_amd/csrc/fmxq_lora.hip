@@ -651,10 +651,7 @@ OutPlan out_plan(int64_t M, int64_t N, int64_t K) {
   // The largest format's limits, so that a plan goes by the sizes alone.
   alignas(16) static uint16_t any;  // an aligned address
   const QmmArgs q{&any, reinterpret_cast<const uint32_t*>(&any), &any, &any, nullptr, &any, M, N, K, K, N, 32, 8};
-  // The thin product reads x once for every 16 outputs, the one for few rows packs it first and works on
-  // whole 64-row steps (us, with the adapters: 4096 x 4096, 16 rows 14.5, 17 rows on the other 19;
-  // 14336 x 4096: 8 rows 28.4, 16 rows 41, 17 rows 30).
-  p.thin = M <= kThinRows && thin_supported(K) && (M <= kThinRows / 2 || N <= ((int64_t)1 << 25) / std::max<int64_t>(K, 1));
+  p.thin = thin_supported(M, N, K);
   const bool chunks = skinny_gemm_supported(K, 32, K) && div_up(M, kSkinnyRows) <= 65535;
   p.skinny = !p.thin && chunks && M <= kSkinnyRows;
   if (!p.thin && !p.skinny && qmm_wide_supported(q)) {

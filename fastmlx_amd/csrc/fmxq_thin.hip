@@ -8,6 +8,8 @@
 //
 // Bound: the dequantization's VALU instructions (5 a weight: two roundings; 6.4e12 weights a second
 // on the whole chip), and for small matrices the launch, the loads' latency and the sum over waves.
+#include <algorithm>
+
 #include "fmxq_common.hpp"
 #include "fmxq_grad_tile.hpp"
 #include "fmxq_mfma_frag.hpp"
@@ -154,11 +156,15 @@ hipError_t launch_thin(const GradGemm& g, hipStream_t stream) {
 }  // namespace
 
 // Byte offsets of 16 rows are 32 bits: x, 8-bit weights.
-bool thin_supported(int64_t K) { return 16 * K * 2 < 0x7ffffff0LL; }
+static bool row_ok(int64_t K) { return 16 * K * 2 < 0x7ffffff0LL; }
+bool thin_supported(int64_t M, int64_t N, int64_t K) {
+  if (M > kThinRows || !row_ok(K)) return false;
+  return M <= 4 || N <= ((int64_t)1 << 29) / M / std::max<int64_t>(K, 1);
+}
 
 hipError_t launch_thin_gemm(const GradGemm& g, hipStream_t stream) {
   if (!g.a || !g.w || !logits_operands(g) || (g.epi != kEpiOut && g.epi != kEpiScores) || (g.epi == kEpiOut && !g.y) ||
-      g.M > kThinRows || !thin_supported(g.lda) || !thin_supported(g.C) || g.lda % 8 || g.splits != 1)
+      g.M > kThinRows || !row_ok(g.lda) || !row_ok(g.C) || g.lda % 8 || g.splits != 1)
     return hipErrorInvalidValue;
   if (g.M < 1 || g.N < 1) return hipSuccess;
   if (g.bits == 4)
