@@ -368,3 +368,37 @@ def test_refuses(gpu):
     with pytest.raises(FmxqError):
         ops.head_logprobs_grad(h, *w, ids[:, :0].contiguous(), none, s[1], s[2], none)
     assert [t.shape[0] for t in f(h[:0], *w, ids[:0], top=3)] == [0] * 5
+
+
+@pytest.mark.parametrize("M,V,K", [(3, 3001, 256), (16, 40000, 1024), (50, 3001, 128), (300, 9000, 128), (1900, 3001, 128)])
+def test_a_dirty_workspace(gpu, M, V, K):
+    """What a workspace held before makes no difference, and nothing is written behind it."""
+    import ctypes
+
+    from fastmlx_amd._lib import load
+
+    announce(f"logprobs dirty workspace {M} {V} {K}")
+    lib = load()
+    h, w, W, ids, gen = case(gpu, M, V, K, 2)
+    a, c = torch.randn(M, 2, generator=gen).to(gpu), torch.randn(M, generator=gen).to(gpu)
+    want = ops.head_logprobs(h, *w, ids, top=7)
+    dh = ops.head_logprobs_grad(h, *w, ids, *want[:3], a, grad_entropy=c)
+    size = ctypes.c_size_t()
+    head = [t.data_ptr() for t in (h, *w, ids)]
+    st = torch.cuda.current_stream().cuda_stream
+    for fill in (0xFF, 0x01):
+        got = [torch.empty_like(t) for t in want]
+        assert lib.fmxq_head_logprobs_workspace(M, V, K, 2, 7, ctypes.byref(size)) == 0
+        ws = torch.full((size.value + 16,), fill, dtype=torch.uint8, device=gpu)
+        assert lib.fmxq_head_logprobs(*head, *(t.data_ptr() for t in got), M, V, K, 2, 7, 1.0, 64, 4, ws.data_ptr(),
+                                      size.value, st) == 0
+        assert bool((ws[size.value:] == fill).all())
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+        assert lib.fmxq_head_logprobs_grad_workspace(M, V, K, 2, ctypes.byref(size)) == 0
+        ws = torch.full((size.value + 16,), fill, dtype=torch.uint8, device=gpu)
+        out = torch.empty_like(dh)
+        assert lib.fmxq_head_logprobs_grad(*head, *(t.data_ptr() for t in want[:3]), a.data_ptr(), c.data_ptr(),
+                                           out.data_ptr(), M, V, K, 2, 1.0, 64, 4, ws.data_ptr(), size.value, st) == 0
+        assert bool((ws[size.value:] == fill).all())
+        assert torch.equal(out, dh)

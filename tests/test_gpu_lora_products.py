@@ -24,6 +24,11 @@ PRODUCTS = [
     (1000, 4100, 320, 4, 72, 4, 64, "mixed"), (500, 8260, 320, 2, 16, 8, 32, "runs"),
     (300, 20001, 320, 3, 8, 4, 32, "mixed"), (1900, 4102, 320, 3, 128, 4, 64, "mixed"),
     (2000, 4101, 96, 1, 24, 8, 32, "runs"), (1900, 4102, 320, 2, 16, 4, 64, "none"),
+    # ... in parts of the contraction, and more weights than one panel holds.
+    (1000, 4100, 1088, 3, 16, 4, 64, "mixed"), (1800, 2052, 1088, 2, 40, 8, 32, "mixed"),
+    (1793, 66004, 4128, 2, 8, 4, 32, "runs"),
+    # Few rows of long ones.
+    (3, 40, 99968, 2, 8, 4, 64, "mixed"), (70, 72, 99968, 2, 8, 8, 64, "mixed"),
 ]
 
 
@@ -102,6 +107,64 @@ def test_streams_and_graphs(gpu, M, N, K):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ops.quantized_matmul_lora(*c[:1], *c[1], *c[2:])), k
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 72, 256), (40, 72, 256), (300, 72, 256), (2048, 4104, 512), (1000, 4100, 320),
+                                   (1900, 4102, 320)])
+def test_any_alignment_of_scales(gpu, M, N, K):
+    """Scales, biases and the adapters' numbers and scales at any multiple of their size: the same bits."""
+    announce(f"lora scales' alignment {M} {N} {K}")
+    gen = torch.Generator().manual_seed(5)
+    x, w, a, b, ids, s = L.make(gen, M, N, K, 3, 16, 4, 64, gpu, "mixed")
+
+    def moved(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=gpu)
+        return buf[1:].view(t.shape).copy_(t)
+
+    w2 = (w[0], moved(w[1]), moved(w[2]))
+    assert torch.equal(ops.quantized_matmul_lora(x, *w2, a, b, moved(ids), moved(s)),
+                       ops.quantized_matmul_lora(x, *w, a, b, ids, s))
+    dy = torch.randn(M, N, generator=gen).bfloat16().to(gpu)
+    for p, q in zip(ops.quantized_matmul_lora_grad(dy, x, *w2, a, b, moved(ids), moved(s)),
+                    ops.quantized_matmul_lora_grad(dy, x, *w, a, b, ids, s)):
+        assert torch.equal(p, q)
+    t = torch.randint(0, N, (M, 1), generator=gen).int().to(gpu)
+    for p, q in zip(ops.head_logprobs(x, *w2, moved(t), top=5), ops.head_logprobs(x, *w, t, top=5)):
+        assert torch.equal(p, q)
+
+
+def test_a_dirty_workspace(gpu):
+    """What a workspace held before makes no difference: through the C entry points, with the workspace
+    filled with NaN bits and with ones, and 16 bytes of guard behind it."""
+    import ctypes
+
+    from fastmlx_amd._lib import load
+
+    lib = load()
+    gen = torch.Generator().manual_seed(6)
+    for M, N, K, E in ((5, 72, 256, 2), (40, 72, 256, 2), (300, 72, 256, 3), (700, 72, 64, 600), (200, 8200, 2048, 3),
+                       (1000, 4100, 1088, 1)):
+        announce(f"dirty workspace {M} {N} {K} {E}")
+        x, w, a, b, ids, s = L.make(gen, M, N, K, E, 8, 4, 64, gpu, "mixed")
+        dy = torch.randn(M, N, generator=gen).bfloat16().to(gpu)
+        want = [ops.quantized_matmul_lora(x, *w, a, b, ids, s), *ops.quantized_matmul_lora_grad(dy, x, *w, a, b, ids, s)]
+        size = ctypes.c_size_t()
+        common = [t.data_ptr() for t in (x, *w, a, b, ids, s)]
+        st = torch.cuda.current_stream().cuda_stream
+        for fill in (0xFF, 0x01):
+            got = [torch.empty_like(t) for t in want]
+            assert lib.fmxq_quantized_matmul_lora_workspace(M, N, K, E, 8, ctypes.byref(size)) == 0
+            ws = torch.full((size.value + 16,), fill, dtype=torch.uint8, device=gpu)
+            assert lib.fmxq_quantized_matmul_lora(*common, got[0].data_ptr(), M, N, K, E, 8, 64, 4, ws.data_ptr(),
+                                                  size.value, st) == 0
+            assert bool((ws[size.value:] == fill).all())
+            assert lib.fmxq_quantized_matmul_lora_grad_workspace(M, N, K, E, 8, ctypes.byref(size)) == 0
+            ws = torch.full((size.value + 16,), fill, dtype=torch.uint8, device=gpu)
+            assert lib.fmxq_quantized_matmul_lora_grad(dy.data_ptr(), *common, *(t.data_ptr() for t in got[1:]), M, N, K,
+                                                       E, 8, 64, 4, ws.data_ptr(), size.value, st) == 0
+            assert bool((ws[size.value:] == fill).all())
+            for p, q in zip(got, want):
+                assert torch.equal(p, q)
 
 
 def policy_step(x, w, a, b, ids, s, head, tokens, adv, beta, max_norm):
