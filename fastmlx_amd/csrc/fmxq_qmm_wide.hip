@@ -374,14 +374,15 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
     pass(k, std::true_type{});
     __builtin_amdgcn_s_waitcnt(wait_enc(0, 15));
 
-    // (A thread's place anew: what is derived from it behind the loop would else be kept in registers from
-    // the kernel's start, through the loop that has none to spare.)
     // Partial slots hold a tile's fp32 sums in register order: 16-byte piece
     // (j, i, g) of thread t at ((j 8 + i) 4 + g) T + t, so every store and load
     // instruction of a wave covers 1 KiB.
     auto piece = [&](int j, int i, int g) { return ((j * RT + i) * 4 + g) * T * 16; };
+    // A thread's place anew in tiles of 256 rows: what is derived from it behind the loop would else be kept
+    // in registers from the kernel's start, through the loop that has none to spare.  2048 rows, 14336 x
+    // 4096: 224 us and 17 registers spilled, 216 and 2.
     int et = tid;
-    asm volatile("" : "+v"(et));
+    if constexpr (BM == 256) asm volatile("" : "+v"(et));
     const int e32 = et & 31, eh = (et >> 5) & 1, piece_at = et * 16;
     uint32_t efo[4];
 #pragma unroll
