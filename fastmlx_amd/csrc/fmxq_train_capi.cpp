@@ -130,7 +130,9 @@ int clip(const void* const* grads, void* const* outs, const int64_t* counts, con
 // ---- adapters -----------------------------------------------------------------------
 
 constexpr int64_t kMaxRows = (1 << 24) - 1, kMaxWidth = (1 << 22) - 8;
-// Up to here the rows' shrinks are taken one at a time, in any order.
+// Up to here the rows' shrinks are taken one at a time, in any order: one launch, which reads an adapter
+// again for every row (128 rows of 8 adapters, 14336 x 4096, rank 16: 10 us on top of the product; the sort,
+// the shrink and its parts, three launches, 17 us at 256 rows).
 constexpr int64_t kLoraFewRows = 128;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
