@@ -228,14 +228,22 @@ __device__ __forceinline__ void clear(const Zeros& z) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < z.n; i += (int64_t)gridDim.x * 256) z.p[i] = 0u;
 }
 
-// A value as the bf16 values that add up to it.
+// A value as the bf16 values that add up to it.  A finite value's parts are finite, also where it is
+// beyond bf16's largest; an infinity is all in the first part, as infinity less infinity would make
+// NaN of it.
+__device__ __forceinline__ float to_part(float v) {
+  constexpr float kMost = 0x1.fep127f;
+  return fabsf(v) < INFINITY ? __builtin_amdgcn_fmed3f(v, -kMost, kMost) : v;
+}
+__device__ __forceinline__ float left_of(float v, float part) { return fabsf(v) < INFINITY ? v - part : 0.f; }
+
 template <int PARTS>
 __device__ __forceinline__ void store_parts(uint16_t* u, int r, float v) {
 #pragma unroll
   for (int k = 0; k < PARTS; ++k) {
-    const uint32_t h = f32_to_bf16_rne(v);
+    const uint32_t h = f32_to_bf16_rne(to_part(v));
     u[k * r] = (uint16_t)h;
-    v -= bf16_bits_to_f32(h);
+    v = left_of(v, bf16_bits_to_f32(h));
   }
 }
 
@@ -262,15 +270,19 @@ __global__ __launch_bounds__(256) void lora_parts_kernel(LoraRows l, Pair<LoraSh
   hi *= s;
   uint16_t* u = a.u + w.m * parts * l.r + j;
   for (int k = 0; k < parts; ++k) {
-    u32x4 o = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
-               pack_bf16x2(hi[2], hi[3])};
+    u32x4 o;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      o[x] = pack_bf16x2(to_part(lo[2 * x]), to_part(lo[2 * x + 1]));
+      o[2 + x] = pack_bf16x2(to_part(hi[2 * x]), to_part(hi[2 * x + 1]));
+    }
     *reinterpret_cast<u32x4*>(u + k * l.r) = o;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      lo[2 * x] -= bf16_lo(o[x]);
-      lo[2 * x + 1] -= bf16_hi(o[x]);
-      hi[2 * x] -= bf16_lo(o[2 + x]);
-      hi[2 * x + 1] -= bf16_hi(o[2 + x]);
+      lo[2 * x] = left_of(lo[2 * x], bf16_lo(o[x]));
+      lo[2 * x + 1] = left_of(lo[2 * x + 1], bf16_hi(o[x]));
+      hi[2 * x] = left_of(hi[2 * x], bf16_lo(o[2 + x]));
+      hi[2 * x + 1] = left_of(hi[2 * x + 1], bf16_hi(o[2 + x]));
     }
   }
 }

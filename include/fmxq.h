@@ -402,7 +402,10 @@ int fmxq_moe_unsort_grad(const uint16_t* dout, const uint16_t* y, const uint32_t
  * int32, below zero for a row without one; lora_scales [E] fp32; E <= 2048.  deq(W) is
  * fmxq_dequantize's, bit for bit; everything is summed in fp32 and y rounded to bf16 once (so a row
  * without adapter may differ from fmxq_quantized_matmul's in its last bit).  An adapter of E or more
- * counts as none and raises the error flag.  x, w, a, b and y are 16-byte aligned. */
+ * counts as none and raises the error flag.  x, w, a, b and y are 16-byte aligned.
+ * A sum x . A_e^T beyond fp32's range is an infinity, and y and the gradients have the formula's.  Results
+ * are not finite exactly where the formula's are not, but an infinite operand of a, b, x or dy may give
+ * NaN there in place of an infinity. */
 int fmxq_quantized_matmul_lora(const uint16_t* x, const uint32_t* w, const uint16_t* scales,
                                const uint16_t* biases, const uint16_t* a, const uint16_t* b,
                                const int32_t* adapters, const float* lora_scales, uint16_t* y, int64_t M,
