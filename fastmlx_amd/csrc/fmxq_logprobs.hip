@@ -11,10 +11,11 @@
 // with `others` the sum of the other tokens' exponentials, -log p of the likeliest token is
 // log1p(others) and H = log1p(others) + sum_v p_v (top - l_v): sums of positive terms, which keep
 // their precision in rows that are sure.
-// The likeliest tokens: the n largest logits lie in the n tiles whose largest are highest, so of the
-// exponentials, which the product leaves in bf16, a row reads those tiles only.  What comes within
-// their rounding of the n-th is a candidate, whose logit is summed again in 64 bits: that decides
-// the order, and equal ones go to the lowest token.
+// The likeliest tokens: the n largest logits lie in the n tiles whose largest are highest, but for what
+// fp32 sums are off by, so of the exponentials, which the product leaves in bf16, a row reads the tiles
+// that come within that of the n-th.  What comes within that and bf16's rounding of it is a
+// candidate, whose logit is summed again in 64 bits: that decides the order, and equal ones go to
+// the lowest token.
 // Gradient: the logits' product again, whose epilogue writes dl (without the given tokens) in bf16,
 // and dl . deq(W); the given tokens' share enters at the end in fp32, as 1 - p from log p.
 #include <algorithm>
@@ -29,9 +30,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxTop = 64;
-// Tiles beside the n highest that are looked at, for logits whose fp32 sums order them wrongly.
-constexpr int kSpareTiles = 8;
-// Candidates: within this of the n-th logit (units of log 2): two roundings to bf16 are 0.0057.
+// Candidates: within this of the n-th logit (units of log 2), beside what fp32 sums are off by: two
+// roundings to bf16 are 0.0057.
 constexpr float kNear = 0.0225f;
 // Exponentials below 2^-kLost are taken as lost.
 constexpr float kLost = 120.f, kLostBelow = 0x1p-120f;
@@ -43,12 +43,16 @@ __device__ __forceinline__ double wave_sum64(double v) {
 }
 
 // The logit of token v for row m in units of log 2, summed in 64 bits (its products are exact
-// there); NaN counts as the lowest.
-__device__ __forceinline__ double logit64(const HeadScore& a, int64_t m, int v) {
+// there); NaN counts as the lowest.  With SIZE also the sum of the products' magnitudes, and whether
+// the row has a value other than 0.
+template <bool SIZE>
+__device__ __forceinline__ double logit64(const HeadScore& a, int64_t m, int v, float* size, bool* some) {
   constexpr int B = 4;  // chunks of 512 columns that are requested together
   const uint16_t* h = a.h + m * a.K;
   const int K = (int)a.K;
   double t = 0.;
+  float mag = 0.f;
+  uint32_t any = 0;
   for (int c0 = 8 * (threadIdx.x & 63); c0 < K; c0 += 512 * B) {
     Packed8 p[B];
     u32x4 x[B];
@@ -67,11 +71,23 @@ __device__ __forceinline__ double logit64(const HeadScore& a, int64_t m, int v) 
       for (int j = 0; j < 4; ++j) {
         t = __builtin_fma((double)wv[2 * j], (double)bf16_lo(x[i][j]), t);
         t = __builtin_fma((double)wv[2 * j + 1], (double)bf16_hi(x[i][j]), t);
+        if constexpr (SIZE) {
+          mag += fabsf(wv[2 * j] * bf16_lo(x[i][j])) + fabsf(wv[2 * j + 1] * bf16_hi(x[i][j]));
+          any |= x[i][j] & 0x7fff7fffu;
+        }
       }
     }
   }
-  t = wave_sum64(t) * (1.4426950408889634 / (double)a.temperature);
+  const double scale = 1.4426950408889634 / (double)a.temperature;
+  t = wave_sum64(t) * scale;
+  if constexpr (SIZE) {
+    *size = wave_sum(mag) * (float)scale;
+    *some = __any(any != 0);
+  }
   return t == t ? t : -__builtin_huge_val();
+}
+__device__ __forceinline__ double logit64(const HeadScore& a, int64_t m, int v) {
+  return logit64<false>(a, m, v, nullptr, nullptr);
 }
 
 // Floats in their order as whole numbers.
@@ -145,10 +161,10 @@ struct ScoreShared {
   uint32_t sel[258], keys[kKeptTiles];
   uint64_t red[T / 64];
   float sum[2][T / 64];
-  uint32_t tiles[kMaxTop + kSpareTiles];
-  float tops[kMaxTop + kSpareTiles], least;
-  uint32_t ntiles, ncand, nbest;
-  uint32_t scan[T / 64];
+  uint32_t tiles[T + 128];
+  double lead;
+  float size;
+  uint32_t zeros, ntiles, ncand, nbest;
   double bl[2][kMaxTop], cl[kCandidates];
   int bi[2][kMaxTop], ci[kCandidates];
 };
@@ -216,7 +232,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   for (int i = 0; i < W; ++i) lead = s.red[i] > lead ? s.red[i] : lead;
   const uint32_t lt = 0xffffffffu - (uint32_t)lead;
   const float top = key_value((uint32_t)(lead >> 32));
-  const int first = (int)((int64_t)lt * tw + st[lt].first);
+  const int first = (int)((int64_t)lt * tw + st[lt].first);  // (past the vocabulary in a row that is not finite)
   float others = 0.f, low = 0.f;
 #pragma unroll 4
   for (uint32_t t = tid; t < nt; t += T) {
@@ -247,109 +263,105 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
     a.lse[m] = bad ? nan : __builtin_fmaf(top, kLn2, lz);
     a.entropy[m] = bad ? nan : lz + kLn2 * (low / (1.f + others));
   }
-  // log p of a token from its logit; the likeliest one's is what the others leave.
-  auto logp = [&](int id, double l) {
-    return bad ? nan : id == first ? -lz : (float)((l - (double)top) * 0.6931471805599453 - (double)lz);
-  };
-  for (int j = wave; j < a.k; j += W) {
-    const int id = a.ids[m * a.k + j];
-    const bool on = id >= 0 && id < a.V;
-    const double l = on && id != first ? logit64(a, m, __builtin_amdgcn_readfirstlane(id)) : 0.;
-    if (lane == 0) {
-      a.logp[m * a.k + j] = on ? logp(id, l) : 0.f;
-      if (id >= a.V) atomicOr(a.flag, 1u);
+  const int n = a.top, k = a.k;
+  if (n + k == 0) return;
+  // The given tokens' logits, and that of the likeliest, in 64 bits.
+  for (int j = wave; j <= k; j += W) {
+    const int id = j < k ? a.ids[m * k + j] : first;
+    if (j < k && id >= a.V && lane == 0) atomicOr(a.flag, 1u);
+    if (bad || id < 0 || id >= a.V) continue;
+    const int v = __builtin_amdgcn_readfirstlane(id);
+    if (j < k) {
+      const double l = v == first ? 0. : logit64(a, m, v);
+      if (lane == 0) s.cl[j] = l;
+    } else {
+      float size;
+      bool some;
+      const double l = logit64<true>(a, m, v, &size, &some);
+      if (lane == 0) {
+        s.lead = l;
+        s.size = size;
+        s.zeros = !some;
+      }
     }
   }
-  const int n = a.top;
+  if (tid == 0) s.ntiles = s.ncand = s.nbest = 0;
+  __syncthreads();
+  // log p of a token from its logit, relative to the likeliest one's, which is what the others leave.
+  auto logp = [&](int id, double l) {
+    return bad ? nan : id == first ? -lz : (float)((l - s.lead) * 0.6931471805599453 - (double)lz);
+  };
+  if (tid < k) {
+    const int id = a.ids[m * k + tid];
+    a.logp[m * k + tid] = id >= 0 && id < a.V ? logp(id, s.cl[tid]) : 0.f;
+  }
   if (n == 0) return;
   int32_t* ids = a.top_ids + m * n;
   float* lps = a.top_logp + m * n;
-  if (bad || (others == (float)(a.V - 1) && low == 0.f)) {
-    // No order, or (a row of zeros, for one) all logits alike.
+  if (bad || s.zeros) {
+    // No order, or a row of zeros, whose logits are all alike.
     for (int i = tid; i < n; i += T) {
       ids[i] = bad ? -1 : i;
       lps[i] = -lz;
     }
     return;
   }
-  if (tid == 0) s.ntiles = s.ncand = s.nbest = 0;
-  __syncthreads();
-  const uint32_t want = (uint32_t)(n + kSpareTiles);
   auto tile_key = [&](uint32_t t) { return kept ? s.keys[t] : order_key(st[t].top); };
-  if (nt <= want) {
-    for (uint32_t t = tid; t < nt; t += T) s.tiles[t] = t;
-    if (tid == 0) s.ntiles = nt;
-  } else {
-    uint32_t equal;
-    const uint32_t key = select_key<T>(nt, want, tile_key, s.sel, &equal);
-    // Higher ones in any order; of the equal ones the first: a range of tiles a thread.
-    const uint32_t per = (nt + T - 1) / T, t0 = tid * per, t1 = t0 + per < nt ? t0 + per : nt;
-    uint32_t mine = 0;
-    for (uint32_t t = t0; t < t1; ++t) mine += tile_key(t) == key;
-    uint32_t inc = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t u = (uint32_t)__shfl_up((int)inc, o, 64);
-      if (lane >= o) inc += u;
-    }
-    if (lane == 63) s.scan[wave] = inc;
-    __syncthreads();
-    uint32_t at = inc - mine;
-    for (int i = 0; i < wave; ++i) at += s.scan[i];
-    for (uint32_t t = t0; t < t1; ++t) {
-      const uint32_t k = tile_key(t);
-      if (k > key || (k == key && at++ < equal)) s.tiles[atomicAdd(&s.ntiles, 1u)] = t;
-    }
-  }
-  __syncthreads();
-  const uint32_t L = s.ntiles, cols = L * (uint32_t)tw;
   const int sh = __builtin_ctz(tw);
   const uint16_t* er = e + m * lde;
-  // A column of the chosen tiles: its token and its logit to bf16's precision, or where its
-  // exponential leaves the type's range, `lost` below the tile's largest (which it is at least).
-  auto column = [&](uint32_t i, int* id, float lost) {
-    const uint32_t t = s.tiles[i >> sh];
-    const int64_t v = (int64_t)t * tw + (i & (tw - 1));
+  // Column c of a tile: its token and its logit to bf16's precision, or where its exponential leaves
+  // the type's range, `lost` below the tile's largest (which it is at least).
+  auto column = [&](uint32_t t, uint32_t c, int* id, float lost) {
+    const int64_t v = (int64_t)t * tw + c;
     *id = (int)v;
     if (v >= a.V) return -INFINITY;
     const float x = bf16_bits_to_f32(er[v]);
     return st[t].top - (x < kLostBelow ? lost : -__builtin_amdgcn_logf(x));
   };
-  // A logit that n columns reach: the n-th highest tile's largest, or of few tiles the n-th column's.
-  float least;
-  if (L >= (uint32_t)n) {
-    if ((uint32_t)tid < L) s.tops[tid] = key_value(tile_key(s.tiles[tid]));
-    __syncthreads();
-    if ((uint32_t)tid < L) {
-      const float mine = s.tops[tid];
-      int above = 0, alike = 0;
-      for (uint32_t i = 0; i < L; ++i) {
-        above += s.tops[i] > mine;
-        alike += s.tops[i] == mine;
-      }
-      if (above < n && n <= above + alike) s.least = mine;  // the same value from every such thread
-    }
-    __syncthreads();
-    least = s.least - kNear;
+  // The n-th logit: a bound below it that n columns reach, the n-th highest tile's largest, or of few
+  // tiles the n-th column's.
+  uint32_t equal;
+  float nth;
+  if (nt >= (uint32_t)n) {
+    nth = key_value(select_key<T>(nt, n, tile_key, s.sel, &equal));
   } else {
-    uint32_t equal;
-    least = key_value(select_key<T>(cols, n, [&](uint32_t i) {
-              int id;
-              return order_key(column(i, &id, INFINITY));
-            }, s.sel, &equal)) - kNear;
+    nth = key_value(select_key<T>(nt * (uint32_t)tw, n, [&](uint32_t i) {
+            int id;
+            return order_key(column(i >> sh, i & (tw - 1), &id, INFINITY));
+          }, s.sel, &equal));
   }
+  // Two fp32 logits that differ by more than this are in their exact order: twice what a sum of K
+  // products is off by, for tokens whose products are up to twice as large as the likeliest one's.
+  const float off = 4.f * (float)(a.K + 16) * 0x1p-24f * fmaxf(s.size, fabsf(nth));
+  const float tile_least = nt >= (uint32_t)n ? nth - off : -INFINITY, least = nth - (kNear + off);
   int set = 0;
-  for (uint32_t i0 = 0; i0 < cols; i0 += T) {
-    int id;
-    const uint32_t i = i0 + tid;
-    if (i < cols && column(i, &id, kLost) >= least && id < a.V) s.ci[atomicAdd(&s.ncand, 1u)] = id;
-    __syncthreads();
-    const bool full = s.ncand > s.kCandidates - T;
-    __syncthreads();
-    if (full) {
-      join_candidates<T>(a, m, n, set, set ^ 1, s);
-      set ^= 1;
+  for (uint32_t t0 = 0; t0 < nt;) {
+    // Tiles that may hold one, as many as the list does, and their columns.
+    for (; t0 < nt; t0 += T) {
+      const bool full = s.ntiles > 128;
+      __syncthreads();
+      if (full) break;
+      const uint32_t t = t0 + tid;
+      if (t < nt && key_value(tile_key(t)) >= tile_least) s.tiles[atomicAdd(&s.ntiles, 1u)] = t;
+      __syncthreads();
     }
+    const uint32_t cols = s.ntiles * (uint32_t)tw;
+    for (uint32_t i0 = 0; i0 < cols; i0 += T) {
+      int id;
+      const uint32_t i = i0 + tid;
+      if (i < cols && column(s.tiles[i >> sh], i & (tw - 1), &id, kLost) >= least && id < a.V)
+        s.ci[atomicAdd(&s.ncand, 1u)] = id;
+      __syncthreads();
+      const bool full = s.ncand > s.kCandidates - T;
+      __syncthreads();
+      if (full) {
+        join_candidates<T>(a, m, n, set, set ^ 1, s);
+        set ^= 1;
+      }
+    }
+    __syncthreads();
+    if (tid == 0) s.ntiles = 0;
+    __syncthreads();
   }
   join_candidates<T>(a, m, n, set, set ^ 1, s);
   set ^= 1;

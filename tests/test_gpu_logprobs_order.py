@@ -1,0 +1,82 @@
+"""The likeliest tokens where fp32 logits do not tell them apart: low temperatures, large hidden states,
+more near ties than a few tiles hold."""
+import pytest
+import torch
+
+import grad_ref as R
+from fastmlx_amd import ops
+from gpu_util import announce
+from test_gpu_logprobs import case, check_scores
+
+pytestmark = pytest.mark.gpu
+
+ROWS = [10, 60, 300, 1800]  # one for each product
+
+
+def copies(gpu, M, V, K, n, small, seed=1):
+    """n tokens whose weights are one row's but for scales of four groups, where h is `small` of its size
+    elsewhere: their logits differ by less than fp32 sums of the whole row see."""
+    h, w, W, ids, gen = case(gpu, M, V, K, 1, seed=seed)
+    words, s, b = (t.clone() for t in w)
+    at = torch.randperm(V, generator=gen)[:n].to(gpu)
+    words[at], s[at], b[at] = w[0][0], w[1][0], w[2][0]
+    s[at, :4] = (s[at, :4].float() * (0.5 + torch.rand(n, 4, generator=gen).to(gpu))).bfloat16()
+    h[:] = (W[0] * (0.5 + 0.01 * torch.randn(M, 1, generator=gen).to(gpu))).bfloat16()
+    h[:, :256] *= small
+    w = (words, s, b)
+    return h, w, R.values(*w, 4, 64), ids
+
+
+def falling(got):
+    assert bool((got[4][:, 1:] <= got[4][:, :-1]).all()), "top_logp falls"
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("T", [1.0, 1e-4, 1e-7])
+def test_near_ties_at_low_temperatures(gpu, M, T):
+    announce(f"near ties {M} {T}")
+    h, w, W, ids = copies(gpu, M, 4000, 512, 60, 1e-7)
+    got, _ = check_scores(h, w, W, ids, 50, T=T)
+    falling(got)
+
+
+@pytest.mark.parametrize("M", ROWS)
+def test_near_ties_of_large_hidden_states(gpu, M):
+    announce(f"near ties of large states {M}")
+    h, w, W, ids = copies(gpu, M, 4000, 512, 60, 1e-7, seed=2)
+    got, _ = check_scores((h.float() * 2.0 ** 17).bfloat16(), w, W, ids, 50)
+    falling(got)
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_near_ties_in_every_tile(gpu, M, top):
+    """More of them than there are tiles: their exact order decides, whatever their tiles' largest."""
+    announce(f"near ties in every tile {M} {top}")
+    h, w, W, ids = copies(gpu, M, 40000, 512, 3000, 1e-7, seed=3)
+    got, _ = check_scores(h, w, W, ids, top)
+    falling(got)
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("V", [4, 50])
+def test_tokens_alike_to_fp32(gpu, M, V):
+    """All logits the same in fp32, none in 64 bits."""
+    announce(f"alike to fp32 {M} {V}")
+    h, w, W, ids = copies(gpu, M, V, 512, V, 1e-10, seed=4)
+    got, _ = check_scores(h, w, W, ids, V)
+    falling(got)
+
+
+@pytest.mark.parametrize("M", ROWS)
+def test_weights_of_zeros(gpu, M):
+    """A head of zeros, for any hidden state: all logits are 0, and the lower tokens come first."""
+    V = 3000
+    announce(f"zeros {M}")
+    h, w, W, ids, _ = case(gpu, M, V, 128, 1)
+    w = (w[0], torch.zeros_like(w[1]), torch.zeros_like(w[2]))
+    got = ops.head_logprobs(h, *w, ids, top=40)
+    assert torch.equal(got[3].long(), torch.arange(40, device=gpu).expand(M, 40))
+    flat = torch.log(torch.tensor(float(V), dtype=torch.float64, device=gpu))
+    for t in (got[1], got[2], -got[4]):
+        R.check(t, flat.expand(t.shape), (flat * 4 * R.U32).expand(t.shape), "flat")
