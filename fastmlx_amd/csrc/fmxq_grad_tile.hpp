@@ -230,8 +230,9 @@ __device__ __forceinline__ void store_stats(const GradGemm& g, f32x16 (&acc)[MI]
 // What log probabilities need of a tile of 32 NJ columns (HeadTile), in units of log 2: its largest
 // logit m and the first column that has it, and of the other columns the sums of 2^(l - m) and of
 // 2^(l - m) (m - l).  That column takes no part in the sums, so that where one token takes nearly
-// everything, what the others leave is not the difference of near equals.  With e, also bf16(2^(l - m)),
-// zeros from column N to the tile's end.
+// everything, what the others leave is not the difference of near equals.  A logit of minus infinity (0
+// times infinity in the second sum), as any other that is not finite, leaves NaN.  With e, also
+// bf16(2^(l - m)), zeros from column N to the tile's end.
 template <int MI, int NJ>
 __device__ __forceinline__ void store_scores(const GradGemm& g, f32x16 (&acc)[MI][NJ], int64_t mw,
                                              int64_t mend, int64_t nw) {
@@ -274,7 +275,7 @@ __device__ __forceinline__ void store_scores(const GradGemm& g, f32x16 (&acc)[MI
           v[e] = c + e < left ? __builtin_amdgcn_exp2f(-d) : 0.f;
           const float w = (uint32_t)(c + e) == first || c + e >= left ? 0.f : v[e];
           sum += w;
-          low = __builtin_fmaf(w, w == 0.f ? 0.f : d, low);
+          low = __builtin_fmaf(w, c + e < left ? d : 0.f, low);
         }
         if (g.e && m < mend)
           *reinterpret_cast<u32x2*>(g.e + m * g.lde + nw + c) =

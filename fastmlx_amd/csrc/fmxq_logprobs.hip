@@ -241,7 +241,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
     const float sum = t == lt ? h.sum : (1.f + h.sum) * f;
     others += sum;
     low += h.low * f;
-    if (t != lt && sum > 0.f) low = __builtin_fmaf(d, sum, low);
+    low = __builtin_fmaf(d, sum, low);
   }
   others = wave_sum(others);
   low = wave_sum(low);
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
     others += s.sum[0][i];
     low += s.sum[1][i];
   }
-  const bool bad = !(fabsf(top) < INFINITY) || !(others < INFINITY);
+  const bool bad = !(fabsf(top) < INFINITY) || !(others < INFINITY) || !(low < INFINITY);
   const float nan = __builtin_nanf("");
   const float lz = bad ? nan : log1pf(others);
   if (tid == 0) {

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(512, 8) void thin_kernel(GradGemm g) {
       ex[i] = c < left ? __builtin_amdgcn_exp2f(-d) : 0.f;
       const float t = c == first || c >= left ? 0.f : ex[i];
       sum += t;
-      low = __builtin_fmaf(t, t == 0.f ? 0.f : d, low);
+      low = __builtin_fmaf(t, c < left ? d : 0.f, low);
     }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);

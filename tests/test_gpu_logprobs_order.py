@@ -1,5 +1,5 @@
 """The likeliest tokens where fp32 logits do not tell them apart: low temperatures, large hidden states,
-more near ties than a few tiles hold."""
+more near ties than a few tiles hold; logits that are not finite."""
 import pytest
 import torch
 
@@ -80,3 +80,19 @@ def test_weights_of_zeros(gpu, M):
     flat = torch.log(torch.tensor(float(V), dtype=torch.float64, device=gpu))
     for t in (got[1], got[2], -got[4]):
         R.check(t, flat.expand(t.shape), (flat * 4 * R.U32).expand(t.shape), "flat")
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("V", [3000, 37])
+def test_a_logit_of_minus_infinity(gpu, M, V):
+    """One such logit makes its row's numbers NaN, whatever else is in its tile."""
+    announce(f"minus infinity {M} {V}")
+    h, (words, s, b), W, ids, _ = case(gpu, M, V, 128, 2, absent=0.0)
+    h[:, :64] = h[:, :64].abs() + 0.125
+    b[V // 2, 0] = float("-inf")
+    got = ops.head_logprobs(h, words, s, b, ids, top=9)
+    for i in (0, 1, 2, 4):
+        assert got[i].isnan().all(), i
+    assert bool((got[3] == -1).all())
+    a = torch.ones(M, 2, device=gpu)
+    assert ops.head_logprobs_grad(h, words, s, b, ids, *got[:3], a).isnan().all()
