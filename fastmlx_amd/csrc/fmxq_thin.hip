@@ -158,7 +158,7 @@ hipError_t launch_thin(const GradGemm& g, hipStream_t stream) {
 // Byte offsets of 16 rows are 32 bits: x, 8-bit weights.
 static bool row_ok(int64_t K) { return 16 * K * 2 < 0x7ffffff0LL; }
 bool thin_supported(int64_t M, int64_t N, int64_t K) {
-  if (M > kThinRows || !row_ok(K)) return false;
+  if (M > kThinRows || !row_ok(K) || (N + 15) / 16 >= kMaxBlocks) return false;
   return M <= 4 || N <= ((int64_t)1 << 29) / M / std::max<int64_t>(K, 1);
 }
 

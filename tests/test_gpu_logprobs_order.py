@@ -1,5 +1,5 @@
 """The likeliest tokens where fp32 logits do not tell them apart: low temperatures, large hidden states,
-more near ties than a few tiles hold; logits that are not finite."""
+more near ties than a few tiles hold; logits that are not finite; a vocabulary of more than 2^27 tokens."""
 import pytest
 import torch
 
@@ -96,3 +96,25 @@ def test_a_logit_of_minus_infinity(gpu, M, V):
     assert bool((got[3] == -1).all())
     a = torch.ones(M, 2, device=gpu)
     assert ops.head_logprobs_grad(h, words, s, b, ids, *got[:3], a).isnan().all()
+
+
+@pytest.mark.parametrize("M", [1, 4, 5])
+def test_a_vocabulary_beyond_the_few_row_products_blocks(gpu, M):
+    """2^27 tokens and more, of which a few have weights other than zero."""
+    V, K = 2 ** 27 + 5000, 32
+    announce(f"{V} tokens, {M} rows")
+    words = torch.zeros(V, K // 8, dtype=torch.int32, device=gpu)
+    s, b = (torch.zeros(V, 1, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    gen = torch.Generator().manual_seed(5)
+    at = torch.tensor([0, 17, 2 ** 26, 2 ** 27 - 1, 2 ** 27 + 4096, V - 1], device=gpu)
+    b[at, 0] = torch.tensor([1.0, 3.0, -2.0, 2.5, 3.5, 2.0], device=gpu).bfloat16()
+    h = torch.rand(M, K, generator=gen).bfloat16().to(gpu)
+    ids = at[torch.arange(M, device=gpu) % 6][:, None].int()
+    got = ops.head_logprobs(h, words, s, b, ids, top=3, group_size=32)
+    l = h.double().sum(-1, keepdim=True) * b[at, 0].double()
+    lse = torch.log(V - 6 + l.exp().sum(-1))
+    # Sums of 2^27 terms of 1: each thread's and the tiles' in fp32, a few thousand one after another.
+    tol = 2.0 ** -10 + 0 * lse
+    R.check(got[2], lse, tol, "lse")
+    R.check(got[0][:, 0], l.gather(1, (torch.arange(M, device=gpu) % 6)[:, None])[:, 0] - lse, tol, "logp")
+    assert torch.equal(got[3].long(), at[[4, 1, 3]].expand(M, 3))
