@@ -622,12 +622,14 @@ hipError_t launch_lora_outer(const LoraRows& l, const LoraOuter* o, int n, hipSt
   return hipGetLastError();
 }
 
+int64_t lora_turn_blocks(int64_t C, int64_t ldo, int64_t E) { return div_up(C, 32) * div_up(ldo, 32) * E; }
+
 hipError_t launch_lora_turn(const LoraRows& l, const LoraTurn* t, int n, hipStream_t stream) {
   if (n < 1 || n > 2 || l.E < 1) return hipErrorInvalidValue;
   int64_t blocks = 0, first = 0;
   for (int i = 0; i < n; ++i) {
     if (t[i].R < 1 || t[i].C < 1) return hipErrorInvalidValue;
-    blocks += div_up(t[i].C, 32) * div_up(t[i].ldo, 32);
+    blocks += lora_turn_blocks(t[i].C, t[i].ldo, 1);
     if (i == 0) first = blocks;
   }
   if (blocks * l.E >= kLoraMaxBlocks) return hipErrorInvalidValue;

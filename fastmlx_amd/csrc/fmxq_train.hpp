@@ -99,6 +99,7 @@ struct LoraTurn {
   uint16_t* out;
   int64_t R, C, ldo;
 };
+int64_t lora_turn_blocks(int64_t C, int64_t ldo, int64_t E);
 hipError_t launch_lora_turn(const LoraRows& l, const LoraTurn* t, int n, hipStream_t stream);
 
 // y [M, N] = x [M, K] . deq(W)^T with fmxq_dequantize's bits and an adapter's part, rounded once.

@@ -198,12 +198,12 @@ int lora_sizes(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad, con
   if (M > kMaxRows || N > kMaxWidth || K > kMaxWidth)
     return fail(FMXQ_ERR_SHAPE, "%s: M=%lld, N=%lld or K=%lld too large", op, (long long)M,
                 (long long)N, (long long)K);
+  // (A and B, and both outer products, share a launch.)
   const int64_t rows = (M + 127) / 128, cols = (std::max(N, K) + 255) / 256;
-  const int64_t turned = (std::max(N, K) / 32 + 1) * (fmxq::kLoraMaxRank / 32) * E;
   if (rows * cols >= fmxq::kLoraMaxBlocks ||
-      (grad && (turned >= fmxq::kLoraMaxBlocks ||
-                std::max(fmxq::lora_outer_blocks(M, N, E), fmxq::lora_outer_blocks(M, K, E)) >=
-                    fmxq::kLoraMaxBlocks)))
+      (grad && (fmxq::lora_turn_blocks(K, r, E) + fmxq::lora_turn_blocks(r, up(N, 8), E) >=
+                    fmxq::kLoraMaxBlocks ||
+                fmxq::lora_outer_blocks(M, N, E) + fmxq::lora_outer_blocks(M, K, E) >= fmxq::kLoraMaxBlocks)))
     return fail(FMXQ_ERR_SHAPE, "%s: %lld rows of %lld and %lld for %lld adapters are too many", op,
                 (long long)M, (long long)N, (long long)K, (long long)E);
   return FMXQ_OK;
