@@ -782,8 +782,8 @@ def _clip_call(grads, outs, max_norm):
 
 def grad_norm(grads):
     """The norm over many gradients: the root of the sum of all their squares, summed in 64 bits.
-    grads: a list of float32 or bfloat16 tensors of one device.  Returns a float32 scalar tensor,
-    without waiting for it."""
+    grads: float32 or bfloat16 tensors of one device.  Returns a float32 scalar tensor, without
+    waiting for it."""
     if _fast is not None:
         r = _fast.clip(grads, None, 0.0)
         if r is not None:
@@ -797,8 +797,13 @@ def clip_grad_norm(grads, max_norm: float, outs=None):
     outs: the results' tensors, of the gradients' shapes and types (new ones without); they may
     be the gradients themselves.  A norm that is zero, infinite or NaN leaves the values as they
     are, so a step can be skipped by the norm alone."""
+    many = (list, tuple)  # others (a generator, for one) are walked once
+    if not isinstance(grads, many):
+        grads = list(grads)
     if outs is None:
         outs = [torch.empty_like(g) for g in grads]
+    elif not isinstance(outs, many):
+        outs = list(outs)
     if _fast is not None:
         r = _fast.clip(grads, outs, float(max_norm))
         if r is not None:
