@@ -377,13 +377,17 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
     // Partial slots hold a tile's fp32 sums in register order: 16-byte piece
     // (j, i, g) of thread t at ((j 8 + i) 4 + g) T + t, so every store and load
     // instruction of a wave covers 1 KiB.
-    auto piece = [&](int j, int i, int g) { return ((j * RT + i) * 4 + g) * T * 16; };
     // A thread's place anew in tiles of 256 rows: what is derived from it behind the loop would else be kept
-    // in registers from the kernel's start, through the loop that has none to spare.  2048 rows, 14336 x
-    // 4096: 224 us and 17 registers spilled, 216 and 2.
+    // in registers from the kernel's start, through the loop that has none to spare (2048 rows, 14336 x 4096:
+    // 226 us and 17 registers spilled, 222 and 2; 8 bits in groups of 64 247, 240).  Not where that costs: in
+    // tiles of 128 rows (512 rows 66 us, 69 that way), and 8 bits in groups of 32 (246, 252).
+    constexpr bool ANEW = BM == 256 && (EXACT || BITS == 4 || GS > 32);
     int et = tid;
-    if constexpr (BM == 256) asm volatile("" : "+v"(et));
-    const int e32 = et & 31, eh = (et >> 5) & 1, piece_at = et * 16;
+    if constexpr (ANEW) asm volatile("" : "+v"(et));
+    const int e32 = ANEW ? et & 31 : r32, eh = ANEW ? (et >> 5) & 1 : h;
+    auto piece = [&](int j, int i, int g) { return ((j * RT + i) * 4 + g) * T * 16; };
+    auto piece_v = [&](int j, int i, int g) { return ANEW ? et * 16 : piece(j, i, g) + tid * 16; };
+    auto piece_s = [&](int j, int i, int g) { return ANEW ? piece(j, i, g) : 0; };
     uint32_t efo[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) efo[s] = e32 * 128 + (((4 * eh + s) ^ swz(e32)) << 4);
@@ -400,8 +404,8 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
           for (int g = 0; g < 4; ++g) {
             const f32x4 v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2],
                              acc[j][i][4 * g + 3]};
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), pres, piece_at,
-                                                   piece(j, i, g), 16 /* sc1 */);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), pres, piece_v(j, i, g),
+                                                   piece_s(j, i, g), 16 /* sc1 */);
           }
       __builtin_amdgcn_s_waitcnt(wait_enc(0, 15));
       __syncthreads();
@@ -476,7 +480,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             part[j][g] = __builtin_bit_cast(
-                f32x4, __builtin_amdgcn_raw_buffer_load_b128(pres, piece_at, piece(j, i, g), 16 /* sc1 */));
+                f32x4, __builtin_amdgcn_raw_buffer_load_b128(pres, piece_v(j, i, g), piece_s(j, i, g), 16 /* sc1 */));
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
