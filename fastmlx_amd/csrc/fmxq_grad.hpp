@@ -149,8 +149,10 @@ hipError_t launch_sum_slices(const float* slices, int splits, uint16_t* y, int64
 // dst [M, ld] = src [M, N] with zeros in columns N .. ld.
 hipError_t launch_pad_rows(const uint16_t* src, uint16_t* dst, int64_t M, int64_t N, int64_t ld,
                            hipStream_t stream);
-// fmxq_quantized_matmul_grad, its checks included, with an adapter's part (fmxq_grad_capi.cpp).
-int input_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
+// fmxq_quantized_matmul_grad, its checks included, with an adapter's part (fmxq_grad_capi.cpp).  ld: the
+// values from one row of dy to the next, N, or where N is no multiple of 8 also that next one, 16-byte
+// aligned and zero past N: such a copy may lie where the workspace begins, where the call would put its own.
+int input_grad(const uint16_t* dy, int64_t ld, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
                const LoraAdd& lora, uint16_t* dx, int64_t M, int64_t N, int64_t K, int group_size, int bits,
                void* workspace, size_t workspace_bytes, void* stream, const char* op);
 // A loss over a quantized head (fmxq_head.hip).  ids [M, k]: the targets (k = 1, teacher

@@ -154,12 +154,12 @@ GradPlan grad_plan(int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
-// dy as the product reads it: itself, or a copy with padded rows in the workspace.
-int grad_operand(const uint16_t* dy, void* pad, int64_t M, int64_t N, hipStream_t s,
+// dy (rows of ld values) as the product reads it: itself, or a copy with padded rows in the workspace.
+int grad_operand(const uint16_t* dy, int64_t ld, void* pad, int64_t M, int64_t N, hipStream_t s,
                  fmxq::GradGemm* g, const char* op) {
   g->a = dy;
-  g->lda = g->a_cols = N;
-  if (N % 8 == 0 && aligned16(dy)) return FMXQ_OK;
+  g->lda = g->a_cols = ld;
+  if (ld % 8 == 0 && aligned16(dy)) return FMXQ_OK;
   g->a = static_cast<uint16_t*>(pad);
   g->lda = g->a_cols = pad_cols(N);
   return hip_status(fmxq::launch_pad_rows(dy, static_cast<uint16_t*>(pad), M, N, g->lda, s), op);
@@ -209,7 +209,7 @@ int row_sizes(int64_t T, int64_t k, int64_t D, const char* op) {
 
 }  // namespace
 
-int fmxq::input_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scales,
+int fmxq::input_grad(const uint16_t* dy, int64_t ld, const uint32_t* w, const uint16_t* scales,
                      const uint16_t* biases, const LoraAdd& lora, uint16_t* dx, int64_t M, int64_t N,
                      int64_t K, int group_size, int bits, void* workspace, size_t workspace_bytes,
                      void* stream, const char* op) {
@@ -231,7 +231,7 @@ int fmxq::input_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* scal
     return rc;
   char* ws = static_cast<char*>(workspace);
   fmxq::GradGemm g;
-  if (int rc = grad_operand(dy, ws + moved_at, M, N, s, &g, op)) return rc;
+  if (int rc = grad_operand(dy, ld, ws + moved_at, M, N, s, &g, op)) return rc;
   g.M = M;
   g.N = K;
   g.C = N;
@@ -393,7 +393,7 @@ int fmxq_quantized_matmul_grad(const uint16_t* dy, const uint32_t* w, const uint
                                const uint16_t* biases, uint16_t* dx, int64_t M, int64_t N,
                                int64_t K, int group_size, int bits, void* workspace,
                                size_t workspace_bytes, void* stream) {
-  return fmxq::input_grad(dy, w, scales, biases, fmxq::LoraAdd{}, dx, M, N, K, group_size, bits, workspace,
+  return fmxq::input_grad(dy, N, w, scales, biases, fmxq::LoraAdd{}, dx, M, N, K, group_size, bits, workspace,
                           workspace_bytes, stream, "quantized_matmul_grad");
 }
 
@@ -429,7 +429,7 @@ int fmxq_gather_qmm_grad(const uint16_t* dy, const uint32_t* w, const uint16_t* 
   uint32_t* flag = nullptr;
   if (int rc = device_flag(s, &flag)) return rc;
   fmxq::GradGemm g;
-  if (int rc = grad_operand(dy, workspace, S, N, s, &g, op)) return rc;
+  if (int rc = grad_operand(dy, N, workspace, S, N, s, &g, op)) return rc;
   g.M = S;
   g.N = K;
   g.C = N;

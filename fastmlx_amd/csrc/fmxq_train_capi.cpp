@@ -142,7 +142,7 @@ struct LoraPlan {
   int64_t n8;
   int splits, splits_dy;
   fmxq::OutPlan out;
-  size_t u, t, order, pos, offsets, hist, none, du, dt, at, bt, part_a, part_b, product, pad, bytes;
+  size_t u, t, order, pos, offsets, hist, none, du, dt, at, bt, part_a, part_b, product, bytes;
 };
 
 // Workspace of the forward pass (product: that of x . deq(W)^T) or of the gradients (of dy . deq(W)).
@@ -180,8 +180,7 @@ LoraPlan lora_plan(int64_t M, int64_t N, int64_t K, int64_t E, int r, bool grad,
     product = p.out.bytes;
   }
   p.product = take((int64_t)product);
-  p.pad = take(grad && N % 8 ? M * p.n8 * 2 : 0);  // at the end: an aligned copy of dy may follow
-  p.bytes = at;
+  p.bytes = at;  // (an aligned copy of dy may follow)
   return p;
 }
 
@@ -336,10 +335,10 @@ int fmxq_quantized_matmul_lora_grad(const uint16_t* dy, const uint16_t* x, const
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes + (moved ? (size_t)(M * N * 2) : 0), op))
     return rc;
   char* ws = static_cast<char*>(workspace);
-  // dy in rows of 16-byte units.
+  // dy in rows of 16-byte units: a copy, where it takes one, serves all that reads dy.
   const uint16_t* g = dy;
   if (moved || N % 8) {
-    uint16_t* pad = reinterpret_cast<uint16_t*>(ws + p.pad);
+    uint16_t* pad = reinterpret_cast<uint16_t*>(ws + (moved ? p.bytes : p.product));
     if (int rc = hip_status(fmxq::launch_pad_rows(dy, pad, M, N, p.n8, s), op)) return rc;
     g = pad;
   }
@@ -360,7 +359,7 @@ int fmxq_quantized_matmul_lora_grad(const uint16_t* dy, const uint16_t* x, const
     return rc;
   if (int rc = hip_status(fmxq::launch_lora_outer(l, outers, 2, s), op)) return rc;
   const fmxq::LoraAdd add{shrinks[1].u, at, adapters, E, K, r, fmxq::kLoraParts};
-  return fmxq::input_grad(moved ? g : dy, w, scales, biases, add, dx, M, N, K, group_size, bits,
+  return fmxq::input_grad(g, p.n8, w, scales, biases, add, dx, M, N, K, group_size, bits,
                           ws + p.product, base, stream, op);
 }
 

@@ -20,3 +20,17 @@ def lora_grad_workspace(M, N, K, E, r):
 def test_adapters_of_both_sides_together(N, K, E, r, want):
     got = lora_grad_workspace(1, N, K, E, r)
     assert got == ("FMXQ_OK" if want == "OK" else "FMXQ_ERR_" + want)
+
+
+def test_one_padded_copy_of_dy():
+    """Rows that are no multiple of 8 values are copied once: into the input gradient's own place."""
+    def bytes_of(name, *sizes):
+        n = ctypes.c_size_t()
+        assert getattr(_lib.load(), name)(*sizes, ctypes.byref(n)) == 0
+        return n.value
+
+    # The adapters' own parts are the same for 4097 and for 4104 values, but for the outer products' parts of 7 rows.
+    M, K = 600, 512
+    odd, even = (bytes_of("fmxq_quantized_matmul_lora_grad_workspace", M, N, K, 1, 8) -
+                 bytes_of("fmxq_quantized_matmul_grad_workspace", M, N, K) for N in (4097, 4104))
+    assert odd <= even
