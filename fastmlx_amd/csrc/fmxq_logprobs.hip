@@ -298,8 +298,9 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   if (n == 0) return;
   int32_t* ids = a.top_ids + m * n;
   float* lps = a.top_logp + m * n;
-  if (bad || s.zeros) {
-    // No order, or a row of zeros, whose logits are all alike.
+  if (bad || s.zeros || (top == 0.f && others == (float)(a.V - 1) && low == 0.f)) {
+    // No order, or a row of zeros, or a head of zeros for the row (all of its logits 0 in fp32): all
+    // alike.  (The search would sum every token again: 100 ms for one row of 128256 x 4096.)
     for (int i = tid; i < n; i += T) {
       ids[i] = bad ? -1 : i;
       lps[i] = -lz;

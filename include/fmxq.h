@@ -329,7 +329,8 @@ int fmxq_head_workspace(int64_t M, int64_t V, int64_t K, int top_k, bool with_gr
  * that of logits summed in 64 bits, equal ones to the lower token, at any temperature: every token whose
  * fp32 logit comes within its error of the last of them is summed again.  (The error of a sum of K products,
  * (K + 16) 2^-24 of their magnitudes' sum, is taken from the likeliest token, twice over: a token whose
- * products are larger than that, and cancel, may be missed among near ties.)  A row with a logit that is not
+ * products are larger than that, and cancel, may be missed among near ties.)  Logits that are
+ * all 0 in fp32 count as equal.  A row with a logit that is not
  * finite (minus infinity too), or with two further apart than fp32 holds, gives NaN and top_ids -1. */
 int fmxq_head_logprobs(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
                        const uint16_t* biases, const int32_t* ids, float* logp, float* entropy, float* lse,
