@@ -90,6 +90,21 @@ __device__ __forceinline__ float excess(float d) {
   return s * (d * d);
 }
 
+// log(1 + a / b) for 0 <= a <= b, relative to itself: 2 atanh(a / (2 b + a)), whose series over at most
+// 1/3 is cut off below 1e-8 of it.
+__device__ __forceinline__ float log1p_ratio(float a, float b) {
+  const float t = a / (2.f * b + a), u = t * t;
+  float s = 1.f / 15;
+  s = __builtin_fmaf(s, u, 1.f / 13);
+  s = __builtin_fmaf(s, u, 1.f / 11);
+  s = __builtin_fmaf(s, u, 1.f / 9);
+  s = __builtin_fmaf(s, u, 1.f / 7);
+  s = __builtin_fmaf(s, u, 1.f / 5);
+  s = __builtin_fmaf(s, u, 1.f / 3);
+  s = __builtin_fmaf(s, u, 1.f);
+  return 2.f * t * s;
+}
+
 // A row's tokens, lane j's entry among them, from the row's final (m, sum over the tokens that are
 // not wanted) and the entry's logit l2: exponentials relative to 2^top.
 //

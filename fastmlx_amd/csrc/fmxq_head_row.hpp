@@ -1,5 +1,5 @@
-// fmxq_head_row.hpp -- single rows of a quantized head, and logarithms near zero, as the losses
-// (fmxq_head.hip) and the log probabilities (fmxq_logprobs.hip) use them.
+// fmxq_head_row.hpp -- single rows of a quantized head, as the losses (fmxq_head.hip) and the log
+// probabilities (fmxq_logprobs.hip) read them.
 #pragma once
 #include "fmxq_common.hpp"
 #include "fmxq_grad_tile.hpp"
@@ -41,21 +41,6 @@ __device__ __forceinline__ void deq8(const Packed8& p, int bits, float* v) {
     v[2 * j] = bf16_lo(t);
     v[2 * j + 1] = bf16_hi(t);
   }
-}
-
-// log(1 + a / b) for 0 <= a <= b, relative to itself: 2 atanh(a / (2 b + a)), whose series over at most
-// 1/3 is cut off below 1e-8 of it.
-__device__ __forceinline__ float log1p_ratio(float a, float b) {
-  const float t = a / (2.f * b + a), u = t * t;
-  float s = 1.f / 15;
-  s = __builtin_fmaf(s, u, 1.f / 13);
-  s = __builtin_fmaf(s, u, 1.f / 11);
-  s = __builtin_fmaf(s, u, 1.f / 9);
-  s = __builtin_fmaf(s, u, 1.f / 7);
-  s = __builtin_fmaf(s, u, 1.f / 5);
-  s = __builtin_fmaf(s, u, 1.f / 3);
-  s = __builtin_fmaf(s, u, 1.f);
-  return 2.f * t * s;
 }
 
 }  // namespace fmxq
