@@ -6,8 +6,10 @@
 // which those of the largest fp32 value have room, in an order that the sizes alone decide: a
 // thread's, a block's, then the blocks' sums.  Every block of the second pass adds the blocks'
 // sums up again (8 KB from the cache), which costs less than a launch between the passes.
-// Bound: HBM.  The second pass walks the tiles from the last to the first, because what the
-// first pass read last is what the last-level cache still holds.
+// Bound: HBM (448 fp32 tensors of 0.34 GB 194 us, 5.2 TB/s of the three passes over them; bf16 99 us,
+// 5.1), and the two launches where there is little (14 tensors of one layer 10 us).  The second pass walks
+// a table's tiles from the last to the first, because what the first pass read last is what the last-level
+// cache still holds: of one table, that is; with more of them it begins with the first table again.
 #include "fmxq_common.hpp"
 #include "fmxq_train.hpp"
 
@@ -128,7 +130,8 @@ __global__ __launch_bounds__(kT) void clip_scale_kernel(ClipTable t, const doubl
   const uint32_t tid = threadIdx.x;
   const double v = norm_of(sums, red);
   if (norm && blockIdx.x == 0 && tid == 0) *norm = (float)v;
-  // A norm of zero, infinity or NaN says nothing about a scale: the gradients stay as they are.
+  // A norm of zero, infinity or NaN says nothing about a scale: the gradients stay as they are.  (In 64
+  // bits: finite gradients whose norm is past fp32's range are scaled by it.)
   const double c = (double)max_norm / v;
   const float f = v > 0. && v < __builtin_huge_val() && c < 1. ? (float)c : 1.f;
   for (uint32_t k = blockIdx.x; k < t.tiles; k += gridDim.x) {

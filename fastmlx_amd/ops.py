@@ -458,8 +458,9 @@ def head_logprobs(h, w, scales, biases, ids, top: int = 0, temperature: float = 
     an id below zero for an absent entry (0 in logp).  With l = logits / temperature and p =
     softmax(l): (logp [M, k], entropy [M], lse [M]) float32, and with ``top`` (up to 64) also
     (top_ids [M, top] int32, top_logp [M, top]), likeliest first, equal ones to the lower token.
-    An id past the vocabulary counts as absent, and device_error reports it.  A row whose logits are
-    not finite gives NaN and top_ids -1."""
+    The order is that of logits summed in 64 bits, at any temperature.  An id past the vocabulary counts
+    as absent, and device_error reports it.  A row with a logit that is not finite gives NaN and
+    top_ids -1."""
     if _fast is not None:
         r = _fast.head_logprobs(h, w, scales, biases, ids, top, float(temperature), group_size, bits)
         if r is not None:
@@ -698,7 +699,8 @@ def quantized_matmul_lora(x, w, scales, biases, a, b, adapters, lora_scales, gro
     x [..., K] bf16; w [N, K*bits/32]; a [E, r, K] and b [E, N, r] bf16, r a multiple of 8 up to
     128 (zeros fill smaller ranks); adapters [...] int32, below zero for a row without one;
     lora_scales [E] float32.  Returns y [..., N] bf16, summed in float32 and rounded once.  An adapter
-    past the last counts as none, and device_error reports it."""
+    past the last counts as none, and device_error reports it.  y is not finite exactly where the
+    formula is not, but an infinite operand may give NaN in place of an infinity."""
     if _fast is not None:
         r = _fast.qmm_lora(x, w, scales, biases, a, b, adapters, lora_scales, group_size, bits)
         if r is not None:
@@ -795,8 +797,9 @@ def clip_grad_norm(grads, max_norm: float, outs=None):
     """Gradients scaled by min(1, max_norm / norm), norm as grad_norm has it -> (outs, norm).
 
     outs: the results' tensors, of the gradients' shapes and types (new ones without); they may
-    be the gradients themselves.  A norm that is zero, infinite or NaN leaves the values as they
-    are, so a step can be skipped by the norm alone."""
+    be the gradients themselves.  Values stay as they are where the norm is zero, or where an infinity
+    or NaN among them makes it one, so a step can be skipped by the norm alone.  (Finite gradients whose
+    norm is past float32's range are scaled by its 64-bit value; the norm returned is infinite.)"""
     many = (list, tuple)  # others (a generator, for one) are walked once
     if not isinstance(grads, many):
         grads = list(grads)

@@ -439,7 +439,9 @@ int fmxq_grad_norm(const void* const* grads, const int64_t* counts, const int* b
 /* ... and the gradients scaled to a norm of max_norm >= 0 at most:
  *     outs[i] = grads[i] min(1, max_norm / norm),
  * in grads[i]'s type.  outs[i] may be grads[i]; otherwise no result may share memory with another or
- * with a gradient.  A norm that is zero, infinite or NaN leaves the values as they are. */
+ * with a gradient.  Values stay as they are where the norm is zero, or where an infinity or NaN among them
+ * makes it one.  (Finite gradients whose norm is past fp32's range are scaled by its 64-bit value; norm
+ * is an infinity then too.) */
 int fmxq_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* counts,
                         const int* bf16, int64_t n, float max_norm, float* norm, void* workspace,
                         size_t workspace_bytes, void* stream);
