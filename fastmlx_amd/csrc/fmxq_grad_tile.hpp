@@ -290,8 +290,11 @@ __device__ __forceinline__ void store_scores(const GradGemm& g, f32x16 (&acc)[MI
 
 // The gradient of log probabilities and entropy for the logits of a tile:
 //   d = -p (a + c (log p + entropy)),  p = 2^(l - lse),
-// as bf16 in e, zeros for the row's wanted tokens (whose share enters later) and from column N to
-// the tile's end.
+// as bf16 in e, zeros for the row's wanted tokens (whose share enters later, in fp32) and from column N to
+// the tile's end.  bf16, which the product behind takes: an entry is off by 2^-8 of itself at most, as in the
+// losses' gradients, before the result's own rounding.  (1000 rows, 128256 x 4096: dh is 0.00184 off in the 2-norm,
+// of which its own rounding alone is 0.00166; 37 rows 0.00169.  What is left in a second bf16 value would be
+// as many rows again for that product: 1.08 and 1.96 ms of a step of 3.3.)
 template <int MI, int NJ>
 __device__ __forceinline__ void store_coef(const GradGemm& g, const f32x16 (&acc)[MI][NJ],
                                            const uint32_t (&out)[MI][NJ], int64_t mw, int64_t mend,

@@ -4,8 +4,9 @@
 //   dx = dy deq(W) + dt A_e,  dt = s_e dy B_e
 //   dA_e = sum dt^T x,  dB_e = s_e sum dy^T t   over e's rows, t = x A_e^T
 // t and dt are fp32, as the sums of parts of the contraction.  As an operand of a matrix product
-// each is a few bf16 values that add up to it: two (16 bits of it) where the result is bf16, three
-// (all 24) for the fp32 gradients, so that no step rounds to bf16 but the result's.
+// each is a few bf16 values that add up to it: two (off by 2^-17 of it, where the result's own
+// rounding to bf16 is 2^-8) for y and dx, three (all 24 bits) for the fp32 gradients, so that no
+// step rounds to bf16 but the result's.
 //
 // The products with W take the adapter's part in their epilogue (add_lora): y and dx are written once,
 // from fp32 sums.  Here are the narrow products around them.  Their rows are ordered by adapter

@@ -491,9 +491,10 @@ __global__ __launch_bounds__(WAVES * 64, 1) void qmm_wide_kernel(WideArgs wa) {
       if constexpr (EXACT) {
         // ... a row group at a time, its adapters in turn; a row keeps its own one's part, so that another's
         // infinities do not reach it.  (2048 rows, 14336 x 4096: 262 us without an adapter, 275 with rank 16, and
-        // with rank 64 of 8 adapters in any order 286 with what comes before; u from global memory, whose
+        // with rank 64 of 8 adapters in runs of rows 285 with what comes before; u from global memory, whose
         // latency each group then waits for, 325.  The sums started from the adapters' part: 326, the loop
-        // then spills.)
+        // then spills.  A group of 32 rows is walked once for every adapter in it: rows in any order take 392
+        // with 8 adapters of rank 64, and 672 with 64 of them.)
         const LoraAdd& lo = wa.lora;
         const int64_t m = m0 + 32 * i + e32;
         int e = lo.u ? adapter_of(lo, m < a.M ? m : a.M - 1) : -1;

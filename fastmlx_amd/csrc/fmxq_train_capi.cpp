@@ -130,9 +130,13 @@ int clip(const void* const* grads, void* const* outs, const int64_t* counts, con
 // ---- adapters -----------------------------------------------------------------------
 
 constexpr int64_t kMaxRows = (1 << 24) - 1, kMaxWidth = (1 << 22) - 8;
-// Up to here the rows' shrinks are taken one at a time, in any order: one launch, which reads an adapter
-// again for every row (128 rows of 8 adapters, 14336 x 4096, rank 16: 10 us on top of the product; the sort,
-// the shrink and its parts, three launches, 17 us at 256 rows).
+// Up to here the rows' shrinks are taken one at a time, in any order: one launch, which reads an adapter and x
+// again for every value; above, the sort, the shrink and its parts, three launches, which read an adapter once for
+// 32 rows that share it.  (us that way and the other, 4 bits, 14336 x 4096.  128 rows: one adapter of rank 16
+// 46 and 51, of rank 128 69 and 73; 8 adapters in any order, rank 16 64 and 79, rank 128 167 and 194.  256 rows:
+// 61 and 64, 92 and 86; 77 and 90, 198 and 203.  Of 14336 values a row, 4096 outputs, 128 rows of one adapter of
+// rank 128 100 and 84, of 8 200 and 214; rank 64 and lower as above.  So depth times rank decides nearer to the
+// border than rows alone do.)
 constexpr int64_t kLoraFewRows = 128;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
