@@ -287,9 +287,15 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
   }
   if (tid == 0) s.ntiles = s.ncand = s.nbest = 0;
   __syncthreads();
-  // log p of a token from its logit, relative to the likeliest one's, which is what the others leave.
+  // log p of a token from its logit, relative to the likeliest one's, which is what the others leave: their
+  // sum relative to that one's 64-bit logit too, so that what its fp32 sum is off by is in neither.
+  const float d = bad ? nan : (float)((double)top - s.lead);
+  const float left = bad             ? nan
+                     : others == 0.f ? 0.f
+                     : d < 64.f      ? log1pf(others * __builtin_amdgcn_exp2f(d))
+                                     : __builtin_fmaf(d, kLn2, logf(others));
   auto logp = [&](int id, double l) {
-    return bad ? nan : id == first ? -lz : (float)((l - s.lead) * 0.6931471805599453 - (double)lz);
+    return bad ? nan : id == first ? -left : (float)((l - s.lead) * 0.6931471805599453 - (double)left);
   };
   if (tid < k) {
     const int id = a.ids[m * k + tid];
@@ -303,7 +309,7 @@ __global__ __launch_bounds__(T) void head_score_kernel(HeadScore a, const HeadTi
     // alike.  (The search would sum every token again: 100 ms for one row of 128256 x 4096.)
     for (int i = tid; i < n; i += T) {
       ids[i] = bad ? -1 : i;
-      lps[i] = -lz;
+      lps[i] = -left;
     }
     return;
   }

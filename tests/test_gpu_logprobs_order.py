@@ -118,3 +118,36 @@ def test_a_vocabulary_beyond_the_few_row_products_blocks(gpu, M):
     R.check(got[2], lse, tol, "lse")
     R.check(got[0][:, 0], l.gather(1, (torch.arange(M, device=gpu) % 6)[:, None])[:, 0] - lse, tol, "logp")
     assert torch.equal(got[3].long(), at[[4, 1, 3]].expand(M, 3))
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("V", [3, 5000])
+@pytest.mark.parametrize("T", [1.0, 1e-6])
+@pytest.mark.parametrize("part", [1, 3])
+def test_a_likeliest_token_that_fp32_rounds(gpu, M, V, T, part):
+    """The likeliest token's logit 8.5 + part / 32 as 2^20 + 8.5 + part / 32 - 2^20, which fp32 rounds (down for 1, up
+    for 3); the others' is 8 exactly: what its sum is off by reaches other tokens' numbers by its probability only,
+    and its own by what the others have.  At the low temperature it is off by thousands, and the others have nothing."""
+    announce(f"rounded leader {M} {V} {T} {part}")
+    K = 512
+    words = torch.zeros(V, K // 8, dtype=torch.int32, device=gpu)
+    s = torch.zeros(V, K // 64, dtype=torch.bfloat16, device=gpu)  # all weights of a group are its bias
+    b = torch.zeros_like(s)
+    b[:, 0] = 8.0
+    lead = V // 2
+    b[lead] = torch.tensor([2.0 ** 20, 0, 0, 8.5, part / 32, 0, 0, -2.0 ** 20], device=gpu).bfloat16()
+    h = torch.zeros(M, K, dtype=torch.bfloat16, device=gpu)
+    h[:, ::64] = 1.0
+    ids = torch.tensor([[0, lead]], dtype=torch.int32, device=gpu).expand(M, 2).contiguous()
+    got = ops.head_logprobs(h, words, s, b, ids, top=2, temperature=T)
+    l = torch.full((V,), 8.0 / T, dtype=torch.float64, device=gpu)
+    l[lead] = (8.5 + part / 32) / T
+    lse = torch.logsumexp(l, -1)
+    p = float((l[lead] - lse).exp())
+    # Of the leader 8 products of 2^20 at most, of the others the scaling to units of log 2 and back; two logarithms.
+    el = (10 * R.U32 * 2 ** 21 + 8 * R.U32 * 8) / T
+    tol = torch.tensor([p * el, (1 - p) * (8 * R.U32 * 8 / T + 16 * R.U32)], dtype=torch.float64, device=gpu)
+    want = l[ids.long()] - lse
+    R.check(got[0], want, tol + 32 * R.U32 * (1 + want.abs()), "logp")
+    assert bool((got[3] == torch.tensor([lead, 0], dtype=torch.int32, device=gpu)).all())
+    assert torch.equal(got[4], got[0].flip(1))
