@@ -325,13 +325,14 @@ int fmxq_head_workspace(int64_t M, int64_t V, int64_t K, int top_k, bool with_gr
  *     entropy[t] = -sum_v p_v log p_v,
  * and the `top` tokens of the largest l with their log probabilities, in falling order: top_ids and
  * top_logp [M, top], 0 <= top <= min(64, V).  ids and logp [M, k], 0 <= k <= 64; an id below zero is
- * absent (logp 0), one of V or more too, which raises the error flag.  The order of the top tokens is
- * that of logits summed in 64 bits, equal ones to the lower token, at any temperature: every token whose
- * fp32 logit comes within its error of the last of them is summed again.  (The error of a sum of K products,
- * (K + 16) 2^-24 of their magnitudes' sum, is taken from the likeliest token, twice over: a token whose
- * products are larger than that, and cancel, may be missed among near ties.)  Logits that are
- * all 0 in fp32 count as equal.  A row with a logit that is not
- * finite (minus infinity too), or with two further apart than fp32 holds, gives NaN and top_ids -1. */
+ * absent (logp 0), one of V or more too, which raises the error flag.
+ * The order of the top tokens is that of logits summed in 64 bits, equal ones to the lower token, at any
+ * temperature: every token whose fp32 logit comes within its error of the last of them is summed again.
+ * (The error of a sum of K products, (K + 16) 2^-24 of their magnitudes' sum, is taken from the likeliest
+ * token, twice over: a token whose products are larger than that, and cancel, may be missed among near
+ * ties.)  Logits that are all 0 in fp32 count as equal.
+ * A row with a logit that is not finite (minus infinity too), or with two further apart than fp32 holds,
+ * gives NaN and top_ids -1. */
 int fmxq_head_logprobs(const uint16_t* h, const uint32_t* w, const uint16_t* scales,
                        const uint16_t* biases, const int32_t* ids, float* logp, float* entropy, float* lse,
                        int32_t* top_ids, float* top_logp, int64_t M, int64_t V, int64_t K, int k, int top,
